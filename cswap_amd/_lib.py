@@ -120,6 +120,17 @@ _SIGNATURES = {
     "cswap_test_zvc_packed_hint": (i32, [sz]),
     "cswap_test_zfp_encode_route": (i32, [sz, sz, sz, pd, pd, u, u, i32]),
     "cswap_zvc_compress_fused_static": (i32, [vp, i32, i32, vp, vp, vp, vp, vp]),
+    "cswap_q8_code_pitch": (sz, [sz]),
+    "cswap_q8_scale_pitch": (sz, [sz]),
+    "cswap_q8_pack": (i32, [vp, i32, sz, sz, pd, vp, vp, vp]),
+    "cswap_q8_unpack": (i32, [vp, vp, sz, sz, vp, i32, pd, vp]),
+    "cswap_q8_act_forward": (i32, [i32, vp, i32, sz, sz, pd, vp, pd, vp, vp, vp]),
+    "cswap_q8_act_backward": (i32, [i32, vp, i32, sz, sz, pd, vp, vp, vp, pd, vp]),
+    "cswap_layer_norm_forward": (i32, [vp, i32, sz, sz, pd, vp, vp, i32, C.c_float, vp, pd, vp, vp, vp, vp, vp]),
+    "cswap_layer_norm_workspace_bytes": (sz, [sz, sz]),
+    "cswap_layer_norm_backward": (i32, [vp, i32, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
+    "cswap_q8_weight_grad_workspace_bytes": (sz, [sz, sz, sz]),
+    "cswap_q8_weight_grad": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, vp, vp, i32, vp, sz, vp]),
     "cswap_probe_nnz": (i32, [vp, sz, vp, vp]),
     "cswap_costs_default": (None, [C.POINTER(Costs)]),
     "cswap_policy_bytes": (sz, [i32, sz, sz, u, i32, sz, sz, sz]),

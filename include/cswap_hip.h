@@ -249,6 +249,77 @@ size_t cswap_zvc_set_single_pass_bytes(size_t bytes);
 int cswap_zvc_compress_fused_static(const float* d_in, int n, int process, int* d_begin, int* d_nnz,
                                     float* d_values, uint32_t* d_mask, cswap_stream_t stream);
 
+/* ------------------------------------------------- 8-bit checkpoints (q8) -----
+ * No counterpart in the reference, which compresses activations to move them.  A
+ * checkpoint holds an activation of rows x cols values in one byte and a 32nd each,
+ * for a backward pass that reads it as it is: groups of 32 consecutive values of a row
+ * (the last one of a row may be shorter) share the power of two 2^e,
+ * e = clamp(floor(log2(largest magnitude)) - 6, -126, 121), held as the byte e + 127, and
+ * a value x is held as the signed byte q = clamp(rint(x / 2^e), -127, 127) and stands
+ * for q * 2^e.  It is off by at most 2^(e-1), by less than 2^e where |x| > 127 * 2^e: by
+ * at most 2^-7 of the group's largest magnitude.  A group that holds a NaN or an
+ * infinity stands for NaN in all its values (byte 255, codes 0).  -0 becomes +0.
+ * Codes do not depend on who computes them, and q * 2^e is a bf16 and an fp32 value
+ * exactly (an fp16 value, too, if x was one).
+ * Layout: d_codes[rows][cswap_q8_code_pitch(cols)], every byte of which is written (0
+ * behind a row's last value), 8-byte aligned, and d_scales[rows][cswap_q8_scale_pitch(cols)].
+ * If cols is a multiple of 32 both are those of one row of rows * cols values.
+ *
+ * Strides are in elements between the starts of rows, 0 = cols; a row itself is
+ * contiguous and may start at any element.  rows may be 0.  Outputs must not overlap
+ * inputs.  CSWAP_E_UNSUPPORTED beyond 2^31 - 1 pieces of 8 values, each row rounded up to
+ * whole groups. */
+typedef enum { CSWAP_DT_F32 = 0, CSWAP_DT_BF16 = 1, CSWAP_DT_F16 = 2 } cswap_dtype;
+size_t cswap_q8_code_pitch(size_t cols);  /* cols rounded up to a multiple of 32 */
+size_t cswap_q8_scale_pitch(size_t cols); /* groups of a row */
+int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride,
+                  int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
+/* Rounds once where `dtype` does not hold q * 2^e. */
+int cswap_q8_unpack(const int8_t* d_codes, const uint8_t* d_scales, size_t rows, size_t cols,
+                    void* d_out, int dtype, ptrdiff_t stride, cswap_stream_t stream);
+
+/* y = f(x) and the checkpoint of x in one pass; dx = dy f'(x^) from the checkpoint x^.
+ * f in fp32 whatever the type: x Phi(x), its tanh form, x / (1 + exp(-x)).  y is 0 where x is
+ * minus infinity. */
+typedef enum { CSWAP_ACT_GELU = 0, CSWAP_ACT_GELU_TANH = 1, CSWAP_ACT_SILU = 2 } cswap_act;
+int cswap_q8_act_forward(int kind, const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
+                         void* d_y, ptrdiff_t y_stride, int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
+int cswap_q8_act_backward(int kind, const void* d_dy, int dtype, size_t rows, size_t cols, ptrdiff_t dy_stride,
+                          const int8_t* d_codes, const uint8_t* d_scales, void* d_dx, ptrdiff_t dx_stride,
+                          cswap_stream_t stream);
+
+/* Layer norm over rows of up to 16384 values (CSWAP_E_UNSUPPORTED beyond).  Forward:
+ * y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps), per row in fp32; gamma and
+ * beta (param_dtype) may be NULL; the checkpoint of x is made where d_codes and d_scales are
+ * given.  Backward takes x either as it is (d_x, d_codes = d_scales = NULL) or as its checkpoint
+ * (d_x = NULL), with the mean and rstd of the forward pass; d_dgamma and d_dbeta (param_dtype)
+ * may be NULL, and where neither is wanted so may d_ws.  Their sums over rows are made in fp32 in
+ * a fixed order: the same call gives the same bits.  d_ws: cswap_layer_norm_workspace_bytes,
+ * 4-byte aligned, with no preparation; calls that overlap must not share one. */
+int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
+                             const void* d_gamma, const void* d_beta, int param_dtype, float eps,
+                             void* d_y, ptrdiff_t y_stride, float* d_mean, float* d_rstd,
+                             int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
+size_t cswap_layer_norm_workspace_bytes(size_t rows, size_t cols);
+int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t cols, ptrdiff_t dy_stride,
+                              const void* d_x, ptrdiff_t x_stride, const int8_t* d_codes, const uint8_t* d_scales,
+                              const float* d_mean, const float* d_rstd, const void* d_gamma, int param_dtype,
+                              void* d_dx, ptrdiff_t dx_stride, void* d_dgamma, void* d_dbeta,
+                              void* d_ws, size_t ws_bytes, cswap_stream_t stream);
+
+/* Gradients of a linear layer y = x W^T + b (W: n x k) from the checkpoint x^ of its input
+ * (rows x k): dw[n][k] = sum over rows of dy[.][n] x^[.][k], db[n] = sum over rows of dy[.][n]
+ * (NULL: not wanted), in out_dtype, contiguous.  Products are exact for fp32 and bf16 dy and
+ * summed in fp32, in a fixed order; for fp16 dy x^ is rounded to fp16, which changes nothing if
+ * the checkpoint was made from fp16.  rows = 0 gives zeros.  n and k up to 2^20.  d_ws:
+ * cswap_q8_weight_grad_workspace_bytes, 16-byte aligned, with no preparation; calls that overlap
+ * must not share one. */
+size_t cswap_q8_weight_grad_workspace_bytes(size_t rows, size_t n, size_t k);
+int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride,
+                         const int8_t* d_codes, const uint8_t* d_scales, size_t k,
+                         void* d_dw, void* d_db, int out_dtype, void* d_ws, size_t ws_bytes,
+                         cswap_stream_t stream);
+
 /* ---------------------------------------------------------------- probe -----
  * One fused read pass: *d_nnz = number of elements != 0 (the quantity the
  * reference derives from PreGPUcompression + PreAcc, Execution.h:89-92). */
