@@ -214,7 +214,8 @@ def test_layer_norm_of_a_row_that_is_not_finite_leaves_the_others():
 
 # ---------------------------------------------------------------- weight gradient
 GRADS = [(1, 1, 1), (1, 130, 40), (7, 33, 65), (64, 256, 256), (31, 100, 193), (333, 129, 257), (1000, 300, 96), (2050, 64, 128),
-         (700, 520, 130), (4100, 17, 300), (128, 128, 128), (515, 1000, 193)]
+         (700, 520, 130), (4100, 17, 300), (128, 128, 128), (515, 1000, 193),
+         (2050, 2900, 2850)]    # the last one in the larger tiles, with rows, columns and both features cut off
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
