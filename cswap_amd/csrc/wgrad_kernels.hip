@@ -34,17 +34,10 @@ __device__ inline f16v mma(F16, uint4 a, uint4 b, f16v c)
 template <typename T> struct Feed {  // the type that the matrix instructions see, and how many of it make one dY
   typedef T type;
   static constexpr int parts = 1;
-  static constexpr uint32_t one = 0x3f803f80u;
 };
 template <> struct Feed<F32> {
   typedef BF16 type;
   static constexpr int parts = 3;
-  static constexpr uint32_t one = 0x3f803f80u;
-};
-template <> struct Feed<F16> {
-  typedef F16 type;
-  static constexpr int parts = 1;
-  static constexpr uint32_t one = 0x3c003c00u;
 };
 
 struct GradShape {
@@ -77,7 +70,7 @@ __device__ inline void split3(const float v[8], uint4 out[3])
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_s4;
 
-// eight m of one column for each lane, from two transposing reads of four; `at` as `Reader` has it
+// eight m of one column for each lane, from two transposing reads of four
 __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
 {
   const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at));
@@ -86,20 +79,40 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
   return make_uint4(x.x, x.y, y.x, y.y);
 }
 
-// A workgroup of four wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows at a time.
+// A workgroup of four wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.
+//
+// The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m: the
+// transposing reads take four rows at once, which have to lie in different banks.  a_at and b_at are the places of value
+// (m, column) of either operand, in 16-bit units.
+template <typename T, int TN, int TK, int BK> struct GradTile {
+  static constexpr int P = Feed<T>::parts;
+  static constexpr int kAPlane = BK * TN, kStage = P * kAPlane + BK * TK;
+  static __device__ inline int a_at(int m, int col) { return m * TN + 8 * ((col >> 3) ^ ((m & 3) << 2)) + (col & 7); }
+  static __device__ inline int b_at(int m, int col)
+  {
+    // pieces of 16 codes leave a lane as two chunks: those of all pieces first, then those of the others, so that neighbouring
+    // lanes write neighbouring chunks
+    const int piece = col >> 4, h = (col >> 3) & 1;
+    return P * kAPlane + m * TK + 8 * (h * (TK / 16) + (piece ^ (2 * (m & 3)) ^ (TK == 256 ? 8 * h : 0))) + (col & 7);
+  }
+};
+
 template <typename T, int TN, int TK, int BK>
 __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::value* __restrict__ dy,
                                                              const int8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, GradShape s,
-                                                             float* __restrict__ dw, float* __restrict__ db)
+                                                             float* __restrict__ dw, float* __restrict__ db,
+                                                             const char* __restrict__ spare)
 {
-  constexpr int P = Feed<T>::parts;
+  typedef GradTile<T, TN, TK, BK> Tile;
   typedef typename Feed<T>::type M;
+  typedef typename T::value V;
+  constexpr int P = Feed<T>::parts, W = T::bytes / 2;               // 16-byte words of a chunk of dY
   constexpr int FN = TN / 64, FK = TK / 64;                       // 32 x 32 pieces of a wavefront's quarter
+  constexpr int kSteps = BK / 16;                                   // matrix instructions' depth
   constexpr int kAChunks = TN / 8, kARows = 256 / kAChunks, kALoads = BK / kARows;
   constexpr int kBPieces = TK / 16, kBRows = 256 / kBPieces, kBLoads = BK / kBRows;
-  constexpr int kAPlane = BK * TN, kStage = P * kAPlane + BK * TK;  // 16-bit values
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kStage];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][Tile::kStage];
 
   const uint32_t tile = blockIdx.x;
   const uint32_t tk = tile % s.tiles_k, rest = tile / s.tiles_k, tn = rest % s.tiles_n, split = rest / s.tiles_n;
@@ -108,142 +121,192 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
   const uint32_t stages = (to - from + BK - 1) / BK;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
 
+  // A stage is plain if all of its loads are in the tensors: columns behind a row's last one read what lies there, which goes
+  // into columns of the product that nobody stores.  Rows that are not there have to be zeros in both operands; the stages from
+  // the first one that is not plain on (the last rows of the tensors) are brought in value by value.
+  const size_t dy_end = (size_t)(s.rows - 1) * s.dy_stride + s.n;
+  uint32_t plain = stages;
+  while (plain > 0) {
+    const uint32_t end = from + plain * BK;
+    if (end <= to && (size_t)(end - 1) * s.dy_stride + n0 + TN <= dy_end &&
+        (size_t)(end - 1) * s.code_pitch + k0 + TK <= (size_t)s.rows * s.code_pitch)
+      break;
+    --plain;
+  }
+  // The loop asks for a plain stage in every turn, the last one again where there is no other; without any it reads the spare
+  // room behind the workspace's sums, and what it reads is not used.
+  const size_t dy_stride = plain ? s.dy_stride : 0, code_pitch = plain ? s.code_pitch : 0, scale_pitch = plain ? s.scale_pitch : 0;
+  const char* const dy_from = plain ? reinterpret_cast<const char*>(dy + (size_t)from * s.dy_stride + n0) : spare;
+  const char* const codes_from = plain ? reinterpret_cast<const char*>(codes) + (size_t)from * s.code_pitch + k0 : spare;
+  const char* const scales_from = plain ? reinterpret_cast<const char*>(scales) + (size_t)from * s.scale_pitch + k0 / kGroup : spare;
+
   // staging: this thread's column chunk and first row of either operand
   const int a_chunk = tid % kAChunks, a_row = tid / kAChunks, b_piece = tid % kBPieces, b_row = tid / kBPieces;
-  const uint32_t a_col = n0 + 8 * a_chunk, b_col = k0 + 16 * b_piece;
-  const int a_valid = a_col + 8 <= s.n ? 8 : a_col < s.n ? (int)(s.n - a_col) : 0;
-  const bool b_here = b_col < s.code_pitch;
-  const bool a_edge = n0 + TN > s.n, b_edge = k0 + TK > s.code_pitch;
-  u4_any a_raw[kALoads][T::bytes / 2], b_raw[kBLoads];
+  const uint32_t a_off = ((uint32_t)a_row * (uint32_t)dy_stride + 8 * a_chunk) * (uint32_t)sizeof(V);
+  const uint32_t b_off = (uint32_t)b_row * (uint32_t)code_pitch + 16 * b_piece;
+  const uint32_t c_off = (uint32_t)b_row * (uint32_t)scale_pitch + b_piece / 2;
+  u4_any a_raw[kALoads][W], b_raw[kBLoads];
   uint32_t b_scale[kBLoads];
-
-  auto load = [&](uint32_t m0) {
-    const bool whole = m0 + BK <= to;
+  auto load_a = [&](uint32_t st, int i) {
+    const char* base = dy_from + (size_t)(st * BK + i * kARows) * dy_stride * sizeof(V);
 #pragma unroll
-    for (int i = 0; i < kALoads; ++i) {
-      const uint32_t m = m0 + a_row + i * kARows;
-      const typename T::value* p = dy + (size_t)m * s.dy_stride + a_col;
-      if (whole && !a_edge) {
+    for (int h = 0; h < W; ++h) a_raw[i][h] = *reinterpret_cast<const u4_any*>(base + a_off + 16 * h);
+  };
+  auto load_b = [&](uint32_t st, int i) {
+    b_raw[i] = *reinterpret_cast<const u4_any*>(codes_from + (size_t)(st * BK + i * kBRows) * code_pitch + b_off);
+    b_scale[i] = *reinterpret_cast<const uint8_t*>(scales_from + (size_t)(st * BK + i * kBRows) * scale_pitch + c_off);
+  };
+  auto store_a = [&](uint16_t* buf, int i) {
+    uint16_t* at = buf + Tile::a_at(a_row + i * kARows, 8 * a_chunk);
+    if constexpr (P == 3) {
+      float v[8];
+      uint4 w[3];
 #pragma unroll
-        for (int h = 0; h < T::bytes / 2; ++h) a_raw[i][h] = reinterpret_cast<const u4_any*>(p)[h];
-      } else {
+      for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(a_raw[i][0][e]), v[4 + e] = __uint_as_float(a_raw[i][1][e]);
+      split3(v, w);
 #pragma unroll
-        for (int h = 0; h < T::bytes / 2; ++h) a_raw[i][h] = (u4_any){0, 0, 0, 0};
-        if (m < to) {
-          if (a_valid == 8) {
-#pragma unroll
-            for (int h = 0; h < T::bytes / 2; ++h) a_raw[i][h] = reinterpret_cast<const u4_any*>(p)[h];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 7; ++e)
-              if (e < a_valid) {
-                if (T::bytes == 4) a_raw[i][(e / 4) % (T::bytes / 2)][e % 4] = reinterpret_cast<const uint32_t*>(p)[e];
-                else a_raw[i][0][e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-              }
-          }
-        }
-      }
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(at + p * Tile::kAPlane) = w[p];
+    } else {
+      *reinterpret_cast<uint4*>(at) = make_uint4(a_raw[i][0][0], a_raw[i][0][1], a_raw[i][0][2], a_raw[i][0][3]);
     }
+  };
+  auto store_b = [&](uint16_t* buf, int i) {
+    const float unit = unit_of(b_scale[i]);
 #pragma unroll
-    for (int i = 0; i < kBLoads; ++i) {
-      const uint32_t m = m0 + b_row + i * kBRows;
-      b_raw[i] = (u4_any){0, 0, 0, 0}, b_scale[i] = 1;
-      if ((whole && !b_edge) || (b_here && m < to)) {
-        b_raw[i] = *reinterpret_cast<const u4_any*>(codes + (size_t)m * s.code_pitch + b_col);
-        b_scale[i] = scales[(size_t)m * s.scale_pitch + b_col / kGroup];
-      }
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+      decode_chunk(make_uint2(b_raw[i][2 * h], b_raw[i][2 * h + 1]), unit, v);
+      *reinterpret_cast<uint4*>(buf + Tile::b_at(b_row + i * kBRows, 16 * b_piece + 8 * h)) =
+          make_uint4(to_pair<M>(v[0], v[1]), to_pair<M>(v[2], v[3]), to_pair<M>(v[4], v[5]), to_pair<M>(v[6], v[7]));
     }
   };
 
-  // The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m:
-  // the transposing reads take four rows at once, which have to lie in different banks.
-  auto store = [&](uint16_t* buf) {
+  // db: the columns of dY, each stage's added up by one of the workgroups that have them
+  float b_sum[8] = {}, b_edge = 0.0f;
+  auto add_columns = [&] {
 #pragma unroll
-    for (int i = 0; i < kALoads; ++i) {
-      const int m = a_row + i * kARows;
-      uint16_t* at = buf + m * TN + 8 * (a_chunk ^ ((m & 3) << 2));
+    for (int i = 0; i < kALoads; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        b_sum[e] += T::bytes == 4 ? __uint_as_float(a_raw[i][(e / 4) % W][e % 4])
+                                  : to_float<T>((V)(uint16_t)(a_raw[i][0][e / 2] >> (16 * (e & 1))));
+  };
+
+  auto stage_by_value = [&](uint16_t* buf, uint32_t m0, bool mine) {
+    const int c = tid % TN;
+    for (int m = tid / TN; m < BK; m += 256 / TN) {
+      const bool here = m0 + m < to && n0 + c < s.n;
+      const V raw = here ? dy[(size_t)(m0 + m) * s.dy_stride + n0 + c] : (V)0;
+      if (mine) b_edge += to_float<T>(raw);
       if constexpr (P == 3) {
-        float v[8];
-        uint4 w[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(a_raw[i][0][e]), v[4 + e] = __uint_as_float(a_raw[i][1][e]);
-        split3(v, w);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(at + p * kAPlane) = w[p];
+        const uint32_t a0 = __float_as_uint(raw) & 0xffff0000u;
+        const float r = raw - __uint_as_float(a0);
+        const uint32_t a1 = __float_as_uint(r) & 0xffff0000u;
+        uint16_t* at = buf + Tile::a_at(m, c);
+        at[0] = (uint16_t)(a0 >> 16), at[Tile::kAPlane] = (uint16_t)(a1 >> 16);
+        at[2 * Tile::kAPlane] = (uint16_t)(__float_as_uint(r - __uint_as_float(a1)) >> 16);
       } else {
-        *reinterpret_cast<uint4*>(at) = make_uint4(a_raw[i][0][0], a_raw[i][0][1], a_raw[i][0][2], a_raw[i][0][3]);
+        buf[Tile::a_at(m, c)] = raw;
       }
     }
-#pragma unroll
-    for (int i = 0; i < kBLoads; ++i) {
-      const int m = b_row + i * kBRows;
-      const float unit = unit_of(b_scale[i]);
-      uint16_t* row = buf + P * kAPlane + m * TK;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-        decode_chunk(make_uint2(b_raw[i][2 * h], b_raw[i][2 * h + 1]), unit, v);
-        *reinterpret_cast<uint4*>(row + 8 * (h * kBPieces + (b_piece ^ (2 * (m & 3)) ^ (TK == 256 ? 8 * h : 0)))) =
-            make_uint4(to_pair<M>(v[0], v[1]), to_pair<M>(v[2], v[3]), to_pair<M>(v[4], v[5]), to_pair<M>(v[6], v[7]));
-      }
+    const int k = tid % TK;
+    for (int m = tid / TK; m < BK; m += 256 / TK) {
+      float v = 0.0f;
+      if (m0 + m < to && k0 + k < s.k)
+        v = (float)codes[(size_t)(m0 + m) * s.code_pitch + k0 + k] *
+            unit_of(scales[(size_t)(m0 + m) * s.scale_pitch + (k0 + k) / kGroup]);
+      buf[Tile::b_at(m, k)] = from_float<M>(v);
     }
   };
 
   // reading: a lane supplies the address of four values of row 8 (lane / 32) + (lane % 16) / 4 and gets column lane % 32
-  const int quad_row = (lane & 15) >> 2, m_lane = 8 * (lane >> 5) + quad_row;
+  const int m_lane = 8 * (lane >> 5) + ((lane & 15) >> 2), c_lane = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   int a_at[FN], b_at[FK];
 #pragma unroll
-  for (int i = 0; i < FN; ++i) {
-    const int col = ((wave >> 1) * FN + i) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    a_at[i] = m_lane * TN + 8 * ((col >> 3) ^ (quad_row << 2)) + (col & 7);
-  }
+  for (int i = 0; i < FN; ++i) a_at[i] = Tile::a_at(m_lane, ((wave >> 1) * FN + i) * 32 + c_lane);
 #pragma unroll
-  for (int j = 0; j < FK; ++j) {
-    const int col = ((wave & 1) * FK + j) * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const int piece = col >> 4, h = (col >> 3) & 1;
-    b_at[j] = P * kAPlane + m_lane * TK + 8 * (h * kBPieces + (piece ^ (2 * quad_row) ^ (TK == 256 ? 8 * h : 0))) + (col & 7);
-  }
+  for (int j = 0; j < FK; ++j) b_at[j] = Tile::b_at(m_lane, ((wave & 1) * FK + j) * 32 + c_lane);
 
-  f16v acc[FN][FK] = {}, acc_b[FN] = {};
-  if (stages) {
-    load(from);
-    store(lds[0]);
-    if (stages > 1) load(from + BK);
-  }
-  for (uint32_t st = 0; st < stages; ++st) {
-    __syncthreads();
-    const uint16_t* buf = lds[st & 1];
-    // the sum of dY's columns: a product with ones, each stage by one of the wavefronts that have its columns
-    const bool bias = db && st % (2 * s.tiles_k) == 2 * tk + (wave & 1);
+  f16v acc[FN][FK] = {};
+  uint4 a[2][FN], b[2][FK];
+  auto read_a = [&](const uint16_t* buf, int c, int p, uint4* to_a) {
 #pragma unroll
-    for (int c = 0; c < BK / 16; ++c) {
-      uint4 b[FK];
+    for (int i = 0; i < FN; ++i) to_a[i] = read_turned(buf + p * Tile::kAPlane + a_at[i] + c * 16 * TN, 4 * TN);
+  };
+  auto read_b = [&](const uint16_t* buf, int c, uint4* to_b) {
 #pragma unroll
-      for (int j = 0; j < FK; ++j) b[j] = read_turned(buf + b_at[j] + c * 16 * TK, 4 * TK);
+    for (int j = 0; j < FK; ++j) to_b[j] = read_turned(buf + b_at[j] + c * 16 * TK, 4 * TK);
+  };
+
+  // One stage's products.  Meanwhile the next one goes from registers to LDS and the one after that is asked for; the fragments of
+  // a step are read while the step before multiplies.
+  auto compute = [&](const uint16_t* buf, uint16_t* next, uint32_t after) {
+    read_b(buf, 0, b[0]);
+    read_a(buf, 0, P - 1, a[0]);
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p) {
-        uint4 a[FN];
+    for (int c = 0; c < kSteps; ++c) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i) a[i] = read_turned(buf + p * kAPlane + a_at[i] + c * 16 * TN, 4 * TN);
+      for (int q = 0; q < P; ++q) {
+        constexpr int kParts = kSteps * P;
+        const int part = c * P + q, at = part & 1;
+        if (q + 1 < P) {
+          read_a(buf, c, P - 2 - q, a[at ^ 1]);
+        } else if (c + 1 < kSteps) {
+          read_b(buf, c + 1, b[(c + 1) & 1]);
+          read_a(buf, c + 1, P - 1, a[at ^ 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < kALoads; ++i)
+          if (i * kParts / kALoads == part) {
+            store_a(next, i);
+            load_a(after, i);
+          }
+#pragma unroll
+        for (int i = 0; i < kBLoads; ++i)
+          if (i * kParts / kBLoads == part) {
+            store_b(next, i);
+            load_b(after, i);
+          }
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
-          for (int j = 0; j < FK; ++j) acc[i][j] = mma(M(), a[i], b[j], acc[i][j]);
-        if (bias) {
-          const uint32_t o = Feed<T>::one;
-#pragma unroll
-          for (int i = 0; i < FN; ++i) acc_b[i] = mma(M(), a[i], make_uint4(o, o, o, o), acc_b[i]);
-        }
+          for (int j = 0; j < FK; ++j) acc[i][j] = mma(M(), a[at][i], b[c & 1][j], acc[i][j]);
       }
     }
-    if (st + 1 < stages) {
-      store(lds[(st + 1) & 1]);
-      if (st + 2 < stages) load(from + (st + 2) * BK);
+  };
+
+  auto load = [&](uint32_t st) {
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) load_a(st, i);
+#pragma unroll
+    for (int i = 0; i < kBLoads; ++i) load_b(st, i);
+  };
+  auto my_turn = [&](uint32_t st) { return db && st % s.tiles_k == tk; };
+  const uint32_t last = plain ? plain - 1 : 0;
+
+  if (plain) {
+    load(0);
+    if (my_turn(0)) add_columns();
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) store_a(lds[0], i);
+#pragma unroll
+    for (int i = 0; i < kBLoads; ++i) store_b(lds[0], i);
+  } else if (stages) {
+    stage_by_value(lds[0], from, my_turn(0));
+  }
+  load(min(1u, last));
+  for (uint32_t st = 0; st < stages; ++st) {
+    __syncthreads();
+    if (st + 1 < plain && my_turn(st + 1)) add_columns();
+    uint16_t* next = lds[(st + 1) & 1];
+    compute(lds[st & 1], next, min(st + 2, last));
+    if (st + 1 < stages && st + 1 >= plain) {
+      __syncthreads();  // the turn has left something there
+      stage_by_value(next, from + (st + 1) * BK, my_turn(st + 1));
     }
   }
 
   float* out = dw + (size_t)split * s.n * s.k;
-  float* out_b = db + (size_t)((split * s.tiles_k + tk) * 2 + (wave & 1)) * s.n;
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
@@ -255,24 +318,77 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
         const uint32_t k = k0 + ((wave & 1) * FK + j) * 32 + (lane & 31);
         if (k < s.k) out[(size_t)n * s.k + k] = acc[i][j][r];
       }
-      if (db && (lane & 31) == 0) out_b[n] = acc_b[i][r];
     }
+  if (db) {
+    float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows + 256 / TN][TN]
+    static_assert(sizeof(lds) >= sizeof(float) * (kARows + 256 / TN) * TN, "room for the columns' sums");
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[a_row * TN + 8 * a_chunk + e] = b_sum[e];
+    sums[kARows * TN + tid] = b_edge;
+    __syncthreads();
+    if (tid < TN && n0 + tid < s.n) {
+      float v = 0.0f;
+      for (int r = 0; r < kARows + 256 / TN; ++r) v += sums[r * TN + tid];
+      db[(size_t)(split * s.tiles_k + tk) * s.n + n0 + tid] = v;
+    }
+  }
 }
 
-// out[i] = sum over `parts` of part[.][i], rounded once
-template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_kernel(const float* __restrict__ part,
-                                                                                       uint32_t parts, size_t count,
-                                                                                       typename O::value* __restrict__ out)
+// out[i] = sum over `parts` of part[.][i], rounded once: dW from its splits, four values a thread, and behind them db
+struct GradSums {
+  const float *dw, *db;
+  size_t dw_count, dw_groups;  // workgroups that sum dW
+  uint32_t dw_parts, db_parts, n;
+};
+
+template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_kernel(GradSums s, typename O::value* __restrict__ dw,
+                                                                                       typename O::value* __restrict__ db)
 {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (size_t)gridDim.x * 256) {
+  if (blockIdx.x < s.dw_groups) {
+    const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at + 4 <= s.dw_count) {
+      float v[4] = {};
+#pragma unroll 4
+      for (uint32_t p = 0; p < s.dw_parts; ++p) {
+        const u4_any w = *reinterpret_cast<const u4_any*>(s.dw + (size_t)p * s.dw_count + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(w[i]);
+      }
+      if constexpr (O::bytes == 4)
+        *reinterpret_cast<u4_any*>(dw + at) =
+            (u4_any){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      else
+        *reinterpret_cast<u2_any*>(dw + at) = (u2_any){to_pair<O>(v[0], v[1]), to_pair<O>(v[2], v[3])};
+    } else {
+      for (size_t i = at; i < s.dw_count; ++i) {
+        float v = 0.0f;
+        for (uint32_t p = 0; p < s.dw_parts; ++p) v += s.dw[(size_t)p * s.dw_count + i];
+        dw[i] = from_float<O>(v);
+      }
+    }
+  } else {
+    // 32 columns a workgroup, eight lanes to a column
+    __shared__ float sum[8][32];
+    const uint32_t i = (uint32_t)(blockIdx.x - s.dw_groups) * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5;
     float v = 0.0f;
-    for (uint32_t p = 0; p < parts; ++p) v += part[(size_t)p * count + i];
-    out[i] = from_float<O>(v);
+    if (i < s.n)
+      for (uint32_t p = seg; p < s.db_parts; p += 8) v += s.db[(size_t)p * s.n + i];
+    sum[seg][threadIdx.x & 31] = v;
+    __syncthreads();
+    if (seg == 0 && i < s.n) {
+#pragma unroll
+      for (int k = 1; k < 8; ++k) v += sum[k][threadIdx.x];
+      db[i] = from_float<O>(v);
+    }
   }
 }
 
 // ---------------------------------------------------------------- launches
-constexpr size_t kMaxGradSide = (size_t)1 << 20;  // features on either side
+constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
+constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 16 rows are 32 bits
+
+constexpr size_t kSpareBytes = 1024 + 32;           // 256 columns of fp32, and 16 bytes from the last of them on
 
 struct GradPlan {
   bool large;  // 256 x 256 tiles, else 128 x 128
@@ -298,7 +414,7 @@ static GradPlan grad_plan(size_t rows, size_t n, size_t k)
   return p;
 }
 
-static size_t bias_parts(const GradPlan& p) { return (size_t)p.splits * p.tiles_k * 2; }
+static size_t bias_parts(const GradPlan& p) { return (size_t)p.splits * p.tiles_k; }
 
 }  // namespace q8
 }  // namespace cswap
@@ -312,7 +428,7 @@ extern "C" size_t cswap_q8_weight_grad_workspace_bytes(size_t rows, size_t n, si
 {
   if (!grad_sizes(rows, n, k)) return 0;
   const GradPlan p = grad_plan(rows, n, k);
-  return ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float);
+  return ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float) + kSpareBytes;
 }
 
 extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride, const int8_t* d_codes,
@@ -323,7 +439,7 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   if (int e = check_rows(rows, n, &dy_stride)) return e;
   if (int e = check_rows(rows, k, &unused)) return e;
   if (!dtype_known(dtype) || !dtype_known(out_dtype)) return CSWAP_E_ARG;
-  if (!grad_sizes(rows, n, k)) return CSWAP_E_UNSUPPORTED;
+  if (!grad_sizes(rows, n, k) || (size_t)dy_stride > kMaxGradStride) return CSWAP_E_UNSUPPORTED;
   if (!value_ptr(d_dw, out_dtype) || (d_db && !value_ptr(d_db, out_dtype))) return CSWAP_E_ARG;
   if (rows && (!value_ptr(d_dy, dtype) || !checkpoint_ptrs(d_codes, d_scales))) return CSWAP_E_ARG;
   if (!value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
@@ -339,22 +455,18 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
     constexpr int BK = T::bytes == 4 ? 32 : 64;
     auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK> : weight_grad_kernel<T, 128, 128, BK>;
     hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(256), 0, st,
-                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, part, d_db ? part_b : nullptr);
+                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, part, d_db ? part_b : nullptr,
+                       reinterpret_cast<const char*>(part_b + bias_parts(p) * n));
     return check_launch();
   };
   if (int e = dtype == CSWAP_DT_F32 ? launch(F32()) : dtype == CSWAP_DT_BF16 ? launch(BF16()) : launch(F16())) return e;
-  const auto reduce = [&](auto t, const float* from, size_t parts, size_t count, void* out) {
+  const size_t dw_groups = (n * k + 1023) / 1024;
+  const GradSums sums = {part, part_b, n * k, dw_groups, p.splits, (uint32_t)bias_parts(p), (uint32_t)n};
+  const auto reduce = [&](auto t) {
     typedef decltype(t) O;
-    const size_t want = (count + 255) / 256;
-    hipLaunchKernelGGL(weight_grad_reduce_kernel<O>, dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, from,
-                       (uint32_t)parts, count, static_cast<typename O::value*>(out));
+    hipLaunchKernelGGL(weight_grad_reduce_kernel<O>, dim3((unsigned)(dw_groups + (d_db ? (n + 31) / 32 : 0))), dim3(256), 0, st, sums,
+                       static_cast<typename O::value*>(d_dw), static_cast<typename O::value*>(d_db));
     return check_launch();
   };
-  const auto reduce_to = [&](const float* from, size_t parts, size_t count, void* out) {
-    return out_dtype == CSWAP_DT_F32    ? reduce(F32(), from, parts, count, out)
-           : out_dtype == CSWAP_DT_BF16 ? reduce(BF16(), from, parts, count, out)
-                                        : reduce(F16(), from, parts, count, out);
-  };
-  if (int e = reduce_to(part, p.splits, n * k, d_dw)) return e;
-  return d_db ? reduce_to(part_b, bias_parts(p), n, d_db) : CSWAP_OK;
+  return out_dtype == CSWAP_DT_F32 ? reduce(F32()) : out_dtype == CSWAP_DT_BF16 ? reduce(BF16()) : reduce(F16());
 }
