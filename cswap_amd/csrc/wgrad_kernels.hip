@@ -79,7 +79,7 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
   return make_uint4(x.x, x.y, y.x, y.y);
 }
 
-// A workgroup of four wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.
+// A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.
 //
 // The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m: the
 // transposing reads take four rows at once, which have to lie in different banks.  a_at and b_at are the places of value
@@ -97,8 +97,19 @@ template <typename T, int TN, int TK, int BK> struct GradTile {
   }
 };
 
-template <typename T, int TN, int TK, int BK>
-__global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::value* __restrict__ dy,
+// The same address in all lanes, for the compiler: loads then take it from scalar registers and 32-bit offsets from the lanes.
+typedef const __attribute__((address_space(1))) char* global_bytes;
+typedef const __attribute__((address_space(1))) u4_any* global_u4;
+typedef const __attribute__((address_space(1))) uint8_t* global_u1;
+__device__ inline global_bytes uniform(const char* p)
+{
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (global_bytes)((uint64_t)hi << 32 | lo);
+}
+
+template <typename T, int TN, int TK, int BK, int WK>
+__global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
                                                              const int8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, GradShape s,
                                                              float* __restrict__ dw, float* __restrict__ db,
@@ -108,10 +119,10 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
   typedef typename Feed<T>::type M;
   typedef typename T::value V;
   constexpr int P = Feed<T>::parts, W = T::bytes / 2;               // 16-byte words of a chunk of dY
-  constexpr int FN = TN / 64, FK = TK / 64;                       // 32 x 32 pieces of a wavefront's quarter
+  constexpr int NT = 128 * WK, FN = TN / 64, FK = TK / (32 * WK);  // threads; 32 x 32 pieces of a wavefront's part
   constexpr int kSteps = BK / 16;                                   // matrix instructions' depth
-  constexpr int kAChunks = TN / 8, kARows = 256 / kAChunks, kALoads = BK / kARows;
-  constexpr int kBPieces = TK / 16, kBRows = 256 / kBPieces, kBLoads = BK / kBRows;
+  constexpr int kAChunks = TN / 8, kARows = NT / kAChunks, kALoads = BK / kARows;
+  constexpr int kBPieces = TK / 16, kBRows = NT / kBPieces, kBLoads = BK / kBRows;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][Tile::kStage];
 
   const uint32_t tile = blockIdx.x;
@@ -148,13 +159,13 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
   u4_any a_raw[kALoads][W], b_raw[kBLoads];
   uint32_t b_scale[kBLoads];
   auto load_a = [&](uint32_t st, int i) {
-    const char* base = dy_from + (size_t)(st * BK + i * kARows) * dy_stride * sizeof(V);
+    const global_bytes base = uniform(dy_from + (size_t)(st * BK + i * kARows) * dy_stride * sizeof(V));
 #pragma unroll
-    for (int h = 0; h < W; ++h) a_raw[i][h] = *reinterpret_cast<const u4_any*>(base + a_off + 16 * h);
+    for (int h = 0; h < W; ++h) a_raw[i][h] = *(global_u4)(base + a_off + 16 * h);
   };
   auto load_b = [&](uint32_t st, int i) {
-    b_raw[i] = *reinterpret_cast<const u4_any*>(codes_from + (size_t)(st * BK + i * kBRows) * code_pitch + b_off);
-    b_scale[i] = *reinterpret_cast<const uint8_t*>(scales_from + (size_t)(st * BK + i * kBRows) * scale_pitch + c_off);
+    b_raw[i] = *(global_u4)(uniform(codes_from + (size_t)(st * BK + i * kBRows) * code_pitch) + b_off);
+    b_scale[i] = *(global_u1)(uniform(scales_from + (size_t)(st * BK + i * kBRows) * scale_pitch) + c_off);
   };
   auto store_a = [&](uint16_t* buf, int i) {
     uint16_t* at = buf + Tile::a_at(a_row + i * kARows, 8 * a_chunk);
@@ -194,7 +205,7 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
 
   auto stage_by_value = [&](uint16_t* buf, uint32_t m0, bool mine) {
     const int c = tid % TN;
-    for (int m = tid / TN; m < BK; m += 256 / TN) {
+    for (int m = tid / TN; m < BK; m += NT / TN) {
       const bool here = m0 + m < to && n0 + c < s.n;
       const V raw = here ? dy[(size_t)(m0 + m) * s.dy_stride + n0 + c] : (V)0;
       if (mine) b_edge += to_float<T>(raw);
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
       }
     }
     const int k = tid % TK;
-    for (int m = tid / TK; m < BK; m += 256 / TK) {
+    for (int m = tid / TK; m < BK; m += NT / TK) {
       float v = 0.0f;
       if (m0 + m < to && k0 + k < s.k)
         v = (float)codes[(size_t)(m0 + m) * s.code_pitch + k0 + k] *
@@ -223,9 +234,9 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
   const int m_lane = 8 * (lane >> 5) + ((lane & 15) >> 2), c_lane = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   int a_at[FN], b_at[FK];
 #pragma unroll
-  for (int i = 0; i < FN; ++i) a_at[i] = Tile::a_at(m_lane, ((wave >> 1) * FN + i) * 32 + c_lane);
+  for (int i = 0; i < FN; ++i) a_at[i] = Tile::a_at(m_lane, ((wave / WK) * FN + i) * 32 + c_lane);
 #pragma unroll
-  for (int j = 0; j < FK; ++j) b_at[j] = Tile::b_at(m_lane, ((wave & 1) * FK + j) * 32 + c_lane);
+  for (int j = 0; j < FK; ++j) b_at[j] = Tile::b_at(m_lane, ((wave % WK) * FK + j) * 32 + c_lane);
 
   f16v acc[FN][FK] = {};
   uint4 a[2][FN], b[2][FK];
@@ -311,17 +322,17 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const uint32_t n = n0 + ((wave >> 1) * FN + i) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+      const uint32_t n = n0 + ((wave / WK) * FN + i) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
       if (n >= s.n) continue;
 #pragma unroll
       for (int j = 0; j < FK; ++j) {
-        const uint32_t k = k0 + ((wave & 1) * FK + j) * 32 + (lane & 31);
+        const uint32_t k = k0 + ((wave % WK) * FK + j) * 32 + (lane & 31);
         if (k < s.k) out[(size_t)n * s.k + k] = acc[i][j][r];
       }
     }
   if (db) {
-    float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows + 256 / TN][TN]
-    static_assert(sizeof(lds) >= sizeof(float) * (kARows + 256 / TN) * TN, "room for the columns' sums");
+    float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows + NT / TN][TN]
+    static_assert(sizeof(lds) >= sizeof(float) * (kARows + NT / TN) * TN, "room for the columns' sums");
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[a_row * TN + 8 * a_chunk + e] = b_sum[e];
@@ -329,7 +340,7 @@ __global__ __launch_bounds__(256, 1) void weight_grad_kernel(const typename T::v
     __syncthreads();
     if (tid < TN && n0 + tid < s.n) {
       float v = 0.0f;
-      for (int r = 0; r < kARows + 256 / TN; ++r) v += sums[r * TN + tid];
+      for (int r = 0; r < kARows + NT / TN; ++r) v += sums[r * TN + tid];
       db[(size_t)(split * s.tiles_k + tk) * s.n + n0 + tid] = v;
     }
   }
@@ -453,8 +464,8 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   const auto launch = [&](auto t) {
     typedef decltype(t) T;
     constexpr int BK = T::bytes == 4 ? 32 : 64;
-    auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK> : weight_grad_kernel<T, 128, 128, BK>;
-    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(256), 0, st,
+    auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, 2>;
+    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 256), 0, st,
                        static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, part, d_db ? part_b : nullptr,
                        reinterpret_cast<const char*>(part_b + bias_parts(p) * n));
     return check_launch();
