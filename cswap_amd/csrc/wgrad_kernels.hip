@@ -97,6 +97,22 @@ template <typename T, int TN, int TK, int BK> struct GradTile {
   }
 };
 
+// Which tile and split a workgroup has.  Workgroups go to the eight XCDs in turn, each of which has a cache of its own: an XCD gets
+// neighbouring tiles of one split, up to 16 along k (whose operand is the smaller one) before the next row of tiles.
+struct Place {
+  uint32_t tn, tk, split;
+};
+__device__ inline Place place_of(uint32_t id, uint32_t count, const GradShape& s)
+{
+  const uint32_t each = count / 8, more = count % 8, xcd = id % 8;
+  uint32_t at = xcd * each + min(xcd, more) + id / 8;
+  const uint32_t tiles = s.tiles_n * s.tiles_k, split = at / tiles;
+  at -= split * tiles;
+  const uint32_t column = at / (16 * s.tiles_n), width = min(16u, s.tiles_k - 16 * column);
+  at -= column * 16 * s.tiles_n;
+  return {at / width, 16 * column + at % width, split};
+}
+
 // The same address in all lanes, for the compiler: loads then take it from scalar registers and 32-bit offsets from the lanes.
 typedef const __attribute__((address_space(1))) char* global_bytes;
 typedef const __attribute__((address_space(1))) u4_any* global_u4;
@@ -112,7 +128,7 @@ template <typename T, int TN, int TK, int BK, int WK>
 __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
                                                              const int8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, GradShape s,
-                                                             float* __restrict__ dw, float* __restrict__ db,
+                                                             void* __restrict__ dw, void* __restrict__ db, int out_dtype,
                                                              const char* __restrict__ spare)
 {
   typedef GradTile<T, TN, TK, BK> Tile;
@@ -125,8 +141,8 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
   constexpr int kBPieces = TK / 16, kBRows = NT / kBPieces, kBLoads = BK / kBRows;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][Tile::kStage];
 
-  const uint32_t tile = blockIdx.x;
-  const uint32_t tk = tile % s.tiles_k, rest = tile / s.tiles_k, tn = rest % s.tiles_n, split = rest / s.tiles_n;
+  const Place at = place_of(blockIdx.x, gridDim.x, s);
+  const uint32_t tk = at.tk, tn = at.tn, split = at.split;
   const uint32_t n0 = tn * TN, k0 = tk * TK;
   const uint32_t from = split * s.step_rows, to = min(s.rows, from + s.step_rows);
   const uint32_t stages = (to - from + BK - 1) / BK;
@@ -145,7 +161,7 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
     --plain;
   }
   // The loop asks for a plain stage in every turn, the last one again where there is no other; without any it reads the spare
-  // room behind the workspace's sums, and what it reads is not used.
+  // room at the workspace's start, and what it reads is not used.
   const size_t dy_stride = plain ? s.dy_stride : 0, code_pitch = plain ? s.code_pitch : 0, scale_pitch = plain ? s.scale_pitch : 0;
   const char* const dy_from = plain ? reinterpret_cast<const char*>(dy + (size_t)from * s.dy_stride + n0) : spare;
   const char* const codes_from = plain ? reinterpret_cast<const char*>(codes) + (size_t)from * s.code_pitch + k0 : spare;
@@ -239,6 +255,7 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
   for (int j = 0; j < FK; ++j) b_at[j] = Tile::b_at(m_lane, ((wave % WK) * FK + j) * 32 + c_lane);
 
   f16v acc[FN][FK] = {};
+  static_assert(kSteps % 2 == 0, "a stage begins with the first of either pair of fragments");
   uint4 a[2][FN], b[2][FK];
   auto read_a = [&](const uint16_t* buf, int c, int p, uint4* to_a) {
 #pragma unroll
@@ -249,50 +266,14 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
     for (int j = 0; j < FK; ++j) to_b[j] = read_turned(buf + b_at[j] + c * 16 * TK, 4 * TK);
   };
 
-  // One stage's products.  Meanwhile the next one goes from registers to LDS and the one after that is asked for; the fragments of
-  // a step are read while the step before multiplies.
-  auto compute = [&](const uint16_t* buf, uint16_t* next, uint32_t after) {
-    read_b(buf, 0, b[0]);
-    read_a(buf, 0, P - 1, a[0]);
-#pragma unroll
-    for (int c = 0; c < kSteps; ++c) {
-#pragma unroll
-      for (int q = 0; q < P; ++q) {
-        constexpr int kParts = kSteps * P;
-        const int part = c * P + q, at = part & 1;
-        if (q + 1 < P) {
-          read_a(buf, c, P - 2 - q, a[at ^ 1]);
-        } else if (c + 1 < kSteps) {
-          read_b(buf, c + 1, b[(c + 1) & 1]);
-          read_a(buf, c + 1, P - 1, a[at ^ 1]);
-        }
-#pragma unroll
-        for (int i = 0; i < kALoads; ++i)
-          if (i * kParts / kALoads == part) {
-            store_a(next, i);
-            load_a(after, i);
-          }
-#pragma unroll
-        for (int i = 0; i < kBLoads; ++i)
-          if (i * kParts / kBLoads == part) {
-            store_b(next, i);
-            load_b(after, i);
-          }
-#pragma unroll
-        for (int i = 0; i < FN; ++i)
-#pragma unroll
-          for (int j = 0; j < FK; ++j) acc[i][j] = mma(M(), a[at][i], b[c & 1][j], acc[i][j]);
-      }
-    }
-  };
-
   auto load = [&](uint32_t st) {
 #pragma unroll
     for (int i = 0; i < kALoads; ++i) load_a(st, i);
 #pragma unroll
     for (int i = 0; i < kBLoads; ++i) load_b(st, i);
   };
-  auto my_turn = [&](uint32_t st) { return db && st % s.tiles_k == tk; };
+  // out_dtype: the results themselves leave; else (-1) what this split has of them
+  auto my_turn = [&](uint32_t st) { return db && (out_dtype < 0 ? st % s.tiles_k == tk : tk == 0); };
   const uint32_t last = plain ? plain - 1 : 0;
 
   if (plain) {
@@ -306,31 +287,79 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
     stage_by_value(lds[0], from, my_turn(0));
   }
   load(min(1u, last));
+  __syncthreads();
+  read_b(lds[0], 0, b[0]);
+  read_a(lds[0], 0, P - 1, a[0]);
+  // One stage's products a turn.  Meanwhile the next stage goes from registers to LDS and the one after that is asked for; the
+  // fragments of a step are read while the step before multiplies, those of a stage's first step, behind the barrier, beside
+  // the last products of the stage before.
   for (uint32_t st = 0; st < stages; ++st) {
-    __syncthreads();
-    if (st + 1 < plain && my_turn(st + 1)) add_columns();
+    const uint16_t* buf = lds[st & 1];
     uint16_t* next = lds[(st + 1) & 1];
-    compute(lds[st & 1], next, min(st + 2, last));
-    if (st + 1 < stages && st + 1 >= plain) {
-      __syncthreads();  // the turn has left something there
-      stage_by_value(next, from + (st + 1) * BK, my_turn(st + 1));
+    const uint32_t after = min(st + 2, last);
+    if (st + 1 < plain && my_turn(st + 1)) add_columns();
+    constexpr int kParts = kSteps * P;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const int c = part / P, q = part % P, at = part & 1;
+#pragma unroll
+      for (int i = 0; i < kALoads; ++i)
+        if (i * kParts / kALoads == part) {
+          store_a(next, i);
+          load_a(after, i);
+        }
+#pragma unroll
+      for (int i = 0; i < kBLoads; ++i)
+        if (i * kParts / kBLoads == part) {
+          store_b(next, i);
+          load_b(after, i);
+        }
+      if (q + 1 < P) {
+        read_a(buf, c, P - 2 - q, a[at ^ 1]);
+      } else if (c + 1 < kSteps) {
+        read_b(buf, c + 1, b[(c + 1) & 1]);
+        read_a(buf, c + 1, P - 1, a[at ^ 1]);
+      } else {
+        if (st + 1 < stages && st + 1 >= plain) {
+          __syncthreads();  // the turn has left something there
+          stage_by_value(next, from + (st + 1) * BK, my_turn(st + 1));
+        }
+        __syncthreads();
+        read_b(next, 0, b[0]);
+        read_a(next, 0, P - 1, a[0]);
+      }
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FK; ++j) acc[i][j] = mma(M(), a[at][i], b[c & 1][j], acc[i][j]);
     }
   }
 
-  float* out = dw + (size_t)split * s.n * s.k;
+  auto leave = [&](auto t, void* to) {
+    typedef decltype(t) O;
+    typename O::value* out = static_cast<typename O::value*>(to);
 #pragma unroll
-  for (int i = 0; i < FN; ++i)
+    for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const uint32_t n = n0 + ((wave / WK) * FN + i) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-      if (n >= s.n) continue;
+      for (int r = 0; r < 16; ++r) {
+        const uint32_t n = n0 + ((wave / WK) * FN + i) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+        if (n >= s.n) continue;
 #pragma unroll
-      for (int j = 0; j < FK; ++j) {
-        const uint32_t k = k0 + ((wave % WK) * FK + j) * 32 + (lane & 31);
-        if (k < s.k) out[(size_t)n * s.k + k] = acc[i][j][r];
+        for (int j = 0; j < FK; ++j) {
+          const uint32_t k = k0 + ((wave % WK) * FK + j) * 32 + (lane & 31);
+          if (k < s.k) out[(size_t)n * s.k + k] = from_float<O>(acc[i][j][r]);
+        }
       }
-    }
-  if (db) {
+  };
+  if (out_dtype < 0)
+    leave(F32(), static_cast<float*>(dw) + (size_t)split * s.n * s.k);
+  else if (out_dtype == CSWAP_DT_F32)
+    leave(F32(), dw);
+  else if (out_dtype == CSWAP_DT_BF16)
+    leave(BF16(), dw);
+  else
+    leave(F16(), dw);
+  if (db && (out_dtype < 0 || tk == 0)) {
     float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows + NT / TN][TN]
     static_assert(sizeof(lds) >= sizeof(float) * (kARows + NT / TN) * TN, "room for the columns' sums");
     __syncthreads();
@@ -341,7 +370,15 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
     if (tid < TN && n0 + tid < s.n) {
       float v = 0.0f;
       for (int r = 0; r < kARows + NT / TN; ++r) v += sums[r * TN + tid];
-      db[(size_t)(split * s.tiles_k + tk) * s.n + n0 + tid] = v;
+      const uint32_t n = n0 + tid;
+      if (out_dtype < 0)
+        static_cast<float*>(db)[(size_t)(split * s.tiles_k + tk) * s.n + n] = v;
+      else if (out_dtype == CSWAP_DT_F32)
+        static_cast<float*>(db)[n] = v;
+      else if (out_dtype == CSWAP_DT_BF16)
+        static_cast<uint16_t*>(db)[n] = from_float<BF16>(v);
+      else
+        static_cast<uint16_t*>(db)[n] = from_float<F16>(v);
     }
   }
 }
@@ -399,7 +436,7 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
 constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
 constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 16 rows are 32 bits
 
-constexpr size_t kSpareBytes = 1024 + 32;           // 256 columns of fp32, and 16 bytes from the last of them on
+constexpr size_t kSpareBytes = 1024 + 64;           // 256 columns of fp32, and 16 bytes from the last of them on
 
 struct GradPlan {
   bool large;  // 256 x 256 tiles, else 128 x 128
@@ -439,7 +476,7 @@ extern "C" size_t cswap_q8_weight_grad_workspace_bytes(size_t rows, size_t n, si
 {
   if (!grad_sizes(rows, n, k)) return 0;
   const GradPlan p = grad_plan(rows, n, k);
-  return ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float) + kSpareBytes;
+  return kSpareBytes + (p.splits == 1 ? 0 : ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float));
 }
 
 extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride, const int8_t* d_codes,
@@ -458,7 +495,8 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   const GradPlan p = grad_plan(rows, n, k);
   const GradShape s = {(uint32_t)rows, (uint32_t)n, (uint32_t)k, (uint32_t)groups_of(k), p.step_rows, p.tiles_n, p.tiles_k,
                        (size_t)dy_stride, pitch_of(k)};
-  float* part = static_cast<float*>(d_ws);
+  const bool direct = p.splits == 1;
+  float* part = reinterpret_cast<float*>(static_cast<char*>(d_ws) + kSpareBytes);
   float* part_b = part + (size_t)p.splits * n * k;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
@@ -466,11 +504,12 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
     constexpr int BK = T::bytes == 4 ? 32 : 64;
     auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, 2>;
     hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 256), 0, st,
-                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, part, d_db ? part_b : nullptr,
-                       reinterpret_cast<const char*>(part_b + bias_parts(p) * n));
+                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part, !d_db ? nullptr : direct ? d_db : part_b,
+                       direct ? out_dtype : -1, static_cast<const char*>(d_ws));
     return check_launch();
   };
   if (int e = dtype == CSWAP_DT_F32 ? launch(F32()) : dtype == CSWAP_DT_BF16 ? launch(BF16()) : launch(F16())) return e;
+  if (direct) return CSWAP_OK;
   const size_t dw_groups = (n * k + 1023) / 1024;
   const GradSums sums = {part, part_b, n * k, dw_groups, p.splits, (uint32_t)bias_parts(p), (uint32_t)n};
   const auto reduce = [&](auto t) {
