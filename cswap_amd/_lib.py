@@ -129,7 +129,7 @@ _SIGNATURES = {
     "cswap_layer_norm_forward": (i32, [vp, i32, sz, sz, pd, vp, vp, i32, C.c_float, vp, pd, vp, vp, vp, vp, vp]),
     "cswap_layer_norm_workspace_bytes": (sz, [sz, sz]),
     "cswap_layer_norm_backward": (i32, [vp, i32, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
-    "cswap_q8_weight_grad_workspace_bytes": (sz, [sz, sz, sz]),
+    "cswap_q8_weight_grad_workspace_bytes": (sz, [i32, sz, sz, sz]),
     "cswap_q8_weight_grad": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, vp, vp, i32, vp, sz, vp]),
     "cswap_probe_nnz": (i32, [vp, sz, vp, vp]),
     "cswap_costs_default": (None, [C.POINTER(Costs)]),

@@ -219,30 +219,42 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
                                   : to_float<T>((V)(uint16_t)(a_raw[i][0][e / 2] >> (16 * (e & 1))));
   };
 
+  // Loads are at clamped places, so that several of them are in flight without a branch; what is not there becomes 0.
+  constexpr int kAhead = P == 3 ? 4 : 8;
   auto stage_by_value = [&](uint16_t* buf, uint32_t m0, bool mine) {
-    const int c = tid % TN;
-    for (int m = tid / TN; m < BK; m += NT / TN) {
-      const bool here = m0 + m < to && n0 + c < s.n;
-      const V raw = here ? dy[(size_t)(m0 + m) * s.dy_stride + n0 + c] : (V)0;
-      if (mine) b_edge += to_float<T>(raw);
-      if constexpr (P == 3) {
-        const uint32_t a0 = __float_as_uint(raw) & 0xffff0000u;
-        const float r = raw - __uint_as_float(a0);
-        const uint32_t a1 = __float_as_uint(r) & 0xffff0000u;
+    const uint32_t m_last = to - 1 - m0;
+    {
+      const int c = tid % TN;
+      const bool there = n0 + c < s.n;
+      const V* p = dy + (size_t)m0 * s.dy_stride + (there ? n0 + c : s.n - 1);
+#pragma unroll kAhead
+      for (int j = 0; j < BK * TN / NT; ++j) {
+        const uint32_t m = tid / TN + j * (NT / TN);
+        V raw = p[(size_t)min(m, m_last) * s.dy_stride];
+        if (!there || m > m_last) raw = 0;
+        if (mine) b_edge += to_float<T>(raw);
         uint16_t* at = buf + Tile::a_at(m, c);
-        at[0] = (uint16_t)(a0 >> 16), at[Tile::kAPlane] = (uint16_t)(a1 >> 16);
-        at[2 * Tile::kAPlane] = (uint16_t)(__float_as_uint(r - __uint_as_float(a1)) >> 16);
-      } else {
-        buf[Tile::a_at(m, c)] = raw;
+        if constexpr (P == 3) {
+          const uint32_t a0 = __float_as_uint(raw) & 0xffff0000u;
+          const float r = raw - __uint_as_float(a0);
+          const uint32_t a1 = __float_as_uint(r) & 0xffff0000u;
+          at[0] = (uint16_t)(a0 >> 16), at[Tile::kAPlane] = (uint16_t)(a1 >> 16);
+          at[2 * Tile::kAPlane] = (uint16_t)(__float_as_uint(r - __uint_as_float(a1)) >> 16);
+        } else {
+          at[0] = raw;
+        }
       }
     }
-    const int k = tid % TK;
-    for (int m = tid / TK; m < BK; m += NT / TK) {
-      float v = 0.0f;
-      if (m0 + m < to && k0 + k < s.k)
-        v = (float)codes[(size_t)(m0 + m) * s.code_pitch + k0 + k] *
-            unit_of(scales[(size_t)(m0 + m) * s.scale_pitch + (k0 + k) / kGroup]);
-      buf[Tile::b_at(m, k)] = from_float<M>(v);
+    const int c = tid % TK;
+    const bool there = k0 + c < s.k;
+    const uint32_t k = there ? k0 + c : s.k - 1;
+    const int8_t* p = codes + (size_t)m0 * s.code_pitch + k;
+    const uint8_t* q = scales + (size_t)m0 * s.scale_pitch + k / kGroup;
+#pragma unroll kAhead
+    for (int j = 0; j < BK * TK / NT; ++j) {
+      const uint32_t m = tid / TK + j * (NT / TK), mc = min(m, m_last);
+      const float v = (float)p[(size_t)mc * s.code_pitch] * unit_of(q[(size_t)mc * s.scale_pitch]);
+      buf[Tile::b_at(m, c)] = from_float<M>(there && m <= m_last ? v : 0.0f);
     }
   };
 
@@ -444,22 +456,40 @@ struct GradPlan {
   uint32_t step_rows;
 };
 
-static GradPlan grad_plan(size_t rows, size_t n, size_t k)
+// Tiles and splits with the least estimated time.  Measured on 256 compute units, in us: a workgroup takes `stage` for 64 rows, a
+// compute unit with two workgroups of the small tiles `pair` for 64 rows of both; `fixed` is the rest of a launch; splits cost
+// the sums' launch (5) and their bytes there and back at 5.5 TB/s.  What it decides between, bf16, us of 128 x 128 tiles / 256 x 256:
+// 512 x 2048 x 2048 15.0 / 32.8, 8192 x 768 x 768 30 / 36, 8192 x 2048 x 2048 102 / 86, 32768 x 4096 x 1024 371 / 294, 2048 x 4096 x
+// 4096 92 / 76; and with 256 / 512 workgroups of the small tiles: 2048 x 2048 x 2048 (not split / in two) 36.6 / 40.9, 32768 x 768 x 768
+// 77 / 66.
+static double grad_estimate(bool large, bool f32, size_t tiles, size_t splits, size_t step, size_t n, size_t k)
 {
-  GradPlan p;
-  p.large = (rows + 2047) / 2048 * ((n + 255) / 256) * ((k + 255) / 256) >= 256;
-  const size_t side = p.large ? 256 : 128, resident = p.large ? 256 : 512;
-  p.tiles_n = (unsigned)((n + side - 1) / side), p.tiles_k = (unsigned)((k + side - 1) / side);
-  const size_t tiles = (size_t)p.tiles_n * p.tiles_k;
-  size_t splits = tiles >= resident ? 1 : resident / tiles;
-  const size_t most = (rows + 255) / 256;  // at least 256 rows to a split
-  if (splits > most) splits = most < 1 ? 1 : most;
-  size_t step = (rows + splits - 1) / splits;
-  step = (step + 63) / 64 * 64;
-  if (step == 0) step = 64;
-  p.step_rows = (uint32_t)step;
-  p.splits = (unsigned)(rows ? (rows + step - 1) / step : 1);
-  return p;
+  const double units = (double)step / 64, stage = large ? (f32 ? 4.4 : 1.65) : (f32 ? 1.9 : 0.9), pair = f32 ? 3.2 : 1.2;
+  const size_t groups = tiles * splits, at_once = large ? 256 : 512, rest = groups % at_once;
+  double t = (large ? 11.0 : 8.0) + (double)(groups / at_once) * units * (large ? stage : pair);
+  if (rest) t += units * (!large && rest > 256 ? pair : stage);
+  if (splits > 1) t += 5.0 + (double)(splits * n * k) * 8.0 / 5.5e6;
+  return t;
+}
+
+static GradPlan grad_plan(int dtype, size_t rows, size_t n, size_t k)
+{
+  GradPlan best = {};
+  double least = 0.0;
+  for (int large = 0; large < 2; ++large) {
+    const size_t side = large ? 256 : 128, tiles_n = (n + side - 1) / side, tiles_k = (k + side - 1) / side;
+    const size_t tiles = tiles_n * tiles_k;
+    for (size_t want = 1; want <= 64 && (want == 1 || (want * tiles <= 1024 && want * 64 <= rows)); ++want) {
+      const size_t step = rows ? ((rows + want - 1) / want + 63) / 64 * 64 : 64, splits = rows ? (rows + step - 1) / step : 1;
+      if (splits != want) continue;  // a smaller number has the same steps
+      const double t = grad_estimate(large, dtype == CSWAP_DT_F32, tiles, splits, step, n, k);
+      if (best.splits == 0 || t < least) {
+        least = t;
+        best = {large != 0, (unsigned)tiles_n, (unsigned)tiles_k, (unsigned)splits, (uint32_t)step};
+      }
+    }
+  }
+  return best;
 }
 
 static size_t bias_parts(const GradPlan& p) { return (size_t)p.splits * p.tiles_k; }
@@ -472,10 +502,10 @@ using namespace cswap::q8;
 
 static bool grad_sizes(size_t rows, size_t n, size_t k) { return n && k && n <= kMaxGradSide && k <= kMaxGradSide && rows < ((size_t)1 << 31); }
 
-extern "C" size_t cswap_q8_weight_grad_workspace_bytes(size_t rows, size_t n, size_t k)
+extern "C" size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k)
 {
-  if (!grad_sizes(rows, n, k)) return 0;
-  const GradPlan p = grad_plan(rows, n, k);
+  if (!dtype_known(dtype) || !grad_sizes(rows, n, k)) return 0;
+  const GradPlan p = grad_plan(dtype, rows, n, k);
   return kSpareBytes + (p.splits == 1 ? 0 : ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float));
 }
 
@@ -491,8 +521,8 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   if (!value_ptr(d_dw, out_dtype) || (d_db && !value_ptr(d_db, out_dtype))) return CSWAP_E_ARG;
   if (rows && (!value_ptr(d_dy, dtype) || !checkpoint_ptrs(d_codes, d_scales))) return CSWAP_E_ARG;
   if (!value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
-  if (ws_bytes < cswap_q8_weight_grad_workspace_bytes(rows, n, k)) return CSWAP_E_NOMEM;
-  const GradPlan p = grad_plan(rows, n, k);
+  if (ws_bytes < cswap_q8_weight_grad_workspace_bytes(dtype, rows, n, k)) return CSWAP_E_NOMEM;
+  const GradPlan p = grad_plan(dtype, rows, n, k);
   const GradShape s = {(uint32_t)rows, (uint32_t)n, (uint32_t)k, (uint32_t)groups_of(k), p.step_rows, p.tiles_n, p.tiles_k,
                        (size_t)dy_stride, pitch_of(k)};
   const bool direct = p.splits == 1;

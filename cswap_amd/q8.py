@@ -296,7 +296,7 @@ def q8_weight_grad(dy: torch.Tensor, held: Checkpoint8, bias: bool = True, out_d
         raise TypeError(f"q8_weight_grad: out_dtype {out_dtype}")
     dw = torch.empty((n, k), dtype=out_dtype, device=dy.device)
     db = torch.empty(n, dtype=out_dtype, device=dy.device) if bias else None
-    room = lib().cswap_q8_weight_grad_workspace_bytes(rows, n, k)
+    room = lib().cswap_q8_weight_grad_workspace_bytes(kind, rows, n, k)
     ws = torch.empty(room, dtype=torch.uint8, device=dy.device)
     with _on(dy.device):
         check(lib().cswap_q8_weight_grad(dy.data_ptr(), kind, rows, n, stride, held.codes.data_ptr(), held.scales.data_ptr(),

@@ -314,7 +314,7 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
  * the checkpoint was made from fp16.  rows = 0 gives zeros.  n and k up to 2^20.  d_ws:
  * cswap_q8_weight_grad_workspace_bytes, 16-byte aligned, with no preparation; calls that overlap
  * must not share one. */
-size_t cswap_q8_weight_grad_workspace_bytes(size_t rows, size_t n, size_t k);
+size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k);
 int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride,
                          const int8_t* d_codes, const uint8_t* d_scales, size_t k,
                          void* d_dw, void* d_db, int out_dtype, void* d_ws, size_t ws_bytes,

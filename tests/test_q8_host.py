@@ -19,7 +19,7 @@ def test_sizes():
     assert L().cswap_layer_norm_workspace_bytes(0, 100) == 0
     assert L().cswap_layer_norm_workspace_bytes(10, 16385) == 0
     assert L().cswap_layer_norm_workspace_bytes(1, 100) >= 2 * 4 * 100
-    assert L().cswap_q8_weight_grad_workspace_bytes(10, 0, 5) == 0
+    assert L().cswap_q8_weight_grad_workspace_bytes(1, 10, 0, 5) == 0
 
 
 def test_codec_refuses():
@@ -88,7 +88,7 @@ def test_layer_norm_refuses():
 
 
 def test_weight_grad_refuses():
-    room = L().cswap_q8_weight_grad_workspace_bytes(64, 48, 40)
+    room = L().cswap_q8_weight_grad_workspace_bytes(1, 64, 48, 40)
     good = [A, 1, 64, 48, 0, A, A, 40, A, A, 1, A, room, None]
 
     def f(**kw):
