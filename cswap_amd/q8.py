@@ -17,28 +17,25 @@ as layers with gradients, ``cswap_amd.hooks.hold_saved_tensors`` for whatever a 
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
 
+from . import api
 from ._lib import check, lib
-from .api import _stream
 
 GROUP = 32
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_NO_GUARD = contextlib.nullcontext()
 
 
 class Checkpoint8:
     """An activation in 8 bits: ``codes`` (int8, rows x pitch) and ``scales`` (uint8, rows x groups), and the
     ``shape`` and ``dtype`` of what it was made from.  ``rows`` is the product of the leading dimensions and
     ``cols`` the last one, or 1 and all of it if it was made with ``flat=True``."""
-    __slots__ = ("codes", "scales", "shape", "dtype", "rows", "cols")
+    __slots__ = ("shape", "dtype", "device", "rows", "cols", "_codes", "_scales", "_room", "_at", "_scales_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype):
-        shape = tuple(shape)
         rows, cols = _rows_cols(shape)
         if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.int8 or scales.dtype != torch.uint8:
             raise ValueError("expected codes as a 2-D int8 tensor and scales as a 2-D uint8 tensor")
@@ -46,37 +43,69 @@ class Checkpoint8:
             rows, cols = 1, rows * cols
         groups = -(-cols // GROUP)
         if codes.shape != (rows, groups * GROUP) or scales.shape != (rows, groups):
-            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold a tensor of shape {shape}")
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold a tensor of shape "
+                             f"{tuple(shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
             raise ValueError("codes and scales are contiguous and on one device")
         if dtype not in _DTYPE:
             raise TypeError(f"checkpoints are made of float32, bfloat16 and float16 tensors, not {dtype}")
-        self.codes, self.scales, self.shape, self.dtype, self.rows, self.cols = codes, scales, shape, dtype, rows, cols
+        self.shape, self.dtype, self.device, self.rows, self.cols = tuple(shape), dtype, codes.device, rows, cols
+        self._codes, self._scales, self._room = codes, scales, None
+        self._at, self._scales_at = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _empty(cls, x: torch.Tensor, rows: int, cols: int) -> "Checkpoint8":
+        """Room for the checkpoint of x, in one allocation; the two tensors over it are made when they are asked for."""
+        self = cls.__new__(cls)
+        groups = -(-cols // GROUP)
+        room = torch.empty(rows * groups * (GROUP + 1), dtype=torch.int8, device=x.device)
+        self.shape, self.dtype, self.device, self.rows, self.cols = x.shape, x.dtype, x.device, rows, cols
+        self._codes = self._scales = None
+        self._room = room
+        self._at = at = room.data_ptr()
+        self._scales_at = at + rows * groups * GROUP
+        return self
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            pitch = -(-self.cols // GROUP) * GROUP
+            self._codes = self._room[:self.rows * pitch].view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            groups = -(-self.cols // GROUP)
+            self._scales = self._room[self.rows * groups * GROUP:].view(torch.uint8).view(self.rows, groups)
+        return self._scales
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.rows * -(-self.cols // GROUP) * (GROUP + 1)
+
+    def record_stream(self, stream) -> None:
+        """As ``torch.Tensor.record_stream``: the arrays are used on ``stream``, too."""
+        for t in (self._room, self._codes, self._scales):
+            if t is not None:
+                t.record_stream(stream)
 
     def __repr__(self):
-        return f"Checkpoint8(shape={self.shape}, dtype={self.dtype}, {self.nbytes} bytes)"
+        return f"Checkpoint8(shape={tuple(self.shape)}, dtype={self.dtype}, {self.nbytes} bytes)"
 
 
 # ------------------------------------------------------------------- what the calls have in common
 def _rows_cols(shape):
-    if len(shape) == 0:
-        return 1, 1
-    return math.prod(shape[:-1]), shape[-1]
+    n = len(shape)
+    if n == 2:
+        return shape
+    return (math.prod(shape[:-1]), shape[-1]) if n else (1, 1)
 
 
-def _on(device: torch.device):
-    """The device's current stream is the one to launch on, whichever device is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+def _elsewhere(device: torch.device) -> bool:
+    """Whether another device is the current one: the call is then made again with its tensor's device current, whose
+    stream is the one to launch on."""
+    return device.index != torch.cuda.current_device()
 
 
 def _need(t: torch.Tensor, what: str) -> int:
@@ -106,67 +135,65 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
     return outer[-1][1]
 
 
-def _same(t: torch.Tensor, like, what: str) -> None:
-    if t.device != like.device:
-        raise ValueError(f"{what}: on {t.device}, not on {like.device}")
+def _like(t: torch.Tensor, stride: int) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if stride == 0 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _params(p, cols: int, like: torch.Tensor, what: str):
     if p is None:
         return 0, None
     kind = _need(p, what)
-    _same(p, like, what)
+    if p.device != like.device:
+        raise ValueError(f"{what}: on {p.device}, not on {like.device}")
     if p.numel() != cols or not p.is_contiguous():
         raise ValueError(f"{what}: expected {cols} contiguous values")
     return p.data_ptr(), kind
-
-
-def _empty_checkpoint(x: torch.Tensor, flat: bool = False) -> Checkpoint8:
-    rows, cols = _rows_cols(x.shape)
-    if flat:
-        rows, cols = 1, rows * cols
-    groups = -(-cols // GROUP)
-    codes = torch.empty((rows, groups * GROUP), dtype=torch.int8, device=x.device)
-    scales = torch.empty((rows, groups), dtype=torch.uint8, device=x.device)
-    return Checkpoint8(codes, scales, x.shape, x.dtype)
 
 
 # ------------------------------------------------------------------- codec
 def q8_compress(x: torch.Tensor, flat: bool = False) -> Checkpoint8:
     """The checkpoint of ``x``.  ``flat`` (contiguous tensors): groups run through the whole tensor instead of
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
-    is the same either way, and only such a flat checkpoint has rows for ``q8_weight_grad``."""
+    is the same either way, and only such a flat checkpoint has rows for the backward passes."""
     kind = _need(x, "q8_compress")
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return q8_compress(x, flat)
     stride = _row_stride(x, "q8_compress")
-    if x.numel() == 0 and (x.dim() == 0 or x.shape[-1] == 0):
+    rows, cols = _rows_cols(x.shape)
+    if cols == 0:
         raise ValueError("q8_compress: rows without values")
-    if flat and not x.is_contiguous():
+    if flat and stride:
         raise ValueError("q8_compress: flat checkpoints are made of contiguous tensors")
-    if flat and x.numel() == 0:
-        flat = False
-    held = _empty_checkpoint(x, flat and x.shape[-1:].numel() % GROUP != 0)
-    with _on(x.device):
-        check(lib().cswap_q8_pack(x.data_ptr(), kind, held.rows, held.cols, stride, held.codes.data_ptr(),
-                                  held.scales.data_ptr(), _stream()), "cswap_q8_pack")
+    if flat and rows and cols % GROUP:
+        rows, cols = 1, rows * cols
+    held = Checkpoint8._empty(x, rows, cols)
+    check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, held._at, held._scales_at, api._stream()),
+          "cswap_q8_pack")
     return held
 
 
 def q8_decompress(held: Checkpoint8, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """What ``held`` stands for, in its own type or in ``dtype`` (rounded once where that does not hold it)."""
-    if not held.codes.is_cuda:
+    if held.device.type != "cuda":
         raise ValueError("q8_decompress: expected a checkpoint in device memory")
+    if _elsewhere(held.device):
+        with torch.cuda.device(held.device):
+            return q8_decompress(held, out, dtype)
     if out is None:
         out = torch.empty(held.shape, dtype=dtype or held.dtype, device=held.device)
-    elif tuple(out.shape) != held.shape or (dtype is not None and out.dtype != dtype):
-        raise ValueError(f"q8_decompress: out is {tuple(out.shape)} {out.dtype}")
-    kind = _need(out, "q8_decompress")
-    _same(out, held, "q8_decompress: out")
-    stride = _row_stride(out, "q8_decompress")
-    if stride and held.rows == 1 and out.numel() != out.shape[-1]:
-        raise ValueError("q8_decompress: a flat checkpoint goes into a contiguous tensor")
-    with _on(held.device):
-        check(lib().cswap_q8_unpack(held.codes.data_ptr(), held.scales.data_ptr(), held.rows, held.cols, out.data_ptr(),
-                                    kind, stride, _stream()), "cswap_q8_unpack")
+        stride = 0
+    else:
+        if out.shape != torch.Size(held.shape) or (dtype is not None and out.dtype != dtype):
+            raise ValueError(f"q8_decompress: out is {tuple(out.shape)} {out.dtype}")
+        if out.device != held.device:
+            raise ValueError(f"q8_decompress: out on {out.device}, not on {held.device}")
+        stride = _row_stride(out, "q8_decompress")
+        if stride and held.rows != _rows_cols(held.shape)[0]:
+            raise ValueError("q8_decompress: a flat checkpoint goes into a contiguous tensor")
+    check(lib().cswap_q8_unpack(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), _need(out, "q8_decompress"),
+                                stride, api._stream()), "cswap_q8_unpack")
     return out
 
 
@@ -180,24 +207,26 @@ def _kind_of(kind: str) -> int:
 def q8_act(x: torch.Tensor, kind: str = "gelu"):
     """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu"."""
     k, dtype = _kind_of(kind), _need(x, "q8_act")
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return q8_act(x, kind)
     stride = _row_stride(x, "q8_act")
     rows, cols = _rows_cols(x.shape)
     if cols == 0:
         raise ValueError("q8_act: rows without values")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    held = _empty_checkpoint(x)
-    with _on(x.device):
-        check(lib().cswap_q8_act_forward(k, x.data_ptr(), dtype, rows, cols, stride, y.data_ptr(), 0, held.codes.data_ptr(),
-                                         held.scales.data_ptr(), _stream()), "cswap_q8_act_forward")
+    y = _like(x, stride)
+    held = Checkpoint8._empty(x, rows, cols)
+    check(lib().cswap_q8_act_forward(k, x.data_ptr(), dtype, rows, cols, stride, y.data_ptr(), 0, held._at, held._scales_at,
+                                     api._stream()), "cswap_q8_act_forward")
     return y, held
 
 
 def _need_gradient(dy: torch.Tensor, held, what: str):
     """dy's type and row stride; it goes with an input of held's shape and type."""
     kind = _need(dy, f"{what}: dy")
-    _same(dy, held, f"{what}: dy")
-    if tuple(dy.shape) != tuple(held.shape) or dy.dtype != held.dtype:
-        raise ValueError(f"{what}: dy is {tuple(dy.shape)} {dy.dtype}, the input was {tuple(held.shape)} {held.dtype}")
+    if dy.shape != torch.Size(held.shape) or dy.dtype != held.dtype or dy.device != held.device:
+        raise ValueError(f"{what}: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, the input was {tuple(held.shape)} "
+                         f"{held.dtype} on {held.device}")
     return kind, _row_stride(dy, f"{what}: dy")
 
 
@@ -213,11 +242,13 @@ def q8_act_backward(dy: torch.Tensor, held: Checkpoint8, kind: str = "gelu") -> 
     """``dy * f'(x)``, x as ``held`` has it."""
     k = _kind_of(kind)
     dtype, stride = _need_gradient(dy, held, "q8_act_backward")
+    if _elsewhere(dy.device):
+        with torch.cuda.device(dy.device):
+            return q8_act_backward(dy, held, kind)
     rows, cols = _need_rows(held, "q8_act_backward")
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    with _on(dy.device):
-        check(lib().cswap_q8_act_backward(k, dy.data_ptr(), dtype, rows, cols, stride, held.codes.data_ptr(),
-                                          held.scales.data_ptr(), dx.data_ptr(), 0, _stream()), "cswap_q8_act_backward")
+    dx = _like(dy, stride)
+    check(lib().cswap_q8_act_backward(k, dy.data_ptr(), dtype, rows, cols, stride, held._at, held._scales_at, dx.data_ptr(), 0,
+                                      api._stream()), "cswap_q8_act_backward")
     return dx
 
 
@@ -227,6 +258,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """``(y, mean, rstd, held)``: layer norm over the last dimension, the rows' statistics in fp32, and what the
     backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``."""
     dtype = _need(x, "layer_norm")
+    if _elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps, checkpoint)
     stride = _row_stride(x, "layer_norm")
     rows, cols = _rows_cols(x.shape)
     if cols == 0 or x.dim() == 0:
@@ -235,16 +269,17 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     b, bk = _params(bias, cols, x, "layer_norm: bias")
     if wk is not None and bk is not None and wk != bk:
         raise TypeError("layer_norm: weight and bias have one type")
-    pk = wk if wk is not None else bk if bk is not None else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    held = _empty_checkpoint(x) if checkpoint else x
-    codes, scales = (held.codes.data_ptr(), held.scales.data_ptr()) if checkpoint else (0, 0)
-    at = stats.data_ptr()
-    with _on(x.device):
-        check(lib().cswap_layer_norm_forward(x.data_ptr(), dtype, rows, cols, stride, w, b, pk, eps, y.data_ptr(), 0, at,
-                                             at + 4 * rows, codes, scales, _stream()), "cswap_layer_norm_forward")
-    return y, stats[0], stats[1], held
+    y = _like(x, stride)
+    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
+    if checkpoint:
+        held = Checkpoint8._empty(x, rows, cols)
+        codes, scales = held._at, held._scales_at
+    else:
+        held, codes, scales = x, 0, 0
+    check(lib().cswap_layer_norm_forward(x.data_ptr(), dtype, rows, cols, stride, w, b, wk or bk or 0, eps, y.data_ptr(), 0,
+                                         mean.data_ptr(), rstd.data_ptr(), codes, scales, api._stream()),
+          "cswap_layer_norm_forward")
+    return y, mean, rstd, held
 
 
 def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor | None = None,
@@ -252,9 +287,12 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
     """``(dx, dweight, dbias)``; ``held`` is what ``layer_norm`` returned last.  The parameters' gradients come in
     ``param_dtype`` (the weight's type, else dy's)."""
     dtype, stride = _need_gradient(dy, held, "layer_norm_backward")
+    if _elsewhere(dy.device):
+        with torch.cuda.device(dy.device):
+            return layer_norm_backward(dy, held, mean, rstd, weight, param_dtype)
     if isinstance(held, Checkpoint8):
         rows, cols = _need_rows(held, "layer_norm_backward")
-        x, x_stride, codes, scales = 0, 0, held.codes.data_ptr(), held.scales.data_ptr()
+        x, x_stride, codes, scales = 0, 0, held._at, held._scales_at
     else:
         rows, cols = _rows_cols(held.shape)
         x, x_stride, codes, scales = held.data_ptr(), _row_stride(held, "layer_norm_backward: x"), 0, 0
@@ -262,20 +300,20 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
         if s.dtype != torch.float32 or s.numel() != rows or not s.is_contiguous() or s.device != dy.device:
             raise ValueError(f"layer_norm_backward: mean and rstd are {rows} contiguous fp32 values on {dy.device}")
     w, wk = _params(weight, cols, dy, "layer_norm_backward: weight")
-    param_dtype = param_dtype or (weight.dtype if weight is not None else dy.dtype)
-    if param_dtype not in _DTYPE or (weight is not None and param_dtype != weight.dtype):
+    if wk is not None and param_dtype not in (None, weight.dtype):
+        raise TypeError(f"layer_norm_backward: param_dtype {param_dtype}, the weight has {weight.dtype}")
+    param_dtype = param_dtype or (dy.dtype if weight is None else weight.dtype)
+    pk = _DTYPE.get(param_dtype)
+    if pk is None:
         raise TypeError(f"layer_norm_backward: param_dtype {param_dtype}")
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    grads = torch.empty((2, cols), dtype=param_dtype, device=dy.device)
+    dx = _like(dy, stride)
+    dw, db = torch.empty((2, cols), dtype=param_dtype, device=dy.device).unbind()
     room = lib().cswap_layer_norm_workspace_bytes(rows, cols)
     ws = torch.empty(room, dtype=torch.uint8, device=dy.device)
-    at = grads.data_ptr()
-    with _on(dy.device):
-        check(lib().cswap_layer_norm_backward(dy.data_ptr(), dtype, rows, cols, stride, x, x_stride, codes, scales,
-                                              mean.data_ptr(), rstd.data_ptr(), w, _DTYPE[param_dtype], dx.data_ptr(), 0, at,
-                                              at + cols * grads.element_size(), ws.data_ptr(), room, _stream()),
-              "cswap_layer_norm_backward")
-    return dx, grads[0], grads[1]
+    check(lib().cswap_layer_norm_backward(dy.data_ptr(), dtype, rows, cols, stride, x, x_stride, codes, scales, mean.data_ptr(),
+                                          rstd.data_ptr(), w, pk, dx.data_ptr(), 0, dw.data_ptr(), db.data_ptr(),
+                                          ws.data_ptr(), room, api._stream()), "cswap_layer_norm_backward")
+    return dx, dw, db
 
 
 # ------------------------------------------------------------------- weight gradient
@@ -283,23 +321,29 @@ def q8_weight_grad(dy: torch.Tensor, held: Checkpoint8, bias: bool = True, out_d
     """``(dW, db)`` of ``y = x @ W.T + b`` from ``dy`` and the checkpoint of ``x``: ``dy.T @ x`` and ``dy.sum(0)`` over
     all rows, in ``out_dtype`` (dy's type); ``db`` is None without ``bias``."""
     kind = _need(dy, "q8_weight_grad: dy")
-    _same(dy, held, "q8_weight_grad: dy")
+    if dy.device != held.device:
+        raise ValueError(f"q8_weight_grad: dy on {dy.device}, the input's checkpoint on {held.device}")
+    if _elsewhere(dy.device):
+        with torch.cuda.device(dy.device):
+            return q8_weight_grad(dy, held, bias, out_dtype)
     rows, k = _need_rows(held, "q8_weight_grad")
-    if dy.dim() == 0 or tuple(dy.shape[:-1]) != held.shape[:-1]:
-        raise ValueError(f"q8_weight_grad: dy is {tuple(dy.shape)}, the input was {held.shape}")
+    if dy.dim() == 0 or dy.shape[:-1] != torch.Size(held.shape[:-1]):
+        raise ValueError(f"q8_weight_grad: dy is {tuple(dy.shape)}, the input was {tuple(held.shape)}")
     if dy.dtype == torch.float16 and held.dtype != torch.float16:
         raise TypeError("q8_weight_grad: a float16 dy goes with the checkpoint of a float16 input")
     stride = _row_stride(dy, "q8_weight_grad: dy")
     n = dy.shape[-1]
+    if n == 0:
+        raise ValueError("q8_weight_grad: rows without values")
     out_dtype = out_dtype or dy.dtype
-    if out_dtype not in _DTYPE:
+    out_kind = _DTYPE.get(out_dtype)
+    if out_kind is None:
         raise TypeError(f"q8_weight_grad: out_dtype {out_dtype}")
     dw = torch.empty((n, k), dtype=out_dtype, device=dy.device)
     db = torch.empty(n, dtype=out_dtype, device=dy.device) if bias else None
     room = lib().cswap_q8_weight_grad_workspace_bytes(kind, rows, n, k)
     ws = torch.empty(room, dtype=torch.uint8, device=dy.device)
-    with _on(dy.device):
-        check(lib().cswap_q8_weight_grad(dy.data_ptr(), kind, rows, n, stride, held.codes.data_ptr(), held.scales.data_ptr(),
-                                         k, dw.data_ptr(), db.data_ptr() if bias else 0, _DTYPE[out_dtype], ws.data_ptr(),
-                                         room, _stream()), "cswap_q8_weight_grad")
+    check(lib().cswap_q8_weight_grad(dy.data_ptr(), kind, rows, n, stride, held._at, held._scales_at, k, dw.data_ptr(),
+                                     db.data_ptr() if bias else 0, out_kind, ws.data_ptr(), room, api._stream()),
+          "cswap_q8_weight_grad")
     return dw, db
