@@ -14,34 +14,49 @@
 namespace cswap {
 namespace q8 {
 
-// Lanes that share a row and chunks of 8 values that each of them holds.  A workgroup has 256 threads, as many as one row needs
-// where that is more.
-template <int L, int NC> struct Form {
-  static constexpr int lanes = L, chunks = NC;
-  static constexpr int threads = L > 256 ? L : 256, rows = threads / L, waves = threads / 64;
+// L lanes share a row, each holds NC chunks of 8 values; a workgroup has NT threads.
+template <int L, int NC, int NT> struct Form {
+  static constexpr int lanes = L, chunks = NC, threads = NT, rows = NT / L, waves = NT / 64;
 };
 
-// The sum over the L lanes of a row, in all of them, the same bits in each.  `red` (threads / 64 floats) only where a row has
-// more lanes than a wavefront.
-template <int L> __device__ inline float row_sum(float v, float* red)
-{
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true));   // lane ^ 1
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true));   // lane ^ 2
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));  // 7 - lane
-  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));  // 15 - lane
-  if (L >= 32) v += __shfl_xor(v, 16);
-  if (L >= 64) v += __shfl_xor(v, 32);
-  if (L > 64) {
-    constexpr int W = L / 64;
-    __syncthreads();  // red may still be read by the sum before
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
+#define CSWAP_DPP(v, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
+
+// The sums of two values over the L lanes of a row, in all of them, the same bits in each.  `red` (two buffers of `waves` pairs,
+// taken in turn: a buffer is written again only behind the next sum's barrier) only where a row has more lanes than a wavefront.
+template <int L, int WAVES> struct RowSum {
+  float2 (*red)[WAVES];
+  int turn = 0;
+  __device__ inline float2 operator()(float x, float y)
+  {
+    x += CSWAP_DPP(x, 0xb1), y += CSWAP_DPP(y, 0xb1);    // lane ^ 1
+    x += CSWAP_DPP(x, 0x4e), y += CSWAP_DPP(y, 0x4e);    // lane ^ 2
+    x += CSWAP_DPP(x, 0x141), y += CSWAP_DPP(y, 0x141);  // 7 - lane
+    x += CSWAP_DPP(x, 0x140), y += CSWAP_DPP(y, 0x140);  // 15 - lane
+    if (L >= 32) x = join<16>(x), y = join<16>(y);
+    if (L >= 64) x = join<32>(x), y = join<32>(y);
+    if (L > 64) {
+      constexpr int W = L / 64;
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) red[turn][wave] = make_float2(x, y);
+      __syncthreads();
+      x = y = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) v += red[w];
+      for (int w = 0; w < W; ++w) {
+        const float2 v = red[turn][wave / W * W + w];
+        x += v.x, y += v.y;
+      }
+      turn ^= 1;
+    }
+    return make_float2(x, y);
   }
-  return v;
-}
+  // v + v of lane ^ N: the swap of halves gives either half to both
+  template <int N> static __device__ inline float join(float v)
+  {
+    const unsigned u = __float_as_uint(v);
+    const auto p = N == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+};
 
 struct Params {
   const void* p;  // NULL: none
@@ -63,6 +78,19 @@ __device__ inline void load_params(const Params& q, uint32_t at, int valid, floa
   }
 }
 
+struct GradParams {
+  void *dgamma, *dbeta;  // NULL: not wanted
+  int dtype;
+  __device__ inline void store(bool gamma, uint32_t at, float v) const
+  {
+    void* to = gamma ? dgamma : dbeta;
+    if (!to) return;
+    if (dtype == CSWAP_DT_F32) static_cast<float*>(to)[at] = v;
+    else if (dtype == CSWAP_DT_BF16) static_cast<uint16_t*>(to)[at] = from_float<BF16>(v);
+    else static_cast<uint16_t*>(to)[at] = from_float<F16>(v);
+  }
+};
+
 struct NormShape {
   uint32_t rows, cols, code_chunks;  // code_chunks: chunks of a checkpoint's row, padding included
   float inv_cols, eps;
@@ -80,7 +108,8 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
                                                                   float* __restrict__ mean, float* __restrict__ rstd,
                                                                   uint2* __restrict__ codes, uint8_t* __restrict__ scales)
 {
-  __shared__ float red[F::waves];
+  __shared__ float2 red[2][F::waves];
+  RowSum<F::lanes, F::waves> row_sum = {red};
   const uint32_t lane = threadIdx.x % F::lanes;
   float g[F::chunks][8], b[F::chunks][8];
   int valid[F::chunks];
@@ -116,7 +145,7 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
         }
       }
     }
-    const float mu = row_sum<F::lanes>(sum, red) * s.inv_cols;
+    const float mu = row_sum(sum, 0.0f).x * s.inv_cols;
     float squares = 0.0f;
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c)
@@ -125,7 +154,7 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
         v[c][i] -= mu;
         if (i < valid[c]) squares = __builtin_fmaf(v[c][i], v[c][i], squares);
       }
-    const float r = 1.0f / __builtin_sqrtf(row_sum<F::lanes>(squares, red) * s.inv_cols + s.eps);
+    const float r = 1.0f / __builtin_sqrtf(row_sum(squares, 0.0f).x * s.inv_cols + s.eps);
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
 #pragma unroll
@@ -136,7 +165,42 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
   }
 }
 
-// One workgroup's share of the parameters' gradients: part[workgroup][0 = gamma, 1 = beta][cols].
+// What a lane holds of the next row while it works on this one: values as they lie in memory.
+template <typename T, bool HELD> struct RowChunk {
+  u4_any dy[T::bytes / 2], x[HELD ? 1 : T::bytes / 2];
+  uint2 q;
+  uint32_t scale;
+};
+
+template <typename T> __device__ inline void load_raw(const typename T::value* p, int valid, u4_any raw[T::bytes / 2])
+{
+  constexpr int W = T::bytes / 2;
+  if (valid >= kChunk) {
+#pragma unroll
+    for (int h = 0; h < W; ++h) raw[h] = reinterpret_cast<const u4_any*>(p)[h];
+  } else {
+#pragma unroll
+    for (int h = 0; h < W; ++h) raw[h] = (u4_any){0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < kChunk - 1; ++e)
+      if (e < valid) {
+        if constexpr (T::bytes == 4) raw[e / 4][e % 4] = __float_as_uint(p[e]);
+        else raw[0][e / 2] |= (uint32_t)p[e] << (16 * (e & 1));
+      }
+  }
+}
+
+template <typename T> __device__ inline void widen(const u4_any raw[T::bytes / 2], float v[8])
+{
+#pragma unroll
+  for (int e = 0; e < kChunk; ++e) {
+    if constexpr (T::bytes == 4) v[e] = __uint_as_float(raw[e / 4][e % 4]);
+    else v[e] = to_float<T>((typename T::value)(raw[0][e / 2] >> (16 * (e & 1))));
+  }
+}
+
+// Either the workgroup's share of the parameters' gradients, part[workgroup][0 = gamma, 1 = beta][cols], or, of a single
+// workgroup (part NULL), the gradients.
 template <typename T, typename F, bool HELD>
 __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typename T::value* __restrict__ dy, size_t dy_stride,
                                                                    const typename T::value* __restrict__ x, size_t x_stride,
@@ -144,9 +208,10 @@ __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typenam
                                                                    const uint8_t* __restrict__ scales, NormShape s,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                    Params gamma, typename T::value* __restrict__ dx,
-                                                                   size_t dx_stride, float* __restrict__ part)
+                                                                   size_t dx_stride, float* __restrict__ part, GradParams grads)
 {
-  __shared__ float red[F::waves];
+  __shared__ float2 red[2][F::waves];
+  RowSum<F::lanes, F::waves> row_sum = {red};
   const uint32_t lane = threadIdx.x % F::lanes;
   float g[F::chunks][8], dg[F::chunks][8], db[F::chunks][8];
   int valid[F::chunks];
@@ -158,33 +223,51 @@ __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typenam
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) dg[c][i] = db[c][i] = 0.0f;
   }
-  for (uint32_t base = blockIdx.x * F::rows; base < s.rows; base += gridDim.x * F::rows) {
-    const uint32_t row = base + threadIdx.x / F::lanes;
+  constexpr bool kAhead = F::chunks == 1 || F::lanes == 64;  // registers for two rows
+  RowChunk<T, HELD> next[F::chunks];
+  float next_mu, next_r;
+  auto load = [&](uint32_t row) {
     const bool here = row < s.rows;
-    const float mu = here ? mean[row] : 0.0f, r = here ? rstd[row] : 0.0f;
-    float h[F::chunks][8], u[F::chunks][8], s1 = 0.0f, s2 = 0.0f;
+    next_mu = here ? mean[row] : 0.0f, next_r = here ? rstd[row] : 0.0f;
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
       const uint32_t chunk = lane + c * F::lanes, col = chunk * kChunk;
       const int n = here ? valid[c] : 0;
-      load_chunk<T>(dy + (size_t)row * dy_stride + col, n, u[c]);
+      load_raw<T>(dy + (size_t)row * dy_stride + col, n, next[c].dy);
       if (HELD) {
         const size_t at = (size_t)row * s.code_chunks + chunk;
-        uint2 q = {0u, 0u};
-        uint32_t scale = 1;
-        if (n) q = codes[at], scale = scales[at / kChunksPerGroup];
-        decode_chunk(q, unit_of(scale), h[c]);
+        next[c].q = {0u, 0u}, next[c].scale = 1;
+        if (n) next[c].q = codes[at], next[c].scale = scales[at / kChunksPerGroup];
       } else {
-        load_chunk<T>(x + (size_t)row * x_stride + col, n, h[c]);
+        load_raw<T>(x + (size_t)row * x_stride + col, n, next[c].x);
       }
     }
+  };
+  // the rows of a workgroup walk together: every lane runs every exchange and barrier
+  const uint32_t mine = threadIdx.x / F::lanes;
+  if (kAhead && blockIdx.x * F::rows < s.rows) load(blockIdx.x * F::rows + mine);
+  for (uint32_t base = blockIdx.x * F::rows; base < s.rows; base += gridDim.x * F::rows) {
+    const uint32_t row = base + mine;
+    if (!kAhead) load(row);
+    const float mu = next_mu, r = next_r;
+    float h[F::chunks][8], u[F::chunks][8], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
-      const int n = here ? valid[c] : 0;
+      widen<T>(next[c].dy, u[c]);
+      if constexpr (HELD) decode_chunk(next[c].q, unit_of(next[c].scale), h[c]);
+      else widen<T>(next[c].x, h[c]);
+    }
+    if (kAhead && base + gridDim.x * F::rows < s.rows) load(row + gridDim.x * F::rows);
+#pragma unroll
+    for (int c = 0; c < F::chunks; ++c) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) h[c][i] = (h[c][i] - mu) * r;
+      if (HELD && valid[c] < kChunk) {  // a group of NaN reaches behind the row's end
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) h[c][i] = i < valid[c] ? h[c][i] : 0.0f;
+      }
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
-        h[c][i] = (h[c][i] - mu) * r;
-        if (i >= n) h[c][i] = 0.0f;  // a group of NaN reaches behind the row's end
         dg[c][i] = __builtin_fmaf(u[c][i], h[c][i], dg[c][i]);
         db[c][i] += u[c][i];
         u[c][i] *= g[c][i];
@@ -192,70 +275,90 @@ __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typenam
         s2 = __builtin_fmaf(u[c][i], h[c][i], s2);
       }
     }
-    s1 = row_sum<F::lanes>(s1, red) * s.inv_cols;
-    s2 = row_sum<F::lanes>(s2, red) * s.inv_cols;
+    const float2 sums = row_sum(s1, s2);
+    s1 = sums.x * s.inv_cols, s2 = sums.y * s.inv_cols;
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) u[c][i] = r * (u[c][i] - __builtin_fmaf(h[c][i], s2, s1));
-      if (here) store_chunk<T>(dx + (size_t)row * dx_stride + (lane + c * F::lanes) * kChunk, valid[c], u[c]);
+      if (row < s.rows) store_chunk<T>(dx + (size_t)row * dx_stride + (lane + c * F::lanes) * kChunk, valid[c], u[c]);
     }
   }
-  if (!part) return;
-  float* mine = part + (size_t)blockIdx.x * 2 * s.cols;
-  // the rows of a workgroup one after the other, in a fixed order
-  constexpr int kPass = F::rows > 1 ? F::lanes * F::chunks * kChunk : 1;
-  __shared__ float sum[2][kPass];
-  if (F::rows > 1) {
-    for (int turn = 0; turn < F::rows; ++turn) {
-      if ((int)(threadIdx.x / F::lanes) == turn) {
+  if (!part && !grads.dgamma && !grads.dbeta) return;
+  float* const share = part ? part + (size_t)blockIdx.x * 2 * s.cols : nullptr;
+  if constexpr (F::rows > 1) {
+    // the lanes that have the same columns one after the other, in a fixed order: within a wavefront by exchanges, then a turn for
+    // each quarter of the workgroup's rows
+    constexpr int kCols = F::lanes * F::chunks * kChunk, kWide = F::lanes < 64 ? 64 : F::lanes, kSets = F::threads / kWide;
+    __shared__ __attribute__((aligned(16))) float sum[kSets * 2 * kCols];
 #pragma unroll
-        for (int c = 0; c < F::chunks; ++c)
+    for (int c = 0; c < F::chunks; ++c)
 #pragma unroll
-          for (int i = 0; i < kChunk; ++i) {
-            const uint32_t at = ((lane + c * F::lanes) * kChunk + i) % kPass;
-            if (turn) dg[c][i] += sum[0][at], db[c][i] += sum[1][at];
-            sum[0][at] = dg[c][i], sum[1][at] = db[c][i];
-          }
+      for (int i = 0; i < kChunk; ++i) {
+        if (F::lanes <= 16) dg[c][i] = row_sum.template join<16>(dg[c][i]), db[c][i] = row_sum.template join<16>(db[c][i]);
+        if (F::lanes <= 32) dg[c][i] = row_sum.template join<32>(dg[c][i]), db[c][i] = row_sum.template join<32>(db[c][i]);
       }
-      __syncthreads();
+    if (threadIdx.x % kWide < F::lanes) {
+      float* to = sum + (size_t)(threadIdx.x / kWide) * 2 * kCols;
+#pragma unroll
+      for (int c = 0; c < F::chunks; ++c)
+#pragma unroll
+        for (int i = 0; i < kChunk; i += 4) {
+          const int at = (lane + c * F::lanes) * kChunk + i;
+          *reinterpret_cast<float4*>(to + at) = make_float4(dg[c][i], dg[c][i + 1], dg[c][i + 2], dg[c][i + 3]);
+          *reinterpret_cast<float4*>(to + kCols + at) = make_float4(db[c][i], db[c][i + 1], db[c][i + 2], db[c][i + 3]);
+        }
     }
-    for (uint32_t i = threadIdx.x; i < s.cols; i += F::threads) mine[i] = sum[0][i % kPass], mine[s.cols + i] = sum[1][i % kPass];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 2 * s.cols; i += F::threads) {
+      const uint32_t col = i < s.cols ? i : i - s.cols;
+      const float* from = sum + (i < s.cols ? 0 : kCols) + col;
+      float v = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSets; ++k) v += from[k * 2 * kCols];
+      if (share) share[i] = v;
+      else grads.store(i < s.cols, col, v);
+    }
   } else {
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
       const uint32_t col = (lane + c * F::lanes) * kChunk;
-      store_chunk<F32>(mine + col, valid[c], dg[c]);
-      store_chunk<F32>(mine + s.cols + col, valid[c], db[c]);
+      if (share) {
+        store_chunk<F32>(share + col, valid[c], dg[c]);
+        store_chunk<F32>(share + s.cols + col, valid[c], db[c]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+          if (i < valid[c]) grads.store(true, col + i, dg[c][i]), grads.store(false, col + i, db[c][i]);
+      }
     }
   }
 }
 
-// out[i] = sum over `parts` rows of part[.][i], n values a row; 32 columns a workgroup, eight lanes to a column
-template <typename P>
-__global__ __launch_bounds__(256) void norm_reduce_kernel(const float* __restrict__ part, uint32_t parts, uint32_t cols,
-                                                          typename P::value* __restrict__ dgamma,
-                                                          typename P::value* __restrict__ dbeta)
+// The gradients from `parts` shares: 32 columns a workgroup, 32 lanes to a column
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restrict__ part, uint32_t parts, uint32_t cols,
+                                                           GradParams grads)
 {
-  __shared__ float sum[8][32];
-  const uint32_t i = blockIdx.x * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5, n = 2 * cols;
+  __shared__ float sum[32][33];
+  const uint32_t lane = threadIdx.x & 31, seg = threadIdx.x >> 5, n = 2 * cols, i = blockIdx.x * 32 + lane;
   float v = 0.0f;
-  if (i < n)
-    for (uint32_t p = seg; p < parts; p += 8) v += part[(size_t)p * n + i];
-  sum[seg][threadIdx.x & 31] = v;
+  if (i < n) {
+#pragma unroll 8
+    for (uint32_t p = seg; p < parts; p += 32) v += part[(size_t)p * n + i];
+  }
+  sum[seg][lane] = v;
   __syncthreads();
   if (seg == 0 && i < n) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) v += sum[k][threadIdx.x];
-    typename P::value* out = i < cols ? dgamma : dbeta;
-    if (out) out[i < cols ? i : i - cols] = from_float<P>(v);
+    for (int k = 1; k < 32; ++k) v += sum[k][lane];
+    grads.store(i < cols, i < cols ? i : i - cols, v);
   }
 }
 
 // ---------------------------------------------------------------- launches
 // Rows up to 16384 values: 16 lanes hold 128 values of a row, 1024 lanes with two chunks each the longest.
 constexpr size_t kMaxNormCols = 16384;
-constexpr unsigned kMostForward = 2048, kMostBackward = 512;  // workgroups
+constexpr unsigned kMostForward = 2048, kMostBackward = 256;  // workgroups
 
 template <typename F> static unsigned groups_for(size_t rows, unsigned most)
 {
@@ -263,21 +366,38 @@ template <typename F> static unsigned groups_for(size_t rows, unsigned most)
   return (unsigned)(want < most ? want : most);
 }
 
-template <typename Fn> static auto with_form(size_t cols, Fn&& fn)
+template <typename Fn> static auto with_forward_form(size_t cols, Fn&& fn)
 {
-  if (cols <= 128) return fn(Form<16, 1>());
-  if (cols <= 256) return fn(Form<32, 1>());
-  if (cols <= 512) return fn(Form<64, 1>());
-  if (cols <= 1024) return fn(Form<64, 2>());
-  if (cols <= 2048) return fn(Form<256, 1>());
-  if (cols <= 4096) return fn(Form<256, 2>());
-  if (cols <= 8192) return fn(Form<1024, 1>());
-  return fn(Form<1024, 2>());
+  if (cols <= 128) return fn(Form<16, 1, 256>());
+  if (cols <= 256) return fn(Form<32, 1, 256>());
+  if (cols <= 512) return fn(Form<64, 1, 256>());
+  if (cols <= 1024) return fn(Form<64, 2, 256>());
+  if (cols <= 2048) return fn(Form<256, 1, 256>());
+  if (cols <= 4096) return fn(Form<512, 1, 512>());
+  if (cols <= 8192) return fn(Form<1024, 1, 1024>());
+  return fn(Form<1024, 2, 1024>());
 }
 
+// Large workgroups: as few shares of the parameters' gradients as there are compute units.
+template <typename Fn> static auto with_backward_form(size_t cols, Fn&& fn)
+{
+  if (cols <= 128) return fn(Form<16, 1, 1024>());
+  if (cols <= 256) return fn(Form<32, 1, 1024>());
+  if (cols <= 512) return fn(Form<64, 1, 1024>());
+  if (cols <= 1024) return fn(Form<64, 2, 512>());
+  if (cols <= 2048) return fn(Form<256, 1, 1024>());
+  if (cols <= 4096) return fn(Form<512, 1, 1024>());
+  if (cols <= 8192) return fn(Form<1024, 1, 1024>());
+  return fn(Form<1024, 2, 1024>());
+}
+
+// One workgroup for as many rows as it takes in four turns: it needs no second kernel for the parameters' gradients.
 static unsigned backward_groups(size_t rows, size_t cols)
 {
-  return with_form(cols, [&](auto f) { return groups_for<decltype(f)>(rows, kMostBackward); });
+  return with_backward_form(cols, [&](auto f) {
+    typedef decltype(f) F;
+    return rows <= 4 * F::rows ? 1u : groups_for<F>(rows, kMostBackward);
+  });
 }
 
 template <typename Fn> static int with_type(int dtype, Fn&& fn)
@@ -305,7 +425,8 @@ using namespace cswap::q8;
 extern "C" size_t cswap_layer_norm_workspace_bytes(size_t rows, size_t cols)
 {
   if (cols == 0 || cols > kMaxNormCols || rows == 0) return 0;
-  return (size_t)backward_groups(rows, cols) * 2 * cols * sizeof(float);
+  const size_t groups = backward_groups(rows, cols);
+  return groups > 1 ? groups * 2 * cols * sizeof(float) : 0;
 }
 
 extern "C" int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
@@ -327,7 +448,7 @@ extern "C" int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows,
   hipStream_t st = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    return with_form(cols, [&](auto f) {
+    return with_forward_form(cols, [&](auto f) {
       typedef decltype(f) F;
       auto k = d_codes ? norm_forward_kernel<T, F, true> : norm_forward_kernel<T, F, false>;
       hipLaunchKernelGGL(k, dim3(groups_for<F>(rows, kMostForward)), dim3(F::threads), 0, st,
@@ -361,33 +482,33 @@ extern "C" int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t row
         !value_ptr(d_rstd, CSWAP_DT_F32))
       return CSWAP_E_ARG;
     if (held ? (d_x || !checkpoint_ptrs(d_codes, d_scales)) : !value_ptr(d_x, dtype)) return CSWAP_E_ARG;
-    if (reduce && !value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
-    if (reduce && ws_bytes < cswap_layer_norm_workspace_bytes(rows, cols)) return CSWAP_E_NOMEM;
+    const size_t room = reduce ? cswap_layer_norm_workspace_bytes(rows, cols) : 0;
+    if (room && !value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
+    if (ws_bytes < room) return CSWAP_E_NOMEM;
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   const Params g = {d_gamma, param_dtype};
   const unsigned grid = rows ? backward_groups(rows, cols) : 0;
+  const GradParams grads = {d_dgamma, d_dbeta, param_dtype};
   if (rows) {
     const int e = with_type(dtype, [&](auto t) {
       typedef decltype(t) T;
-      return with_form(cols, [&](auto f) {
+      return with_backward_form(cols, [&](auto f) {
         typedef decltype(f) F;
         auto k = d_codes ? norm_backward_kernel<T, F, true> : norm_backward_kernel<T, F, false>;
-        hipLaunchKernelGGL(k, dim3(grid), dim3(F::threads), 0, st, static_cast<const typename T::value*>(d_dy), (size_t)dy_stride,
-                           static_cast<const typename T::value*>(d_x), (size_t)x_stride, reinterpret_cast<const uint2*>(d_codes),
-                           d_scales, s, d_mean, d_rstd, g, static_cast<typename T::value*>(d_dx), (size_t)dx_stride,
-                           reduce ? static_cast<float*>(d_ws) : nullptr);
+        hipLaunchKernelGGL(k, dim3(grid), dim3(F::threads), 0, st, static_cast<const typename T::value*>(d_dy),
+                           (size_t)dy_stride, static_cast<const typename T::value*>(d_x), (size_t)x_stride,
+                           reinterpret_cast<const uint2*>(d_codes), d_scales, s, d_mean, d_rstd, g,
+                           static_cast<typename T::value*>(d_dx), (size_t)dx_stride,
+                           reduce && grid > 1 ? static_cast<float*>(d_ws) : nullptr,
+                           grid > 1 ? GradParams{nullptr, nullptr, 0} : grads);
         return check_launch();
       });
     });
     if (e) return e;
   }
-  if (!reduce) return CSWAP_OK;
-  return with_type(param_dtype, [&](auto t) {
-    typedef decltype(t) P;
-    hipLaunchKernelGGL(norm_reduce_kernel<P>, dim3((unsigned)((2 * cols + 31) / 32)), dim3(256), 0, st,
-                       static_cast<const float*>(d_ws), grid, (uint32_t)cols, static_cast<typename P::value*>(d_dgamma),
-                       static_cast<typename P::value*>(d_dbeta));
-    return check_launch();
-  });
+  if (!reduce || grid == 1) return CSWAP_OK;
+  hipLaunchKernelGGL(norm_reduce_kernel, dim3((unsigned)((2 * cols + 31) / 32)), dim3(1024), 0, st, static_cast<const float*>(d_ws),
+                     grid, (uint32_t)cols, grads);
+  return check_launch();
 }
