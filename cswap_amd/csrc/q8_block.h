@@ -143,8 +143,9 @@ __device__ inline uint32_t quad_max_bits(const float v[8])
   return m;
 }
 
-// Eight codes (byte i of the pair is value i) and the group's scale byte.
-__device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale)
+// Eight codes (byte i of the pair is value i) and the group's scale byte.  KEEP_SIGN: a value that is not 0 has no code of 0 but 1
+// or -1, the nearest that has its sign.
+template <bool KEEP_SIGN = false> __device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale)
 {
   const int exponent = (int)(max_bits >> 23);
   const int b = max(exponent - 6, 1);
@@ -157,6 +158,11 @@ __device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32
 #pragma unroll
   for (int i = 0; i < kChunk; ++i)
     t[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], inverse, kMagic), kMagic - 127.0f, kMagic + 127.0f));
+  if (KEEP_SIGN) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
+  }
   uint2 q;
   // v_perm_b32 numbers the bytes of its second operand 0 to 3 and those of its first 4 to 7
   q.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400), __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400), 0x05040100);

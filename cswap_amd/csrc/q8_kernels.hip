@@ -49,7 +49,7 @@ __device__ inline void store_codes(uint32_t chunk, uint2 q, uint32_t scale, uint
   if ((chunk & (kChunksPerGroup - 1)) == 0) scales[chunk / kChunksPerGroup] = (uint8_t)scale;
 }
 
-template <typename T, bool FLAT>
+template <typename T, bool FLAT, bool KEEP_SIGN>
 __global__ __launch_bounds__(kThreads) void q8_pack_kernel(const typename T::value* __restrict__ in, size_t stride, Shape s,
                                                            size_t flat_cols, uint2* __restrict__ codes,
                                                            uint8_t* __restrict__ scales)
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kThreads) void q8_pack_kernel(const typename T::val
   float v[kChunk];
   load_chunk<T>(in + offset_of<FLAT>(chunk, p, stride), p.valid, v);
   uint32_t scale;
-  const uint2 q = encode_chunk(v, quad_max_bits(v), &scale);
+  const uint2 q = encode_chunk<KEEP_SIGN>(v, quad_max_bits(v), &scale);
   store_codes(chunk, q, scale, codes, scales);
 }
 
@@ -187,9 +187,11 @@ __global__ __launch_bounds__(kThreads) void q8_act_forward_kernel(const typename
   const Place p = place_of<FLAT>(chunk, s, flat_cols);
   float v[kChunk];
   load_chunk<T>(x + offset_of<FLAT>(chunk, p, x_stride), p.valid, v);
-  uint32_t scale;
-  const uint2 q = encode_chunk(v, quad_max_bits(v), &scale);
-  store_codes(chunk, q, scale, codes, scales);
+  if (codes) {
+    uint32_t scale;
+    const uint2 q = encode_chunk(v, quad_max_bits(v), &scale);
+    store_codes(chunk, q, scale, codes, scales);
+  }
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) v[i] = A::template value<T>(v[i]);
   store_chunk<T>(y + offset_of<FLAT>(chunk, p, y_stride), p.valid, v);
@@ -235,9 +237,11 @@ static int plan(size_t rows, size_t cols, ptrdiff_t* stride_a, ptrdiff_t* stride
   return CSWAP_OK;
 }
 
-template <typename T> static int pack(const void* in, size_t stride, const Call& c, int8_t* codes, uint8_t* scales, hipStream_t st)
+template <typename T>
+static int pack(const void* in, size_t stride, bool keep_sign, const Call& c, int8_t* codes, uint8_t* scales, hipStream_t st)
 {
-  auto k = c.flat ? q8_pack_kernel<T, true> : q8_pack_kernel<T, false>;
+  auto k = keep_sign ? (c.flat ? q8_pack_kernel<T, true, true> : q8_pack_kernel<T, false, true>)
+                     : (c.flat ? q8_pack_kernel<T, true, false> : q8_pack_kernel<T, false, false>);
   hipLaunchKernelGGL(k, dim3(c.grid), dim3(kThreads), 0, st, static_cast<const typename T::value*>(in), stride, c.s, c.flat_cols,
                      reinterpret_cast<uint2*>(codes), scales);
   return check_launch();
@@ -304,8 +308,8 @@ using namespace cswap::q8;
 extern "C" size_t cswap_q8_code_pitch(size_t cols) { return pitch_of(cols); }
 extern "C" size_t cswap_q8_scale_pitch(size_t cols) { return groups_of(cols); }
 
-extern "C" int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride, int8_t* d_codes,
-                             uint8_t* d_scales, cswap_stream_t stream)
+extern "C" int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride, int keep_sign,
+                             int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream)
 {
   Call c;
   if (int e = plan(rows, cols, &stride, nullptr, &c)) return e;
@@ -314,9 +318,9 @@ extern "C" int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t co
   if (!value_ptr(d_in, dtype) || !checkpoint_ptrs(d_codes, d_scales)) return CSWAP_E_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case CSWAP_DT_F32: return pack<F32>(d_in, (size_t)stride, c, d_codes, d_scales, st);
-    case CSWAP_DT_BF16: return pack<BF16>(d_in, (size_t)stride, c, d_codes, d_scales, st);
-    default: return pack<F16>(d_in, (size_t)stride, c, d_codes, d_scales, st);
+    case CSWAP_DT_F32: return pack<F32>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
+    case CSWAP_DT_BF16: return pack<BF16>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
+    default: return pack<F16>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
   }
 }
 
@@ -343,7 +347,8 @@ extern "C" int cswap_q8_act_forward(int kind, const void* d_x, int dtype, size_t
   if (int e = plan(rows, cols, &x_stride, &y_stride, &c)) return e;
   if (!dtype_known(dtype) || !act_known(kind)) return CSWAP_E_ARG;
   if (rows == 0) return CSWAP_OK;
-  if (!value_ptr(d_x, dtype) || !value_ptr(d_y, dtype) || !checkpoint_ptrs(d_codes, d_scales)) return CSWAP_E_ARG;
+  if (!value_ptr(d_x, dtype) || !value_ptr(d_y, dtype)) return CSWAP_E_ARG;
+  if ((d_codes || d_scales) && !checkpoint_ptrs(d_codes, d_scales)) return CSWAP_E_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const size_t xs = (size_t)x_stride, ys = (size_t)y_stride;
   switch (dtype) {

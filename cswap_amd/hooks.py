@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import swap
+from . import q8, swap
 from ._lib import CswapError
 
 E_NOMEM = -4   # CSWAP_E_NOMEM
@@ -292,3 +292,42 @@ class swap_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         for h in self._live.values():      # held and never swapped
             h.keep = None
         self._live.clear()
+
+
+class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
+    """Keeps eligible saved activations on the device in 8 bits (``cswap_amd.q8``) instead of swapping them:
+    contiguous float32, bfloat16 and float16 device tensors of at least ``min_bytes`` that are not parameters or other
+    leaves; everything else is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
+    the largest magnitude among 32 neighbouring values, in the tensor's type; 0 stays 0 and everything else keeps its
+    sign, which is all that a ReLU's backward pass asks of its result.
+
+        with hold_saved_tensors():
+            loss = model(x).sum()
+        loss.backward()
+
+    A tensor that several nodes save is held once for each of them, so a float32 one gains half of its memory where
+    two nodes do and a 16-bit one nothing.  Layers that can read a checkpoint as it is (``cswap_amd.layers8``) need
+    neither the hooks nor the tensor that backward would be given here; what they keep passes through unchanged."""
+
+    def __init__(self, min_bytes: int = 1 << 20):
+        self.min_bytes = min_bytes
+        self.stats = {"held": 0, "bytes_in": 0, "bytes_held": 0, "kept": 0}
+        super().__init__(self._pack, self._unpack)
+
+    def _eligible(self, t: torch.Tensor) -> bool:
+        return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.is_contiguous() and t.dim() >= 1
+                and t.numel() * t.element_size() >= max(1, self.min_bytes) and not isinstance(t, torch.nn.Parameter)
+                and not t.is_leaf)
+
+    def _pack(self, t: torch.Tensor):
+        if not self._eligible(t):
+            self.stats["kept"] += 1
+            return t
+        held = q8.q8_compress(t.detach(), flat=True, keep_sign=True)
+        self.stats["held"] += 1
+        self.stats["bytes_in"] += t.numel() * t.element_size()
+        self.stats["bytes_held"] += held.nbytes
+        return held
+
+    def _unpack(self, held):
+        return q8.q8_decompress(held) if isinstance(held, q8.Checkpoint8) else held

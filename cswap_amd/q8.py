@@ -55,15 +55,20 @@ class Checkpoint8:
 
     @classmethod
     def _empty(cls, x: torch.Tensor, rows: int, cols: int) -> "Checkpoint8":
-        """Room for the checkpoint of x, in one allocation; the two tensors over it are made when they are asked for."""
+        """Room for the checkpoint of x, in one allocation."""
+        room = torch.empty(rows * -(-cols // GROUP) * (GROUP + 1), dtype=torch.int8, device=x.device)
+        return cls._over(room, x.shape, x.dtype, rows, cols)
+
+    @classmethod
+    def _over(cls, room: torch.Tensor, shape, dtype: torch.dtype, rows: int, cols: int) -> "Checkpoint8":
+        """The checkpoint in ``room``: codes, and scales behind them; the tensors over either are made when they are
+        asked for."""
         self = cls.__new__(cls)
-        groups = -(-cols // GROUP)
-        room = torch.empty(rows * groups * (GROUP + 1), dtype=torch.int8, device=x.device)
-        self.shape, self.dtype, self.device, self.rows, self.cols = x.shape, x.dtype, x.device, rows, cols
+        self.shape, self.dtype, self.device, self.rows, self.cols = shape, dtype, room.device, rows, cols
         self._codes = self._scales = None
         self._room = room
         self._at = at = room.data_ptr()
-        self._scales_at = at + rows * groups * GROUP
+        self._scales_at = at + rows * -(-cols // GROUP) * GROUP
         return self
 
     @property
@@ -152,14 +157,15 @@ def _params(p, cols: int, like: torch.Tensor, what: str):
 
 
 # ------------------------------------------------------------------- codec
-def q8_compress(x: torch.Tensor, flat: bool = False) -> Checkpoint8:
+def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) -> Checkpoint8:
     """The checkpoint of ``x``.  ``flat`` (contiguous tensors): groups run through the whole tensor instead of
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
-    is the same either way, and only such a flat checkpoint has rows for the backward passes."""
+    is the same either way, and only such a flat checkpoint has rows for the backward passes.  ``keep_sign``: what is
+    not 0 but rounds to 0 is held as the smallest value with its sign."""
     kind = _need(x, "q8_compress")
     if _elsewhere(x.device):
         with torch.cuda.device(x.device):
-            return q8_compress(x, flat)
+            return q8_compress(x, flat, keep_sign)
     stride = _row_stride(x, "q8_compress")
     rows, cols = _rows_cols(x.shape)
     if cols == 0:
@@ -169,7 +175,7 @@ def q8_compress(x: torch.Tensor, flat: bool = False) -> Checkpoint8:
     if flat and rows and cols % GROUP:
         rows, cols = 1, rows * cols
     held = Checkpoint8._empty(x, rows, cols)
-    check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, held._at, held._scales_at, api._stream()),
+    check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, keep_sign, held._at, held._scales_at, api._stream()),
           "cswap_q8_pack")
     return held
 
@@ -204,19 +210,24 @@ def _kind_of(kind: str) -> int:
     return KINDS[kind]
 
 
-def q8_act(x: torch.Tensor, kind: str = "gelu"):
-    """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu"."""
+def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
+    """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu".  The second is None with
+    ``checkpoint=False``."""
     k, dtype = _kind_of(kind), _need(x, "q8_act")
     if _elsewhere(x.device):
         with torch.cuda.device(x.device):
-            return q8_act(x, kind)
+            return q8_act(x, kind, checkpoint)
     stride = _row_stride(x, "q8_act")
     rows, cols = _rows_cols(x.shape)
     if cols == 0:
         raise ValueError("q8_act: rows without values")
     y = _like(x, stride)
-    held = Checkpoint8._empty(x, rows, cols)
-    check(lib().cswap_q8_act_forward(k, x.data_ptr(), dtype, rows, cols, stride, y.data_ptr(), 0, held._at, held._scales_at,
+    if checkpoint:
+        held = Checkpoint8._empty(x, rows, cols)
+        codes, scales = held._at, held._scales_at
+    else:
+        held, codes, scales = None, 0, 0
+    check(lib().cswap_q8_act_forward(k, x.data_ptr(), dtype, rows, cols, stride, y.data_ptr(), 0, codes, scales,
                                      api._stream()), "cswap_q8_act_forward")
     return y, held
 

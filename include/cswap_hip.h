@@ -272,14 +272,16 @@ int cswap_zvc_compress_fused_static(const float* d_in, int n, int process, int* 
 typedef enum { CSWAP_DT_F32 = 0, CSWAP_DT_BF16 = 1, CSWAP_DT_F16 = 2 } cswap_dtype;
 size_t cswap_q8_code_pitch(size_t cols);  /* cols rounded up to a multiple of 32 */
 size_t cswap_q8_scale_pitch(size_t cols); /* groups of a row */
-int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride,
+/* keep_sign: a value that is not 0 but rounds to 0 is held as 2^e with its sign, so that what asks
+ * only for the sign (a ReLU's backward pass) loses nothing; it is then off by less than 2^e. */
+int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride, int keep_sign,
                   int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
 /* Rounds once where `dtype` does not hold q * 2^e. */
 int cswap_q8_unpack(const int8_t* d_codes, const uint8_t* d_scales, size_t rows, size_t cols,
                     void* d_out, int dtype, ptrdiff_t stride, cswap_stream_t stream);
 
-/* y = f(x) and the checkpoint of x in one pass; dx = dy f'(x^) from the checkpoint x^.
- * f in fp32 whatever the type: x Phi(x), its tanh form, x / (1 + exp(-x)).  y is 0 where x is
+/* y = f(x) and, where d_codes and d_scales are given, the checkpoint of x in one pass;
+ * dx = dy f'(x^) from the checkpoint x^.  f in fp32 whatever the type: x Phi(x), its tanh form, x / (1 + exp(-x)).  y is 0 where x is
  * minus infinity. */
 typedef enum { CSWAP_ACT_GELU = 0, CSWAP_ACT_GELU_TANH = 1, CSWAP_ACT_SILU = 2 } cswap_act;
 int cswap_q8_act_forward(int kind, const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
@@ -293,9 +295,9 @@ int cswap_q8_act_backward(int kind, const void* d_dy, int dtype, size_t rows, si
  * beta (param_dtype) may be NULL; the checkpoint of x is made where d_codes and d_scales are
  * given.  Backward takes x either as it is (d_x, d_codes = d_scales = NULL) or as its checkpoint
  * (d_x = NULL), with the mean and rstd of the forward pass; d_dgamma and d_dbeta (param_dtype)
- * may be NULL, and where neither is wanted so may d_ws.  Their sums over rows are made in fp32 in
- * a fixed order: the same call gives the same bits.  d_ws: cswap_layer_norm_workspace_bytes,
- * 4-byte aligned, with no preparation; calls that overlap must not share one. */
+ * may be NULL, and where neither is wanted or cswap_layer_norm_workspace_bytes is 0 (few rows) so
+ * may d_ws.  Their sums over rows are made in fp32 in a fixed order: the same call gives the same
+ * bits.  d_ws: 4-byte aligned, no preparation; calls that overlap must not share one. */
 int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
                              const void* d_gamma, const void* d_beta, int param_dtype, float eps,
                              void* d_y, ptrdiff_t y_stride, float* d_mean, float* d_rstd,
@@ -311,7 +313,8 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
  * (rows x k): dw[n][k] = sum over rows of dy[.][n] x^[.][k], db[n] = sum over rows of dy[.][n]
  * (NULL: not wanted), in out_dtype, contiguous.  Products are exact for fp32 and bf16 dy and
  * summed in fp32, in a fixed order; for fp16 dy x^ is rounded to fp16, which changes nothing if
- * the checkpoint was made from fp16.  rows = 0 gives zeros.  n and k up to 2^20.  d_ws:
+ * the checkpoint was made from fp16.  A NaN or an infinity in an fp32 dy gives NaN.  rows = 0
+ * gives zeros.  n and k up to 2^20, dy_stride up to 2^24 (CSWAP_E_UNSUPPORTED beyond).  d_ws:
  * cswap_q8_weight_grad_workspace_bytes, 16-byte aligned, with no preparation; calls that overlap
  * must not share one. */
 size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k);

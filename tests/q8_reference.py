@@ -19,7 +19,7 @@ def power_of_two(e):
     return ((e.long() + 1023) << 52).view(torch.float64)
 
 
-def pack(x):
+def pack(x, keep_sign=False):
     """codes (rows x pitch, int8), scales (rows x groups, uint8) of a 2-D tensor of any type."""
     x = x.detach().cpu().double()
     rows, cols = x.shape
@@ -33,6 +33,8 @@ def pack(x):
     zero = g.abs().amax(dim=2, keepdim=True) == 0
     e = torch.where(zero, torch.full_like(ex, -126), (ex - 7).clamp(-126, 121))
     q = torch.round(g * power_of_two(-e)).clamp(-127, 127)
+    if keep_sign:
+        q = torch.where(q == 0, torch.sign(g), q)
     scales = torch.where(finite, e + 127, torch.full_like(e, 255)).to(torch.uint8)
     return q.to(torch.int8).view(rows, -1), scales.view(rows, groups)
 
@@ -45,8 +47,8 @@ def unpack(codes, scales, cols):
     return (codes.view(*scales.shape, GROUP) * unit.unsqueeze(2)).view(codes.shape)[:, :cols]
 
 
-def held(x):
-    return unpack(*pack(x), x.shape[1])
+def held(x, keep_sign=False):
+    return unpack(*pack(x, keep_sign), x.shape[1])
 
 
 # ---------------------------------------------------------------- activation functions: value, slope

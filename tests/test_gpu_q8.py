@@ -78,6 +78,23 @@ def test_codec_of_rows_with_gaps_and_odd_starts(dtype):
     assert bool((big[:, :3] == 5).all()) and bool((big[:, 133:] == 5).all())         # what lies between rows is left alone
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_signs_that_are_kept(dtype):
+    """What is not 0 has a code that is not 0, with its sign; the other codes are the same."""
+    x = values(50, 130, dtype, 31)
+    x[::3, ::7] = 0.0
+    x[1::3, 1::5] *= 1e-4
+    x[0, 64:96] = torch.finfo(dtype).tiny
+    x[0, 64], x[0, 65] = 1.0, -torch.finfo(dtype).tiny
+    plain, kept = q8().q8_compress(x.cuda()), q8().q8_compress(x.cuda(), keep_sign=True)
+    assert torch.equal(plain.scales, kept.scales)
+    a, b, sign = plain.codes.cpu().int(), kept.codes.cpu().int(), torch.zeros(50, 160, dtype=torch.int32)
+    sign[:, :130] = torch.sign(x.float()).int()
+    assert int((sign[a == 0] != 0).sum()) > 100
+    assert torch.equal(b, torch.where(a == 0, sign, a))
+    assert torch.equal(torch.sign(q8().q8_decompress(kept).float()).cpu(), torch.sign(x.float()))
+
+
 def test_flat_checkpoints():
     x = values(6, 4 * 5, F32).view(6, 4, 5)
     held = q8().q8_compress(x.cuda(), flat=True)

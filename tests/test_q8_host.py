@@ -18,26 +18,27 @@ def test_sizes():
         assert L().cswap_q8_code_pitch(cols) == pitch and L().cswap_q8_scale_pitch(cols) == groups
     assert L().cswap_layer_norm_workspace_bytes(0, 100) == 0
     assert L().cswap_layer_norm_workspace_bytes(10, 16385) == 0
-    assert L().cswap_layer_norm_workspace_bytes(1, 100) >= 2 * 4 * 100
+    assert L().cswap_layer_norm_workspace_bytes(1, 100) == 0            # one workgroup takes all rows
+    assert L().cswap_layer_norm_workspace_bytes(100000, 100) >= 2 * 2 * 4 * 100
     assert L().cswap_q8_weight_grad_workspace_bytes(1, 10, 0, 5) == 0
 
 
 def test_codec_refuses():
     pack, unpack = L().cswap_q8_pack, L().cswap_q8_unpack
-    assert pack(None, 0, 4, 32, 0, A, A, None) == ARG
-    assert pack(A, 0, 4, 32, 0, None, A, None) == ARG
-    assert pack(A, 0, 4, 32, 0, A, None, None) == ARG
-    assert pack(A, 0, 4, 32, 0, A + 4, A, None) == ARG          # codes are 8-byte aligned
-    assert pack(A + 2, 0, 4, 32, 0, A, A, None) == ARG          # fp32 values 4-byte aligned
-    assert pack(A + 1, 1, 4, 32, 0, A, A, None) == ARG
-    assert pack(A, 3, 4, 32, 0, A, A, None) == ARG
-    assert pack(A, 0, 4, 0, 0, A, A, None) == ARG
-    assert pack(A, 0, 4, 32, 31, A, A, None) == ARG             # rows overlap
-    assert pack(A, 0, 4, 32, -32, A, A, None) == ARG
-    assert pack(A, 0, 1 << 40, 32, 0, A, A, None) == UNSUPPORTED
-    assert pack(A, 0, 1, 1 << 40, 0, A, A, None) == UNSUPPORTED
-    assert pack(A, 0, 1 << 29, 32, 0, A, A, None) == UNSUPPORTED  # 2^31 pieces
-    assert pack(None, 0, 0, 32, 0, None, None, None) == 0
+    assert pack(None, 0, 4, 32, 0, 0, A, A, None) == ARG
+    assert pack(A, 0, 4, 32, 0, 0, None, A, None) == ARG
+    assert pack(A, 0, 4, 32, 0, 0, A, None, None) == ARG
+    assert pack(A, 0, 4, 32, 0, 0, A + 4, A, None) == ARG          # codes are 8-byte aligned
+    assert pack(A + 2, 0, 4, 32, 0, 0, A, A, None) == ARG          # fp32 values 4-byte aligned
+    assert pack(A + 1, 1, 4, 32, 0, 0, A, A, None) == ARG
+    assert pack(A, 3, 4, 32, 0, 0, A, A, None) == ARG
+    assert pack(A, 0, 4, 0, 0, 0, A, A, None) == ARG
+    assert pack(A, 0, 4, 32, 31, 0, A, A, None) == ARG             # rows overlap
+    assert pack(A, 0, 4, 32, -32, 0, A, A, None) == ARG
+    assert pack(A, 0, 1 << 40, 32, 0, 0, A, A, None) == UNSUPPORTED
+    assert pack(A, 0, 1, 1 << 40, 0, 0, A, A, None) == UNSUPPORTED
+    assert pack(A, 0, 1 << 29, 32, 0, 0, A, A, None) == UNSUPPORTED  # 2^31 pieces
+    assert pack(None, 0, 0, 32, 0, 0, None, None, None) == 0
     assert unpack(None, A, 4, 32, A, 0, 0, None) == ARG
     assert unpack(A, A, 4, 32, None, 0, 0, None) == ARG
     assert unpack(A, A, 4, 32, A, 7, 0, None) == ARG
@@ -50,6 +51,8 @@ def test_activations_refuse():
     assert fwd(-1, A, 0, 4, 32, 0, A, 0, A, A, None) == ARG
     assert fwd(0, A, 0, 4, 32, 0, None, 0, A, A, None) == ARG
     assert fwd(0, A, 0, 4, 32, 0, A, 8, A, A, None) == ARG
+    assert fwd(0, A, 0, 4, 32, 0, A, 0, A, None, None) == ARG   # codes and scales, or neither
+    assert fwd(0, A, 0, 4, 32, 0, A, 0, None, A, None) == ARG
     assert fwd(0, None, 0, 0, 32, 0, None, 0, None, None, None) == 0
     assert bwd(0, A, 0, 4, 32, 0, None, A, A, 0, None) == ARG
     assert bwd(5, A, 0, 4, 32, 0, A, A, A, 0, None) == ARG
@@ -71,8 +74,8 @@ def test_layer_norm_refuses():
     assert f(_13=None) == ARG and f(_14=None) == ARG and f(_5=A + 1) == ARG
     assert f(_3=16385) == UNSUPPORTED
     assert f(_2=0, _0=None) == 0
-    room = L().cswap_layer_norm_workspace_bytes(4, 32)
-    good = [A, 0, 4, 32, 0, None, 0, A, A, A, A, A, 0, A, 0, A, A, A, room, None]
+    room = L().cswap_layer_norm_workspace_bytes(4000, 32)
+    good = [A, 0, 4000, 32, 0, None, 0, A, A, A, A, A, 0, A, 0, A, A, A, room, None]
 
     def b(**kw):
         a = list(good)
