@@ -172,24 +172,6 @@ template <typename T, bool HELD> struct RowChunk {
   uint32_t scale;
 };
 
-template <typename T> __device__ inline void load_raw(const typename T::value* p, int valid, u4_any raw[T::bytes / 2])
-{
-  constexpr int W = T::bytes / 2;
-  if (valid >= kChunk) {
-#pragma unroll
-    for (int h = 0; h < W; ++h) raw[h] = reinterpret_cast<const u4_any*>(p)[h];
-  } else {
-#pragma unroll
-    for (int h = 0; h < W; ++h) raw[h] = (u4_any){0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < kChunk - 1; ++e)
-      if (e < valid) {
-        if constexpr (T::bytes == 4) raw[e / 4][e % 4] = __float_as_uint(p[e]);
-        else raw[0][e / 2] |= (uint32_t)p[e] << (16 * (e & 1));
-      }
-  }
-}
-
 template <typename T> __device__ inline void widen(const u4_any raw[T::bytes / 2], float v[8])
 {
 #pragma unroll

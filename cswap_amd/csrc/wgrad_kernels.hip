@@ -124,12 +124,13 @@ __device__ inline global_bytes uniform(const char* p)
   return (global_bytes)((uint64_t)hi << 32 | lo);
 }
 
+__device__ char spare[1024 + 16];  // 256 columns of fp32, and 16 bytes from the last of them on
+
 template <typename T, int TN, int TK, int BK, int WK>
 __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
                                                              const int8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, GradShape s,
-                                                             void* __restrict__ dw, void* __restrict__ db, int out_dtype,
-                                                             const char* __restrict__ spare)
+                                                             void* __restrict__ dw, void* __restrict__ db, int out_dtype)
 {
   typedef GradTile<T, TN, TK, BK> Tile;
   typedef typename Feed<T>::type M;
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
 
   // A stage is plain if all of its loads are in the tensors: columns behind a row's last one read what lies there, which goes
   // into columns of the product that nobody stores.  Rows that are not there have to be zeros in both operands; the stages from
-  // the first one that is not plain on (the last rows of the tensors) are brought in value by value.
+  // the first one that is not plain on (the last rows of the tensors) are loaded chunk by chunk as far as they are there.
   const size_t dy_end = (size_t)(s.rows - 1) * s.dy_stride + s.n;
   uint32_t plain = stages;
   while (plain > 0) {
@@ -160,8 +161,8 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
       break;
     --plain;
   }
-  // The loop asks for a plain stage in every turn, the last one again where there is no other; without any it reads the spare
-  // room at the workspace's start, and what it reads is not used.
+  // The loop asks for a plain stage in every turn, the last one again where there is no other; without any it reads
+  // a spare array, and what it reads is not used.
   const size_t dy_stride = plain ? s.dy_stride : 0, code_pitch = plain ? s.code_pitch : 0, scale_pitch = plain ? s.scale_pitch : 0;
   const char* const dy_from = plain ? reinterpret_cast<const char*>(dy + (size_t)from * s.dy_stride + n0) : spare;
   const char* const codes_from = plain ? reinterpret_cast<const char*>(codes) + (size_t)from * s.code_pitch + k0 : spare;
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
   };
 
   // db: the columns of dY, each stage's added up by one of the workgroups that have them
-  float b_sum[8] = {}, b_edge = 0.0f;
+  float b_sum[8] = {};
   auto add_columns = [&] {
 #pragma unroll
     for (int i = 0; i < kALoads; ++i)
@@ -219,42 +220,23 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
                                   : to_float<T>((V)(uint16_t)(a_raw[i][0][e / 2] >> (16 * (e & 1))));
   };
 
-  // Loads are at clamped places, so that several of them are in flight without a branch; what is not there becomes 0.
-  constexpr int kAhead = P == 3 ? 4 : 8;
-  auto stage_by_value = [&](uint16_t* buf, uint32_t m0, bool mine) {
-    const uint32_t m_last = to - 1 - m0;
-    {
-      const int c = tid % TN;
-      const bool there = n0 + c < s.n;
-      const V* p = dy + (size_t)m0 * s.dy_stride + (there ? n0 + c : s.n - 1);
-#pragma unroll kAhead
-      for (int j = 0; j < BK * TN / NT; ++j) {
-        const uint32_t m = tid / TN + j * (NT / TN);
-        V raw = p[(size_t)min(m, m_last) * s.dy_stride];
-        if (!there || m > m_last) raw = 0;
-        if (mine) b_edge += to_float<T>(raw);
-        uint16_t* at = buf + Tile::a_at(m, c);
-        if constexpr (P == 3) {
-          const uint32_t a0 = __float_as_uint(raw) & 0xffff0000u;
-          const float r = raw - __uint_as_float(a0);
-          const uint32_t a1 = __float_as_uint(r) & 0xffff0000u;
-          at[0] = (uint16_t)(a0 >> 16), at[Tile::kAPlane] = (uint16_t)(a1 >> 16);
-          at[2 * Tile::kAPlane] = (uint16_t)(__float_as_uint(r - __uint_as_float(a1)) >> 16);
-        } else {
-          at[0] = raw;
-        }
-      }
+  // A stage that is not plain: every chunk that is there, and zeros.
+  auto load_guarded = [&](uint32_t m0) {
+    const uint32_t a_col = n0 + 8 * a_chunk, b_col = k0 + 16 * b_piece;
+    const int valid = a_col + 8 <= s.n ? 8 : a_col < s.n ? (int)(s.n - a_col) : 0;
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) {
+      const uint32_t m = m0 + a_row + i * kARows;
+      load_raw<T>(dy + (size_t)m * s.dy_stride + a_col, m < to ? valid : 0, a_raw[i]);
     }
-    const int c = tid % TK;
-    const bool there = k0 + c < s.k;
-    const uint32_t k = there ? k0 + c : s.k - 1;
-    const int8_t* p = codes + (size_t)m0 * s.code_pitch + k;
-    const uint8_t* q = scales + (size_t)m0 * s.scale_pitch + k / kGroup;
-#pragma unroll kAhead
-    for (int j = 0; j < BK * TK / NT; ++j) {
-      const uint32_t m = tid / TK + j * (NT / TK), mc = min(m, m_last);
-      const float v = (float)p[(size_t)mc * s.code_pitch] * unit_of(q[(size_t)mc * s.scale_pitch]);
-      buf[Tile::b_at(m, c)] = from_float<M>(there && m <= m_last ? v : 0.0f);
+#pragma unroll
+    for (int i = 0; i < kBLoads; ++i) {
+      const uint32_t m = m0 + b_row + i * kBRows;
+      b_raw[i] = (u4_any){0, 0, 0, 0}, b_scale[i] = 1;
+      if (m < to && b_col < s.code_pitch) {
+        b_raw[i] = *reinterpret_cast<const u4_any*>(codes + (size_t)m * s.code_pitch + b_col);
+        b_scale[i] = scales[(size_t)m * s.scale_pitch + b_col / kGroup];
+      }
     }
   };
 
@@ -288,15 +270,17 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
   auto my_turn = [&](uint32_t st) { return db && (out_dtype < 0 ? st % s.tiles_k == tk : tk == 0); };
   const uint32_t last = plain ? plain - 1 : 0;
 
-  if (plain) {
-    load(0);
+  auto store = [&](uint16_t* buf) {
+#pragma unroll
+    for (int i = 0; i < kALoads; ++i) store_a(buf, i);
+#pragma unroll
+    for (int i = 0; i < kBLoads; ++i) store_b(buf, i);
+  };
+  if (stages) {
+    if (plain) load(0);
+    else load_guarded(from);
     if (my_turn(0)) add_columns();
-#pragma unroll
-    for (int i = 0; i < kALoads; ++i) store_a(lds[0], i);
-#pragma unroll
-    for (int i = 0; i < kBLoads; ++i) store_b(lds[0], i);
-  } else if (stages) {
-    stage_by_value(lds[0], from, my_turn(0));
+    store(lds[0]);
   }
   load(min(1u, last));
   __syncthreads();
@@ -333,8 +317,10 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
         read_a(buf, c + 1, P - 1, a[at ^ 1]);
       } else {
         if (st + 1 < stages && st + 1 >= plain) {
+          load_guarded(from + (st + 1) * BK);
+          if (my_turn(st + 1)) add_columns();
           __syncthreads();  // the turn has left something there
-          stage_by_value(next, from + (st + 1) * BK, my_turn(st + 1));
+          store(next);
         }
         __syncthreads();
         read_b(next, 0, b[0]);
@@ -372,16 +358,15 @@ __global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename
   else
     leave(F16(), dw);
   if (db && (out_dtype < 0 || tk == 0)) {
-    float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows + NT / TN][TN]
-    static_assert(sizeof(lds) >= sizeof(float) * (kARows + NT / TN) * TN, "room for the columns' sums");
+    float* sums = reinterpret_cast<float*>(lds[0]);                 // [kARows][TN]
+    static_assert(sizeof(lds) >= sizeof(float) * kARows * TN, "room for the columns' sums");
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[a_row * TN + 8 * a_chunk + e] = b_sum[e];
-    sums[kARows * TN + tid] = b_edge;
     __syncthreads();
     if (tid < TN && n0 + tid < s.n) {
       float v = 0.0f;
-      for (int r = 0; r < kARows + NT / TN; ++r) v += sums[r * TN + tid];
+      for (int r = 0; r < kARows; ++r) v += sums[r * TN + tid];
       const uint32_t n = n0 + tid;
       if (out_dtype < 0)
         static_cast<float*>(db)[(size_t)(split * s.tiles_k + tk) * s.n + n] = v;
@@ -448,7 +433,6 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
 constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
 constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 16 rows are 32 bits
 
-constexpr size_t kSpareBytes = 1024 + 64;           // 256 columns of fp32, and 16 bytes from the last of them on
 
 struct GradPlan {
   bool large;  // 256 x 256 tiles, else 128 x 128
@@ -494,6 +478,12 @@ static GradPlan grad_plan(int dtype, size_t rows, size_t n, size_t k)
 
 static size_t bias_parts(const GradPlan& p) { return (size_t)p.splits * p.tiles_k; }
 
+// Sums of the splits; none where the tiles leave as results.
+static size_t grad_room(const GradPlan& p, size_t n, size_t k)
+{
+  return p.splits == 1 ? 0 : ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float);
+}
+
 }  // namespace q8
 }  // namespace cswap
 
@@ -505,8 +495,7 @@ static bool grad_sizes(size_t rows, size_t n, size_t k) { return n && k && n <= 
 extern "C" size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k)
 {
   if (!dtype_known(dtype) || !grad_sizes(rows, n, k)) return 0;
-  const GradPlan p = grad_plan(dtype, rows, n, k);
-  return kSpareBytes + (p.splits == 1 ? 0 : ((size_t)p.splits * n * k + bias_parts(p) * n) * sizeof(float));
+  return grad_room(grad_plan(dtype, rows, n, k), n, k);
 }
 
 extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride, const int8_t* d_codes,
@@ -520,13 +509,14 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   if (!grad_sizes(rows, n, k) || (size_t)dy_stride > kMaxGradStride) return CSWAP_E_UNSUPPORTED;
   if (!value_ptr(d_dw, out_dtype) || (d_db && !value_ptr(d_db, out_dtype))) return CSWAP_E_ARG;
   if (rows && (!value_ptr(d_dy, dtype) || !checkpoint_ptrs(d_codes, d_scales))) return CSWAP_E_ARG;
-  if (!value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
-  if (ws_bytes < cswap_q8_weight_grad_workspace_bytes(dtype, rows, n, k)) return CSWAP_E_NOMEM;
   const GradPlan p = grad_plan(dtype, rows, n, k);
+  const size_t room = grad_room(p, n, k);
+  if (room && !value_ptr(d_ws, CSWAP_DT_F32)) return CSWAP_E_ARG;
+  if (ws_bytes < room) return CSWAP_E_NOMEM;
   const GradShape s = {(uint32_t)rows, (uint32_t)n, (uint32_t)k, (uint32_t)groups_of(k), p.step_rows, p.tiles_n, p.tiles_k,
                        (size_t)dy_stride, pitch_of(k)};
   const bool direct = p.splits == 1;
-  float* part = reinterpret_cast<float*>(static_cast<char*>(d_ws) + kSpareBytes);
+  float* part = static_cast<float*>(d_ws);
   float* part_b = part + (size_t)p.splits * n * k;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
@@ -535,7 +525,7 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
     auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, 2>;
     hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 256), 0, st,
                        static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part, !d_db ? nullptr : direct ? d_db : part_b,
-                       direct ? out_dtype : -1, static_cast<const char*>(d_ws));
+                       direct ? out_dtype : -1);
     return check_launch();
   };
   if (int e = dtype == CSWAP_DT_F32 ? launch(F32()) : dtype == CSWAP_DT_BF16 ? launch(BF16()) : launch(F16())) return e;

@@ -37,12 +37,13 @@ class Checkpoint8:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype):
         rows, cols = _rows_cols(shape)
-        if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+        if codes.dtype is not torch.int8 or scales.dtype is not torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
             raise ValueError("expected codes as a 2-D int8 tensor and scales as a 2-D uint8 tensor")
-        if codes.shape[0] != rows and codes.shape[0] == 1:
+        held, pitch = codes.shape
+        if held != rows and held == 1:
             rows, cols = 1, rows * cols
         groups = -(-cols // GROUP)
-        if codes.shape != (rows, groups * GROUP) or scales.shape != (rows, groups):
+        if held != rows or pitch != groups * GROUP or scales.shape != (rows, groups):
             raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold a tensor of shape "
                              f"{tuple(shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device):
@@ -107,10 +108,13 @@ def _rows_cols(shape):
     return (math.prod(shape[:-1]), shape[-1]) if n else (1, 1)
 
 
-def _elsewhere(device: torch.device) -> bool:
-    """Whether another device is the current one: the call is then made again with its tensor's device current, whose
-    stream is the one to launch on."""
-    return device.index != torch.cuda.current_device()
+def _stream_of(device: torch.device):
+    """The current stream of the current device, if that is ``device``; else None: the call is then made again with
+    its tensor's device current, whose stream is the one to launch on."""
+    index = torch.cuda.current_device()
+    if device.index != index:
+        return None
+    return api._raw_stream(index) if api._raw_stream is not None else api._stream()
 
 
 def _need(t: torch.Tensor, what: str) -> int:
@@ -145,12 +149,13 @@ def _like(t: torch.Tensor, stride: int) -> torch.Tensor:
     return torch.empty_like(t) if stride == 0 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _params(p, cols: int, like: torch.Tensor, what: str):
+def _param(p, cols: int, device: torch.device, what: str):
+    """Address and type of a parameter (0 and None: there is none)."""
     if p is None:
         return 0, None
-    kind = _need(p, what)
-    if p.device != like.device:
-        raise ValueError(f"{what}: on {p.device}, not on {like.device}")
+    kind = _DTYPE.get(p.dtype)
+    if kind is None or p.device != device:
+        raise TypeError(f"{what}: a float32, bfloat16 or float16 tensor on {device}, not {p.dtype} on {p.device}")
     if p.numel() != cols or not p.is_contiguous():
         raise ValueError(f"{what}: expected {cols} contiguous values")
     return p.data_ptr(), kind
@@ -162,9 +167,10 @@ def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) ->
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
     is the same either way, and only such a flat checkpoint has rows for the backward passes.  ``keep_sign``: what is
     not 0 but rounds to 0 is held as the smallest value with its sign."""
-    kind = _need(x, "q8_compress")
-    if _elsewhere(x.device):
-        with torch.cuda.device(x.device):
+    kind, device = _need(x, "q8_compress"), x.device
+    stream = _stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
             return q8_compress(x, flat, keep_sign)
     stride = _row_stride(x, "q8_compress")
     rows, cols = _rows_cols(x.shape)
@@ -175,31 +181,33 @@ def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) ->
     if flat and rows and cols % GROUP:
         rows, cols = 1, rows * cols
     held = Checkpoint8._empty(x, rows, cols)
-    check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, keep_sign, held._at, held._scales_at, api._stream()),
+    check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, keep_sign, held._at, held._scales_at, stream),
           "cswap_q8_pack")
     return held
 
 
 def q8_decompress(held: Checkpoint8, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """What ``held`` stands for, in its own type or in ``dtype`` (rounded once where that does not hold it)."""
-    if held.device.type != "cuda":
+    device = held.device
+    if device.type != "cuda":
         raise ValueError("q8_decompress: expected a checkpoint in device memory")
-    if _elsewhere(held.device):
-        with torch.cuda.device(held.device):
+    stream = _stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
             return q8_decompress(held, out, dtype)
     if out is None:
-        out = torch.empty(held.shape, dtype=dtype or held.dtype, device=held.device)
+        out = torch.empty(held.shape, dtype=dtype or held.dtype, device=device)
         stride = 0
     else:
         if out.shape != torch.Size(held.shape) or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"q8_decompress: out is {tuple(out.shape)} {out.dtype}")
-        if out.device != held.device:
-            raise ValueError(f"q8_decompress: out on {out.device}, not on {held.device}")
+        if out.device != device:
+            raise ValueError(f"q8_decompress: out on {out.device}, not on {device}")
         stride = _row_stride(out, "q8_decompress")
         if stride and held.rows != _rows_cols(held.shape)[0]:
             raise ValueError("q8_decompress: a flat checkpoint goes into a contiguous tensor")
     check(lib().cswap_q8_unpack(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), _need(out, "q8_decompress"),
-                                stride, api._stream()), "cswap_q8_unpack")
+                                stride, stream), "cswap_q8_unpack")
     return out
 
 
@@ -214,7 +222,8 @@ def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
     """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu".  The second is None with
     ``checkpoint=False``."""
     k, dtype = _kind_of(kind), _need(x, "q8_act")
-    if _elsewhere(x.device):
+    stream = _stream_of(x.device)
+    if stream is None:
         with torch.cuda.device(x.device):
             return q8_act(x, kind, checkpoint)
     stride = _row_stride(x, "q8_act")
@@ -228,17 +237,17 @@ def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
     else:
         held, codes, scales = None, 0, 0
     check(lib().cswap_q8_act_forward(k, x.data_ptr(), dtype, rows, cols, stride, y.data_ptr(), 0, codes, scales,
-                                     api._stream()), "cswap_q8_act_forward")
+                                     stream), "cswap_q8_act_forward")
     return y, held
 
 
 def _need_gradient(dy: torch.Tensor, held, what: str):
     """dy's type and row stride; it goes with an input of held's shape and type."""
-    kind = _need(dy, f"{what}: dy")
-    if dy.shape != torch.Size(held.shape) or dy.dtype != held.dtype or dy.device != held.device:
+    kind = _need(dy, what)
+    if tuple(dy.shape) != tuple(held.shape) or dy.dtype != held.dtype or dy.device != held.device:
         raise ValueError(f"{what}: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, the input was {tuple(held.shape)} "
                          f"{held.dtype} on {held.device}")
-    return kind, _row_stride(dy, f"{what}: dy")
+    return kind, _row_stride(dy, what)
 
 
 def _need_rows(held: Checkpoint8, what: str):
@@ -253,13 +262,14 @@ def q8_act_backward(dy: torch.Tensor, held: Checkpoint8, kind: str = "gelu") -> 
     """``dy * f'(x)``, x as ``held`` has it."""
     k = _kind_of(kind)
     dtype, stride = _need_gradient(dy, held, "q8_act_backward")
-    if _elsewhere(dy.device):
+    stream = _stream_of(dy.device)
+    if stream is None:
         with torch.cuda.device(dy.device):
             return q8_act_backward(dy, held, kind)
     rows, cols = _need_rows(held, "q8_act_backward")
     dx = _like(dy, stride)
     check(lib().cswap_q8_act_backward(k, dy.data_ptr(), dtype, rows, cols, stride, held._at, held._scales_at, dx.data_ptr(), 0,
-                                      api._stream()), "cswap_q8_act_backward")
+                                      stream), "cswap_q8_act_backward")
     return dx
 
 
@@ -268,27 +278,29 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
                checkpoint: bool = True):
     """``(y, mean, rstd, held)``: layer norm over the last dimension, the rows' statistics in fp32, and what the
     backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``."""
-    dtype = _need(x, "layer_norm")
-    if _elsewhere(x.device):
-        with torch.cuda.device(x.device):
+    dtype, device = _need(x, "layer_norm"), x.device
+    stream = _stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
             return layer_norm(x, weight, bias, eps, checkpoint)
     stride = _row_stride(x, "layer_norm")
     rows, cols = _rows_cols(x.shape)
     if cols == 0 or x.dim() == 0:
         raise ValueError("layer_norm: rows without values")
-    w, wk = _params(weight, cols, x, "layer_norm: weight")
-    b, bk = _params(bias, cols, x, "layer_norm: bias")
+    w, wk = _param(weight, cols, device, "layer_norm: weight")
+    b, bk = _param(bias, cols, device, "layer_norm: bias")
     if wk is not None and bk is not None and wk != bk:
         raise TypeError("layer_norm: weight and bias have one type")
     y = _like(x, stride)
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
+    mean = torch.empty(rows, dtype=torch.float32, device=device)
+    rstd = torch.empty_like(mean)
     if checkpoint:
         held = Checkpoint8._empty(x, rows, cols)
         codes, scales = held._at, held._scales_at
     else:
         held, codes, scales = x, 0, 0
     check(lib().cswap_layer_norm_forward(x.data_ptr(), dtype, rows, cols, stride, w, b, wk or bk or 0, eps, y.data_ptr(), 0,
-                                         mean.data_ptr(), rstd.data_ptr(), codes, scales, api._stream()),
+                                         mean.data_ptr(), rstd.data_ptr(), codes, scales, stream),
           "cswap_layer_norm_forward")
     return y, mean, rstd, held
 
@@ -298,8 +310,10 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
     """``(dx, dweight, dbias)``; ``held`` is what ``layer_norm`` returned last.  The parameters' gradients come in
     ``param_dtype`` (the weight's type, else dy's)."""
     dtype, stride = _need_gradient(dy, held, "layer_norm_backward")
-    if _elsewhere(dy.device):
-        with torch.cuda.device(dy.device):
+    device = dy.device
+    stream = _stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
             return layer_norm_backward(dy, held, mean, rstd, weight, param_dtype)
     if isinstance(held, Checkpoint8):
         rows, cols = _need_rows(held, "layer_norm_backward")
@@ -308,9 +322,9 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
         rows, cols = _rows_cols(held.shape)
         x, x_stride, codes, scales = held.data_ptr(), _row_stride(held, "layer_norm_backward: x"), 0, 0
     for s in (mean, rstd):
-        if s.dtype != torch.float32 or s.numel() != rows or not s.is_contiguous() or s.device != dy.device:
-            raise ValueError(f"layer_norm_backward: mean and rstd are {rows} contiguous fp32 values on {dy.device}")
-    w, wk = _params(weight, cols, dy, "layer_norm_backward: weight")
+        if s.dtype is not torch.float32 or s.numel() != rows or not s.is_contiguous() or s.device != device:
+            raise ValueError(f"layer_norm_backward: mean and rstd are {rows} contiguous fp32 values on {device}")
+    w, wk = _param(weight, cols, device, "layer_norm_backward: weight")
     if wk is not None and param_dtype not in (None, weight.dtype):
         raise TypeError(f"layer_norm_backward: param_dtype {param_dtype}, the weight has {weight.dtype}")
     param_dtype = param_dtype or (dy.dtype if weight is None else weight.dtype)
@@ -318,12 +332,13 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
     if pk is None:
         raise TypeError(f"layer_norm_backward: param_dtype {param_dtype}")
     dx = _like(dy, stride)
-    dw, db = torch.empty((2, cols), dtype=param_dtype, device=dy.device).unbind()
+    dw = torch.empty(cols, dtype=param_dtype, device=device)
+    db = torch.empty_like(dw)
     room = lib().cswap_layer_norm_workspace_bytes(rows, cols)
-    ws = torch.empty(room, dtype=torch.uint8, device=dy.device)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
     check(lib().cswap_layer_norm_backward(dy.data_ptr(), dtype, rows, cols, stride, x, x_stride, codes, scales, mean.data_ptr(),
                                           rstd.data_ptr(), w, pk, dx.data_ptr(), 0, dw.data_ptr(), db.data_ptr(),
-                                          ws.data_ptr(), room, api._stream()), "cswap_layer_norm_backward")
+                                          ws.data_ptr() if room else 0, room, stream), "cswap_layer_norm_backward")
     return dx, dw, db
 
 
@@ -331,14 +346,15 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
 def q8_weight_grad(dy: torch.Tensor, held: Checkpoint8, bias: bool = True, out_dtype: torch.dtype | None = None):
     """``(dW, db)`` of ``y = x @ W.T + b`` from ``dy`` and the checkpoint of ``x``: ``dy.T @ x`` and ``dy.sum(0)`` over
     all rows, in ``out_dtype`` (dy's type); ``db`` is None without ``bias``."""
-    kind = _need(dy, "q8_weight_grad: dy")
-    if dy.device != held.device:
-        raise ValueError(f"q8_weight_grad: dy on {dy.device}, the input's checkpoint on {held.device}")
-    if _elsewhere(dy.device):
-        with torch.cuda.device(dy.device):
+    kind, device = _need(dy, "q8_weight_grad: dy"), dy.device
+    if device != held.device:
+        raise ValueError(f"q8_weight_grad: dy on {device}, the input's checkpoint on {held.device}")
+    stream = _stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
             return q8_weight_grad(dy, held, bias, out_dtype)
     rows, k = _need_rows(held, "q8_weight_grad")
-    if dy.dim() == 0 or dy.shape[:-1] != torch.Size(held.shape[:-1]):
+    if dy.dim() == 0 or tuple(dy.shape[:-1]) != tuple(held.shape[:-1]):
         raise ValueError(f"q8_weight_grad: dy is {tuple(dy.shape)}, the input was {tuple(held.shape)}")
     if dy.dtype == torch.float16 and held.dtype != torch.float16:
         raise TypeError("q8_weight_grad: a float16 dy goes with the checkpoint of a float16 input")
@@ -350,11 +366,11 @@ def q8_weight_grad(dy: torch.Tensor, held: Checkpoint8, bias: bool = True, out_d
     out_kind = _DTYPE.get(out_dtype)
     if out_kind is None:
         raise TypeError(f"q8_weight_grad: out_dtype {out_dtype}")
-    dw = torch.empty((n, k), dtype=out_dtype, device=dy.device)
-    db = torch.empty(n, dtype=out_dtype, device=dy.device) if bias else None
+    dw = torch.empty((n, k), dtype=out_dtype, device=device)
+    db = torch.empty(n, dtype=out_dtype, device=device) if bias else None
     room = lib().cswap_q8_weight_grad_workspace_bytes(kind, rows, n, k)
-    ws = torch.empty(room, dtype=torch.uint8, device=dy.device)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
     check(lib().cswap_q8_weight_grad(dy.data_ptr(), kind, rows, n, stride, held._at, held._scales_at, k, dw.data_ptr(),
-                                     db.data_ptr() if bias else 0, out_kind, ws.data_ptr(), room, api._stream()),
+                                     db.data_ptr() if bias else 0, out_kind, ws.data_ptr() if room else 0, room, stream),
           "cswap_q8_weight_grad")
     return dw, db

@@ -315,8 +315,8 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
  * summed in fp32, in a fixed order; for fp16 dy x^ is rounded to fp16, which changes nothing if
  * the checkpoint was made from fp16.  A NaN or an infinity in an fp32 dy gives NaN.  rows = 0
  * gives zeros.  n and k up to 2^20, dy_stride up to 2^24 (CSWAP_E_UNSUPPORTED beyond).  d_ws:
- * cswap_q8_weight_grad_workspace_bytes, 16-byte aligned, with no preparation; calls that overlap
- * must not share one. */
+ * cswap_q8_weight_grad_workspace_bytes (NULL where that is 0), 4-byte aligned, no preparation;
+ * calls that overlap must not share one. */
 size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k);
 int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptrdiff_t dy_stride,
                          const int8_t* d_codes, const uint8_t* d_scales, size_t k,

@@ -91,8 +91,9 @@ def test_layer_norm_refuses():
 
 
 def test_weight_grad_refuses():
-    room = L().cswap_q8_weight_grad_workspace_bytes(1, 64, 48, 40)
-    good = [A, 1, 64, 48, 0, A, A, 40, A, A, 1, A, room, None]
+    assert L().cswap_q8_weight_grad_workspace_bytes(1, 64, 48, 40) == 0      # results leave from the tiles
+    room = L().cswap_q8_weight_grad_workspace_bytes(1, 20000, 48, 40)
+    good = [A, 1, 20000, 48, 0, A, A, 40, A, A, 1, A, room, None]
 
     def f(**kw):
         a = list(good)
