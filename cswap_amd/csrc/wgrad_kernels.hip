@@ -127,7 +127,7 @@ __device__ inline global_bytes uniform(const char* p)
 __device__ char spare[1024 + 16];  // 256 columns of fp32, and 16 bytes from the last of them on
 
 template <typename T, int TN, int TK, int BK, int WK>
-__global__ __launch_bounds__(128 * WK, 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
+__global__ __launch_bounds__(128 * WK, TN == 128 && WK == 4 ? 4 : 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
                                                              const int8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, GradShape s,
                                                              void* __restrict__ dw, void* __restrict__ db, int out_dtype)
@@ -448,7 +448,7 @@ struct GradPlan {
 // 77 / 66.
 static double grad_estimate(bool large, bool f32, size_t tiles, size_t splits, size_t step, size_t n, size_t k)
 {
-  const double units = (double)step / 64, stage = large ? (f32 ? 4.4 : 1.65) : (f32 ? 1.9 : 0.9), pair = f32 ? 3.2 : 1.2;
+  const double units = (double)step / 64, stage = large ? (f32 ? 4.4 : 1.65) : (f32 ? 1.9 : 0.77), pair = f32 ? 3.2 : 1.2;
   const size_t groups = tiles * splits, at_once = large ? 256 : 512, rest = groups % at_once;
   double t = (large ? 11.0 : 8.0) + (double)(groups / at_once) * units * (large ? stage : pair);
   if (rest) t += units * (!large && rest > 256 ? pair : stage);
@@ -521,9 +521,9 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
     typedef decltype(t) T;
-    constexpr int BK = T::bytes == 4 ? 32 : 64;
-    auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, 2>;
-    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 256), 0, st,
+    constexpr int BK = T::bytes == 4 ? 32 : 64, kSmall = T::bytes == 4 ? 2 : 4;
+    auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, kSmall>;
+    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 128 * kSmall), 0, st,
                        static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part, !d_db ? nullptr : direct ? d_db : part_b,
                        direct ? out_dtype : -1);
     return check_launch();
