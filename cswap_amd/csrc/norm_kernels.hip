@@ -101,6 +101,15 @@ __device__ inline int valid_at(uint32_t col, uint32_t cols)
   return col + kChunk <= cols ? kChunk : col < cols ? (int)(cols - col) : 0;
 }
 
+template <typename T> __device__ inline void widen(const u4_any raw[T::bytes / 2], float v[8])
+{
+#pragma unroll
+  for (int e = 0; e < kChunk; ++e) {
+    if constexpr (T::bytes == 4) v[e] = __uint_as_float(raw[e / 4][e % 4]);
+    else v[e] = to_float<T>((typename T::value)(raw[0][e / 2] >> (16 * (e & 1))));
+  }
+}
+
 template <typename T, typename F, bool HOLD>
 __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename T::value* __restrict__ x, size_t x_stride,
                                                                   NormShape s, Params gamma, Params beta,
@@ -120,18 +129,26 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
     load_params(gamma, col, valid[c], 1.0f, g[c]);
     load_params(beta, col, valid[c], 0.0f, b[c]);
   }
+  u4_any next[F::chunks][T::bytes / 2];
+  auto load = [&](uint32_t row) {
+#pragma unroll
+    for (int c = 0; c < F::chunks; ++c)
+      load_raw<T>(x + (size_t)row * x_stride + (lane + c * F::lanes) * kChunk, row < s.rows ? valid[c] : 0, next[c]);
+  };
   // the rows of a workgroup walk together: every lane runs every exchange and barrier
+  const uint32_t mine = threadIdx.x / F::lanes;
+  load(blockIdx.x * F::rows + mine);
   for (uint32_t base = blockIdx.x * F::rows; base < s.rows; base += gridDim.x * F::rows) {
-    const uint32_t row = base + threadIdx.x / F::lanes;
+    const uint32_t row = base + mine;
     const bool here = row < s.rows;
     float v[F::chunks][8], sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < F::chunks; ++c) {
-      const uint32_t col = (lane + c * F::lanes) * kChunk;
-      load_chunk<T>(x + (size_t)row * x_stride + col, here ? valid[c] : 0, v[c]);
+      widen<T>(next[c], v[c]);
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) sum += v[c][i];
     }
+    if (base + gridDim.x * F::rows < s.rows) load(row + gridDim.x * F::rows);
     if (HOLD) {
 #pragma unroll
       for (int c = 0; c < F::chunks; ++c) {
@@ -152,7 +169,8 @@ __global__ __launch_bounds__(F::threads) void norm_forward_kernel(const typename
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) {
         v[c][i] -= mu;
-        if (i < valid[c]) squares = __builtin_fmaf(v[c][i], v[c][i], squares);
+        const float d = i < valid[c] ? v[c][i] : 0.0f;
+        squares = __builtin_fmaf(d, d, squares);
       }
     const float r = 1.0f / __builtin_sqrtf(row_sum(squares, 0.0f).x * s.inv_cols + s.eps);
 #pragma unroll
@@ -171,15 +189,6 @@ template <typename T, bool HELD> struct RowChunk {
   uint2 q;
   uint32_t scale;
 };
-
-template <typename T> __device__ inline void widen(const u4_any raw[T::bytes / 2], float v[8])
-{
-#pragma unroll
-  for (int e = 0; e < kChunk; ++e) {
-    if constexpr (T::bytes == 4) v[e] = __uint_as_float(raw[e / 4][e % 4]);
-    else v[e] = to_float<T>((typename T::value)(raw[0][e / 2] >> (16 * (e & 1))));
-  }
-}
 
 // Either the workgroup's share of the parameters' gradients, part[workgroup][0 = gamma, 1 = beta][cols], or, of a single
 // workgroup (part NULL), the gradients.
@@ -340,7 +349,8 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
 // ---------------------------------------------------------------- launches
 // Rows up to 16384 values: 16 lanes hold 128 values of a row, 1024 lanes with two chunks each the longest.
 constexpr size_t kMaxNormCols = 16384;
-constexpr unsigned kMostForward = 2048, kMostBackward = 256;  // workgroups
+constexpr unsigned kForwardThreads = 256 * 1024;  // of all workgroups
+constexpr unsigned kMostBackward = 256;            // workgroups
 
 template <typename F> static unsigned groups_for(size_t rows, unsigned most)
 {
@@ -355,8 +365,8 @@ template <typename Fn> static auto with_forward_form(size_t cols, Fn&& fn)
   if (cols <= 512) return fn(Form<64, 1, 256>());
   if (cols <= 1024) return fn(Form<64, 2, 256>());
   if (cols <= 2048) return fn(Form<256, 1, 256>());
-  if (cols <= 4096) return fn(Form<512, 1, 512>());
-  if (cols <= 8192) return fn(Form<1024, 1, 1024>());
+  if (cols <= 4096) return fn(Form<256, 2, 256>());
+  if (cols <= 8192) return fn(Form<512, 2, 512>());
   return fn(Form<1024, 2, 1024>());
 }
 
@@ -433,7 +443,7 @@ extern "C" int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows,
     return with_forward_form(cols, [&](auto f) {
       typedef decltype(f) F;
       auto k = d_codes ? norm_forward_kernel<T, F, true> : norm_forward_kernel<T, F, false>;
-      hipLaunchKernelGGL(k, dim3(groups_for<F>(rows, kMostForward)), dim3(F::threads), 0, st,
+      hipLaunchKernelGGL(k, dim3(groups_for<F>(rows, kForwardThreads / F::threads)), dim3(F::threads), 0, st,
                          static_cast<const typename T::value*>(d_x), (size_t)x_stride, s, g, b,
                          static_cast<typename T::value*>(d_y), (size_t)y_stride, d_mean, d_rstd,
                          reinterpret_cast<uint2*>(d_codes), d_scales);
