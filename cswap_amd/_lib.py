@@ -119,6 +119,7 @@ _SIGNATURES = {
     "cswap_test_zfp_store_hint": (i32, [C.c_ulonglong] * 4 + [u]),
     "cswap_test_zvc_packed_hint": (i32, [sz]),
     "cswap_test_zfp_encode_route": (i32, [sz, sz, sz, pd, pd, u, u, i32]),
+    "cswap_test_weight_grad_plan": (i32, [i32, sz, sz, sz]),
     "cswap_zvc_compress_fused_static": (i32, [vp, i32, i32, vp, vp, vp, vp, vp]),
     "cswap_q8_code_pitch": (sz, [sz]),
     "cswap_q8_scale_pitch": (sz, [sz]),

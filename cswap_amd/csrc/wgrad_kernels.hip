@@ -7,10 +7,24 @@
 // 16-bit rate instead of one of the fp32 rate, which is a sixteenth of it.  An fp16 dY meets x^ as fp16, which is exact where
 // the checkpoint was made from fp16.
 //
-// Both operands run along m in memory's slow direction, and a matrix instruction wants eight consecutive m of one row or
-// column in a lane: they are turned round on their way into LDS.
+// Both operands run along m, memory's slow direction, and a matrix instruction wants eight consecutive m of one row or column
+// in a lane.  dY goes to LDS as it lies in memory and the codes as the 16-bit values that they stand for, and both are read
+// by the transposing LDS reads of this chip.  (The first form turned them round in registers, in pieces of 2 x 8 values loaded
+// two at a time: 16384 x 4096 x 1024 bf16 2084 us.)
+//
+// What bounds it: the matrix instructions, at the clock that they leave.  16384 x 4096 x 1024 bf16: 136 us and 12 for the sum
+// of four splits, 930 TFLOP/s in all, where torch's product of the same bf16 matrices takes 180-195 us; the matrix units are
+// busy 54 % of the time that a compute unit is, at 2.05 of 2.4 GHz.  The rest is issue: 100 vector instructions and 56 LDS
+// instructions to 32 matrix instructions in a wavefront's stage.  fp32 of that size 390 us (353 TFLOP/s; torch's fp32
+// product 950).  8192 x 8192 x 2048 bf16 262 us, 1050 TFLOP/s (torch 248).
+//
+// Measured and not kept: four wavefronts to a 256 x 256 tile (4096^3 fp16 163 : 149 us; a wavefront alone on its SIMD issues
+// one instruction in four cycles, and a stage has 400 of them), an order of instructions given to the compiler group by group
+// (four patterns, +-3 %), db as a product with ones (its sums did not fit the registers beside the tile: 268 us, half of it
+// moves between register files).
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
+#include "../../include/cswap_test_hooks.h"
 #include "common.h"
 #include "q8_block.h"
 
@@ -79,7 +93,9 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
   return make_uint4(x.x, x.y, y.x, y.y);
 }
 
-// A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.
+// A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.  Tiles of
+// 256 x 256 read LDS 1.5 times for what they multiply where those of 128 x 128 read it 3 times, and need a quarter of the cache
+// traffic; one fits a compute unit (128 KB of LDS for two stages), of the small ones two.
 //
 // The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m: the
 // transposing reads take four rows at once, which have to lie in different banks.  a_at and b_at are the places of value
@@ -99,10 +115,10 @@ template <typename T, int TN, int TK, int BK> struct GradTile {
 
 // Which tile and split a workgroup has.  Workgroups go to the eight XCDs in turn, each of which has a cache of its own: an XCD gets
 // neighbouring tiles of one split, up to 16 along k (whose operand is the smaller one) before the next row of tiles.
-struct Place {
+struct TilePlace {
   uint32_t tn, tk, split;
 };
-__device__ inline Place place_of(uint32_t id, uint32_t count, const GradShape& s)
+__device__ inline TilePlace tile_place(uint32_t id, uint32_t count, const GradShape& s)
 {
   const uint32_t each = count / 8, more = count % 8, xcd = id % 8;
   uint32_t at = xcd * each + min(xcd, more) + id / 8;
@@ -127,10 +143,9 @@ __device__ inline global_bytes uniform(const char* p)
 __device__ char spare[1024 + 16];  // 256 columns of fp32, and 16 bytes from the last of them on
 
 template <typename T, int TN, int TK, int BK, int WK>
-__global__ __launch_bounds__(128 * WK, TN == 128 && WK == 4 ? 4 : 2) void weight_grad_kernel(const typename T::value* __restrict__ dy,
-                                                             const int8_t* __restrict__ codes,
-                                                             const uint8_t* __restrict__ scales, GradShape s,
-                                                             void* __restrict__ dw, void* __restrict__ db, int out_dtype)
+__global__ __launch_bounds__(128 * WK, TN == 128 && WK == 4 ? 4 : 2) void weight_grad_kernel(
+    const typename T::value* __restrict__ dy, const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, GradShape s,
+    void* __restrict__ dw, void* __restrict__ db, int out_dtype)
 {
   typedef GradTile<T, TN, TK, BK> Tile;
   typedef typename Feed<T>::type M;
@@ -142,7 +157,7 @@ __global__ __launch_bounds__(128 * WK, TN == 128 && WK == 4 ? 4 : 2) void weight
   constexpr int kBPieces = TK / 16, kBRows = NT / kBPieces, kBLoads = BK / kBRows;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][Tile::kStage];
 
-  const Place at = place_of(blockIdx.x, gridDim.x, s);
+  const TilePlace at = tile_place(blockIdx.x, gridDim.x, s);
   const uint32_t tk = at.tk, tn = at.tn, split = at.split;
   const uint32_t n0 = tn * TN, k0 = tk * TK;
   const uint32_t from = split * s.step_rows, to = min(s.rows, from + s.step_rows);
@@ -417,8 +432,10 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
     __shared__ float sum[8][32];
     const uint32_t i = (uint32_t)(blockIdx.x - s.dw_groups) * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5;
     float v = 0.0f;
-    if (i < s.n)
+    if (i < s.n) {
+#pragma unroll 8
       for (uint32_t p = seg; p < s.db_parts; p += 8) v += s.db[(size_t)p * s.n + i];
+    }
     sum[seg][threadIdx.x & 31] = v;
     __syncthreads();
     if (seg == 0 && i < s.n) {
@@ -431,8 +448,7 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
 
 // ---------------------------------------------------------------- launches
 constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
-constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 16 rows are 32 bits
-
+constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 32 rows are 32 bits
 
 struct GradPlan {
   bool large;  // 256 x 256 tiles, else 128 x 128
@@ -490,7 +506,16 @@ static size_t grad_room(const GradPlan& p, size_t n, size_t k)
 using namespace cswap;
 using namespace cswap::q8;
 
-static bool grad_sizes(size_t rows, size_t n, size_t k) { return n && k && n <= kMaxGradSide && k <= kMaxGradSide && rows < ((size_t)1 << 31); }
+static bool grad_sizes(size_t rows, size_t n, size_t k)
+{
+  return n && k && n <= kMaxGradSide && k <= kMaxGradSide && rows < ((size_t)1 << 31);
+}
+
+extern "C" int cswap_test_weight_grad_plan(int dtype, size_t rows, size_t n, size_t k)
+{
+  const GradPlan p = grad_plan(dtype, rows, n, k);
+  return (int)p.splits * (p.large ? -1 : 1);
+}
 
 extern "C" size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k)
 {
@@ -524,8 +549,8 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
     constexpr int BK = T::bytes == 4 ? 32 : 64, kSmall = T::bytes == 4 ? 2 : 4;
     auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, kSmall>;
     hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 128 * kSmall), 0, st,
-                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part, !d_db ? nullptr : direct ? d_db : part_b,
-                       direct ? out_dtype : -1);
+                       static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part,
+                       !d_db ? nullptr : direct ? d_db : part_b, direct ? out_dtype : -1);
     return check_launch();
   };
   if (int e = dtype == CSWAP_DT_F32 ? launch(F32()) : dtype == CSWAP_DT_BF16 ? launch(BF16()) : launch(F16())) return e;

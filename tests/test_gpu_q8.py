@@ -232,7 +232,7 @@ def test_layer_norm_of_a_row_that_is_not_finite_leaves_the_others():
 # ---------------------------------------------------------------- weight gradient
 GRADS = [(1, 1, 1), (1, 130, 40), (7, 33, 65), (64, 256, 256), (31, 100, 193), (333, 129, 257), (1000, 300, 96), (2050, 64, 128),
          (700, 520, 130), (4100, 17, 300), (128, 128, 128), (515, 1000, 193),
-         (2050, 2900, 2850)]    # the last one in the larger tiles, with rows, columns and both features cut off
+         (2050, 2900, 2850), (8200, 1500, 1400)]    # the larger tiles, the rows not split and split, everything cut off somewhere
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -276,6 +276,18 @@ def test_weight_grad_keeps_the_last_bits_of_fp32():
     dw, _ = q8().q8_weight_grad(dy.cuda(), q8().q8_compress(x.cuda()))
     want = dy.double().t() @ kept
     ref.check(dw, want, 2 * ref.U * want.abs(), F32, "dw")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,n,k", [(3001, 777, 333), (16384, 768, 768), (16000, 300, 2000), (200, 5000, 70)])
+def test_weight_grad_of_whole_numbers_is_exact(dtype, rows, n, k):
+    """Sums below 2^24: every order of fp32 additions gives the exact result, and a value left out or taken twice shows."""
+    g = torch.Generator().manual_seed(rows + n + k)
+    x, dy = torch.randint(-9, 10, (rows, k), generator=g), torch.randint(-9, 10, (rows, n), generator=g)
+    x[:, ::32] = 9
+    dw, db = q8().q8_weight_grad(dy.to(dtype).cuda(), q8().q8_compress(x.to(dtype).cuda()), out_dtype=F32)
+    assert torch.equal(dw.cpu(), (dy.float().t() @ x.float()))
+    assert torch.equal(db.cpu(), dy.sum(0).float())
 
 
 def test_weight_grad_of_values_that_are_not_finite():

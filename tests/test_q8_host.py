@@ -107,6 +107,25 @@ def test_weight_grad_refuses():
     assert f(_3=(1 << 20) + 1) == UNSUPPORTED and f(_7=(1 << 20) + 1) == UNSUPPORTED
 
 
+def test_weight_grad_layout():
+    """Tiles and splits as they measured best (negative: 256 x 256 tiles), and the same in the workspace's size."""
+    plan, room = L().cswap_test_weight_grad_plan, L().cswap_q8_weight_grad_workspace_bytes
+    f32, bf16 = 0, 1
+    for rows, n, k in ((1, 1, 1), (64, 256, 256), (512, 2048, 2048), (512, 768, 4096), (0, 100, 100)):
+        assert plan(bf16, rows, n, k) == 1 and room(bf16, rows, n, k) == 0
+    for rows, n, k in ((2048, 4096, 4096), (8192, 4096, 4096), (4096, 4096, 4096)):
+        assert plan(bf16, rows, n, k) == -1 and plan(f32, rows, n, k) == -1
+    for rows, n, k in ((16384, 4096, 1024), (32768, 1024, 1024), (8192, 2048, 2048)):
+        assert plan(bf16, rows, n, k) <= -4
+    for rows, n, k in ((8192, 256, 256), (8192, 768, 768), (32768, 256, 256), (4100, 17, 300)):
+        assert plan(bf16, rows, n, k) >= 2
+    for dtype in (f32, bf16):
+        for rows, n, k in ((5000, 300, 100), (70000, 33, 65), (16384, 768, 768), (1 << 20, 128, 128)):
+            splits = abs(plan(dtype, rows, n, k))
+            side = 256 if plan(dtype, rows, n, k) < 0 else 128
+            assert 2 <= splits <= 64 and room(dtype, rows, n, k) == 4 * splits * (n * k + n * -(-k // side))
+
+
 # ---------------------------------------------------------------- the torch side
 def checkpoint(shape, rows, cols, dtype=torch.float32):
     from cswap_amd.q8 import Checkpoint8
@@ -144,6 +163,41 @@ def test_tensors_that_are_refused():
         q8.q8_compress(x.double())
     with pytest.raises(ValueError):
         q8.q8_act(x, "relu")
+
+
+def test_a_tensor_on_another_device_makes_that_device_current(monkeypatch):
+    """The launch is on the tensor's device: where another is current, the call is made again with it current."""
+    import contextlib
+
+    from cswap_amd import api, q8
+
+    current, launched = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        was, current[0] = current[0], d.index
+        yield
+        current[0] = was
+
+    class OnDevice1(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        device = property(lambda self: torch.device("cuda", 1))
+
+    x = torch.zeros(4, 40).as_subclass(OnDevice1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(q8.Checkpoint8, "_empty", classmethod(lambda cls, t, rows, cols: checkpoint((4, 40), rows, cols)))
+
+    class Lib:
+        @staticmethod
+        def cswap_q8_pack(*a):
+            launched.append((current[0], a[-1]))
+            return 0
+
+    monkeypatch.setattr(q8, "lib", lambda: Lib)
+    q8.q8_compress(x)
+    assert launched == [(1, 1001)] and current == [0]
 
 
 def test_row_strides():
