@@ -9,7 +9,8 @@ import torch
 
 from cswap_amd import api, swap
 from cswap_amd._lib import Costs
-from cswap_amd.hooks import swap_saved_tensors
+from cswap_amd.hooks import hold_saved_tensors, swap_saved_tensors
+from cswap_amd.layers8 import checkpoint_layers
 from cswap_amd.planner import PolicyMaker, run_planned_iteration
 from cswap_amd.workloads import dummy_layer_compute, vgg16_modules
 
@@ -296,7 +297,9 @@ def bench_transformer_step(dev, layers: int = 4, batch: int = 32, seq: int = 512
     out, so the [batch, heads, seq, seq] probabilities are saved as in
     configuration 5; GELU feed-forward of 4 x hidden) with and without swapping
     through the saved-tensor hooks.  No ReLU anywhere: the selector has only ZFP
-    and raw to choose from."""
+    and raw to choose from.  Then without the link: what is saved held in 8 bits on
+    the device by hooks, the linear, norm and GELU layers with checkpoints that
+    their backward passes read, and both."""
     import math
 
     torch.manual_seed(0)
@@ -310,13 +313,14 @@ def bench_transformer_step(dev, layers: int = 4, batch: int = 32, seq: int = 512
             self.ln2 = torch.nn.LayerNorm(hidden)
             self.fc1 = torch.nn.Linear(hidden, 4 * hidden)
             self.fc2 = torch.nn.Linear(4 * hidden, hidden)
+            self.act = torch.nn.GELU()
 
         def forward(self, x):
             b, s, h = x.shape
             q, k, v = self.qkv(self.ln1(x)).view(b, s, 3, heads, h // heads).permute(2, 0, 3, 1, 4)
             p = torch.softmax(q @ k.transpose(-1, -2) / math.sqrt(h // heads), dim=-1)
             x = x + self.proj((p @ v).transpose(1, 2).reshape(b, s, h))
-            return x + self.fc2(torch.nn.functional.gelu(self.fc1(self.ln2(x))))
+            return x + self.fc2(self.act(self.fc1(self.ln2(x))))
 
     net = torch.nn.Sequential(*[Block() for _ in range(layers)]).to(dev)
     x = torch.randn(batch, seq, hidden, device=dev)
@@ -344,4 +348,18 @@ def bench_transformer_step(dev, layers: int = 4, batch: int = 32, seq: int = 512
     res["staging_pool_MB"] = round(staging / 1e6, 1)
     _swap_rows(res, eng, step, params, min_bytes, 9)
     eng.close()
+
+    def held(label, make_ctx):
+        for p in params:
+            p.grad = None
+        ms, mb, st = _measure_step(step, params, make_ctx, 9)
+        res[label] = {"step_ms": round(ms[0], 2), "step_ms_best": round(ms[1], 2), "step_peak_MB": round(mb, 1)}
+        if st is not None:
+            res[label].update(held_tensors=st["held"], held_from_MB=round(st["bytes_in"] / 1e6, 1),
+                              held_MB=round(st["bytes_held"] / 1e6, 1))
+
+    held("held_8bit", lambda: hold_saved_tensors(min_bytes))
+    checkpoint_layers(net)
+    held("layers_8bit", lambda: None)
+    held("layers_and_held_8bit", lambda: hold_saved_tensors(min_bytes))
     return res

@@ -307,7 +307,9 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
 
     A tensor that several nodes save is held once for each of them, so a float32 one gains half of its memory where
     two nodes do and a 16-bit one nothing.  Layers that can read a checkpoint as it is (``cswap_amd.layers8``) need
-    neither the hooks nor the tensor that backward would be given here; what they keep passes through unchanged."""
+    neither the hooks nor the tensor that backward would be given here; what they keep passes through unchanged.
+    Operators whose backward pass compares saved tensors with one another (``amax``, ``median``) find no equal
+    values any more: keep them outside."""
 
     def __init__(self, min_bytes: int = 1 << 20):
         self.min_bytes = min_bytes
@@ -331,3 +333,6 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
 
     def _unpack(self, held):
         return q8.q8_decompress(held) if isinstance(held, q8.Checkpoint8) else held
+
+    def close(self):
+        """Nothing is left to release: there so that this context goes where ``swap_saved_tensors`` does."""
