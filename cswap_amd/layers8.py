@@ -98,9 +98,11 @@ class _Linear(torch.autograd.Function):
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, held: Checkpoint8 | None = None):
     """``x @ weight.T + bias``; ``held``: x's checkpoint, if there is one already.  Under autocast in its type, as
     torch's linear is (``held`` is then of x in that type)."""
+    if not torch.is_grad_enabled():
+        return F.linear(x, weight, bias)
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
-        x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
+        x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias))
         with torch.autocast("cuda", enabled=False):
             return _Linear.apply(x, weight, bias, held)
     return _Linear.apply(x, weight, bias, held)
@@ -128,8 +130,10 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5):
     """Layer norm over the last dimension; under autocast in fp32, as torch's is."""
-    if torch.is_autocast_enabled("cuda"):
+    if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:
         x = x.float()
+    if not torch.is_grad_enabled():
+        return q8.layer_norm(_rows(x), weight, bias, eps, checkpoint=False)[0]
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
@@ -152,6 +156,8 @@ class _Act(torch.autograd.Function):
 
 def activation(x: torch.Tensor, kind: str = "gelu"):
     """"gelu", "gelu_tanh" or "silu" of x."""
+    if not torch.is_grad_enabled():
+        return q8.q8_act(_rows(x), kind, checkpoint=False)[0]
     return _Act.apply(x, kind)
 
 

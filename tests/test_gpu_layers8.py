@@ -182,6 +182,22 @@ def test_a_shared_checkpoint_and_partial_gradients():
         layers8.linear(leaf, w[0], None, held=layers8.hold(x[:40]))
 
 
+def test_without_gradients_nothing_is_made(monkeypatch):
+    """Where gradients are off, parameters that could have them make no checkpoint, and results are the same."""
+    from cswap_amd import layers8, q8
+
+    model = layers8.checkpoint_layers(block(dtype=BF16))
+    x = randn(30, 96, dtype=BF16, seed=35)
+    want = model(x).detach()
+    monkeypatch.setattr(q8.Checkpoint8, "_empty", None)
+    with torch.no_grad():
+        assert torch.equal(model(x), want)
+        with torch.autocast("cuda", dtype=BF16):
+            assert model(x.float()).dtype == BF16
+    with torch.inference_mode():
+        assert torch.equal(model(x), want)
+
+
 def test_gradients_that_are_views():
     """What sum() and a transposition hand to backward: expanded and strided gradients, and inputs that are views."""
     from cswap_amd import layers8
