@@ -143,7 +143,7 @@ __device__ inline global_bytes uniform(const char* p)
 __device__ char spare[1024 + 16];  // 256 columns of fp32, and 16 bytes from the last of them on
 
 template <typename T, int TN, int TK, int BK, int WK>
-__global__ __launch_bounds__(128 * WK, TN == 128 && WK == 4 ? 4 : 2) void weight_grad_kernel(
+__global__ __launch_bounds__(128 * WK, TN * TK == 128 * 128 && WK == 4 ? 4 : 2) void weight_grad_kernel(
     const typename T::value* __restrict__ dy, const int8_t* __restrict__ codes, const uint8_t* __restrict__ scales, GradShape s,
     void* __restrict__ dw, void* __restrict__ db, int out_dtype)
 {
@@ -450,24 +450,31 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
 constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
 constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 32 rows are 32 bits
 
+// Tiles of dW: n x k features.
+enum GradForm { kSmallTile, kMiddleTile, kLargeTile, kGradForms };
+constexpr size_t kTileN[kGradForms] = {128, 128, 256}, kTileK[kGradForms] = {128, 256, 256};
+
 struct GradPlan {
-  bool large;  // 256 x 256 tiles, else 128 x 128
+  int form;
   unsigned tiles_n, tiles_k, splits;
   uint32_t step_rows;
 };
 
 // Tiles and splits with the least estimated time.  Measured on 256 compute units, in us: a workgroup takes `stage` for 64 rows, a
 // compute unit with two workgroups of the small tiles `pair` for 64 rows of both; `fixed` is the rest of a launch; splits cost
-// the sums' launch (5) and their bytes there and back at 5.5 TB/s.  What it decides between, bf16, us of 128 x 128 tiles / 256 x 256:
-// 512 x 2048 x 2048 15.0 / 32.8, 8192 x 768 x 768 30 / 36, 8192 x 2048 x 2048 102 / 86, 32768 x 4096 x 1024 371 / 294, 2048 x 4096 x
-// 4096 92 / 76; and with 256 / 512 workgroups of the small tiles: 2048 x 2048 x 2048 (not split / in two) 36.6 / 40.9, 32768 x 768 x 768
-// 77 / 66.
-static double grad_estimate(bool large, bool f32, size_t tiles, size_t splits, size_t step, size_t n, size_t k)
+// the sums' launch (5) and their bytes there and back at 5.5 TB/s.  What it decides between, small : middle : large tiles in us,
+// each with its best splits.  bf16: 512 x 2048 x 2048 14 : 18 : 33, 8192 x 768 x 768 28.5 : 28.6 : 36, 8192 x 1024 x 1024 39.7 : 37.6 :
+// 43, 8192 x 2048 x 2048 102 : 91 : 86, 32768 x 4096 x 1024 371 : 328 : 273, 2048 x 4096 x 4096 92 : 84 : 71; fp32: 8192 x 768 x 768
+// 52 : 42 : 50, 2048 x 2048 x 2048 68 : 61 : 70, 8192 x 4096 x 1024 222 : 184 : 180, 32768 x 768 x 4096 677 : 561 : 514.  Small tiles with
+// one : two workgroups a compute unit, bf16: 2048 x 2048 x 2048 (not split : in two) 36.6 : 40.9, 32768 x 768 x 768 77 : 66.
+static double grad_estimate(int form, bool f32, size_t tiles, size_t splits, size_t step, size_t n, size_t k)
 {
-  const double units = (double)step / 64, stage = large ? (f32 ? 4.4 : 1.65) : (f32 ? 1.9 : 0.77), pair = f32 ? 3.2 : 1.2;
-  const size_t groups = tiles * splits, at_once = large ? 256 : 512, rest = groups % at_once;
-  double t = (large ? 11.0 : 8.0) + (double)(groups / at_once) * units * (large ? stage : pair);
-  if (rest) t += units * (!large && rest > 256 ? pair : stage);
+  constexpr double kFixed[kGradForms] = {8.0, 9.5, 11.0};
+  constexpr double kStage[2][kGradForms] = {{0.77, 1.05, 1.65}, {1.9, 2.35, 4.4}}, kPair[2] = {1.2, 3.2};
+  const size_t groups = tiles * splits, at_once = form == kSmallTile ? 512 : 256, rest = groups % at_once;
+  const double units = (double)step / 64, stage = kStage[f32][form], both = form == kSmallTile ? kPair[f32] : stage;
+  double t = kFixed[form] + (double)(groups / at_once) * units * both;
+  if (rest) t += units * (rest > 256 ? both : stage);
   if (splits > 1) t += 5.0 + (double)(splits * n * k) * 8.0 / 5.5e6;
   return t;
 }
@@ -476,16 +483,16 @@ static GradPlan grad_plan(int dtype, size_t rows, size_t n, size_t k)
 {
   GradPlan best = {};
   double least = 0.0;
-  for (int large = 0; large < 2; ++large) {
-    const size_t side = large ? 256 : 128, tiles_n = (n + side - 1) / side, tiles_k = (k + side - 1) / side;
+  for (int form = 0; form < kGradForms; ++form) {
+    const size_t tiles_n = (n + kTileN[form] - 1) / kTileN[form], tiles_k = (k + kTileK[form] - 1) / kTileK[form];
     const size_t tiles = tiles_n * tiles_k;
     for (size_t want = 1; want <= 64 && (want == 1 || (want * tiles <= 1024 && want * 64 <= rows)); ++want) {
       const size_t step = rows ? ((rows + want - 1) / want + 63) / 64 * 64 : 64, splits = rows ? (rows + step - 1) / step : 1;
       if (splits != want) continue;  // a smaller number has the same steps
-      const double t = grad_estimate(large, dtype == CSWAP_DT_F32, tiles, splits, step, n, k);
+      const double t = grad_estimate(form, dtype == CSWAP_DT_F32, tiles, splits, step, n, k);
       if (best.splits == 0 || t < least) {
         least = t;
-        best = {large != 0, (unsigned)tiles_n, (unsigned)tiles_k, (unsigned)splits, (uint32_t)step};
+        best = {form, (unsigned)tiles_n, (unsigned)tiles_k, (unsigned)splits, (uint32_t)step};
       }
     }
   }
@@ -514,7 +521,7 @@ static bool grad_sizes(size_t rows, size_t n, size_t k)
 extern "C" int cswap_test_weight_grad_plan(int dtype, size_t rows, size_t n, size_t k)
 {
   const GradPlan p = grad_plan(dtype, rows, n, k);
-  return (int)p.splits * (p.large ? -1 : 1);
+  return (int)p.splits + 1000 * p.form;
 }
 
 extern "C" size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k)
@@ -546,9 +553,12 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto launch = [&](auto t) {
     typedef decltype(t) T;
+    // stages of 32 rows in fp32, whose three planes need the room; a small tile's codes are then too few for eight wavefronts
     constexpr int BK = T::bytes == 4 ? 32 : 64, kSmall = T::bytes == 4 ? 2 : 4;
-    auto kernel = p.large ? weight_grad_kernel<T, 256, 256, BK, 4> : weight_grad_kernel<T, 128, 128, BK, kSmall>;
-    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.large ? 512 : 128 * kSmall), 0, st,
+    auto kernel = p.form == kLargeTile    ? weight_grad_kernel<T, 256, 256, BK, 4>
+                  : p.form == kMiddleTile ? weight_grad_kernel<T, 128, 256, BK, 4>
+                                          : weight_grad_kernel<T, 128, 128, BK, kSmall>;
+    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.form == kSmallTile ? 128 * kSmall : 512), 0, st,
                        static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part,
                        !d_db ? nullptr : direct ? d_db : part_b, direct ? out_dtype : -1);
     return check_launch();

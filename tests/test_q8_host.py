@@ -108,22 +108,23 @@ def test_weight_grad_refuses():
 
 
 def test_weight_grad_layout():
-    """Tiles and splits as they measured best (negative: 256 x 256 tiles), and the same in the workspace's size."""
+    """Tiles (1000s: 0 small, 1 middle, 2 large) and splits as they measured best, and the same in the workspace's size."""
     plan, room = L().cswap_test_weight_grad_plan, L().cswap_q8_weight_grad_workspace_bytes
     f32, bf16 = 0, 1
     for rows, n, k in ((1, 1, 1), (64, 256, 256), (512, 2048, 2048), (512, 768, 4096), (0, 100, 100)):
         assert plan(bf16, rows, n, k) == 1 and room(bf16, rows, n, k) == 0
     for rows, n, k in ((2048, 4096, 4096), (8192, 4096, 4096), (4096, 4096, 4096)):
-        assert plan(bf16, rows, n, k) == -1 and plan(f32, rows, n, k) == -1
+        assert plan(bf16, rows, n, k) == 2001 and plan(f32, rows, n, k) == 2001
     for rows, n, k in ((16384, 4096, 1024), (32768, 1024, 1024), (8192, 2048, 2048)):
-        assert plan(bf16, rows, n, k) <= -4
-    for rows, n, k in ((8192, 256, 256), (8192, 768, 768), (32768, 256, 256), (4100, 17, 300)):
-        assert plan(bf16, rows, n, k) >= 2
+        assert plan(bf16, rows, n, k) >= 2004
+    for rows, n, k in ((8192, 768, 768), (2048, 2048, 2048), (2048, 768, 4096)):
+        assert 1002 <= plan(f32, rows, n, k) < 2000
+    for rows, n, k in ((8192, 256, 256), (32768, 256, 256), (4100, 17, 300)):
+        assert 2 <= plan(bf16, rows, n, k) <= 64
     for dtype in (f32, bf16):
         for rows, n, k in ((5000, 300, 100), (70000, 33, 65), (16384, 768, 768), (1 << 20, 128, 128)):
-            splits = abs(plan(dtype, rows, n, k))
-            side = 256 if plan(dtype, rows, n, k) < 0 else 128
-            assert 2 <= splits <= 64 and room(dtype, rows, n, k) == 4 * splits * (n * k + n * -(-k // side))
+            form, splits = divmod(plan(dtype, rows, n, k), 1000)
+            assert 2 <= splits <= 64 and room(dtype, rows, n, k) == 4 * splits * (n * k + n * -(-k // (128, 256, 256)[form]))
 
 
 # ---------------------------------------------------------------- the torch side
