@@ -55,12 +55,6 @@ class Checkpoint8:
         self._at, self._scales_at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _empty(cls, x: torch.Tensor, rows: int, cols: int) -> "Checkpoint8":
-        """Room for the checkpoint of x, in one allocation."""
-        room = torch.empty(rows * -(-cols // GROUP) * (GROUP + 1), dtype=torch.int8, device=x.device)
-        return cls._over(room, x.shape, x.dtype, rows, cols)
-
-    @classmethod
     def _over(cls, room: torch.Tensor, shape, dtype: torch.dtype, rows: int, cols: int) -> "Checkpoint8":
         """The checkpoint in ``room``: codes, and scales behind them; the tensors over either are made when they are
         asked for."""
@@ -144,6 +138,21 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
     return outer[-1][1]
 
 
+def _empty_checkpoint(x: torch.Tensor, rows: int, cols: int, device: torch.device) -> Checkpoint8:
+    """Room for the checkpoint of x, in one allocation (``Checkpoint8._over``, without the call: it is on every path)."""
+    codes = rows * -(-cols // GROUP) * GROUP
+    held = _new_checkpoint(Checkpoint8)
+    held._room = room = torch.empty(codes + codes // GROUP, dtype=torch.int8, device=device)
+    held._at = at = room.data_ptr()
+    held._scales_at = at + codes
+    held._codes = held._scales = None
+    held.shape, held.dtype, held.device, held.rows, held.cols = x.shape, x.dtype, device, rows, cols
+    return held
+
+
+_new_checkpoint = object.__new__
+
+
 def _like(t: torch.Tensor, stride: int) -> torch.Tensor:
     """A contiguous tensor of t's shape and type."""
     return torch.empty_like(t) if stride == 0 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
@@ -180,7 +189,7 @@ def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) ->
         raise ValueError("q8_compress: flat checkpoints are made of contiguous tensors")
     if flat and rows and cols % GROUP:
         rows, cols = 1, rows * cols
-    held = Checkpoint8._empty(x, rows, cols)
+    held = _empty_checkpoint(x, rows, cols, device)
     check(lib().cswap_q8_pack(x.data_ptr(), kind, rows, cols, stride, keep_sign, held._at, held._scales_at, stream),
           "cswap_q8_pack")
     return held
@@ -221,10 +230,10 @@ def _kind_of(kind: str) -> int:
 def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
     """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu".  The second is None with
     ``checkpoint=False``."""
-    k, dtype = _kind_of(kind), _need(x, "q8_act")
-    stream = _stream_of(x.device)
+    k, dtype, device = _kind_of(kind), _need(x, "q8_act"), x.device
+    stream = _stream_of(device)
     if stream is None:
-        with torch.cuda.device(x.device):
+        with torch.cuda.device(device):
             return q8_act(x, kind, checkpoint)
     stride = _row_stride(x, "q8_act")
     rows, cols = _rows_cols(x.shape)
@@ -232,7 +241,7 @@ def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
         raise ValueError("q8_act: rows without values")
     y = _like(x, stride)
     if checkpoint:
-        held = Checkpoint8._empty(x, rows, cols)
+        held = _empty_checkpoint(x, rows, cols, device)
         codes, scales = held._at, held._scales_at
     else:
         held, codes, scales = None, 0, 0
@@ -295,7 +304,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     mean = torch.empty(rows, dtype=torch.float32, device=device)
     rstd = torch.empty_like(mean)
     if checkpoint:
-        held = Checkpoint8._empty(x, rows, cols)
+        held = _empty_checkpoint(x, rows, cols, device)
         codes, scales = held._at, held._scales_at
     else:
         held, codes, scales = x, 0, 0

@@ -189,7 +189,7 @@ def test_without_gradients_nothing_is_made(monkeypatch):
     model = layers8.checkpoint_layers(block(dtype=BF16))
     x = randn(30, 96, dtype=BF16, seed=35)
     want = model(x).detach()
-    monkeypatch.setattr(q8.Checkpoint8, "_empty", None)
+    monkeypatch.setattr(q8, "_empty_checkpoint", None)
     with torch.no_grad():
         assert torch.equal(model(x), want)
         with torch.autocast("cuda", dtype=BF16):

@@ -188,7 +188,7 @@ def test_a_tensor_on_another_device_makes_that_device_current(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", device)
     monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
-    monkeypatch.setattr(q8.Checkpoint8, "_empty", classmethod(lambda cls, t, rows, cols: checkpoint((4, 40), rows, cols)))
+    monkeypatch.setattr(q8, "_empty_checkpoint", lambda t, rows, cols, device: checkpoint((4, 40), rows, cols))
 
     class Lib:
         @staticmethod
