@@ -21,7 +21,7 @@
 // Measured and not kept: four wavefronts to a 256 x 256 tile (4096^3 fp16 163 : 149 us; a wavefront alone on its SIMD issues
 // one instruction in four cycles, and a stage has 400 of them), an order of instructions given to the compiler group by group
 // (four patterns, +-3 %), db as a product with ones (its sums did not fit the registers beside the tile: 268 us, half of it
-// moves between register files).
+// moves between register files), the two wavefronts of a SIMD held half a step apart by barriers (4096^3 bf16 155 : 159-168).
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
 #include "../../include/cswap_test_hooks.h"
@@ -93,9 +93,10 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
   return make_uint4(x.x, x.y, y.x, y.y);
 }
 
-// A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.  Tiles of
-// 256 x 256 read LDS 1.5 times for what they multiply where those of 128 x 128 read it 3 times, and need a quarter of the cache
-// traffic; one fits a compute unit (128 KB of LDS for two stages), of the small ones two.
+// A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.  A
+// product of 32 x 32 x 16 takes 0.75 fragments from LDS in a tile of 256 x 256, 1 in one of 128 x 256 and 1.5 in one of 128 x 128, and
+// the small ones read either operand twice as often from the caches; of the large and middle ones one fits a compute unit (128 KB
+// of LDS for two stages), of the small ones two, and more of them there are where dW is small.
 //
 // The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m: the
 // transposing reads take four rows at once, which have to lie in different banks.  a_at and b_at are the places of value
