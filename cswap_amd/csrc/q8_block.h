@@ -12,8 +12,6 @@
 // lanes and its maximum two DPP steps.
 #pragma once
 #include <hip/hip_runtime.h>
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <stdint.h>
 #include "../../include/cswap_hip.h"
 

@@ -257,7 +257,7 @@ int cswap_zvc_compress_fused_static(const float* d_in, int n, int process, int* 
  * e = clamp(floor(log2(largest magnitude)) - 6, -126, 121), held as the byte e + 127, and
  * a value x is held as the signed byte q = clamp(rint(x / 2^e), -127, 127) and stands
  * for q * 2^e.  It is off by at most 2^(e-1), by less than 2^e where |x| > 127 * 2^e: by
- * at most 2^-7 of the group's largest magnitude.  A group that holds a NaN or an
+ * at most 2^-7 of the group's largest magnitude (of 2^-120 where that is less).  A group that holds a NaN or an
  * infinity stands for NaN in all its values (byte 255, codes 0).  -0 becomes +0.
  * Codes do not depend on who computes them, and q * 2^e is a bf16 and an fp32 value
  * exactly (an fp16 value, too, if x was one).
@@ -281,8 +281,8 @@ int cswap_q8_unpack(const int8_t* d_codes, const uint8_t* d_scales, size_t rows,
                     void* d_out, int dtype, ptrdiff_t stride, cswap_stream_t stream);
 
 /* y = f(x) and, where d_codes and d_scales are given, the checkpoint of x in one pass;
- * dx = dy f'(x^) from the checkpoint x^.  f in fp32 whatever the type: x Phi(x), its tanh form, x / (1 + exp(-x)).  y is 0 where x is
- * minus infinity. */
+ * dx = dy f'(x^) from the checkpoint x^.  f in fp32 whatever the type: x Phi(x), its tanh
+ * form, x / (1 + exp(-x)).  Where x is minus infinity y is 0 (at most 1e-35 off it). */
 typedef enum { CSWAP_ACT_GELU = 0, CSWAP_ACT_GELU_TANH = 1, CSWAP_ACT_SILU = 2 } cswap_act;
 int cswap_q8_act_forward(int kind, const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
                          void* d_y, ptrdiff_t y_stride, int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
@@ -313,8 +313,8 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
  * (rows x k): dw[n][k] = sum over rows of dy[.][n] x^[.][k], db[n] = sum over rows of dy[.][n]
  * (NULL: not wanted), in out_dtype, contiguous.  Products are exact for fp32 and bf16 dy and
  * summed in fp32, in a fixed order; for fp16 dy x^ is rounded to fp16, which changes nothing if
- * the checkpoint was made from fp16.  A NaN or an infinity in an fp32 dy gives NaN.  rows = 0
- * gives zeros.  n and k up to 2^20, dy_stride up to 2^24 (CSWAP_E_UNSUPPORTED beyond).  d_ws:
+ * the checkpoint was made from fp16.  Of an fp32 dy the bits below 2^-133 are cut off, and a
+ * NaN or an infinity in it gives NaN.  rows = 0 gives zeros.  n and k up to 2^20, dy_stride up to 2^24 (CSWAP_E_UNSUPPORTED beyond).  d_ws:
  * cswap_q8_weight_grad_workspace_bytes (NULL where that is 0), 4-byte aligned, no preparation;
  * calls that overlap must not share one. */
 size_t cswap_q8_weight_grad_workspace_bytes(int dtype, size_t rows, size_t n, size_t k);

@@ -52,7 +52,8 @@ def test_codec_at_the_ends_of_the_range(dtype):
     least = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}[dtype]
     rows = [[0.0] * 40, [-0.0] * 40, [fi.max] * 40, [-fi.max, 1.0] * 20, [least] * 40, [fi.tiny, -least] * 20,
             [math.inf] + [1.0] * 39, [1.0] * 39 + [-math.inf], [1.0, math.nan] + [2.0] * 38,
-            [127.5, -127.5, 127.49, 126.5, 64.5, 63.5, 0.5, 1.5] * 5, [128.0, 127.75, -127.9, 1.0] * 10, [1e-30] + [3.0] * 39]
+            [127.5, -127.5, 127.49, 126.5, 64.5, 63.5, 0.5, 1.5] * 5, [128.0, 127.75, -127.9, 1.0] * 10, [1e-30] + [3.0] * 39,
+            [1.5 * 2.0 ** -127] * 40, [2.0 ** -127, -2.0 ** -126, 2.0 ** -120, 2.0 ** -121] * 10]
     x = torch.tensor(rows, dtype=torch.float64).to(dtype)
     held = q8().q8_compress(x.cuda())
     codes, scales = ref.pack(x)
@@ -288,6 +289,22 @@ def test_weight_grad_of_whole_numbers_is_exact(dtype, rows, n, k):
     dw, db = q8().q8_weight_grad(dy.to(dtype).cuda(), q8().q8_compress(x.to(dtype).cuda()), out_dtype=F32)
     assert torch.equal(dw.cpu(), (dy.float().t() @ x.float()))
     assert torch.equal(db.cpu(), dy.sum(0).float())
+
+
+def test_weight_grad_of_subnormal_values():
+    """fp16 below 2^-14 in either operand, bf16 and fp32 below 2^-126: nothing is flushed."""
+    g = torch.Generator().manual_seed(24)
+    small = torch.randint(-1000, 1001, (200, 70), generator=g).double() * 2.0 ** -24
+    for x, dy in ((values(200, 70, F16, 25), small[:, :40].to(F16)), (small.to(F16), values(200, 40, F16, 26))):
+        dw, db = q8().q8_weight_grad(dy.cuda(), q8().q8_compress(x.cuda()), out_dtype=F32)
+        d, kept = dy.double(), ref.held(x)
+        ref.check(dw, ref.weight_grad(d, kept)[0], ref.weight_grad_error(d, kept)[0], F32, "dw")
+        ref.check(db, ref.weight_grad(d, kept)[1], ref.weight_grad_error(d, kept)[1], F32, "db")
+    for dtype in (BF16, F32):
+        dy = (torch.randint(1, 128, (1, 40), generator=g).double() * 2.0 ** -133).to(dtype)
+        dw, db = q8().q8_weight_grad(dy.cuda(), q8().q8_compress(torch.full((1, 32), 64.0, dtype=dtype).cuda()), out_dtype=F32)
+        assert torch.equal(dw.cpu().double(), dy.double().t() * torch.full((1, 32), 64.0, dtype=torch.float64))
+        assert torch.equal(db.cpu().double(), dy.double()[0])
 
 
 def test_weight_grad_of_values_that_are_not_finite():
