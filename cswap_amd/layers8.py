@@ -9,8 +9,9 @@ stays on the device in one byte a value, and the layer's backward pass reads it 
     y = layers8.linear(x, weight, bias)     # or function by function
 
 Outputs are those of the layers without checkpoints (linear layers run torch's own product); gradients are
-computed from inputs that are off by at most 2^-7 of the largest magnitude among 32 neighbours.  Without
-gradients to come nothing is kept.  Layers that share an input (the projections of an attention layer) can
+computed from inputs that are off by at most 2^-7 of the largest magnitude among 32 neighbours (a layer norm whose
+rows have a mean of many times their deviation is better left as it is).  Without gradients to come nothing is
+kept.  Layers that share an input (the projections of an attention layer) can
 share its checkpoint: ``held = layers8.hold(x)``, then ``linear(x, w, b, held=held)`` for each.  Double
 backward is refused, as are tensors that ``cswap_amd.q8`` refuses.
 """

@@ -286,7 +286,9 @@ def q8_act_backward(dy: torch.Tensor, held: Checkpoint8, kind: str = "gelu") -> 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
                checkpoint: bool = True):
     """``(y, mean, rstd, held)``: layer norm over the last dimension, the rows' statistics in fp32, and what the
-    backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``."""
+    backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``.  A checkpoint is off by up to
+    2^-7 of the largest magnitude nearby, mean included: rows whose mean is many times their deviation are better kept
+    as they are."""
     dtype, device = _need(x, "layer_norm"), x.device
     stream = _stream_of(device)
     if stream is None:
