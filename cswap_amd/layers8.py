@@ -8,7 +8,8 @@ stays on the device in one byte a value, and the layer's backward pass reads it 
     layers8.checkpoint_layers(model)        # nn.Linear, nn.LayerNorm, nn.GELU, nn.SiLU of a model, in place
     y = layers8.linear(x, weight, bias)     # or function by function
 
-Outputs are those of the layers without checkpoints (linear layers run torch's own product); gradients are
+Outputs are those of the layers without checkpoints (linear layers run torch's own product; norms and activation
+functions are computed in fp32 and rounded once, which may differ from torch's in the last place); gradients are
 computed from inputs that are off by at most 2^-7 of the largest magnitude among 32 neighbours (a layer norm whose
 rows have a mean of many times their deviation is better left as it is).  Without gradients to come nothing is
 kept.  Layers that share an input (the projections of an attention layer) can
