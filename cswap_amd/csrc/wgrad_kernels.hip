@@ -396,17 +396,44 @@ __global__ __launch_bounds__(128 * WK, TN * TK == 128 * 128 && WK == 4 ? 4 : 2) 
   }
 }
 
-// out[i] = sum over `parts` of part[.][i], rounded once: dW from its splits, four values a thread, and behind them db
+// out[i] = sum over `parts` of part[.][i], rounded once: dW from its splits, and behind it db.  Of few splits a thread sums four
+// values; of many, which a small dW has, eight lanes sum one.
 struct GradSums {
   const float *dw, *db;
   size_t dw_count, dw_groups;  // workgroups that sum dW
   uint32_t dw_parts, db_parts, n;
 };
+constexpr uint32_t kFewSplits = 16;
+
+// 32 values a workgroup, eight lanes to a value
+template <typename O> __device__ inline void sum_by_eight(const float* part, uint32_t parts, size_t count, size_t group,
+                                                          typename O::value* out)
+{
+  __shared__ float sum[8][32];
+  const uint32_t lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
+  const size_t i = group * 32 + lane;
+  float v = 0.0f;
+  if (i < count) {
+#pragma unroll 8
+    for (uint32_t p = seg; p < parts; p += 8) v += part[(size_t)p * count + i];
+  }
+  sum[seg][lane] = v;
+  __syncthreads();
+  if (seg == 0 && i < count) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += sum[k][lane];
+    out[i] = from_float<O>(v);
+  }
+}
 
 template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_kernel(GradSums s, typename O::value* __restrict__ dw,
                                                                                        typename O::value* __restrict__ db)
 {
-  if (blockIdx.x < s.dw_groups) {
+  if (blockIdx.x >= s.dw_groups) {
+    sum_by_eight<O>(s.db, s.db_parts, s.n, blockIdx.x - s.dw_groups, db);
+  } else if (s.dw_parts > kFewSplits) {
+    sum_by_eight<O>(s.dw, s.dw_parts, s.dw_count, blockIdx.x, dw);
+  } else {
     const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (at + 4 <= s.dw_count) {
       float v[4] = {};
@@ -427,22 +454,6 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
         for (uint32_t p = 0; p < s.dw_parts; ++p) v += s.dw[(size_t)p * s.dw_count + i];
         dw[i] = from_float<O>(v);
       }
-    }
-  } else {
-    // 32 columns a workgroup, eight lanes to a column
-    __shared__ float sum[8][32];
-    const uint32_t i = (uint32_t)(blockIdx.x - s.dw_groups) * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5;
-    float v = 0.0f;
-    if (i < s.n) {
-#pragma unroll 8
-      for (uint32_t p = seg; p < s.db_parts; p += 8) v += s.db[(size_t)p * s.n + i];
-    }
-    sum[seg][threadIdx.x & 31] = v;
-    __syncthreads();
-    if (seg == 0 && i < s.n) {
-#pragma unroll
-      for (int k = 1; k < 8; ++k) v += sum[k][threadIdx.x];
-      db[i] = from_float<O>(v);
     }
   }
 }
@@ -487,9 +498,9 @@ static GradPlan grad_plan(int dtype, size_t rows, size_t n, size_t k)
   for (int form = 0; form < kGradForms; ++form) {
     const size_t tiles_n = (n + kTileN[form] - 1) / kTileN[form], tiles_k = (k + kTileK[form] - 1) / kTileK[form];
     const size_t tiles = tiles_n * tiles_k;
-    for (size_t want = 1; want <= 64 && (want == 1 || (want * tiles <= 1024 && want * 64 <= rows)); ++want) {
+    // every number of splits up to 16, then an eighth more each time: the estimate is not finer, and a call takes this long
+    for (size_t want = 1; want == 1 || (want <= 512 && want * tiles <= 1024 && want * 64 <= rows); want += want < 16 ? 1 : want / 8) {
       const size_t step = rows ? ((rows + want - 1) / want + 63) / 64 * 64 : 64, splits = rows ? (rows + step - 1) / step : 1;
-      if (splits != want) continue;  // a smaller number has the same steps
       const double t = grad_estimate(form, dtype == CSWAP_DT_F32, tiles, splits, step, n, k);
       if (best.splits == 0 || t < least) {
         least = t;
@@ -566,7 +577,7 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
   };
   if (int e = dtype == CSWAP_DT_F32 ? launch(F32()) : dtype == CSWAP_DT_BF16 ? launch(BF16()) : launch(F16())) return e;
   if (direct) return CSWAP_OK;
-  const size_t dw_groups = (n * k + 1023) / 1024;
+  const size_t dw_groups = p.splits > kFewSplits ? (n * k + 31) / 32 : (n * k + 1023) / 1024;
   const GradSums sums = {part, part_b, n * k, dw_groups, p.splits, (uint32_t)bias_parts(p), (uint32_t)n};
   const auto reduce = [&](auto t) {
     typedef decltype(t) O;

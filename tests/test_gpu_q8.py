@@ -280,7 +280,7 @@ def test_weight_grad_keeps_the_last_bits_of_fp32():
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("rows,n,k", [(3001, 777, 333), (16384, 768, 768), (16000, 300, 2000), (200, 5000, 70), (20001, 603, 701)])
+@pytest.mark.parametrize("rows,n,k", [(3001, 777, 333), (16384, 768, 768), (16000, 300, 2000), (200, 5000, 70), (20001, 603, 701), (100003, 33, 17)])
 def test_weight_grad_of_whole_numbers_is_exact(dtype, rows, n, k):
     """Sums below 2^24: every order of fp32 additions gives the exact result, and a value left out or taken twice shows."""
     g = torch.Generator().manual_seed(rows + n + k)
