@@ -284,8 +284,7 @@ __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typenam
   if (!part && !grads.dgamma && !grads.dbeta) return;
   float* const share = part ? part + (size_t)blockIdx.x * 2 * s.cols : nullptr;
   if constexpr (F::rows > 1) {
-    // the lanes that have the same columns one after the other, in a fixed order: within a wavefront by exchanges, then a turn for
-    // each quarter of the workgroup's rows
+    // the lanes that have the same columns, in a fixed order: those of a wavefront by exchanges, then the sets through LDS
     constexpr int kCols = F::lanes * F::chunks * kChunk, kWide = F::lanes < 64 ? 64 : F::lanes, kSets = F::threads / kWide;
     __shared__ __attribute__((aligned(16))) float sum[kSets * 2 * kCols];
 #pragma unroll

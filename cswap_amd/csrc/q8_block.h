@@ -148,16 +148,21 @@ template <typename T> __device__ inline void store_chunk(typename T::value* p, i
 // The unit that a scale byte stands for; 255 gives infinity.
 __device__ inline float unit_of(uint32_t scale) { return __uint_as_float(scale << 23); }
 
-// The largest magnitude of the group that this lane's quad holds, as its bits: NaN and infinity compare largest.  All four
+// The larger, the smaller of two values; NaN where either is.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ inline float smaller(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+
+// The largest magnitude of the group that this lane's quad holds, as its bits: NaN compares largest, then infinity.  All four
 // lanes of the quad have to run this.
 __device__ inline uint32_t quad_max_bits(const float v[8])
 {
-  uint32_t m = 0;
+  // v_maximum3_f32 takes magnitudes and passes NaN on
+  float m = larger(__builtin_fabsf(v[0]), __builtin_fabsf(v[1]));
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xb1, 0xf, 0xf, true));  // lane ^ 1
-  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4e, 0xf, 0xf, true));  // lane ^ 2
-  return m;
+  for (int i = 2; i < kChunk; i += 2) m = larger(larger(m, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+  m = larger(m, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, m), 0xb1, 0xf, 0xf, true)));  // lane ^ 1
+  m = larger(m, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, m), 0x4e, 0xf, 0xf, true)));  // lane ^ 2
+  return __float_as_uint(m) & 0x7fffffffu;
 }
 
 // Eight codes (byte i of the pair is value i) and the group's scale byte.  KEEP_SIGN: a value that is not 0 has no code of 0 but 1

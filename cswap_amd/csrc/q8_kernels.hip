@@ -85,51 +85,55 @@ __global__ __launch_bounds__(kThreads) void q8_unpack_kernel(const uint2* __rest
 }
 
 // ---------------------------------------------------------------- activation functions
-// Each gives y(x) and its slope in fp32.  v_exp_f32 and v_rcp_f32 are off by one unit in the last place.
+// Each gives y(x) and its slope in fp32.  v_exp_f32 and v_rcp_f32 are off by one unit in the last place and take four turns of
+// the vector unit each, of 18 to 30 in all for a value with its conversions: at 6 TB/s of 16-bit values these count.
 constexpr float kLog2e = 1.4426950408889634f;
 
-// 1 / (1 + exp(-z)) from 2^(-z log2 e); the exponent is held below 126 so that both it and 1 - s stay finite: e * s is 1 - s
-// without the cancellation.  A comparison with NaN is false, so NaN goes through.
+// s = 1 / (1 + e) and 1 - s = e s, the second without the cancellation, from e = 2^a, a = -z log2 e.  The callers hold a below 126,
+// so that e and e s are finite.
 struct Sigmoid {
   float s, one_minus;
 };
-__device__ inline Sigmoid sigmoid(float z)
+__device__ inline Sigmoid sigmoid(float a)
 {
-  float a = -z * kLog2e;
-  a = a > 126.0f ? 126.0f : a;
   const float e = __builtin_amdgcn_exp2f(a);
   const float s = __builtin_amdgcn_rcpf(1.0f + e);
   return {s, e * s};
 }
 
+// x s(x).  Below -87 the function is less than 2e-36 off 0, and s must not meet a large x.
 struct Silu {
-  // below -100 the function is less than 1e-41 off 0, and s, held at 2^-126, must not meet a large x
   template <typename T> static __device__ inline float value(float x)
   {
-    return (x < -100.0f ? -100.0f : x) * sigmoid(x).s;
+    x = larger(x, -87.0f);
+    return x * sigmoid(x * -kLog2e).s;
   }
   template <typename T> static __device__ inline float slope(float x)
   {
-    const Sigmoid g = sigmoid(x);
-    const float xc = x < -100.0f ? -100.0f : x;
-    return g.s * __builtin_fmaf(xc, g.one_minus, 1.0f);
+    x = larger(x, -87.0f);
+    const Sigmoid g = sigmoid(x * -kLog2e);
+    return g.s * __builtin_fmaf(x, g.one_minus, 1.0f);
   }
 };
 
-// x s(2 u), u = sqrt(2/pi) (x + 0.044715 x^3)
+// x s(2 u), u = sqrt(2/pi) (x + 0.044715 x^3); below -10 the same.  Beyond 10 the sigmoid is 1, and the cubic's slope must not
+// overflow.
 struct GeluTanh {
   static constexpr float kC2 = 1.5957691216057308f, kC2A = kC2 * 0.044715f;  // 2 sqrt(2/pi) and that times a
+  static __device__ inline Sigmoid parts(float x, float xx)
+  {
+    return sigmoid(x * __builtin_fmaf(-kLog2e * kC2A, xx, -kLog2e * kC2));
+  }
   template <typename T> static __device__ inline float value(float x)
   {
-    const float z = x * __builtin_fmaf(kC2A, x * x, kC2);
-    return (x < -12.0f ? -12.0f : x) * sigmoid(z).s;
+    x = larger(x, -10.0f);
+    return x * parts(x, x * x).s;
   }
   template <typename T> static __device__ inline float slope(float x)
   {
-    // beyond 12 the sigmoid is 0 or 1 in fp32; the cubic's slope must not overflow there
-    x = x > 12.0f ? 12.0f : x < -12.0f ? -12.0f : x;
+    x = smaller(larger(x, -10.0f), 10.0f);
     const float xx = x * x;
-    const Sigmoid g = sigmoid(x * __builtin_fmaf(kC2A, xx, kC2));
+    const Sigmoid g = parts(x, xx);
     return g.s * __builtin_fmaf(x * g.one_minus, __builtin_fmaf(3.0f * kC2A, xx, kC2), 1.0f);
   }
 };
@@ -171,10 +175,9 @@ struct Gelu {
   }
   template <typename T> static __device__ inline float value(float x)
   {
-    // x >= 0: x - x tail, else x tail; the product with the tail is 0 at infinity, not NaN
-    const float z = __builtin_fabsf(x);
-    const float zc = z > 1e30f ? 1e30f : z;
-    return __builtin_fmaf(-zc, parts<T>(x).tail, x > 0.0f ? x : 0.0f);
+    // x >= 0: x - x tail, else x tail; the product with the tail is 0 at infinity, not NaN (a NaN comes with the tail)
+    const float z = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.0f, 1e30f);
+    return __builtin_fmaf(-z, parts<T>(x).tail, __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()));
   }
   template <typename T> static __device__ inline float slope(float x)
   {
