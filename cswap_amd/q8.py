@@ -50,7 +50,7 @@ class Checkpoint8:
             raise ValueError("codes and scales are contiguous and on one device")
         if dtype not in _DTYPE:
             raise TypeError(f"checkpoints are made of float32, bfloat16 and float16 tensors, not {dtype}")
-        self.shape, self.dtype, self.device, self.rows, self.cols = tuple(shape), dtype, codes.device, rows, cols
+        self.shape, self.dtype, self.device, self.rows, self.cols = torch.Size(shape), dtype, codes.device, rows, cols
         self._codes, self._scales, self._room = codes, scales, None
         self._at, self._scales_at = codes.data_ptr(), scales.data_ptr()
 
@@ -59,7 +59,7 @@ class Checkpoint8:
         """The checkpoint in ``room``: codes, and scales behind them; the tensors over either are made when they are
         asked for."""
         self = cls.__new__(cls)
-        self.shape, self.dtype, self.device, self.rows, self.cols = shape, dtype, room.device, rows, cols
+        self.shape, self.dtype, self.device, self.rows, self.cols = torch.Size(shape), dtype, room.device, rows, cols
         self._codes = self._scales = None
         self._room = room
         self._at = at = room.data_ptr()
@@ -102,22 +102,27 @@ def _rows_cols(shape):
     return (math.prod(shape[:-1]), shape[-1]) if n else (1, 1)
 
 
-def _stream_of(device: torch.device):
-    """The current stream of the current device, if that is ``device``; else None: the call is then made again with
-    its tensor's device current, whose stream is the one to launch on."""
-    index = torch.cuda.current_device()
-    if device.index != index:
-        return None
-    return api._raw_stream(index) if api._raw_stream is not None else api._stream()
+# torch's own short cut to the current device's number, as api has one to the stream's handle
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _need(t: torch.Tensor, what: str) -> int:
+def _begin(t: torch.Tensor, what: str):
+    """Type and device of a tensor in device memory, and the stream to launch on: the current one of its device, if that
+    is the current device, else None. The call is then made again with its device current."""
     kind = _DTYPE.get(t.dtype)
     if kind is None:
         raise TypeError(f"{what}: float32, bfloat16 or float16, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{what}: expected a tensor in device memory")
-    return kind
+    device = t.device
+    return kind, device, _stream_of(device)
+
+
+def _stream_of(device: torch.device):
+    index = device.index
+    if index != _current_device():
+        return None
+    return api._raw_stream(index) if api._raw_stream is not None else api._stream()
 
 
 def _row_stride(t: torch.Tensor, what: str) -> int:
@@ -176,12 +181,11 @@ def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) ->
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
     is the same either way, and only such a flat checkpoint has rows for the backward passes.  ``keep_sign``: what is
     not 0 but rounds to 0 is held as the smallest value with its sign."""
-    kind, device = _need(x, "q8_compress"), x.device
-    stream = _stream_of(device)
+    kind, device, stream = _begin(x, "q8_compress")
     if stream is None:
         with torch.cuda.device(device):
             return q8_compress(x, flat, keep_sign)
-    stride = _row_stride(x, "q8_compress")
+    stride = 0 if x.is_contiguous() else _row_stride(x, "q8_compress")
     rows, cols = _rows_cols(x.shape)
     if cols == 0:
         raise ValueError("q8_compress: rows without values")
@@ -205,17 +209,20 @@ def q8_decompress(held: Checkpoint8, out: torch.Tensor | None = None, dtype: tor
         with torch.cuda.device(device):
             return q8_decompress(held, out, dtype)
     if out is None:
-        out = torch.empty(held.shape, dtype=dtype or held.dtype, device=device)
-        stride = 0
+        dtype = dtype or held.dtype
+        out = torch.empty(held.shape, dtype=dtype, device=device)
+        kind, stride = _DTYPE.get(dtype), 0
+        if kind is None:
+            raise TypeError(f"q8_decompress: float32, bfloat16 or float16, not {dtype}")
     else:
-        if out.shape != torch.Size(held.shape) or (dtype is not None and out.dtype != dtype):
+        if out.shape != held.shape or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"q8_decompress: out is {tuple(out.shape)} {out.dtype}")
         if out.device != device:
             raise ValueError(f"q8_decompress: out on {out.device}, not on {device}")
-        stride = _row_stride(out, "q8_decompress")
+        kind, stride = _begin(out, "q8_decompress: out")[0], _row_stride(out, "q8_decompress")
         if stride and held.rows != _rows_cols(held.shape)[0]:
             raise ValueError("q8_decompress: a flat checkpoint goes into a contiguous tensor")
-    check(lib().cswap_q8_unpack(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), _need(out, "q8_decompress"),
+    check(lib().cswap_q8_unpack(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), kind,
                                 stride, stream), "cswap_q8_unpack")
     return out
 
@@ -230,12 +237,12 @@ def _kind_of(kind: str) -> int:
 def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
     """``(f(x), checkpoint of x)`` in one pass; ``kind``: "gelu", "gelu_tanh" or "silu".  The second is None with
     ``checkpoint=False``."""
-    k, dtype, device = _kind_of(kind), _need(x, "q8_act"), x.device
-    stream = _stream_of(device)
+    k = _kind_of(kind)
+    dtype, device, stream = _begin(x, "q8_act")
     if stream is None:
         with torch.cuda.device(device):
             return q8_act(x, kind, checkpoint)
-    stride = _row_stride(x, "q8_act")
+    stride = 0 if x.is_contiguous() else _row_stride(x, "q8_act")
     rows, cols = _rows_cols(x.shape)
     if cols == 0:
         raise ValueError("q8_act: rows without values")
@@ -251,12 +258,12 @@ def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
 
 
 def _need_gradient(dy: torch.Tensor, held, what: str):
-    """dy's type and row stride; it goes with an input of held's shape and type."""
-    kind = _need(dy, what)
-    if tuple(dy.shape) != tuple(held.shape) or dy.dtype != held.dtype or dy.device != held.device:
+    """``_begin`` of dy, and its row stride; it goes with an input of held's shape and type."""
+    kind, device, stream = _begin(dy, what)
+    if dy.shape != held.shape or dy.dtype != held.dtype or device != held.device:
         raise ValueError(f"{what}: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, the input was {tuple(held.shape)} "
                          f"{held.dtype} on {held.device}")
-    return kind, _row_stride(dy, what)
+    return kind, device, stream, 0 if dy.is_contiguous() else _row_stride(dy, what)
 
 
 def _need_rows(held: Checkpoint8, what: str):
@@ -270,10 +277,9 @@ def _need_rows(held: Checkpoint8, what: str):
 def q8_act_backward(dy: torch.Tensor, held: Checkpoint8, kind: str = "gelu") -> torch.Tensor:
     """``dy * f'(x)``, x as ``held`` has it."""
     k = _kind_of(kind)
-    dtype, stride = _need_gradient(dy, held, "q8_act_backward")
-    stream = _stream_of(dy.device)
+    dtype, device, stream, stride = _need_gradient(dy, held, "q8_act_backward")
     if stream is None:
-        with torch.cuda.device(dy.device):
+        with torch.cuda.device(device):
             return q8_act_backward(dy, held, kind)
     rows, cols = _need_rows(held, "q8_act_backward")
     dx = _like(dy, stride)
@@ -289,12 +295,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``.  A checkpoint is off by up to
     2^-7 of the largest magnitude nearby, mean included: rows whose mean is many times their deviation are better kept
     as they are."""
-    dtype, device = _need(x, "layer_norm"), x.device
-    stream = _stream_of(device)
+    dtype, device, stream = _begin(x, "layer_norm")
     if stream is None:
         with torch.cuda.device(device):
             return layer_norm(x, weight, bias, eps, checkpoint)
-    stride = _row_stride(x, "layer_norm")
+    stride = 0 if x.is_contiguous() else _row_stride(x, "layer_norm")
     rows, cols = _rows_cols(x.shape)
     if cols == 0 or x.dim() == 0:
         raise ValueError("layer_norm: rows without values")
@@ -320,9 +325,7 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
                         param_dtype: torch.dtype | None = None):
     """``(dx, dweight, dbias)``; ``held`` is what ``layer_norm`` returned last.  The parameters' gradients come in
     ``param_dtype`` (the weight's type, else dy's)."""
-    dtype, stride = _need_gradient(dy, held, "layer_norm_backward")
-    device = dy.device
-    stream = _stream_of(device)
+    dtype, device, stream, stride = _need_gradient(dy, held, "layer_norm_backward")
     if stream is None:
         with torch.cuda.device(device):
             return layer_norm_backward(dy, held, mean, rstd, weight, param_dtype)
@@ -357,20 +360,20 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
 def q8_weight_grad(dy: torch.Tensor, held: Checkpoint8, bias: bool = True, out_dtype: torch.dtype | None = None):
     """``(dW, db)`` of ``y = x @ W.T + b`` from ``dy`` and the checkpoint of ``x``: ``dy.T @ x`` and ``dy.sum(0)`` over
     all rows, in ``out_dtype`` (dy's type); ``db`` is None without ``bias``."""
-    kind, device = _need(dy, "q8_weight_grad: dy"), dy.device
+    kind, device, stream = _begin(dy, "q8_weight_grad: dy")
     if device != held.device:
         raise ValueError(f"q8_weight_grad: dy on {device}, the input's checkpoint on {held.device}")
-    stream = _stream_of(device)
     if stream is None:
         with torch.cuda.device(device):
             return q8_weight_grad(dy, held, bias, out_dtype)
     rows, k = _need_rows(held, "q8_weight_grad")
-    if dy.dim() == 0 or tuple(dy.shape[:-1]) != tuple(held.shape[:-1]):
+    shape = dy.shape
+    if len(shape) == 0 or shape[:-1] != held.shape[:-1]:
         raise ValueError(f"q8_weight_grad: dy is {tuple(dy.shape)}, the input was {tuple(held.shape)}")
     if dy.dtype == torch.float16 and held.dtype != torch.float16:
         raise TypeError("q8_weight_grad: a float16 dy goes with the checkpoint of a float16 input")
-    stride = _row_stride(dy, "q8_weight_grad: dy")
-    n = dy.shape[-1]
+    stride = 0 if dy.is_contiguous() else _row_stride(dy, "q8_weight_grad: dy")
+    n = shape[-1]
     if n == 0:
         raise ValueError("q8_weight_grad: rows without values")
     out_dtype = out_dtype or dy.dtype

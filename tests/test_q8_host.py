@@ -185,7 +185,7 @@ def test_a_tensor_on_another_device_makes_that_device_current(monkeypatch):
         device = property(lambda self: torch.device("cuda", 1))
 
     x = torch.zeros(4, 40).as_subclass(OnDevice1)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(q8, "_current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", device)
     monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
     monkeypatch.setattr(q8, "_empty_checkpoint", lambda t, rows, cols, device: checkpoint((4, 40), rows, cols))
