@@ -9,8 +9,8 @@
 // 1024 values is one wavefront's or less, so nothing waits for a barrier; longer ones share a sum through LDS with one barrier
 // each.  Either kernel asks for a workgroup's next row before it works on this one.
 //
-// Tensors in turn: 16384 x 768 bf16 forward 15.0 us (4.2 TB/s; one row at a time 16.1), backward 19.7 with its sums (44 in the first
-// form: a row at a time, 512 shares, 8 lanes to sum a column); 2048 x 8192 fp32 32.3 and 38.7 (4.7 and 3.9 TB/s); 4096 x 16384
+// Tensors in turn: 16384 x 768 bf16 forward 13.5 us (4.7 TB/s), backward 17.6 with its sums (44 in the first form: a row at a
+// time, 512 shares, 8 lanes to sum a column); 2048 x 8192 fp32 32.3 and 38.7 (4.7 and 3.9 TB/s); 4096 x 16384
 // bf16 66 and 81.  Shares by wavefronts of 1024 threads in rows of 513 to 1024 values spill (16384 x 768 fp32 backward 38 : 24 us with 512 threads).
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(F::threads) void norm_backward_kernel(const typenam
 #pragma unroll
     for (int i = 0; i < kChunk; ++i) dg[c][i] = db[c][i] = 0.0f;
   }
-  constexpr bool kAhead = F::chunks == 1 || F::lanes == 64;  // registers for two rows
+  constexpr bool kAhead = F::chunks == 1 || F::lanes <= 64;  // registers for two rows
   RowChunk<T, HELD> next[F::chunks];
   float next_mu, next_r;
   auto load = [&](uint32_t row) {
@@ -363,21 +363,33 @@ template <typename F> static unsigned groups_for(size_t rows, unsigned most)
   return (unsigned)(want < most ? want : most);
 }
 
-template <typename Fn> static auto with_forward_form(size_t cols, Fn&& fn)
+// Many rows of 513 to 768 values in a 16-bit type: half a wavefront with three chunks a lane, none idle at 768 (16384 x 768 bf16
+// forward 13.6 us, with a wavefront and two chunks 14.9; backward 17.5 and 20.1; 8192 rows 9.2 and 9.6, 12.7 and 12.8, 4096 rows
+// 6.1 and 6.3, 9.9 and 9.6).  In fp32 it is 28.5 and 26.5, 29.6 and 29.3.
+template <typename T> static bool half_wave(size_t rows, size_t cols)
 {
+  return T::bytes == 2 && cols > 512 && cols <= 768 && rows >= 8192;
+}
+
+template <typename T, typename Fn> static auto with_forward_form(size_t rows, size_t cols, Fn&& fn)
+{
+  if constexpr (T::bytes == 2)
+    if (half_wave<T>(rows, cols)) return fn(Form<32, 3, 256>());
   if (cols <= 128) return fn(Form<16, 1, 256>());
   if (cols <= 256) return fn(Form<32, 1, 256>());
   if (cols <= 512) return fn(Form<64, 1, 256>());
   if (cols <= 1024) return fn(Form<64, 2, 256>());
-  if (cols <= 2048) return fn(Form<256, 1, 256>());
+  if (cols <= 2048) return fn(Form<128, 2, 256>());  // 8192 x 1536 bf16 14.7 us, with 256 lanes 17.7; fp32 25.3 and 24.7
   if (cols <= 4096) return fn(Form<256, 2, 256>());
   if (cols <= 8192) return fn(Form<512, 2, 512>());
   return fn(Form<1024, 2, 1024>());
 }
 
 // Large workgroups: as few shares of the parameters' gradients as there are compute units.
-template <typename Fn> static auto with_backward_form(size_t cols, Fn&& fn)
+template <typename T, typename Fn> static auto with_backward_form(size_t rows, size_t cols, Fn&& fn)
 {
+  if constexpr (T::bytes == 2)
+    if (half_wave<T>(rows, cols)) return fn(Form<32, 3, 512>());
   if (cols <= 128) return fn(Form<16, 1, 1024>());
   if (cols <= 256) return fn(Form<32, 1, 1024>());
   if (cols <= 512) return fn(Form<64, 1, 1024>());
@@ -391,7 +403,7 @@ template <typename Fn> static auto with_backward_form(size_t cols, Fn&& fn)
 // One workgroup for as many rows as it takes in four turns: it needs no second kernel for the parameters' gradients.
 static unsigned backward_groups(size_t rows, size_t cols)
 {
-  return with_backward_form(cols, [&](auto f) {
+  return with_backward_form<F32>(rows, cols, [&](auto f) {  // of any type: there are kMostBackward where forms differ
     typedef decltype(f) F;
     return rows <= 4 * F::rows ? 1u : groups_for<F>(rows, kMostBackward);
   });
@@ -445,7 +457,7 @@ extern "C" int cswap_layer_norm_forward(const void* d_x, int dtype, size_t rows,
   hipStream_t st = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    return with_forward_form(cols, [&](auto f) {
+    return with_forward_form<T>(rows, cols, [&](auto f) {
       typedef decltype(f) F;
       auto k = d_codes ? norm_forward_kernel<T, F, true> : norm_forward_kernel<T, F, false>;
       hipLaunchKernelGGL(k, dim3(groups_for<F>(rows, kForwardThreads / F::threads)), dim3(F::threads), 0, st,
@@ -490,7 +502,7 @@ extern "C" int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t row
   if (rows) {
     const int e = with_type(dtype, [&](auto t) {
       typedef decltype(t) T;
-      return with_backward_form(cols, [&](auto f) {
+      return with_backward_form<T>(rows, cols, [&](auto f) {
         typedef decltype(f) F;
         auto k = d_codes ? norm_backward_kernel<T, F, true> : norm_backward_kernel<T, F, false>;
         hipLaunchKernelGGL(k, dim3(grid), dim3(F::threads), 0, st, static_cast<const typename T::value*>(d_dy),

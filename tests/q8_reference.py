@@ -106,8 +106,8 @@ def norm(x, kept, dy, w, b, eps):
 
 
 def norm_error(x, kept, dy, w, b, eps):
-    """Bounds on what fp32 leaves of them.  A row's sums have at most 16 terms in a lane and 4 + 2 + 16 joins: k = 40 with
-    the factor 1 / cols.  The parameters' sums: one rounding a row at most, and 80 for the joins."""
+    """Bounds on what fp32 leaves of them.  A row's sums have at most 16 terms in a lane and 4 + 2 + 16 joins, or 24 and 5:
+    k = 40 with the factor 1 / cols.  The parameters' sums: one rounding a row at most, and 80 for the joins."""
     k = 40
     mu = x.mean(dim=1, keepdim=True)
     d = x - mu

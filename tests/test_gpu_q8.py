@@ -96,6 +96,23 @@ def test_signs_that_are_kept(dtype):
     assert torch.equal(torch.sign(q8().q8_decompress(kept).float()).cpu(), torch.sign(x.float()))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_signs_that_are_kept(dtype):
+    """What is not 0 has a code that is not 0, with its sign; the other codes are the same."""
+    x = values(50, 130, dtype, 31)
+    x[::3, ::7] = 0.0
+    x[1::3, 1::5] *= 1e-4
+    x[0, 64:96] = torch.finfo(dtype).tiny
+    x[0, 64], x[0, 65] = 1.0, -torch.finfo(dtype).tiny
+    plain, kept = q8().q8_compress(x.cuda()), q8().q8_compress(x.cuda(), keep_sign=True)
+    assert torch.equal(plain.scales, kept.scales)
+    a, b, sign = plain.codes.cpu().int(), kept.codes.cpu().int(), torch.zeros(50, 160, dtype=torch.int32)
+    sign[:, :130] = torch.sign(x.float()).int()
+    assert int((sign[a == 0] != 0).sum()) > 100
+    assert torch.equal(b, torch.where(a == 0, sign, a))
+    assert torch.equal(torch.sign(q8().q8_decompress(kept).float()).cpu(), torch.sign(x.float()))
+
+
 def test_flat_checkpoints():
     x = values(6, 4 * 5, F32).view(6, 4, 5)
     held = q8().q8_compress(x.cuda(), flat=True)
@@ -199,6 +216,23 @@ def test_layer_norm_of_many_rows_twice_gives_the_same_bits(rows):
     want, err = ref.norm(*args), ref.norm_error(*args)
     for name, got, at in zip(("y", "dx", "dw", "db"), outs[0], (0, 3, 4, 5)):
         ref.check(got, want[at], err[at], BF16, name)
+
+
+@pytest.mark.parametrize("checkpoint", [True, False])
+@pytest.mark.parametrize("dtype,rows,cols", [(BF16, 8197, 513), (F16, 8192, 768), (BF16, 9001, 700), (BF16, 8191, 640)], ids=str)
+def test_layer_norm_of_many_rows_of_513_to_768_values(dtype, rows, cols, checkpoint):
+    m = q8()
+    x, dy = values(rows, cols, dtype, 41), values(rows, cols, dtype, 42, 0.1)
+    w, b = values(1, cols, F32, 43)[0], values(1, cols, F32, 44)[0]
+    y, mean, rstd, held = m.layer_norm(x.cuda(), w.cuda(), b.cuda(), 1e-5, checkpoint=checkpoint)
+    dx, dw, db = m.layer_norm_backward(dy.cuda(), held, mean, rstd, w.cuda())
+    if checkpoint:
+        assert torch.equal(held.codes.cpu(), ref.pack(x)[0]) and torch.equal(held.scales.cpu(), ref.pack(x)[1])
+    args = (x.double(), ref.held(x) if checkpoint else x.double(), dy.double(), w.double(), b.double(), 1e-5)
+    for name, got, want, err, t in zip(("y", "mean", "rstd", "dx", "dw", "db"), (y, mean, rstd, dx, dw, db), ref.norm(*args),
+                                       ref.norm_error(*args), (dtype, F32, F32, dtype, F32, F32)):
+        assert got.dtype == t
+        ref.check(got, want, err, t, name)
 
 
 def test_layer_norm_without_parameters_and_with_a_large_mean():
