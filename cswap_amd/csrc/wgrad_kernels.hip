@@ -94,9 +94,10 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
 }
 
 // A workgroup of 2 x WK wavefronts makes a TN x TK tile of dW from one split of the rows, BK rows (a stage) at a time.  A
-// product of 32 x 32 x 16 takes 0.75 fragments from LDS in a tile of 256 x 256, 1 in one of 128 x 256 and 1.5 in one of 128 x 128, and
-// the small ones read either operand twice as often from the caches; of the large and middle ones one fits a compute unit (128 KB
-// of LDS for two stages), of the small ones two, and more of them there are where dW is small.
+// product of 32 x 32 x 16 takes 0.75 fragments from LDS in a tile of 256 x 256, 1 in one of 128 x 256, 1.25 in a narrow one of
+// 64 x 256 and 1.5 in one of 128 x 128, and the small ones read either operand twice as often from the caches; of the large and
+// middle ones one fits a compute unit (128 KB of LDS for two stages), of the others two, and more of them there are where dW is
+// small.
 //
 // The tile of a stage lies in LDS as it does in memory, m by m, in chunks of 16 bytes whose order within a row depends on m: the
 // transposing reads take four rows at once, which have to lie in different banks.  a_at and b_at are the places of value
@@ -104,7 +105,11 @@ __device__ inline uint4 read_turned(const uint16_t* at, int four_rows)
 template <typename T, int TN, int TK, int BK> struct GradTile {
   static constexpr int P = Feed<T>::parts;
   static constexpr int kAPlane = BK * TN, kStage = P * kAPlane + BK * TK;
-  static __device__ inline int a_at(int m, int col) { return m * TN + 8 * ((col >> 3) ^ ((m & 3) << 2)) + (col & 7); }
+  static __device__ inline int a_at(int m, int col)
+  {
+    // in a tile of 64 columns two rows take all banks: of four, two differ in the order
+    return m * TN + 8 * ((col >> 3) ^ (TN == 64 ? (m & 2) << 1 : (m & 3) << 2)) + (col & 7);
+  }
   static __device__ inline int b_at(int m, int col)
   {
     // pieces of 16 codes leave a lane as two chunks: those of all pieces first, then those of the others, so that neighbouring
@@ -462,9 +467,13 @@ template <typename O> __global__ __launch_bounds__(256) void weight_grad_reduce_
 constexpr size_t kMaxGradSide = (size_t)1 << 20;    // features on either side
 constexpr size_t kMaxGradStride = (size_t)1 << 24;  // a workgroup's offsets within 32 rows are 32 bits
 
-// Tiles of dW: n x k features.
-enum GradForm { kSmallTile, kMiddleTile, kLargeTile, kGradForms };
-constexpr size_t kTileN[kGradForms] = {128, 128, 256}, kTileK[kGradForms] = {128, 256, 256};
+// Tiles of dW: n x k features.  The narrow ones are for an fp32 dY of few columns, whose three products of those that are not there
+// cost the most: in us, narrow : others, 32768 x 8 x 2048 37 : 55, 32768 x 64 x 4096 72 : 102, 8192 x 64 x 768 19.1 : 20.3, but
+// 32768 x 320 x 256 37 : 33; bf16 32768 x 64 x 4096 50.5 : 51.9, 8192 x 64 x 2048 23.8 : 18.6.
+enum GradForm { kSmallTile, kMiddleTile, kLargeTile, kNarrowTile, kGradForms };
+constexpr size_t kTileN[kGradForms] = {128, 128, 256, 64}, kTileK[kGradForms] = {128, 256, 256, 256};
+
+static bool narrow_fits(int dtype, size_t n, size_t k) { return dtype == CSWAP_DT_F32 && n <= 64 && k > 128; }
 
 struct GradPlan {
   int form;
@@ -473,7 +482,7 @@ struct GradPlan {
 };
 
 // Tiles and splits with the least estimated time.  Measured on 256 compute units, in us: a workgroup takes `stage` for 64 rows, a
-// compute unit with two workgroups of the small tiles `pair` for 64 rows of both; `fixed` is the rest of a launch; splits cost
+// compute unit with two workgroups of the small or narrow tiles `pair` for 64 rows of both; `fixed` is the rest of a launch; splits cost
 // the sums' launch (5) and their bytes there and back at 5.5 TB/s.  What it decides between, small : middle : large tiles in us,
 // each with its best splits.  bf16: 512 x 2048 x 2048 14 : 18 : 33, 8192 x 768 x 768 28.5 : 28.6 : 36, 8192 x 1024 x 1024 39.7 : 37.6 :
 // 43, 8192 x 2048 x 2048 102 : 91 : 86, 32768 x 4096 x 1024 371 : 328 : 273, 2048 x 4096 x 4096 92 : 84 : 71; fp32: 8192 x 768 x 768
@@ -481,10 +490,12 @@ struct GradPlan {
 // one : two workgroups a compute unit, bf16: 2048 x 2048 x 2048 (not split : in two) 36.6 : 40.9, 32768 x 768 x 768 77 : 66.
 static double grad_estimate(int form, bool f32, size_t tiles, size_t splits, size_t step, size_t n, size_t k)
 {
-  constexpr double kFixed[kGradForms] = {8.0, 9.5, 11.0};
-  constexpr double kStage[2][kGradForms] = {{0.77, 1.05, 1.65}, {1.9, 2.35, 4.4}}, kPair[2] = {1.2, 3.2};
-  const size_t groups = tiles * splits, at_once = form == kSmallTile ? 512 : 256, rest = groups % at_once;
-  const double units = (double)step / 64, stage = kStage[f32][form], both = form == kSmallTile ? kPair[f32] : stage;
+  constexpr double kFixed[kGradForms] = {8.0, 9.5, 11.0, 8.0};
+  constexpr double kStage[2][kGradForms] = {{0.77, 1.05, 1.65}, {1.9, 2.35, 4.4, 1.75}};
+  constexpr double kPair[2][kGradForms] = {{1.2, 1.05, 1.65}, {3.2, 2.35, 4.4, 3.0}};
+  const bool two = form == kSmallTile || form == kNarrowTile;
+  const size_t groups = tiles * splits, at_once = two ? 512 : 256, rest = groups % at_once;
+  const double units = (double)step / 64, stage = kStage[f32][form], both = kPair[f32][form];
   double t = kFixed[form] + (double)(groups / at_once) * units * both;
   if (rest) t += units * (rest > 256 ? both : stage);
   if (splits > 1) t += 5.0 + (double)(splits * n * k) * 8.0 / 5.5e6;
@@ -496,6 +507,7 @@ static GradPlan grad_plan(int dtype, size_t rows, size_t n, size_t k)
   GradPlan best = {};
   double least = 0.0;
   for (int form = 0; form < kGradForms; ++form) {
+    if (form == kNarrowTile && !narrow_fits(dtype, n, k)) continue;
     const size_t tiles_n = (n + kTileN[form] - 1) / kTileN[form], tiles_k = (k + kTileK[form] - 1) / kTileK[form];
     const size_t tiles = tiles_n * tiles_k;
     // every number of splits up to 16, then an eighth more each time: the estimate is not finer, and a call takes this long
@@ -570,7 +582,10 @@ extern "C" int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, si
     auto kernel = p.form == kLargeTile    ? weight_grad_kernel<T, 256, 256, BK, 4>
                   : p.form == kMiddleTile ? weight_grad_kernel<T, 128, 256, BK, 4>
                                           : weight_grad_kernel<T, 128, 128, BK, kSmall>;
-    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(p.form == kSmallTile ? 128 * kSmall : 512), 0, st,
+    unsigned threads = p.form == kSmallTile ? 128 * kSmall : 512;
+    if constexpr (T::bytes == 4)
+      if (p.form == kNarrowTile) kernel = weight_grad_kernel<T, 64, 256, BK, 2>, threads = 256;
+    hipLaunchKernelGGL(kernel, dim3(p.tiles_n * p.tiles_k * p.splits), dim3(threads), 0, st,
                        static_cast<const typename T::value*>(d_dy), d_codes, d_scales, s, direct ? d_dw : part,
                        !d_db ? nullptr : direct ? d_db : part_b, direct ? out_dtype : -1);
     return check_launch();

@@ -58,7 +58,7 @@ int cswap_test_zfp_store_hint(unsigned long long base, unsigned long long pitch,
 int cswap_test_zfp_decode_runs(size_t nx, size_t ny, size_t nz, ptrdiff_t sy, ptrdiff_t sz, unsigned base);
 
 /* How cswap_q8_weight_grad lays out a call: the number of splits of the rows, and 1000 more with
- * tiles of 128 x 256 features, 2000 more with 256 x 256 (else 128 x 128).  Host only. */
+ * tiles of 128 x 256 features, 2000 more with 256 x 256, 3000 more with 64 x 256 (else 128 x 128).  Host only. */
 int cswap_test_weight_grad_plan(int dtype, size_t rows, size_t n, size_t k);
 
 #ifdef __cplusplus

@@ -325,6 +325,23 @@ def test_weight_grad_of_whole_numbers_is_exact(dtype, rows, n, k):
     assert torch.equal(db.cpu(), dy.sum(0).float())
 
 
+@pytest.mark.parametrize("rows,n,k", [(12000, 8, 2048), (30000, 64, 300), (9001, 49, 1000), (20011, 33, 131), (70, 17, 4000),
+                                      (700, 1, 257)])
+def test_weight_grad_of_few_outputs_in_fp32(rows, n, k):
+    """dy has 24 bits, whose three parts each matter, and a row of x at most one value that is not 0: a sum is off by one
+    rounding for each part of each product that is not 0 (parts have dy's sign, so their magnitudes add up to its own)."""
+    g = torch.Generator().manual_seed(rows + n + k)
+    dy = (torch.randint(-(1 << 24) + 1, 1 << 24, (rows, n), generator=g).double() * 2.0 ** -23).to(F32)
+    x = torch.zeros(rows, k)
+    x[torch.arange(rows), torch.randint(0, k, (rows,), generator=g)] = 3.0
+    held = q8().q8_compress(x.cuda())
+    dw, db = q8().q8_weight_grad(dy.cuda(), held)
+    kept = ref.held(x)
+    terms = 2 + 3 * int((x != 0).sum(0).max())
+    ref.check(dw, dy.double().t() @ kept, terms * ref.U * (dy.double().abs().t() @ kept.abs()), F32, "dw")
+    ref.check(db, dy.double().sum(0), ref.weight_grad_error(dy.double(), kept)[1], F32, "db")
+
+
 def test_weight_grad_of_subnormal_values():
     """fp16 below 2^-14 in either operand, bf16 and fp32 below 2^-126: nothing is flushed."""
     g = torch.Generator().manual_seed(24)

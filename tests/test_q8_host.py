@@ -127,6 +127,17 @@ def test_weight_grad_layout():
             assert 2 <= splits <= 512 and room(dtype, rows, n, k) == 4 * splits * (n * k + n * -(-k // (128, 256, 256)[form]))
 
 
+def test_weight_grad_layout_of_few_outputs():
+    """Narrow tiles (3000s) where an fp32 dY has no more columns than they."""
+    plan, room = L().cswap_test_weight_grad_plan, L().cswap_q8_weight_grad_workspace_bytes
+    for rows, n, k in ((12000, 8, 2048), (30000, 64, 300), (9001, 33, 1000)):
+        form, splits = divmod(plan(0, rows, n, k), 1000)
+        assert form == 3 and room(0, rows, n, k) == 4 * splits * (n * k + n * -(-k // 256))
+        assert plan(1, rows, n, k) < 3000
+    for rows, n, k in ((30000, 65, 300), (30000, 192, 2048), (30000, 64, 128)):
+        assert plan(0, rows, n, k) < 3000
+
+
 # ---------------------------------------------------------------- the torch side
 def checkpoint(shape, rows, cols, dtype=torch.float32):
     from cswap_amd.q8 import Checkpoint8
