@@ -185,11 +185,6 @@ template <bool KEEP_SIGN = false> __device__ inline uint2 encode_chunk(const flo
     for (int i = 0; i < kChunk; ++i)
       if (t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
   }
-  if (KEEP_SIGN) {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i)
-      if (t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
-  }
   uint2 q;
   // v_perm_b32 numbers the bytes of its second operand 0 to 3 and those of its first 4 to 7
   q.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400), __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400), 0x05040100);
