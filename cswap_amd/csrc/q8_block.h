@@ -165,9 +165,15 @@ __device__ inline uint32_t quad_max_bits(const float v[8])
   return __float_as_uint(m) & 0x7fffffffu;
 }
 
-// Eight codes (byte i of the pair is value i) and the group's scale byte.  KEEP_SIGN: a value that is not 0 has no code of 0 but 1
-// or -1, the nearest that has its sign.
-template <bool KEEP_SIGN = false> __device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale)
+// What becomes of a value that is not 0 but rounds to 0: the code 0, or 1 or -1, the nearest that has its sign, in every group or in
+// those that have no more than kMostLost of them.  Of one sign, as probabilities are, such codes add up to a bias: rows of a
+// softmax over 512 logits N(0, 9) sum to 1.20 with all signs kept and to 0.991 with few or none (0.998 to 1.0002 for N(0, 1) to N(0, 2.25)
+// with few).
+enum Signs { kRounded = 0, kAllSigns = 1, kFewSigns = 2 };
+constexpr int kMostLost = 2;
+
+// Eight codes (byte i of the pair is value i) and the group's scale byte.  With kFewSigns all four lanes of the quad have to run this.
+template <int SIGNS = kRounded> __device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale)
 {
   const int exponent = (int)(max_bits >> 23);
   const int b = max(exponent - 6, 1);
@@ -180,10 +186,19 @@ template <bool KEEP_SIGN = false> __device__ inline uint2 encode_chunk(const flo
 #pragma unroll
   for (int i = 0; i < kChunk; ++i)
     t[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], inverse, kMagic), kMagic - 127.0f, kMagic + 127.0f));
-  if (KEEP_SIGN) {
+  if (SIGNS != kRounded) {
+    bool keep = true;
+    if (SIGNS == kFewSigns) {
+      int lost = 0;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) lost += t[i] == __float_as_uint(kMagic) && v[i] != 0.0f;
+      lost += __builtin_amdgcn_mov_dpp(lost, 0xb1, 0xf, 0xf, true);  // lane ^ 1
+      lost += __builtin_amdgcn_mov_dpp(lost, 0x4e, 0xf, 0xf, true);  // lane ^ 2
+      keep = lost <= kMostLost;
+    }
 #pragma unroll
     for (int i = 0; i < kChunk; ++i)
-      if (t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
+      if (keep && t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
   }
   uint2 q;
   // v_perm_b32 numbers the bytes of its second operand 0 to 3 and those of its first 4 to 7

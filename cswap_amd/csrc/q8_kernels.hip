@@ -56,7 +56,7 @@ __device__ inline void store_codes(uint32_t chunk, uint2 q, uint32_t scale, uint
   if ((chunk & (kChunksPerGroup - 1)) == 0) scales[chunk / kChunksPerGroup] = (uint8_t)scale;
 }
 
-template <typename T, bool FLAT, bool KEEP_SIGN>
+template <typename T, bool FLAT, int SIGNS>
 __global__ __launch_bounds__(kThreads) void q8_pack_kernel(const typename T::value* __restrict__ in, size_t stride, Shape s,
                                                            size_t flat_cols, uint2* __restrict__ codes,
                                                            uint8_t* __restrict__ scales)
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kThreads) void q8_pack_kernel(const typename T::val
   float v[kChunk];
   load_chunk<T>(in + offset_of<FLAT>(chunk, p, stride), p.valid, v);
   uint32_t scale;
-  const uint2 q = encode_chunk<KEEP_SIGN>(v, quad_max_bits(v), &scale);
+  const uint2 q = encode_chunk<SIGNS>(v, quad_max_bits(v), &scale);
   store_codes(chunk, q, scale, codes, scales);
 }
 
@@ -248,10 +248,11 @@ static int plan(size_t rows, size_t cols, ptrdiff_t* stride_a, ptrdiff_t* stride
 }
 
 template <typename T>
-static int pack(const void* in, size_t stride, bool keep_sign, const Call& c, int8_t* codes, uint8_t* scales, hipStream_t st)
+static int pack(const void* in, size_t stride, int keep_sign, const Call& c, int8_t* codes, uint8_t* scales, hipStream_t st)
 {
-  auto k = keep_sign ? (c.flat ? q8_pack_kernel<T, true, true> : q8_pack_kernel<T, false, true>)
-                     : (c.flat ? q8_pack_kernel<T, true, false> : q8_pack_kernel<T, false, false>);
+  auto k = keep_sign == CSWAP_Q8_FEW_SIGNS ? (c.flat ? q8_pack_kernel<T, true, kFewSigns> : q8_pack_kernel<T, false, kFewSigns>)
+           : keep_sign                     ? (c.flat ? q8_pack_kernel<T, true, kAllSigns> : q8_pack_kernel<T, false, kAllSigns>)
+                                           : (c.flat ? q8_pack_kernel<T, true, kRounded> : q8_pack_kernel<T, false, kRounded>);
   hipLaunchKernelGGL(k, dim3(c.grid), dim3(kThreads), 0, st, static_cast<const typename T::value*>(in), stride, c.s, c.flat_cols,
                      reinterpret_cast<uint2*>(codes), scales);
   return check_launch();
@@ -328,9 +329,9 @@ extern "C" int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t co
   if (!value_ptr(d_in, dtype) || !checkpoint_ptrs(d_codes, d_scales)) return CSWAP_E_ARG;
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case CSWAP_DT_F32: return pack<F32>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
-    case CSWAP_DT_BF16: return pack<BF16>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
-    default: return pack<F16>(d_in, (size_t)stride, keep_sign != 0, c, d_codes, d_scales, st);
+    case CSWAP_DT_F32: return pack<F32>(d_in, (size_t)stride, keep_sign, c, d_codes, d_scales, st);
+    case CSWAP_DT_BF16: return pack<BF16>(d_in, (size_t)stride, keep_sign, c, d_codes, d_scales, st);
+    default: return pack<F16>(d_in, (size_t)stride, keep_sign, c, d_codes, d_scales, st);
   }
 }
 

@@ -294,12 +294,22 @@ class swap_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         self._live.clear()
 
 
+# nodes that save their result and ask for its sign: relu, and leaky_relu in place
+_SAVE_SIGNS = ("ReluBackward0", "LeakyReluBackward1")
+
+
 class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     """Keeps eligible saved activations on the device in 8 bits (``cswap_amd.q8``) instead of swapping them:
     contiguous float32, bfloat16 and float16 device tensors of at least ``min_bytes`` that are not parameters or other
     leaves; everything else is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
-    the largest magnitude among 32 neighbouring values, in the tensor's type; 0 stays 0 and everything else keeps its
-    sign, which is all that a ReLU's backward pass asks of its result.
+    the largest magnitude among 32 neighbouring values, in the tensor's type.  0 stays 0; another value that rounds to
+    0 keeps its sign where one or two of 32 neighbours do so, and is then off by up to 2^-6 of the largest.  Beside more
+    of them it becomes 0: held as something else they would add up (the probabilities of a softmax to 1.2 and more).
+
+    What a ReLU saves for itself, of which its backward pass asks only for the sign, keeps the sign of every value.
+    ``keep_sign`` holds all tensors so, off by up to 2^-6 of the largest and with that bias: for models with operators
+    that divide by what they saved (``log``, ``sqrt``, division by a tensor), whose gradient is infinite where that has
+    become 0, or that ask for the sign of inputs far below their neighbours.
 
         with hold_saved_tensors():
             loss = model(x).sum()
@@ -311,8 +321,9 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     Operators whose backward pass compares saved tensors with one another (``amax``, ``median``) find no equal
     values any more: keep them outside."""
 
-    def __init__(self, min_bytes: int = 1 << 20):
+    def __init__(self, min_bytes: int = 1 << 20, keep_sign: bool = False):
         self.min_bytes = min_bytes
+        self.keep_sign = keep_sign
         self.stats = {"held": 0, "bytes_in": 0, "bytes_held": 0, "kept": 0}
         super().__init__(self._pack, self._unpack)
 
@@ -321,11 +332,21 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
                 and t.numel() * t.element_size() >= max(1, self.min_bytes) and not isinstance(t, torch.nn.Parameter)
                 and not t.is_leaf)
 
+    @staticmethod
+    def _of_a_relu(t: torch.Tensor) -> bool:
+        """A result that its own operator saves for the sign.  It does so before anybody else can: who saves the same
+        tensor later uses its values."""
+        node = t.grad_fn
+        if type(node).__name__ not in _SAVE_SIGNS or "cswap_amd.hooks" in node.metadata:
+            return False
+        node.metadata["cswap_amd.hooks"] = True
+        return True
+
     def _pack(self, t: torch.Tensor):
         if not self._eligible(t):
             self.stats["kept"] += 1
             return t
-        held = q8.q8_compress(t.detach(), flat=True, keep_sign=True)
+        held = q8.q8_compress(t.detach(), flat=True, keep_sign=True if self.keep_sign or self._of_a_relu(t) else q8.FEW)
         self.stats["held"] += 1
         self.stats["bytes_in"] += t.numel() * t.element_size()
         self.stats["bytes_held"] += held.nbytes

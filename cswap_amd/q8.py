@@ -27,6 +27,7 @@ from ._lib import check, lib
 GROUP = 32
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FEW = 2     # for keep_sign
 
 
 class Checkpoint8:
@@ -176,11 +177,12 @@ def _param(p, cols: int, device: torch.device, what: str):
 
 
 # ------------------------------------------------------------------- codec
-def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) -> Checkpoint8:
+def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool | int = False) -> Checkpoint8:
     """The checkpoint of ``x``.  ``flat`` (contiguous tensors): groups run through the whole tensor instead of
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
     is the same either way, and only such a flat checkpoint has rows for the backward passes.  ``keep_sign``: what is
-    not 0 but rounds to 0 is held as the smallest value with its sign."""
+    not 0 but rounds to 0 is held as the smallest value with its sign, off by up to 2^-6 of the group's largest magnitude;
+    ``FEW``: in groups that have one or two such values, where it does not add up to a bias."""
     kind, device, stream = _begin(x, "q8_compress")
     if stream is None:
         with torch.cuda.device(device):

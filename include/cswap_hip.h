@@ -273,7 +273,10 @@ typedef enum { CSWAP_DT_F32 = 0, CSWAP_DT_BF16 = 1, CSWAP_DT_F16 = 2 } cswap_dty
 size_t cswap_q8_code_pitch(size_t cols);  /* cols rounded up to a multiple of 32 */
 size_t cswap_q8_scale_pitch(size_t cols); /* groups of a row */
 /* keep_sign: a value that is not 0 but rounds to 0 is held as 2^e with its sign, so that what asks
- * only for the sign (a ReLU's backward pass) loses nothing; it is then off by less than 2^e. */
+ * only for the sign (a ReLU's backward pass) loses nothing; it is then off by less than 2^e, at most
+ * 2^-6 of the group's largest magnitude.  Many such values of one sign add up to a bias (rows of a
+ * softmax sum to 1.2 and more): CSWAP_Q8_FEW_SIGNS does so only in groups that have one or two of them. */
+typedef enum { CSWAP_Q8_ROUND = 0, CSWAP_Q8_SIGNS = 1, CSWAP_Q8_FEW_SIGNS = 2 } cswap_q8_signs;
 int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride, int keep_sign,
                   int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
 /* Rounds once where `dtype` does not hold q * 2^e. */
