@@ -19,14 +19,16 @@ constexpr int kThreads = 256;
 
 // rows x cols values, a lane per chunk.  cpr: chunks of a row, its group padding included, so four neighbouring lanes are a
 // group and no quad crosses a row.
+// Columns are counted in chunks: a row may have more than 2^32 values, but fewer than 2^31 chunks.
 struct Shape {
-  uint32_t cols, chunks;
+  uint32_t chunks, full;  // of the call; of a row those whose 8 values are all there
+  int tail;               // values of the chunk behind these
   RowDivisor cpr;
 };
 
 struct Place {
-  uint32_t row, col;  // of the chunk's first value
-  int valid;          // values of the chunk that are there: 8, fewer at a row's end, 0 behind it
+  uint32_t row, at;  // the row, and the chunk in it
+  int valid;         // values of the chunk that are there: 8, fewer at a row's end, 0 behind it
 };
 
 // FLAT: one row (a tensor whose rows are whole groups without gaps is one), chunk numbers are positions.
@@ -35,19 +37,19 @@ template <bool FLAT> __device__ inline Place place_of(uint32_t chunk, const Shap
   Place p;
   if (FLAT) {
     const size_t at = (size_t)chunk * kChunk;
-    p.row = 0, p.col = 0;
+    p.row = 0, p.at = 0;
     p.valid = at + kChunk <= flat_cols ? kChunk : at < flat_cols ? (int)(flat_cols - at) : 0;
   } else {
     p.row = divide(chunk, s.cpr);
-    p.col = (chunk - p.row * s.cpr.d) * kChunk;
-    p.valid = p.col + kChunk <= s.cols ? kChunk : p.col < s.cols ? (int)(s.cols - p.col) : 0;
+    p.at = chunk - p.row * s.cpr.d;
+    p.valid = p.at < s.full ? kChunk : p.at == s.full ? s.tail : 0;
   }
   return p;
 }
 
 template <bool FLAT> __device__ inline size_t offset_of(uint32_t chunk, const Place& p, size_t stride)
 {
-  return FLAT ? (size_t)chunk * kChunk : (size_t)p.row * stride + p.col;
+  return FLAT ? (size_t)chunk * kChunk : (size_t)p.row * stride + (size_t)p.at * kChunk;
 }
 
 __device__ inline void store_codes(uint32_t chunk, uint2 q, uint32_t scale, uint2* codes, uint8_t* scales)
@@ -242,7 +244,7 @@ static int plan(size_t rows, size_t cols, ptrdiff_t* stride_a, ptrdiff_t* stride
   c->flat = rows <= 1 || (cols % kGroup == 0 && *stride_a == (ptrdiff_t)cols && (!stride_b || *stride_b == (ptrdiff_t)cols));
   const size_t cpr = pitch_of(cols) / kChunk, chunks = rows * cpr;
   c->flat_cols = rows * cols;
-  c->s = {(uint32_t)(c->flat ? 0 : cols), (uint32_t)chunks, c->flat ? RowDivisor{1, 0, 0} : row_divisor((uint32_t)cpr)};
+  c->s = {(uint32_t)chunks, (uint32_t)(cols / kChunk), (int)(cols % kChunk), c->flat ? RowDivisor{1, 0, 0} : row_divisor((uint32_t)cpr)};
   c->grid = (unsigned)((chunks + kThreads - 1) / kThreads);
   return CSWAP_OK;
 }
