@@ -125,6 +125,7 @@ _SIGNATURES = {
     "cswap_q8_scale_pitch": (sz, [sz]),
     "cswap_q8_pack": (i32, [vp, i32, sz, sz, pd, i32, vp, vp, vp]),
     "cswap_q8_unpack": (i32, [vp, vp, sz, sz, vp, i32, pd, vp]),
+    "cswap_q8_unpack_held": (i32, [vp, vp, sz, sz, vp, i32, pd, vp]),
     "cswap_q8_act_forward": (i32, [i32, vp, i32, sz, sz, pd, vp, pd, vp, vp, vp]),
     "cswap_q8_act_backward": (i32, [i32, vp, i32, sz, sz, pd, vp, vp, vp, pd, vp]),
     "cswap_layer_norm_forward": (i32, [vp, i32, sz, sz, pd, vp, vp, i32, C.c_float, vp, pd, vp, vp, vp, vp, vp]),

@@ -165,15 +165,18 @@ __device__ inline uint32_t quad_max_bits(const float v[8])
   return __float_as_uint(m) & 0x7fffffffu;
 }
 
-// What becomes of a value that is not 0 but rounds to 0: the code 0, or 1 or -1, the nearest that has its sign, in every group or in
-// those that have no more than kMostLost of them.  Of one sign, as probabilities are, such codes add up to a bias: rows of a
+// What becomes of a value that is not 0 but rounds to 0: the code 0, or 1 or -1, the nearest that has its sign, in every group or
+// (kHold) in those that have no more than kMostLost of them.  Of one sign, as probabilities are, such codes add up to a bias: rows of a
 // softmax over 512 logits N(0, 9) sum to 1.20 with all signs kept and to 0.991 with few or none (0.998 to 1.0002 for N(0, 1) to N(0, 2.25)
-// with few).
-enum Signs { kRounded = 0, kAllSigns = 1, kFewSigns = 2 };
+// with few).  kHold has minus infinity, which masks leave, as a value of its own, too: the code -128.
+enum Signs { kRounded = 0, kAllSigns = 1, kHold = 2 };
 constexpr int kMostLost = 2;
+constexpr uint32_t kMaskCode = 0x80;
 
-// Eight codes (byte i of the pair is value i) and the group's scale byte.  With kFewSigns all four lanes of the quad have to run this.
-template <int SIGNS = kRounded> __device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale)
+// Eight codes (byte i of the pair is value i) and the group's scale byte.  With kHold all four lanes of the quad have to run this, and v has 0
+// in the places of `masked` (bit i: value i).
+template <int SIGNS = kRounded>
+__device__ inline uint2 encode_chunk(const float v[8], uint32_t max_bits, uint32_t* scale, uint32_t masked = 0)
 {
   const int exponent = (int)(max_bits >> 23);
   const int b = max(exponent - 6, 1);
@@ -188,7 +191,7 @@ template <int SIGNS = kRounded> __device__ inline uint2 encode_chunk(const float
     t[i] = __float_as_uint(__builtin_amdgcn_fmed3f(__builtin_fmaf(v[i], inverse, kMagic), kMagic - 127.0f, kMagic + 127.0f));
   if (SIGNS != kRounded) {
     bool keep = true;
-    if (SIGNS == kFewSigns) {
+    if (SIGNS == kHold) {
       int lost = 0;
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) lost += t[i] == __float_as_uint(kMagic) && v[i] != 0.0f;
@@ -199,6 +202,11 @@ template <int SIGNS = kRounded> __device__ inline uint2 encode_chunk(const float
 #pragma unroll
     for (int i = 0; i < kChunk; ++i)
       if (keep && t[i] == __float_as_uint(kMagic)) t[i] = v[i] > 0.0f ? 1u : v[i] < 0.0f ? 0xffu : 0u;
+  }
+  if (SIGNS == kHold) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (masked >> i & 1) t[i] = kMaskCode;
   }
   uint2 q;
   // v_perm_b32 numbers the bytes of its second operand 0 to 3 and those of its first 4 to 7
@@ -214,6 +222,20 @@ __device__ inline void decode_chunk(uint2 q, float unit, float v[8])
 {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = code_value(q.x, i) * unit, v[4 + i] = code_value(q.y, i) * unit;
+}
+
+// Minus infinity where the code is -128, which no other value has.
+__device__ inline void decode_masked(float unit, float v[8])
+{
+  const float code = -128.0f * unit;
+  float least = smaller(v[0], v[1]);
+#pragma unroll
+  for (int i = 2; i < kChunk; i += 2) least = smaller(smaller(least, v[i]), v[i + 1]);
+  if (least <= code) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (v[i] <= code) v[i] = -__builtin_inff();
+  }
 }
 
 // ---------------------------------------------------------------- rows of chunks

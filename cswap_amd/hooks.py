@@ -311,6 +311,12 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     that divide by what they saved (``log``, ``sqrt``, division by a tensor), whose gradient is infinite where that has
     become 0, or that ask for the sign of inputs far below their neighbours.
 
+    Minus infinity, as masks leave it, comes back as it is and does not touch its neighbours (with ``keep_sign`` it does as
+    the others do): NaN and plus infinity make their 32 neighbours NaN, and beside a mask of the type's lowest value the
+    others become 0.  What ``log_softmax`` saves is kept as it is, since its backward pass takes the exponential: 2^-7 of a
+    log-probability of -10 is 8 % of the probability.  An operator that must not get what is said here can be run in
+    ``torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)`` inside: the innermost hooks are the ones that apply.
+
         with hold_saved_tensors():
             loss = model(x).sum()
         loss.backward()
@@ -319,7 +325,8 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     two nodes do and a 16-bit one nothing.  Layers that can read a checkpoint as it is (``cswap_amd.layers8``) need
     neither the hooks nor the tensor that backward would be given here; what they keep passes through unchanged.
     Operators whose backward pass compares saved tensors with one another (``amax``, ``median``) find no equal
-    values any more: keep them outside."""
+    values any more, and those that take the exponential of a saved difference (``logsumexp``, ``logaddexp``) get the
+    error of logits as a factor: keep them outside."""
 
     def __init__(self, min_bytes: int = 1 << 20, keep_sign: bool = False):
         self.min_bytes = min_bytes
@@ -330,7 +337,7 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     def _eligible(self, t: torch.Tensor) -> bool:
         return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.is_contiguous() and t.dim() >= 1
                 and t.numel() * t.element_size() >= max(1, self.min_bytes) and not isinstance(t, torch.nn.Parameter)
-                and not t.is_leaf)
+                and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0")
 
     @staticmethod
     def _of_a_relu(t: torch.Tensor) -> bool:
@@ -346,14 +353,14 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         if not self._eligible(t):
             self.stats["kept"] += 1
             return t
-        held = q8.q8_compress(t.detach(), flat=True, keep_sign=True if self.keep_sign or self._of_a_relu(t) else q8.FEW)
+        held = q8.q8_compress(t.detach(), flat=True, keep_sign=True if self.keep_sign or self._of_a_relu(t) else q8._HOLD)
         self.stats["held"] += 1
         self.stats["bytes_in"] += t.numel() * t.element_size()
         self.stats["bytes_held"] += held.nbytes
         return held
 
     def _unpack(self, held):
-        return q8.q8_decompress(held) if isinstance(held, q8.Checkpoint8) else held
+        return q8._give_back(held) if isinstance(held, q8.Checkpoint8) else held
 
     def close(self):
         """Nothing is left to release: there so that this context goes where ``swap_saved_tensors`` does."""

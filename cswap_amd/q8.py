@@ -27,7 +27,7 @@ from ._lib import check, lib
 GROUP = 32
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-FEW = 2     # for keep_sign
+_HOLD = 2    # keep_sign of the saved-tensor hooks: few signs, and minus infinity, which only _give_back knows
 
 
 class Checkpoint8:
@@ -177,12 +177,11 @@ def _param(p, cols: int, device: torch.device, what: str):
 
 
 # ------------------------------------------------------------------- codec
-def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool | int = False) -> Checkpoint8:
+def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) -> Checkpoint8:
     """The checkpoint of ``x``.  ``flat`` (contiguous tensors): groups run through the whole tensor instead of
     starting at each row, which saves the padding of short rows; a tensor whose last dimension is a multiple of 32
     is the same either way, and only such a flat checkpoint has rows for the backward passes.  ``keep_sign``: what is
-    not 0 but rounds to 0 is held as the smallest value with its sign, off by up to 2^-6 of the group's largest magnitude;
-    ``FEW``: in groups that have one or two such values, where it does not add up to a bias."""
+    not 0 but rounds to 0 is held as the smallest value with its sign, off by up to 2^-6 of the group's largest magnitude."""
     kind, device, stream = _begin(x, "q8_compress")
     if stream is None:
         with torch.cuda.device(device):
@@ -226,6 +225,18 @@ def q8_decompress(held: Checkpoint8, out: torch.Tensor | None = None, dtype: tor
             raise ValueError("q8_decompress: a flat checkpoint goes into a contiguous tensor")
     check(lib().cswap_q8_unpack(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), kind,
                                 stride, stream), "cswap_q8_unpack")
+    return out
+
+
+def _give_back(held: Checkpoint8) -> torch.Tensor:
+    """The tensor that the saved-tensor hooks' checkpoint was made of, as far as that holds it."""
+    stream = _stream_of(held.device)
+    if stream is None:
+        with torch.cuda.device(held.device):
+            return _give_back(held)
+    out = torch.empty(held.shape, dtype=held.dtype, device=held.device)
+    check(lib().cswap_q8_unpack_held(held._at, held._scales_at, held.rows, held.cols, out.data_ptr(), _DTYPE[held.dtype], 0,
+                                     stream), "cswap_q8_unpack_held")
     return out
 
 

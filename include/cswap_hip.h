@@ -275,13 +275,18 @@ size_t cswap_q8_scale_pitch(size_t cols); /* groups of a row */
 /* keep_sign: a value that is not 0 but rounds to 0 is held as 2^e with its sign, so that what asks
  * only for the sign (a ReLU's backward pass) loses nothing; it is then off by less than 2^e, at most
  * 2^-6 of the group's largest magnitude.  Many such values of one sign add up to a bias (rows of a
- * softmax sum to 1.2 and more): CSWAP_Q8_FEW_SIGNS does so only in groups that have one or two of them. */
-typedef enum { CSWAP_Q8_ROUND = 0, CSWAP_Q8_SIGNS = 1, CSWAP_Q8_FEW_SIGNS = 2 } cswap_q8_signs;
+ * softmax sum to 1.2 and more).  CSWAP_Q8_HOLD, for what saved-tensor hooks hold, does so only in
+ * groups that have one or two of them, and holds minus infinity as the code -128 and the group's other
+ * values as if it were 0; cswap_q8_unpack_held gives such a checkpoint back, no other function here knows
+ * that code. */
+typedef enum { CSWAP_Q8_ROUND = 0, CSWAP_Q8_SIGNS = 1, CSWAP_Q8_HOLD = 2 } cswap_q8_signs;
 int cswap_q8_pack(const void* d_in, int dtype, size_t rows, size_t cols, ptrdiff_t stride, int keep_sign,
                   int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
 /* Rounds once where `dtype` does not hold q * 2^e. */
 int cswap_q8_unpack(const int8_t* d_codes, const uint8_t* d_scales, size_t rows, size_t cols,
                     void* d_out, int dtype, ptrdiff_t stride, cswap_stream_t stream);
+int cswap_q8_unpack_held(const int8_t* d_codes, const uint8_t* d_scales, size_t rows, size_t cols,
+                         void* d_out, int dtype, ptrdiff_t stride, cswap_stream_t stream);
 
 /* y = f(x) and, where d_codes and d_scales are given, the checkpoint of x in one pass;
  * dx = dy f'(x^) from the checkpoint x^.  f in fp32 whatever the type: x Phi(x), its tanh

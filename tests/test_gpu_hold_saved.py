@@ -1,4 +1,5 @@
-"""What the saved-tensor hooks hold in 8 bits, against 64-bit forms."""
+"""What the saved-tensor hooks hold in 8 bits: signs, probabilities and masks, against 64-bit forms."""
+import math
 import os
 import sys
 
@@ -153,3 +154,68 @@ def test_signs_on_request():
         y = torch.log(leaf * 1.0)
     y.backward(torch.ones_like(y))
     assert bool((leaf.grad[:, ::32] == 1).all()) and bool((leaf.grad[:, 1:32] == 64).all())
+
+
+# ---------------------------------------------------------------- masks
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("shape", [(8, 64), (5, 45)])
+def test_minus_infinity_is_held_beside_its_neighbours(dtype, shape):
+    """Masked places stay minus infinity; the others are held as if those were not there.  NaN and plus infinity make their
+    group NaN."""
+    x = randn(*shape, dtype=dtype, seed=9, scale=3.0)
+    x[1, ::3] = -math.inf
+    x[2] = -math.inf
+    x[3, 7] = -math.inf
+    got = what_is_held(x).cpu().double()
+    masked = torch.isinf(x.cpu())
+    want = held_few(x.masked_fill(masked.to(DEV), 0.0))
+    assert torch.equal(got, torch.where(masked, torch.full_like(want, -math.inf), want.to(dtype).double()))
+    x.view(-1)[40], x.view(-1)[100] = math.nan, math.inf
+    nan = torch.isnan(what_is_held(x).cpu()).view(-1).nonzero().flatten().tolist()
+    assert nan == [*range(32, 64), *range(96, 128)]
+
+
+def test_masked_logits_have_finite_gradients():
+    """logsumexp saves its masked input: gradients within what the held logits, off by 2^-7 of the largest of 32, give."""
+    from cswap_amd.hooks import hold_saved_tensors
+
+    x = randn(16, 96, seed=10)
+    mask = torch.rand(16, 96, generator=torch.Generator().manual_seed(11)) < 0.3
+    mask[:, 5] = False
+    leaf = x.clone().requires_grad_()
+    ctx = hold_saved_tensors(min_bytes=1 << 10)
+    with ctx:
+        y = torch.logsumexp(leaf.masked_fill(mask.to(DEV), -math.inf), -1)
+    y.sum().backward()
+    assert ctx.stats["held"] == 1
+    got, want = leaf.grad.cpu().double(), torch.softmax(x.cpu().double().masked_fill(mask, -math.inf), -1)
+    assert bool((got[mask] == 0).all())
+    off = 2.0 ** -7 * group_max(x.cpu().double().masked_fill(mask, 0.0).view(-1)).view(16, 96)
+    assert bool(((got - want).abs() <= want * (torch.expm1(2 * off) + 200 * ref.U)).all())
+
+
+@pytest.mark.parametrize("lowest", [-math.inf, torch.finfo(F32).min])
+def test_log_probabilities_are_kept_as_they_are(lowest):
+    """log_softmax saves its result for its exponential: masked or not, the gradient is that without the hooks."""
+    from cswap_amd.hooks import hold_saved_tensors
+
+    x, target = randn(64, 1000, seed=12), torch.arange(64, device=DEV)
+    x[:, 500::7] = lowest
+    grads = []
+    for ctx in (None, hold_saved_tensors(min_bytes=0)):
+        leaf = x.clone().requires_grad_()
+        if ctx is None:
+            loss = torch.nn.functional.cross_entropy(leaf, target)
+        else:
+            with ctx:
+                loss = torch.nn.functional.cross_entropy(leaf, target)
+        loss.backward()
+        grads.append(leaf.grad)
+    assert bool(torch.isfinite(grads[0]).all()) and torch.equal(*grads)
+
+
+def group_max(x):
+    """For every value of a 1-D tensor the largest magnitude among its 32."""
+    n = x.numel()
+    g = torch.nn.functional.pad(x.abs(), (0, -n % 32)).view(-1, 32)
+    return g.amax(1, keepdim=True).expand_as(g).reshape(-1)[:n]
