@@ -294,14 +294,24 @@ class swap_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         self._live.clear()
 
 
+def _is_weight(t: torch.Tensor) -> bool:
+    """A view of a parameter, or what autocast made of one."""
+    if isinstance(t._base, torch.nn.Parameter):
+        return True
+    node = t.grad_fn
+    if type(node).__name__ != "ToCopyBackward0":
+        return False
+    return isinstance(getattr(node.next_functions[0][0], "variable", None), torch.nn.Parameter)
+
+
 # nodes that save their result and ask for its sign: relu, and leaky_relu in place
 _SAVE_SIGNS = ("ReluBackward0", "LeakyReluBackward1")
 
 
 class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     """Keeps eligible saved activations on the device in 8 bits (``cswap_amd.q8``) instead of swapping them:
-    contiguous float32, bfloat16 and float16 device tensors of at least ``min_bytes`` that are not parameters or other
-    leaves; everything else is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
+    contiguous float32, bfloat16 and float16 device tensors of at least ``min_bytes`` that are not parameters, views or
+    casts of parameters or other leaves; everything else is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
     the largest magnitude among 32 neighbouring values, in the tensor's type.  0 stays 0; another value that rounds to
     0 keeps its sign where one or two of 32 neighbours do so, and is then off by up to 2^-6 of the largest.  Beside more
     of them it becomes 0: held as something else they would add up (the probabilities of a softmax to 1.2 and more).
@@ -337,7 +347,7 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     def _eligible(self, t: torch.Tensor) -> bool:
         return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.is_contiguous() and t.dim() >= 1
                 and t.numel() * t.element_size() >= max(1, self.min_bytes) and not isinstance(t, torch.nn.Parameter)
-                and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0")
+                and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0" and not _is_weight(t))
 
     @staticmethod
     def _of_a_relu(t: torch.Tensor) -> bool:

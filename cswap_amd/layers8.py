@@ -41,7 +41,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _keep(ctx, held: Checkpoint8 | None, *others) -> None:
-    """Through autograd, which lets them go when backward has used them."""
+    """Through autograd, which lets them go when backward has used them.  Parameters come detached, as leaves: hooks that
+    take a model's saved activations leave those alone, also where they are a cast or a view of a parameter."""
     if held is None:
         ctx.held = None
         ctx.save_for_backward(*others)
@@ -74,9 +75,9 @@ class _Linear(torch.autograd.Function):
             elif tuple(held.shape) != tuple(x.shape) or held.dtype != x.dtype:
                 raise ValueError(f"linear: held is the checkpoint of a {tuple(held.shape)} {held.dtype} tensor, x is "
                                  f"{tuple(x.shape)} {x.dtype}")
-            _keep(ctx, held, weight)
+            _keep(ctx, held, weight.detach())
         else:
-            _keep(ctx, None, weight)
+            _keep(ctx, None, weight.detach())
         return F.linear(x, weight, bias)
 
     @staticmethod
@@ -117,7 +118,7 @@ class _LayerNorm(torch.autograd.Function):
         need = any(ctx.needs_input_grad)
         y, mean, rstd, held = q8.layer_norm(_rows(x), weight, bias, eps, checkpoint=need)
         if need:
-            _keep(ctx, held, mean, rstd, weight)
+            _keep(ctx, held, mean, rstd, None if weight is None else weight.detach())
             ctx.params = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
         return y
 

@@ -1,4 +1,4 @@
-"""What the saved-tensor hooks hold in 8 bits: signs, probabilities and masks, against 64-bit forms."""
+"""What the saved-tensor hooks hold in 8 bits: signs, probabilities, masks and weights, against 64-bit forms."""
 import math
 import os
 import sys
@@ -219,3 +219,82 @@ def group_max(x):
     n = x.numel()
     g = torch.nn.functional.pad(x.abs(), (0, -n % 32)).view(-1, 32)
     return g.amax(1, keepdim=True).expand_as(g).reshape(-1)[:n]
+
+
+# ---------------------------------------------------------------- weights
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+def test_weights_pass_through_under_autocast(dtype):
+    """Layers with checkpoints, hooks and autocast together: the hooks have nothing to hold, and every gradient is to the
+    bit that without them."""
+    from cswap_amd import layers8
+    from cswap_amd.hooks import hold_saved_tensors
+    from torch import nn
+
+    x = randn(128, 96, seed=13)
+    grads = []
+    for hooked in (False, True):
+        torch.manual_seed(14)
+        model = nn.Sequential(nn.LayerNorm(96), nn.Linear(96, 224), nn.GELU(), nn.Linear(224, 96), nn.SiLU()).to(DEV)
+        layers8.checkpoint_layers(model)
+        leaf = x.clone().requires_grad_()
+        ctx = hold_saved_tensors(min_bytes=1 << 10)
+        with torch.autocast("cuda", dtype=dtype):
+            if hooked:
+                with ctx:
+                    y = model(leaf)
+            else:
+                y = model(leaf)
+        assert ctx.stats["held"] == 0
+        y.float().square().sum().backward()
+        grads.append([leaf.grad, *(p.grad for p in model.parameters())])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_weights_that_are_computed_pass_through():
+    """A norm over several dimensions takes its weight as a view, a linear layer one that was made of others."""
+    from cswap_amd import layers8
+    from cswap_amd.hooks import hold_saved_tensors
+
+    x, w = randn(32, 6, 16, seed=15), randn(40, 96, seed=16)
+    grads = []
+    for ctx in (None, hold_saved_tensors(min_bytes=0)):
+        norm = layers8.checkpoint_layers(torch.nn.LayerNorm((6, 16))).to(DEV)
+        with torch.no_grad():
+            norm.weight.copy_(randn(6, 16, seed=17))
+        leaves = x.clone().requires_grad_(), w.clone().requires_grad_()
+
+        def forward():
+            return layers8.linear(norm(leaves[0]).view(32, 96), leaves[1] * 0.3, None)
+
+        if ctx is None:
+            y = forward()
+        else:
+            with ctx:
+                y = forward()
+            assert ctx.stats["held"] == 0
+        y.square().sum().backward()
+        grads.append([norm.weight.grad, norm.bias.grad, *(t.grad for t in leaves)])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_weights_of_torchs_own_layers_pass_through():
+    """A convolution's weight, cast by autocast, and a view of a parameter; their inputs are held."""
+    from cswap_amd.hooks import hold_saved_tensors
+
+    conv = torch.nn.Conv2d(8, 16, 3).to(DEV)
+    x = randn(2, 8, 12, 12, seed=18).requires_grad_()
+    shapes = []
+
+    class Watch(hold_saved_tensors):
+        def _eligible(self, t):
+            take = super()._eligible(t)
+            if take:
+                shapes.append(tuple(t.shape))
+            return take
+
+    with Watch(min_bytes=0):
+        with torch.autocast("cuda", dtype=BF16):
+            conv(x * 1.0)
+        torch.matmul((x * 1.0).view(-1, 16), conv.weight.view(16, 72))
+    assert (16, 8, 3, 3) not in shapes and (16, 72) not in shapes
+    assert (2, 8, 12, 12) in shapes and (144, 16) in shapes

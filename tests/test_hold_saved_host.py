@@ -18,3 +18,42 @@ def test_the_hooks_codec_refuses_what_the_codec_does():
     assert unpack(A, A, 4, 32, A, 7, 0, None) == ARG and unpack(A, A, 4, 0, A, 0, 0, None) == ARG
     assert unpack(A, A, 4, 32, A, 0, 31, None) == ARG and unpack(A, A, 1 << 29, 32, A, 0, 0, None) == UNSUPPORTED
     assert unpack(None, None, 0, 32, None, 0, 0, None) == 0
+
+
+def test_layers_save_their_weights_as_leaves():
+    """Hooks take what is no leaf: a weight that was cast or computed is none, but is no activation either."""
+    from cswap_amd import layers8
+    from cswap_amd.q8 import Checkpoint8
+
+    x, w = torch.randn(4, 32, requires_grad=True), torch.randn(8, 32, requires_grad=True)
+    held = Checkpoint8(torch.zeros(4, 32, dtype=torch.int8), torch.ones(4, 1, dtype=torch.uint8), (4, 32), torch.float32)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(t), t)[1], lambda t: t):
+        scaled = w.to(torch.float64).to(torch.float32)
+        layers8.linear(x, scaled, None, held=held)                   # its checkpoint is kept with it
+        layers8.linear(x, scaled.detach(), torch.zeros(8, requires_grad=True))
+    weights = [t for t in seen if t.shape == (8, 32)]
+    assert len(weights) == 2 and all(t.is_leaf and t.data_ptr() in (scaled.data_ptr(),) for t in weights)
+
+
+def test_what_is_a_weight():
+    from cswap_amd.hooks import _is_weight
+
+    p, x = torch.nn.Parameter(torch.zeros(4, 8)), torch.zeros(4, 8, requires_grad=True)
+    for weight in (p.view(8, 4), p[1:], p.flatten(), p.to(torch.bfloat16), p.half()):
+        assert _is_weight(weight)
+    for other in (x.view(8, 4), x.half(), p * 2, (p * 2).half(), torch.relu(x), p @ x.t()):
+        assert not _is_weight(other)
+
+
+def test_a_weight_that_changed_before_backward_is_noticed():
+    from cswap_amd import layers8
+    from cswap_amd.q8 import Checkpoint8
+
+    x, w = torch.randn(4, 32, requires_grad=True), torch.randn(8, 32, requires_grad=True)
+    held = Checkpoint8(torch.zeros(4, 32, dtype=torch.int8), torch.ones(4, 1, dtype=torch.uint8), (4, 32), torch.float32)
+    y = layers8.linear(x, w, None, held=held)
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
