@@ -360,7 +360,7 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         return True
 
     def _pack(self, t: torch.Tensor):
-        if not self._eligible(t):
+        if not self._eligible(t) or q8._watched() and (q8._traced() or q8._have_tangents(t)):
             self.stats["kept"] += 1
             return t
         held = q8.q8_compress(t.detach(), flat=True, keep_sign=True if self.keep_sign or self._of_a_relu(t) else q8._HOLD)

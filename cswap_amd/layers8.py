@@ -14,7 +14,7 @@ computed from inputs that are off by at most 2^-7 of the largest magnitude among
 rows have a mean of many times their deviation is better left as it is).  Without gradients to come nothing is
 kept.  Layers that share an input (the projections of an attention layer) can
 share its checkpoint: ``held = layers8.hold(x)``, then ``linear(x, w, b, held=held)`` for each.  Double
-backward is refused, as are tensors that ``cswap_amd.q8`` refuses.
+backward, forward-mode derivatives and traces are refused, as are tensors that ``cswap_amd.q8`` refuses.
 """
 from __future__ import annotations
 

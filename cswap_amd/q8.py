@@ -12,7 +12,8 @@ form by its layer's backward pass:
 
 Tensors are float32, bfloat16 or float16 in device memory, ``[..., features]``: the last dimension is
 contiguous and the dimensions before it have one distance between rows.  Every function launches on the
-current stream of the tensor's device and returns without synchronising.  ``cswap_amd.layers8`` has them
+current stream of the tensor's device and returns without synchronising.  Torch sees the outputs but not what makes
+them: functions here refuse to be traced, and tensors with forward-mode derivatives.  ``cswap_amd.layers8`` has them
 as layers with gradients, ``cswap_amd.hooks.hold_saved_tensors`` for whatever a model saves.
 """
 from __future__ import annotations
@@ -20,6 +21,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import api
 from ._lib import check, lib
@@ -105,11 +107,38 @@ def _rows_cols(shape):
 
 # torch's own short cut to the current device's number, as api has one to the stream's handle
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_is_tracing = torch._C._is_tracing
+_modes = torch._C._len_torch_dispatch_stack
 
 
-def _begin(t: torch.Tensor, what: str):
+def _traced() -> bool:
+    return _is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+
+
+def _have_tangents(*tensors) -> bool:
+    return forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
+
+
+def _refuse_what_torch_would_lose(what: str, *tensors) -> None:
+    """Called where something watches: a trace records the outputs' allocation alone and would give back memory as it
+    was, and outputs have no tangent."""
+    if _traced():
+        raise RuntimeError(f"{what}: cannot be traced")
+    if _have_tangents(*tensors):
+        raise RuntimeError(f"{what}: no forward-mode derivatives")
+
+
+def _watched() -> bool:
+    """Something sees more of a tensor than its values: forward-mode differentiation, a trace, a dispatch mode."""
+    return forward_ad._current_level >= 0 or _is_tracing() or _modes() > 0
+
+
+def _begin(t: torch.Tensor, what: str, *others):
     """Type and device of a tensor in device memory, and the stream to launch on: the current one of its device, if that
     is the current device, else None. The call is then made again with its device current."""
+    if forward_ad._current_level >= 0 or _is_tracing() or _modes():     # _watched, without the call: it is on every path
+        _refuse_what_torch_would_lose(what, t, *others)
     kind = _DTYPE.get(t.dtype)
     if kind is None:
         raise TypeError(f"{what}: float32, bfloat16 or float16, not {t.dtype}")
@@ -203,6 +232,8 @@ def q8_compress(x: torch.Tensor, flat: bool = False, keep_sign: bool = False) ->
 def q8_decompress(held: Checkpoint8, out: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """What ``held`` stands for, in its own type or in ``dtype`` (rounded once where that does not hold it)."""
     device = held.device
+    if _watched():
+        _refuse_what_torch_would_lose("q8_decompress", out)
     if device.type != "cuda":
         raise ValueError("q8_decompress: expected a checkpoint in device memory")
     stream = _stream_of(device)
@@ -270,9 +301,9 @@ def q8_act(x: torch.Tensor, kind: str = "gelu", checkpoint: bool = True):
     return y, held
 
 
-def _need_gradient(dy: torch.Tensor, held, what: str):
+def _need_gradient(dy: torch.Tensor, held, what: str, *others):
     """``_begin`` of dy, and its row stride; it goes with an input of held's shape and type."""
-    kind, device, stream = _begin(dy, what)
+    kind, device, stream = _begin(dy, what, held, *others)
     if dy.shape != held.shape or dy.dtype != held.dtype or device != held.device:
         raise ValueError(f"{what}: dy is {tuple(dy.shape)} {dy.dtype} on {dy.device}, the input was {tuple(held.shape)} "
                          f"{held.dtype} on {held.device}")
@@ -308,7 +339,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     backward pass reads: the checkpoint of ``x``, or ``x`` itself with ``checkpoint=False``.  A checkpoint is off by up to
     2^-7 of the largest magnitude nearby, mean included: rows whose mean is many times their deviation are better kept
     as they are."""
-    dtype, device, stream = _begin(x, "layer_norm")
+    dtype, device, stream = _begin(x, "layer_norm", weight, bias)
     if stream is None:
         with torch.cuda.device(device):
             return layer_norm(x, weight, bias, eps, checkpoint)
@@ -338,7 +369,7 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
                         param_dtype: torch.dtype | None = None):
     """``(dx, dweight, dbias)``; ``held`` is what ``layer_norm`` returned last.  The parameters' gradients come in
     ``param_dtype`` (the weight's type, else dy's)."""
-    dtype, device, stream, stride = _need_gradient(dy, held, "layer_norm_backward")
+    dtype, device, stream, stride = _need_gradient(dy, held, "layer_norm_backward", mean, rstd, weight)
     if stream is None:
         with torch.cuda.device(device):
             return layer_norm_backward(dy, held, mean, rstd, weight, param_dtype)
