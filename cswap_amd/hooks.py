@@ -346,8 +346,8 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
 
     def _eligible(self, t: torch.Tensor) -> bool:
         return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.is_contiguous() and t.dim() >= 1
-                and t.numel() * t.element_size() >= max(1, self.min_bytes) and not isinstance(t, torch.nn.Parameter)
-                and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0" and not _is_weight(t))
+                and t.numel() * t.element_size() >= max(1, self.min_bytes) and t.numel() <= q8.MAX_VALUES
+                and not isinstance(t, torch.nn.Parameter) and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0" and not _is_weight(t))
 
     @staticmethod
     def _of_a_relu(t: torch.Tensor) -> bool:

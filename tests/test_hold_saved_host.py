@@ -57,3 +57,36 @@ def test_a_weight_that_changed_before_backward_is_noticed():
         w.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         y.sum().backward()
+
+
+# ---------------------------------------------------------------- sizes
+def test_what_is_too_large_is_saved_as_usual():
+    """The codec's limit is 2^31 - 1 pieces of 8 values, in whole groups of 32."""
+    from cswap_amd import _lib, q8
+    from cswap_amd.hooks import hold_saved_tensors
+
+    most = q8.MAX_VALUES
+    pack = _lib.lib().cswap_q8_pack
+    assert pack(None, 0, 1, most, 0, 2, A, A, None) == ARG           # would run
+    assert pack(None, 0, 1, most + 1, 0, 2, A, A, None) == UNSUPPORTED
+
+    class Large:
+        is_cuda, dtype, is_leaf, grad_fn, _base = True, torch.float32, False, None, None
+
+        def __init__(self, n):
+            self.n = n
+
+        def is_contiguous(self):
+            return True
+
+        def dim(self):
+            return 1
+
+        def numel(self):
+            return self.n
+
+        def element_size(self):
+            return 4
+
+    hooks = hold_saved_tensors()
+    assert hooks._eligible(Large(most)) and not hooks._eligible(Large(most + 1))
