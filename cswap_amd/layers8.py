@@ -70,11 +70,13 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, held):
         if ctx.needs_input_grad[1]:
+            if max(weight.shape) > q8.MAX_FEATURES:
+                raise ValueError(f"linear: up to {q8.MAX_FEATURES} features on either side, not {tuple(weight.shape)}")
             if held is None:
                 held = hold(x)
-            elif tuple(held.shape) != tuple(x.shape) or held.dtype != x.dtype:
-                raise ValueError(f"linear: held is the checkpoint of a {tuple(held.shape)} {held.dtype} tensor, x is "
-                                 f"{tuple(x.shape)} {x.dtype}")
+            elif tuple(held.shape) != tuple(x.shape) or held.dtype != x.dtype or held.device != x.device:
+                raise ValueError(f"linear: held is the checkpoint of a {tuple(held.shape)} {held.dtype} tensor on {held.device}, x is "
+                                 f"{tuple(x.shape)} {x.dtype} on {x.device}")
             _keep(ctx, held, weight.detach())
         else:
             _keep(ctx, None, weight.detach())
@@ -209,11 +211,18 @@ _KINDS = {nn.Linear: Linear8, nn.LayerNorm: LayerNorm8, nn.GELU: GELU8, nn.SiLU:
 def checkpoint_layers(model: nn.Module) -> nn.Module:
     """Every ``nn.Linear``, ``nn.LayerNorm``, ``nn.GELU`` and ``nn.SiLU`` of ``model`` (itself among them) becomes its form here, in place:
     parameters, hooks and state stay as they are.  Classes derived from them are left alone, and so are a SiLU that works
-    in place and a layer norm over more than 16384 values."""
+    in place, a layer norm over more than 16384 values, a linear layer with more than 2^20 features on one side, and either over
+    none."""
     for m in model.modules():
         to = _KINDS.get(type(m))
-        if to is SiLU8 and m.inplace or to is LayerNorm8 and math.prod(m.normalized_shape) > 16384:
-            continue
-        if to is not None:
+        if to is not None and _fits(m):
             m.__class__ = to
     return model
+
+
+def _fits(m: nn.Module) -> bool:
+    if type(m) is nn.SiLU:
+        return not m.inplace
+    if type(m) is nn.LayerNorm:
+        return 0 < math.prod(m.normalized_shape) <= q8.MAX_NORM
+    return type(m) is not nn.Linear or 0 < min(m.weight.shape) and max(m.weight.shape) <= q8.MAX_FEATURES

@@ -28,6 +28,8 @@ from ._lib import check, lib
 
 GROUP = 32
 MAX_VALUES = ((1 << 31) // 4 - 1) * GROUP   # of a flat checkpoint: 2^31 - 1 pieces of 8, in whole groups
+MAX_FEATURES = 1 << 20                      # on either side of a weight gradient
+MAX_NORM = 16384                            # values of a layer norm's row
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HOLD = 2    # keep_sign of the saved-tensor hooks: few signs, and minus infinity, which only _give_back knows

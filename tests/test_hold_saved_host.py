@@ -90,3 +90,33 @@ def test_what_is_too_large_is_saved_as_usual():
 
     hooks = hold_saved_tensors()
     assert hooks._eligible(Large(most)) and not hooks._eligible(Large(most + 1))
+
+
+def test_layers_that_the_kernels_cannot_take_are_left_alone():
+    from cswap_amd import layers8
+    from torch import nn
+
+    def kinds(*layers):
+        with torch.device("meta"):
+            return [type(m).__name__ for m in layers8.checkpoint_layers(nn.Sequential(*(f() for f in layers)))]
+
+    most = 1 << 20
+    assert kinds(lambda: nn.Linear(most, 2), lambda: nn.Linear(most + 1, 2), lambda: nn.Linear(2, most), lambda: nn.Linear(2, most + 1)) \
+        == ["Linear8", "Linear", "Linear8", "Linear"]
+    assert kinds(lambda: nn.Linear(0, 3), lambda: nn.Linear(3, 0), lambda: nn.LayerNorm(0), lambda: nn.LayerNorm((4, 0))) \
+        == ["Linear", "Linear", "LayerNorm", "LayerNorm"]
+    assert kinds(lambda: nn.LayerNorm(16384), lambda: nn.LayerNorm(16385), nn.GELU, nn.SiLU, lambda: nn.SiLU(inplace=True)) \
+        == ["LayerNorm8", "LayerNorm", "GELU8", "SiLU8", "SiLU"]
+
+
+def test_linear_refuses_in_the_forward_pass():
+    from cswap_amd import layers8
+    from cswap_amd.q8 import Checkpoint8
+
+    x = torch.zeros(1, 2, requires_grad=True)
+    with pytest.raises(ValueError, match="features"):
+        layers8.linear(x, torch.zeros((1 << 20) + 1, 2, requires_grad=True))
+    w = torch.zeros(3, 2, requires_grad=True, device="meta")
+    held = Checkpoint8(torch.zeros(1, 32, dtype=torch.int8), torch.zeros(1, 1, dtype=torch.uint8), (1, 2), torch.float32)
+    with pytest.raises(ValueError, match="on cpu, x is"):
+        layers8.linear(x.detach().to("meta"), w, None, held=held)
