@@ -311,7 +311,7 @@ _SAVE_SIGNS = ("ReluBackward0", "LeakyReluBackward1")
 class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
     """Keeps eligible saved activations on the device in 8 bits (``cswap_amd.q8``) instead of swapping them:
     contiguous float32, bfloat16 and float16 device tensors of at least ``min_bytes`` that are not parameters, views or
-    casts of parameters or other leaves; everything else is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
+    casts of parameters or other leaves; everything else (sparse, nested and distributed tensors among it) is saved as usual.  Backward gets what the checkpoint stands for, off by at most 2^-7 of
     the largest magnitude among 32 neighbouring values, in the tensor's type.  0 stays 0; another value that rounds to
     0 keeps its sign where one or two of 32 neighbours do so, and is then off by up to 2^-6 of the largest.  Beside more
     of them it becomes 0: held as something else they would add up (the probabilities of a softmax to 1.2 and more).
@@ -345,7 +345,8 @@ class hold_saved_tensors(torch.autograd.graph.saved_tensors_hooks):
         super().__init__(self._pack, self._unpack)
 
     def _eligible(self, t: torch.Tensor) -> bool:
-        return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.is_contiguous() and t.dim() >= 1
+        return (t.is_cuda and t.dtype in (torch.float32, torch.bfloat16, torch.float16) and t.layout is torch.strided
+                and not t.is_nested and not hasattr(t, "__tensor_flatten__") and t.is_contiguous() and t.dim() >= 1
                 and t.numel() * t.element_size() >= max(1, self.min_bytes) and t.numel() <= q8.MAX_VALUES
                 and not isinstance(t, torch.nn.Parameter) and not t.is_leaf and type(t.grad_fn).__name__ != "LogSoftmaxBackward0" and not _is_weight(t))
 

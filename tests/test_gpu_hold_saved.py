@@ -298,3 +298,26 @@ def test_weights_of_torchs_own_layers_pass_through():
         torch.matmul((x * 1.0).view(-1, 16), conv.weight.view(16, 72))
     assert (16, 8, 3, 3) not in shapes and (16, 72) not in shapes
     assert (2, 8, 12, 12) in shapes and (144, 16) in shapes
+
+
+def test_tensors_of_other_layouts_are_saved_as_usual():
+    from cswap_amd.hooks import hold_saved_tensors
+
+    dense, eye = randn(6, 8, seed=19), torch.eye(6, device=DEV)
+    for make in (lambda: eye.to_sparse_csr(), lambda: eye.to_sparse()):
+        grads = []
+        for ctx in (hold_saved_tensors(min_bytes=0), torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)):
+            s, d = make().requires_grad_(), dense.clone().requires_grad_()
+            with ctx:
+                y = torch.sparse.mm(s * 2.0, d)
+            y.sum().backward()
+            grads.append(d.grad)
+        assert torch.equal(*grads)
+    nested = torch.nested.nested_tensor([dense, dense[:3]])
+    for ctx in (hold_saved_tensors(min_bytes=0), torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)):
+        leaf = nested.clone().detach().requires_grad_()
+        with ctx:
+            y = torch.relu(leaf * 2.0)
+        torch.nested.to_padded_tensor(y, 0.0).sum().backward()
+        grads.append(torch.nested.to_padded_tensor(leaf.grad, 0.0))
+    assert torch.equal(*grads[2:])

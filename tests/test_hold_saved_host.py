@@ -72,6 +72,7 @@ def test_what_is_too_large_is_saved_as_usual():
 
     class Large:
         is_cuda, dtype, is_leaf, grad_fn, _base = True, torch.float32, False, None, None
+        layout, is_nested = torch.strided, False
 
         def __init__(self, n):
             self.n = n
