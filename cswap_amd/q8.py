@@ -162,6 +162,8 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
     """The distance between rows, in elements; 0 (the library's default) where there are no gaps."""
     if t.is_contiguous():
         return 0
+    if t.is_neg():
+        raise ValueError(f"{what}: a view with its sign turned (resolve_neg)")
     shape, stride = t.shape, t.stride()
     if shape[-1] > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: the last dimension has to be contiguous")

@@ -121,3 +121,14 @@ def test_linear_refuses_in_the_forward_pass():
     held = Checkpoint8(torch.zeros(1, 32, dtype=torch.int8), torch.zeros(1, 1, dtype=torch.uint8), (1, 2), torch.float32)
     with pytest.raises(ValueError, match="on cpu, x is"):
         layers8.linear(x.detach().to("meta"), w, None, held=held)
+
+
+def test_a_view_with_its_sign_turned_is_refused():
+    """The imaginary part of a conjugate is a view whose values in memory have the other sign."""
+    from cswap_amd import layers8
+    from cswap_amd.q8 import _row_stride
+
+    t = torch.randn(4, 1, dtype=torch.complex64).conj().imag
+    with pytest.raises(ValueError, match="sign"):
+        _row_stride(t, "t")
+    assert torch.equal(layers8._rows(t), t) and not layers8._rows(t).is_neg()
