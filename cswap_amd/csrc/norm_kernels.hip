@@ -9,9 +9,11 @@
 // 1024 values is one wavefront's or less, so nothing waits for a barrier; longer ones share a sum through LDS with one barrier
 // each.  Either kernel asks for a workgroup's next row before it works on this one.
 //
-// Tensors in turn: 16384 x 768 bf16 forward 13.5 us (4.7 TB/s), backward 17.6 with its sums (44 in the first form: a row at a
-// time, 512 shares, 8 lanes to sum a column); 2048 x 8192 fp32 32.3 and 38.7 (4.7 and 3.9 TB/s); 4096 x 16384
-// bf16 66 and 81.  Shares by wavefronts of 1024 threads in rows of 513 to 1024 values spill (16384 x 768 fp32 backward 38 : 24 us with 512 threads).
+// Calls one behind the other, tensors in turn: 16384 x 768 bf16 forward 13.0 us (4.9 TB/s), backward with its sums 17.0 from the
+// checkpoint and 18.0 from the input (3.7 and 4.2 TB/s; the backward 44 in the first form: a row at a time, 512 shares, 8 lanes to
+// sum a column), fp32 19.1, 23.4 and 30.5; 2048 x 8192 fp32 28.5, 35.3 and 42.1; 4096 x 16384 bf16 64, 81 and 87.  Traced launch by
+// launch 16384 x 768 bf16 takes 15.0-16.3, 15.0-16.0 and 3.0-4.0 for the sums, 2048 x 8192 fp32 30-31, 31-33 and 4.2-4.8.  Shares
+// by wavefronts of 1024 threads in rows of 513 to 1024 values spill (16384 x 768 fp32 backward 38 : 24 us with 512 threads).
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
 #include "common.h"
@@ -363,9 +365,10 @@ template <typename F> static unsigned groups_for(size_t rows, unsigned most)
   return (unsigned)(want < most ? want : most);
 }
 
-// Many rows of 513 to 768 values in a 16-bit type: half a wavefront with three chunks a lane, none idle at 768 (16384 x 768 bf16
-// forward 13.6 us, with a wavefront and two chunks 14.9; backward 17.5 and 20.1; 8192 rows 9.2 and 9.6, 12.7 and 12.8, 4096 rows
-// 6.1 and 6.3, 9.9 and 9.6).  In fp32 it is 28.5 and 26.5, 29.6 and 29.3.
+// Many rows of 513 to 768 values in a 16-bit type: half a wavefront with three chunks a lane, none idle at 768 and fewer
+// everywhere.  This form : a wavefront with two chunks, us forward and backward, bf16: 16384 rows of 768 13.0 : 14.0 and 16.8 :
+// 18.5, of 640 13.0 : 13.7 and 16.6 : 18.3, of 520 12.6 : 13.4 and 16.2 : 18.2; 8192 rows of 768 9.1 : 9.5 and 12.7 : 12.9, of 520
+// 8.7 : 9.1 and 12.2 : 12.6; 4096 rows of 768 6.1 : 6.3 and 9.9 : 9.6.  In fp32 16384 rows of 768 28.5 : 26.5 and 29.6 : 29.3.
 template <typename T> static bool half_wave(size_t rows, size_t cols)
 {
   return T::bytes == 2 && cols > 512 && cols <= 768 && rows >= 8192;

@@ -1,12 +1,13 @@
 // q8_kernels.hip -- 8-bit activation checkpoints: codec, and activation functions whose forward pass leaves the checkpoint
 // of its input and whose backward pass reads it.  The format is in q8_block.h.
 //
-// Memory bounds them all; a lane has 8 values, which is one or two 16-byte accesses and 8 bytes of codes, and a workgroup's
-// are one run.  402 MB of fp32: to codes 103-110 us, back 78-89 (4.7 and 6.0 TB/s, read and written; a copy of 1 GB reaches 5.2).
-// GELU of 16384 x 768 fp32, tensors in turn: forward 21, backward 21.6 us (5.3 TB/s); its tanh form of 16384 x 4096 bf16: 51 and
-// 64 us (6.6 and 5.3 TB/s).  Two chunks a lane changed nothing (+-3 %).  Nontemporal hints: loads cost where a tensor is still in the
-// memory-side cache (50 MB fp32 GELU 18.3 -> 22), stores save 20 % of a bf16 tensor's decoding and cost 17-47 % of an fp32
-// one's; none is used.
+// Memory bounds them all; a lane has 8 values, which is one or two 16-byte accesses and 8 bytes of codes, and a workgroup's are one
+// run.  402 MB of fp32, tensors in turn, each kernel traced: to codes 103-111 us, back 79-91 (4.6-4.9 and 5.6-6.4 TB/s, read and
+// written; a copy of 1 GB reaches 5.2).  GELU of 16384 x 768 fp32 so: forward 21.4-22.2, backward 21.5-22.4 us (5.1-5.3 TB/s); its
+// tanh form of 16384 x 4096 bf16: 50-52 and 63-66 us (6.4-6.8 and 5.1-5.3 TB/s).  One tensor again and again, the form of the codec
+// that hooks use : the plain one: 402 MB of fp32 86 : 86 us, 134 MB of bf16 33.7 : 30.0, 201 MB of bf16 59 : 51.6 to codes.  Two
+// chunks a lane changed nothing (+-3 %).  Nontemporal hints: loads cost where a tensor is still in the memory-side cache (50 MB
+// fp32 GELU 18.3 -> 22), stores save 20 % of a bf16 tensor's decoding and cost 17-47 % of an fp32 one's; none is used.
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
 #include "common.h"
@@ -151,7 +152,7 @@ struct GeluTanh {
 
 // x Phi(x).  With z = |x| the tail Phi(-z) = exp(-z^2 / 2) R(z), R(z) = erfcx(z / sqrt 2) / 2: smooth, so a polynomial in
 // t = 1 / (1 + p z) without a constant term holds it to a relative error, in the far tail too.  Coefficients: least squares
-// weighted towards the smallest largest relative error over z from 0 to 40, 9.0e-8 for nine of them (fp32) and 1.1e-5 for six
+// weighted towards the smallest largest relative error over z from 0 to 40, 1.0e-7 for nine of them (fp32) and 1.1e-5 for six
 // (16-bit types, whose half step is 4.9e-4 and more).  The library's erff costs some 40 instructions, this 22 and 18.
 struct Gelu {
   struct Parts {
