@@ -5,9 +5,10 @@
 // run.  402 MB of fp32, tensors in turn, each kernel traced: to codes 103-111 us, back 79-91 (4.6-4.9 and 5.6-6.4 TB/s, read and
 // written; a copy of 1 GB reaches 5.2).  GELU of 16384 x 768 fp32 so: forward 21.4-22.2, backward 21.5-22.4 us (5.1-5.3 TB/s); its
 // tanh form of 16384 x 4096 bf16: 50-52 and 63-66 us (6.4-6.8 and 5.1-5.3 TB/s).  One tensor again and again, the form of the codec
-// that hooks use : the plain one: 402 MB of fp32 86 : 86 us, 134 MB of bf16 33.7 : 30.0, 201 MB of bf16 59 : 51.6 to codes.  Two
-// chunks a lane changed nothing (+-3 %).  Nontemporal hints: loads cost where a tensor is still in the memory-side cache (50 MB
-// fp32 GELU 18.3 -> 22), stores save 20 % of a bf16 tensor's decoding and cost 17-47 % of an fp32 one's; none is used.
+// that hooks use : the plain one, us to codes and back: 402 MB of fp32 86 : 87 and 87 : 86, 134 MB of bf16 34.0 : 30.0 and 30.2 :
+// 30.1, 201 MB of bf16 59 : 51.5 and 56 : 52.5, of fp16 57 : 50 and 54.5 : 52.  Two chunks a lane changed nothing (+-3 %).
+// Nontemporal hints: loads cost where a tensor is still in the memory-side cache (50 MB fp32 GELU 18.3 -> 22), stores save 20 % of
+// a bf16 tensor's decoding and cost 17-47 % of an fp32 one's; none is used.
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
 #include "common.h"
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void q8_pack_kernel(const typename T::val
   store_codes(chunk, q, scale, codes, scales);
 }
 
-// MASKED: codes of -128 are minus infinity.  A form of its own, since the question costs up to 5 % (196608 x 512 bf16 51.7 : 54 us).
+// MASKED: codes of -128 are minus infinity.  A form of its own, since the question costs up to 6 % (196608 x 512 bf16 52.5 : 56 us).
 template <typename T, bool FLAT, bool MASKED>
 __global__ __launch_bounds__(kThreads) void q8_unpack_kernel(const uint2* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              Shape s, size_t flat_cols, typename T::value* __restrict__ out,

@@ -110,8 +110,8 @@ def _rows_cols(shape):
 
 # torch's own short cut to the current device's number, as api has one to the stream's handle
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_is_tracing = torch._C._is_tracing
-_modes = torch._C._len_torch_dispatch_stack
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
 
 
 def _traced() -> bool:
