@@ -321,3 +321,46 @@ def test_tensors_of_other_layouts_are_saved_as_usual():
         torch.nested.to_padded_tensor(y, 0.0).sum().backward()
         grads.append(torch.nested.to_padded_tensor(leaf.grad, 0.0))
     assert torch.equal(*grads[2:])
+
+
+# ---------------------------------------------------------------- the codec that the hooks use, by itself
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_rows_with_gaps_and_padding(dtype):
+    """The hooks hold tensors as one row; the functions take rows, with groups that begin at each."""
+    from cswap_amd import q8
+
+    x = randn(9, 130, dtype=dtype, seed=20)
+    x[2, 5:60], x[3, 64:96] = -math.inf, 0.0
+    x[3, 70], x[4, 0] = -math.inf, 1e4
+    big = torch.full((9, 141), math.nan, dtype=dtype, device=DEV)
+    big[:, 3:133] = x
+    got = q8._give_back(q8.q8_compress(big[:, 3:133], keep_sign=q8._HOLD)).cpu().double()
+    masked = torch.isinf(x.cpu())
+    rows = x.masked_fill(masked.to(DEV), 0.0)
+    want = torch.cat([held_few(r) for r in rows]).view(9, 130).to(dtype).double()
+    assert torch.equal(got, want.masked_fill(masked, -math.inf))
+
+
+def test_in_a_graph():
+    """Recorded, and replayed with eager work between: every replay holds and gives back what the eager calls do."""
+    from cswap_amd import q8
+
+    x = torch.zeros(300, 193, device=DEV)
+
+    def there_and_back():
+        return q8._give_back(q8.q8_compress(x, flat=True, keep_sign=q8._HOLD))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there_and_back()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = there_and_back()
+    for turn in range(4):
+        x.copy_(randn(300, 193, seed=21 + turn))
+        x[turn] = -math.inf
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, there_and_back()) and bool((out[turn] == -math.inf).all())
