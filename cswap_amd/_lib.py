@@ -60,6 +60,10 @@ class PlanSummary(C.Structure):
                 ("n_selected", C.c_int), ("target_met", C.c_int)]
 
 
+class AdamwOptions(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double)]
+
+
 class ZfpBitstream(C.Structure):
     _fields_ = [("bits", C.c_uint), ("buffer", C.c_uint64), ("ptr", C.c_void_p), ("begin", C.c_void_p),
                 ("end", C.c_void_p)]
@@ -133,6 +137,12 @@ _SIGNATURES = {
     "cswap_layer_norm_backward": (i32, [vp, i32, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
     "cswap_q8_weight_grad_workspace_bytes": (sz, [i32, sz, sz, sz]),
     "cswap_q8_weight_grad": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, vp, vp, i32, vp, sz, vp]),
+    "cswap_adamw_moment_bytes": (sz, [sz]),
+    "cswap_adamw_factors_bytes": (sz, []),
+    "cswap_adamw_step": (i32, [vp, sz, i32, C.POINTER(AdamwOptions), C.c_longlong, vp]),
+    "cswap_adamw_step_counted": (i32, [vp, sz, i32, C.POINTER(AdamwOptions), vp, vp, vp, vp]),
+    "cswap_adamw_pack": (i32, [vp, sz, vp]),
+    "cswap_adamw_unpack": (i32, [vp, sz, vp]),
     "cswap_probe_nnz": (i32, [vp, sz, vp, vp]),
     "cswap_costs_default": (None, [C.POINTER(Costs)]),
     "cswap_policy_bytes": (sz, [i32, sz, sz, u, i32, sz, sz, sz]),

@@ -1,0 +1,356 @@
+"""AdamW over all tensors of a model at once, its moments held in 8 bits or in fp32 (``include/cswap_hip.h``, "AdamW").
+
+The reference leaves the optimiser to its framework (CIFAR10/cifar10.py:98); what a step keeps besides activations are the
+optimiser's two moments, 8 bytes a parameter in fp32 and 2.06 here:
+
+    optimizer = AdamW8(model.parameters(), lr=1e-3)             # torch.optim.AdamW's arguments and defaults
+    loss.backward();  optimizer.step()
+    moments = unpack_moments(optimizer)                         # [(exp_avg, exp_avg_sq)] in fp32
+
+A step is one launch for every 64 tensors, of any mixture of types, on the current stream of their device; nothing waits for it.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from array import array
+
+import torch
+
+from . import q8
+from ._lib import AdamwOptions, check, lib
+
+__all__ = ["AdamW8", "unpack_moments"]
+
+GROUP = 32
+_OWN = ("bits", "master", "capturable")     # how an optimiser holds its state, whatever it loads
+
+
+def _dense_order(t: torch.Tensor) -> bool:
+    """Whether t fills its memory, in whatever order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+class _Plan:
+    """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
+    __slots__ = ("params", "states", "ptrs", "kept", "contiguous", "table", "device", "strides", "moments", "how")
+
+    def __init__(self, optimizer, group, params):
+        bits = group["bits"]
+        self.how = bits, group["capturable"]
+        self.params, self.states = params, [optimizer.state[p] for p in params]
+        self.ptrs = [p.data_ptr() for p in params]
+        self.kept = [(s["exp_avg"], s["exp_avg_sq"], s.get("master")) for s in self.states]
+        self.contiguous = [p.is_contiguous() for p in params]
+        self.strides = [p.stride() for p in params]
+        self.device = params[0].device
+        # rows of cswap_adamw_tensor: seven words, the type in the last
+        self.table, self.moments = array("Q"), []
+        for p, s, kept in zip(params, self.states, self.kept):
+            if p.dtype not in q8._DTYPE:
+                raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
+            _check_state(p, s, kept, bits)
+            m, v, master = kept
+            self.table.extend((p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), p.numel(),
+                               q8._DTYPE[p.dtype]))
+            self.moments.append((m.data_ptr(), v.data_ptr(), p.numel()))
+
+    def holds(self, params, group) -> bool:
+        """Whether the plan is still that of these parameters and of their state."""
+        if len(params) != len(self.params) or self.how != (group["bits"], group["capturable"]):
+            return False
+        for p, mine, ptr, strides, (_, _, n), s, (m, v, master) in zip(params, self.params, self.ptrs, self.strides, self.moments, self.states, self.kept):
+            if p is not mine or p.data_ptr() != ptr or p.stride() != strides or p.numel() != n or p.dtype not in q8._DTYPE:
+                return False
+            if s.get("exp_avg") is not m or s.get("exp_avg_sq") is not v or s.get("master") is not master:
+                return False
+        return True
+
+    def set_gradients(self):
+        """Fills in the gradients' addresses; gives back what has to live until the launch."""
+        copies, addresses, device = [], array("Q"), self.device
+        for p, contiguous, strides, (_, _, n) in zip(self.params, self.contiguous, self.strides, self.moments):
+            g = p.grad
+            if g.layout is not torch.strided:
+                raise RuntimeError("AdamW8: no sparse gradients")
+            if g.dtype is not p.dtype or g.numel() != n or g.device != device:
+                raise TypeError(f"AdamW8: a gradient {tuple(g.shape)} {g.dtype} on {g.device} of a parameter {tuple(p.shape)} {p.dtype} on {device}")
+            if not (contiguous and g.is_contiguous()) and g.stride() != strides or g.is_neg():
+                g = torch.empty_like(p).copy_(g)
+                copies.append(g)
+            addresses.append(g.data_ptr())
+        self.table[1::7] = addresses
+        return copies
+
+
+def _check_state(p, s, kept, bits):
+    """A state that did not come from here, or a parameter that changed under it."""
+    m, v, master = kept
+    n = p.numel()
+    for t in (m, v):
+        if bits == 8:
+            fits = t.dtype is torch.uint8 and t.numel() == -(-n // GROUP) * (GROUP + 1) and t.is_contiguous() and t.data_ptr() % 8 == 0
+        else:
+            fits = t.dtype is torch.float32 and t.numel() == n and (t.stride() == p.stride() or t.is_contiguous() and p.is_contiguous())
+        if not fits or t.device != p.device:
+            raise ValueError(f"AdamW8: a moment {tuple(t.shape)} {t.dtype} on {t.device} of a parameter {tuple(p.shape)} on {p.device} held in "
+                             f"{bits} bits")
+    if bits == 8 and tuple(s.get("strides", p.stride())) != p.stride():
+        raise RuntimeError(f"AdamW8: moments in 8 bits of a parameter with strides {tuple(s['strides'])}, which now has {p.stride()}")
+    if master is not None and (master.dtype is not torch.float32 or master.numel() != n or master.device != p.device or
+                               not (master.stride() == p.stride() or master.is_contiguous() and p.is_contiguous())):
+        raise ValueError(f"AdamW8: a master copy {tuple(master.shape)} {master.dtype} on {master.device} of a parameter {tuple(p.shape)} on {p.device}")
+
+
+class AdamW8(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with ``bits=8`` or 32 for its moments, in each parameter group as it says.
+
+    Parameters are float32, bfloat16 or float16 in device memory; the step is computed in fp32 and rounded to the parameter's
+    type once, to nearest: 16-bit parameters of steps below their last place keep still, unless ``master=True`` keeps fp32
+    copies of them (their ``state[p]["master"]``).  In 8 bits a moment has three bits of mantissa over 2^14 (the second: 2^30) below the
+    largest of 32 neighbours, rounded up and down in turn so that it drifts as it should; a NaN or an infinity in a gradient makes its 32
+    neighbours' moments NaN.  ``state[p]`` has "step", "exp_avg" and "exp_avg_sq", as ``torch.optim.AdamW``'s, which
+    ``load_state_dict`` also takes.
+
+    ``capturable=True``: steps are counted in device memory, so that ``step()`` can be captured into a graph and counts on at each
+    replay; ``lr`` may be an fp32 tensor of one value on the device.  Make one step before capturing.  Parameters that made their
+    first step together then have to have gradients together."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits: int = 8, master: bool = False,
+                 capturable: bool = False):
+        self._plans = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, master=master, capturable=capturable))
+
+    def add_param_group(self, param_group):
+        group = {**self.defaults, **{k: v for k, v in param_group.items() if k != "params"}}
+        _options(group)
+        if group["bits"] not in (8, 32):
+            raise ValueError(f"AdamW8: moments in 8 or 32 bits, not {group['bits']}")
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dtype not in q8._DTYPE:
+                self.param_groups.pop()
+                raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plans = {}
+
+    def _new_state(self, p, group, steps):
+        if not p.is_cuda:
+            raise ValueError("AdamW8: expected parameters in device memory")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW8: a parameter's first step cannot be captured")
+        if not _dense_order(p):
+            raise ValueError(f"AdamW8: a parameter {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
+        s = self.state[p]
+        if group["bits"] == 8:
+            size = lib().cswap_adamw_moment_bytes(p.numel())
+            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(size, dtype=torch.uint8, device=p.device) for _ in range(2))
+            s["strides"] = p.stride()
+        else:
+            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32) for _ in range(2))
+        self._finish_state(p, s, group, 0, steps)
+
+    def _finish_state(self, p, s, group, step, steps):
+        if group["master"] and p.dtype is not torch.float32 and "master" not in s:
+            s["master"] = p.detach().to(torch.float32)
+        if group["capturable"]:      # one counter for those that begin together
+            key = (p.device, step)
+            if key not in steps:
+                steps[key] = torch.full((1,), step, dtype=torch.int64, device=p.device)
+            s["step"] = steps[key]
+        else:
+            s["step"] = step
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for number, group in enumerate(self.param_groups):
+            params = [p for p in group["params"] if p.grad is not None]
+            if not params:
+                continue
+            capturable = group["capturable"]
+            options = _options(group)
+            plans = self._plans.get(number)
+            if plans is None or not all(plan.holds(some, group) for plan, some in zip(plans, _as_split(plans, params))):
+                plans = self._plans[number] = self._make_plans(group, params)
+            if not capturable and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW8: a captured step needs capturable=True")
+            if capturable:
+                _all_together(group, params, self.state)
+            lr = group["lr"] if isinstance(group["lr"], torch.Tensor) else None
+            copies = [plan.set_gradients() for plan in plans]      # whatever they refuse, they refuse before a step is made
+            for plan in plans:
+                if q8._stream_of(plan.device) is not None:
+                    _launch(plan, group, options, lr)
+                else:
+                    with torch.cuda.device(plan.device):
+                        _launch(plan, group, options, lr)
+            del copies
+        return loss
+
+    def _make_plans(self, group, params):
+        """A plan for the parameters of each device that have made as many steps."""
+        steps, split = {}, {}
+        for p in params:
+            if "exp_avg" not in self.state[p]:
+                self._new_state(p, group, steps)
+            step = self.state[p]["step"]
+            if isinstance(step, torch.Tensor) != bool(group["capturable"]):      # the option changed
+                self._finish_state(p, self.state[p], group, int(step), steps)
+                step = self.state[p]["step"]
+            split.setdefault((p.device, id(step) if group["capturable"] else step), []).append(p)
+        return [_Plan(self, group, some) for some in split.values()]
+
+    def load_state_dict(self, state_dict):
+        """Of an ``AdamW8`` or of a ``torch.optim.AdamW``; this optimiser's own ``bits``, ``master`` and ``capturable`` stay, and moments are
+        converted to them (to 8 bits: to nearest)."""
+        for saved in state_dict["param_groups"]:
+            if saved.get("amsgrad") or saved.get("maximize"):
+                raise ValueError("AdamW8: no amsgrad and no maximize")
+        own = [{k: group[k] for k in _OWN} for group in self.param_groups]
+        super().load_state_dict(state_dict)     # casts moments to the parameters' types: they are read from state_dict again
+        self._plans = {}
+        steps = {}
+        for group, mine, saved in zip(self.param_groups, own, state_dict["param_groups"]):
+            group.update(mine)
+            for p, number in zip(group["params"], saved["params"]):
+                kept = state_dict["state"].get(number)
+                if kept:
+                    self._load(p, group, kept, steps)
+
+    @torch.no_grad()
+    def _load(self, p, group, kept, steps):
+        if not p.is_cuda:
+            raise ValueError("AdamW8: expected parameters in device memory")
+        s = self.state[p]
+        s.clear()
+        strides = tuple(kept.get("strides", p.stride()))
+        pair = [kept["exp_avg"], kept["exp_avg_sq"]]
+        size = lib().cswap_adamw_moment_bytes(p.numel())
+        if pair[0].dtype is torch.uint8:
+            if any(t.dtype is not torch.uint8 or t.numel() != size for t in pair):
+                raise ValueError(f"AdamW8: {pair[0].numel()} bytes of moments of a parameter of {p.numel()} values")
+            pair = [t.detach().to(p.device, copy=True).reshape(-1) for t in pair]
+            if group["bits"] != 8 or strides != p.stride():
+                values = [torch.empty_strided(p.shape, strides, dtype=torch.float32, device=p.device) for _ in pair]
+                _convert(_row(*values, *pair), "cswap_adamw_unpack", p.device)
+                pair = values
+        if pair[0].dtype is not torch.uint8:
+            pair = [torch.empty_like(p, dtype=torch.float32).copy_(t.reshape(p.shape)) for t in pair]
+            if group["bits"] == 8:
+                packed = [torch.empty(size, dtype=torch.uint8, device=p.device) for _ in pair]
+                _convert(_row(*pair, *packed), "cswap_adamw_pack", p.device)
+                pair = packed
+        s["exp_avg"], s["exp_avg_sq"] = pair
+        if group["bits"] == 8:
+            s["strides"] = p.stride()
+        if group["master"] and p.dtype is not torch.float32 and kept.get("master") is not None:
+            s["master"] = torch.empty_like(p, dtype=torch.float32).copy_(kept["master"].reshape(p.shape))
+        self._finish_state(p, s, group, int(kept["step"]), steps)
+
+
+def _launch(plan, group, options, lr):
+    table, count, first, stream = plan.table.buffer_info()[0], len(plan.params), plan.states[0], q8._stream_of(plan.device)
+    if group["capturable"]:
+        if lr is not None and lr.device != plan.device:
+            raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
+        factors = torch.empty(lib().cswap_adamw_factors_bytes(), dtype=torch.uint8, device=plan.device)
+        check(lib().cswap_adamw_step_counted(table, count, group["bits"], C.byref(options), first["step"].data_ptr(),
+                                             0 if lr is None else lr.data_ptr(), factors.data_ptr(), stream), "cswap_adamw_step_counted")
+    else:
+        step = first["step"] + 1
+        check(lib().cswap_adamw_step(table, count, group["bits"], C.byref(options), step, stream), "cswap_adamw_step")
+        for s in plan.states:
+            s["step"] = step
+
+
+def _options(group) -> AdamwOptions:
+    lr, (b1, b2) = group["lr"], group["betas"]
+    if isinstance(lr, torch.Tensor):
+        if not group["capturable"] or lr.numel() != 1 or lr.dtype is not torch.float32 or not lr.is_cuda:
+            raise ValueError("AdamW8: lr is a number, or, with capturable=True, an fp32 tensor of one value in device memory")
+        lr = 0.0
+    options = AdamwOptions(lr, b1, b2, group["eps"], group["weight_decay"])
+    if not (0.0 <= lr < 1e30 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and 1e-30 <= group["eps"] < 1e30 and 0.0 <= group["weight_decay"] < 1e30):
+        raise ValueError(f"AdamW8: lr {lr}, betas {(b1, b2)}, eps {group['eps']}, weight_decay {group['weight_decay']}")
+    return options
+
+
+def _as_split(plans, params):
+    """params in the plans' order, as far as they are the same ones."""
+    if len(plans) == 1:
+        return [params]
+    place = {id(p): k for k, plan in enumerate(plans) for p in plan.params}
+    split = [[] for _ in plans]
+    for p in params:
+        split[place.get(id(p), 0)].append(p)
+    return split
+
+
+def _all_together(group, params, state):
+    counters = {id(state[p]["step"]) for p in params}
+    there = {id(p) for p in params}
+    for p in group["params"]:
+        if id(p) not in there and p in state and id(state[p].get("step")) in counters:
+            raise RuntimeError("AdamW8: capturable=True, and a parameter without a gradient shares the count of steps with others that have one")
+
+
+def _row(m, v, m8, v8):
+    return array("Q", (m.data_ptr(), v.data_ptr(), m8.data_ptr(), v8.data_ptr(), m.numel()))
+
+
+def _convert(rows, name, device):
+    """``rows``: cswap_adamw_moments as five words each."""
+    with torch.cuda.device(device):
+        check(getattr(lib(), name)(rows.buffer_info()[0], len(rows) // 5, q8._stream_of(device)), name)
+
+
+def _unpack_rows(optimizer):
+    """Of the parameters that have made a step, in order: the parameter, its group, its state and, where it is held in 8 bits, the two moments'
+    addresses, checked."""
+    for number, group in enumerate(optimizer.param_groups):
+        params = [p for p in group["params"] if "exp_avg" in optimizer.state.get(p, ())]
+        plans = optimizer._plans.get(number, ())
+        if len(plans) == 1 and plans[0].holds(params, group):
+            yield from zip(params, [group] * len(params), plans[0].states, plans[0].moments)
+            continue
+        for p in params:
+            s = optimizer.state[p]
+            _check_state(p, s, (s["exp_avg"], s["exp_avg_sq"], None), group["bits"])
+            yield p, group, s, (s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), p.numel())
+
+
+@torch.no_grad()
+def unpack_moments(optimizer: AdamW8, out=None):
+    """``[(exp_avg, exp_avg_sq)]`` in fp32 of the parameters that have made a step, in their order and layout; ``out``: such a list to
+    write to."""
+    params = list(_unpack_rows(optimizer))
+    if out is None:
+        out = [tuple(torch.empty_like(p, dtype=torch.float32) for _ in range(2)) for p, *_ in params]
+    elif len(out) != len(params):
+        raise ValueError(f"unpack_moments: {len(out)} pairs for {len(params)} parameters")
+    rows = {}
+    for (p, group, s, (m8, v8, n)), (m, v) in zip(params, out):
+        for t in (m, v):
+            if t.dtype is not torch.float32 or t.device != p.device or t.numel() != n or not (
+                    t.is_contiguous() and p.is_contiguous() or t.stride() == p.stride()):
+                raise ValueError(f"unpack_moments: {tuple(t.shape)} {t.dtype} on {t.device} for a parameter {tuple(p.shape)} on {p.device}")
+        if group["bits"] == 8:
+            rows.setdefault(p.device, array("Q")).extend((m.data_ptr(), v.data_ptr(), m8, v8, n))
+        else:
+            m.copy_(s["exp_avg"].view_as(m))
+            v.copy_(s["exp_avg_sq"].view_as(v))
+    for device, some in rows.items():
+        _convert(some, "cswap_adamw_unpack", device)
+    return out

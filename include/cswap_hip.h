@@ -331,6 +331,53 @@ int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptr
                          void* d_dw, void* d_db, int out_dtype, void* d_ws, size_t ws_bytes,
                          cswap_stream_t stream);
 
+/* ------------------------------------------------ AdamW over many tensors -----
+ * No counterpart in the reference, which leaves the optimiser to its framework.  One step, t = 1, 2, ...:
+ *   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) (g g)
+ *   p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ * in fp32 whatever the parameter's type, rounded to it once; with `master`, fp32 copies of 16-bit parameters, p
+ * is read there and written to both.  Products and sums of m' and v' are rounded one by one.
+ *
+ * Moments: bits = 32: fp32 values.  bits = 8: cswap_adamw_moment_bytes(n) bytes, 8-byte aligned: a code for each value,
+ * rounded up to whole groups of 32 (0 behind the last), then a byte for each group.  The 32 values of a group
+ * share 2^e, e = max(floor(log2(largest magnitude)) - 6, -126), held as the byte e + 127; y = |x| / 2^e is held as the exponent and
+ * three bits of y + T, T = 2^-8 for m and 2^-24 for v:
+ *   code = ((bits(y + T) + (u >> 12)) >> 20) - (bits(T) >> 20)   of the fp32 sum, in m with the sign of x in bit 7
+ *   it stands for (fp32 of bits((code << 20) + bits(T)) - T) * 2^e
+ * with the offset u = (i A + t B) mod 2^32 of a step's m and (i B + t A) mod 2^32 of its v, i the value's number in its tensor,
+ * A = 0xC13FA9A9, B = 0x91E10DA5, which rounds up as often as what it cuts off is large; cswap_adamw_pack has
+ * 2^31, to nearest.  Where v's code is 0 m's is 0.  A group with a NaN or an infinity stands for NaN in all its values (byte
+ * 255, codes 0).  All bytes 0 are moments of 0.
+ *
+ * Tensors are contiguous, of any alignment of their type, up to 2^34 - 32 values (CSWAP_E_UNSUPPORTED beyond), and do not overlap; n may be 0.  The array of
+ * tensors is read before the call returns, and is not needed after it.  Options: 0 <= b1, b2 < 1, eps >= 1e-30, lr, wd >= 0. */
+typedef struct {
+  void*       param;
+  const void* grad;             /* param's type */
+  void       *exp_avg, *exp_avg_sq;
+  float*      master;           /* NULL: none */
+  size_t      n;
+  int         dtype;
+} cswap_adamw_tensor;
+typedef struct { double lr, beta1, beta2, eps, weight_decay; } cswap_adamw_options;
+size_t cswap_adamw_moment_bytes(size_t n);
+int cswap_adamw_step(const cswap_adamw_tensor* tensors, size_t count, int bits, const cswap_adamw_options* options, long long step,
+                     cswap_stream_t stream);
+/* The step's number is counted up in device memory, so that a captured call counts on with each replay: *d_step, 8-byte aligned, is the
+ * number of steps made, the learning rate *d_lr (NULL: options->lr); d_factors: cswap_adamw_factors_bytes, 4-byte aligned, no preparation, not shared by
+ * calls that overlap. */
+size_t cswap_adamw_factors_bytes(void);
+int cswap_adamw_step_counted(const cswap_adamw_tensor* tensors, size_t count, int bits, const cswap_adamw_options* options,
+                             long long* d_step, const float* d_lr, void* d_factors, cswap_stream_t stream);
+/* Moments from fp32 to 8 bits and back. */
+typedef struct {
+  float   *exp_avg, *exp_avg_sq;
+  uint8_t *exp_avg8, *exp_avg_sq8;
+  size_t   n;
+} cswap_adamw_moments;
+int cswap_adamw_pack(const cswap_adamw_moments* tensors, size_t count, cswap_stream_t stream);
+int cswap_adamw_unpack(const cswap_adamw_moments* tensors, size_t count, cswap_stream_t stream);
+
 /* ---------------------------------------------------------------- probe -----
  * One fused read pass: *d_nnz = number of elements != 0 (the quantity the
  * reference derives from PreGPUcompression + PreAcc, Execution.h:89-92). */
