@@ -135,6 +135,9 @@ _SIGNATURES = {
     "cswap_layer_norm_forward": (i32, [vp, i32, sz, sz, pd, vp, vp, i32, C.c_float, vp, pd, vp, vp, vp, vp, vp]),
     "cswap_layer_norm_workspace_bytes": (sz, [sz, sz]),
     "cswap_layer_norm_backward": (i32, [vp, i32, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
+    "cswap_group_norm_workspace_bytes": (sz, [sz, sz, sz, sz, i32]),
+    "cswap_group_norm_forward": (i32, [i32, vp, i32, sz, sz, sz, sz, pd, vp, vp, i32, C.c_float, vp, pd, vp, vp, vp, vp, vp, sz, vp]),
+    "cswap_group_norm_backward": (i32, [i32, vp, i32, sz, sz, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
     "cswap_q8_weight_grad_workspace_bytes": (sz, [i32, sz, sz, sz]),
     "cswap_q8_weight_grad": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, vp, vp, i32, vp, sz, vp]),
     "cswap_adamw_moment_bytes": (sz, [sz]),

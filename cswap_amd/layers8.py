@@ -6,6 +6,8 @@ stays on the device in one byte a value, and the layer's backward pass reads it 
 
     import cswap_amd.layers8 as layers8
     layers8.checkpoint_layers(model)        # nn.Linear, nn.LayerNorm, nn.GELU, nn.SiLU of a model, in place
+    layers8.checkpoint_layers(model, group_norm=True)                   # and nn.GroupNorm, for images that lie channels last
+    y = layers8.group_norm(x, 32, weight, bias, act="silu")            # with an activation function in the same call
     y = layers8.linear(x, weight, bias)     # or function by function
 
 Outputs are those of the layers without checkpoints (linear layers run torch's own product; norms and activation
@@ -28,7 +30,7 @@ from torch.autograd.function import once_differentiable
 from . import q8
 from .q8 import Checkpoint8
 
-__all__ = ["hold", "linear", "layer_norm", "activation", "Linear8", "LayerNorm8", "GELU8", "SiLU8", "checkpoint_layers"]
+__all__ = ["hold", "linear", "layer_norm", "group_norm", "activation", "Linear8", "LayerNorm8", "GroupNorm8", "GELU8", "SiLU8", "checkpoint_layers"]
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -142,6 +144,50 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
+# ------------------------------------------------------------------- group norm
+def _channels_last(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it that lies channels last."""
+    try:
+        q8._images(t, "")
+        return t
+    except ValueError:
+        if t.dim() < 2:
+            raise
+        return t.movedim(1, -1).contiguous().movedim(-1, 1)
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        need = any(ctx.needs_input_grad)
+        y, mean, rstd, held = q8.group_norm(_channels_last(x), groups, weight, bias, eps, act, checkpoint=need)
+        if need:
+            _keep(ctx, held, mean, rstd, None if weight is None else weight.detach(), None if bias is None else bias.detach())
+            ctx.params = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+            ctx.how = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        mean, rstd, weight, bias, held = _kept(ctx, 4)
+        groups, act = ctx.how
+        dx, dw, db = q8.group_norm_backward(_channels_last(dy), held, mean, rstd, groups, weight, bias, act, ctx.params)
+        need = ctx.needs_input_grad
+        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None, None, None
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               act: str | None = None):
+    """Group norm of images ``[N, C, ...]``, then ``act`` ("gelu", "gelu_tanh", "silu"; None: none); under autocast in fp32, as torch's is.
+    Images that do not lie channels last are copied so first; the result and the gradient lie so in any case."""
+    if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:
+        x = x.float()
+    if not torch.is_grad_enabled():
+        return q8.group_norm(_channels_last(x), groups, weight, bias, eps, act, checkpoint=False)[0]
+    return _GroupNorm.apply(x, weight, bias, groups, eps, act)
+
+
 # ------------------------------------------------------------------- activation functions
 class _Act(torch.autograd.Function):
     @staticmethod
@@ -189,6 +235,23 @@ class LayerNorm8(nn.LayerNorm):
                           self.eps).view(x.shape)
 
 
+class GroupNorm8(nn.GroupNorm):
+    """``nn.GroupNorm`` whose input is kept in 8 bits; images lie channels last (others are copied so).  ``act``: an activation function behind it
+    in the same call."""
+    act = None
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, device=None, dtype=None, *, act: str | None = None):
+        super().__init__(num_groups, num_channels, eps, affine, device, dtype)
+        if act is not None:
+            q8._kind_of(act)
+        self.act = act
+
+    def forward(self, x):
+        if x.dim() < 2 or x.shape[1] != self.num_channels:
+            raise ValueError(f"GroupNorm8: images of {self.num_channels} channels, not {tuple(x.shape)}")
+        return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.act)
+
+
 class GELU8(nn.GELU):
     """``nn.GELU`` whose input is kept in 8 bits."""
 
@@ -208,13 +271,13 @@ class SiLU8(nn.SiLU):
 _KINDS = {nn.Linear: Linear8, nn.LayerNorm: LayerNorm8, nn.GELU: GELU8, nn.SiLU: SiLU8}
 
 
-def checkpoint_layers(model: nn.Module) -> nn.Module:
+def checkpoint_layers(model: nn.Module, group_norm: bool = False) -> nn.Module:
     """Every ``nn.Linear``, ``nn.LayerNorm``, ``nn.GELU`` and ``nn.SiLU`` of ``model`` (itself among them) becomes its form here, in place:
     parameters, hooks and state stay as they are.  Classes derived from them are left alone, and so are a SiLU that works
     in place, a layer norm over more than 16384 values, a linear layer with more than 2^20 features on one side, and either over
-    none."""
+    none.  ``group_norm=True``: every ``nn.GroupNorm`` of up to 4096 channels in up to 2048 groups, too, for models whose images lie channels last."""
     for m in model.modules():
-        to = _KINDS.get(type(m))
+        to = _KINDS.get(type(m)) or (GroupNorm8 if group_norm and type(m) is nn.GroupNorm else None)
         if to is not None and _fits(m):
             m.__class__ = to
     return model
@@ -225,4 +288,6 @@ def _fits(m: nn.Module) -> bool:
         return not m.inplace
     if type(m) is nn.LayerNorm:
         return 0 < math.prod(m.normalized_shape) <= q8.MAX_NORM
+    if type(m) is nn.GroupNorm:
+        return 0 < m.num_channels <= q8.MAX_CHANNELS and m.num_groups <= q8.MAX_GROUPS
     return type(m) is not nn.Linear or 0 < min(m.weight.shape) and max(m.weight.shape) <= q8.MAX_FEATURES

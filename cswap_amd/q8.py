@@ -8,10 +8,13 @@ form by its layer's backward pass:
     x    = q8_decompress(held)
     y, held = q8_act(x, "gelu");                    dx = q8_act_backward(dy, held, "gelu")
     y, mean, rstd, held = layer_norm(x, w, b);      dx, dw, db = layer_norm_backward(dy, held, mean, rstd, w)
+    y, mean, rstd, held = group_norm(x, 32, w, b, act="silu")          # x: images, channels last
+    dx, dw, db = group_norm_backward(dy, held, mean, rstd, 32, w, b, act="silu")
     dw, db = q8_weight_grad(dy, held)             # of y = x @ w.T + b, held made from x
 
 Tensors are float32, bfloat16 or float16 in device memory, ``[..., features]``: the last dimension is
-contiguous and the dimensions before it have one distance between rows.  Every function launches on the
+contiguous and the dimensions before it have one distance between rows (images of a group norm: ``[N, C, ...]`` that lie so in memory
+with C last, as ``torch.channels_last`` has them).  Every function launches on the
 current stream of the tensor's device and returns without synchronising.  Torch sees the outputs but not what makes
 them: functions here refuse to be traced, and tensors with forward-mode derivatives.  ``cswap_amd.layers8`` has them
 as layers with gradients, ``cswap_amd.hooks.hold_saved_tensors`` for whatever a model saves.
@@ -30,6 +33,7 @@ GROUP = 32
 MAX_VALUES = ((1 << 31) // 4 - 1) * GROUP   # of a flat checkpoint: 2^31 - 1 pieces of 8, in whole groups
 MAX_FEATURES = 1 << 20                      # on either side of a weight gradient
 MAX_NORM = 16384                            # values of a layer norm's row
+MAX_CHANNELS, MAX_GROUPS = 4096, 2048       # of a group norm
 KINDS = {"gelu": 0, "gelu_tanh": 1, "silu": 2}
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _HOLD = 2    # keep_sign of the saved-tensor hooks: few signs, and minus infinity, which only _give_back knows
@@ -402,6 +406,129 @@ def layer_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.
     check(lib().cswap_layer_norm_backward(dy.data_ptr(), dtype, rows, cols, stride, x, x_stride, codes, scales, mean.data_ptr(),
                                           rstd.data_ptr(), w, pk, dx.data_ptr(), 0, dw.data_ptr(), db.data_ptr(),
                                           ws.data_ptr() if room else 0, room, stream), "cswap_layer_norm_backward")
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------- group norm
+def _images(x: torch.Tensor, what: str):
+    """Samples, positions and channels of ``[N, C, ...]``, and the distance between positions (0: no gaps)."""
+    shape, stride, n = x.shape, x.stride(), x.dim()
+    if n < 2:
+        raise ValueError(f"{what}: expected [N, C, ...], not {tuple(shape)}")
+    if x.is_neg():
+        raise ValueError(f"{what}: a view with its sign turned (resolve_neg)")
+    samples, channels = shape[0], shape[1]
+    positions = math.prod(shape[2:])
+    if channels == 0 or positions == 0:
+        raise ValueError(f"{what}: images without values, {tuple(shape)}")
+    if channels > 1 and stride[1] != 1:
+        raise ValueError(f"{what}: channels have to lie next to each other (torch.channels_last)")
+    outer = [(shape[d], stride[d]) for d in (0, *range(2, n)) if shape[d] != 1]
+    if not outer or samples == 0:
+        return samples, positions, channels, 0
+    for (_, a), (size, b) in zip(outer, outer[1:]):
+        if a != size * b:
+            raise ValueError(f"{what}: positions have no one distance (torch.channels_last)")
+    step = outer[-1][1]
+    if step < channels:
+        raise ValueError(f"{what}: positions overlap")
+    return samples, positions, channels, 0 if step == channels else step
+
+
+def _like_images(t: torch.Tensor, stride: int) -> torch.Tensor:
+    """A tensor of t's shape and type, channels last without gaps."""
+    if stride == 0 and t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return torch.empty_like(t)
+    shape = t.shape
+    return torch.empty((shape[0], *shape[2:], shape[1]), dtype=t.dtype, device=t.device).movedim(-1, 1)
+
+
+_NO_ACT = 3
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+               act: str | None = None, checkpoint: bool = True):
+    """``(y, mean, rstd, held)``: group norm of images ``[N, C, ...]`` that lie channels last, then the activation function ``act``
+    ("gelu", "gelu_tanh", "silu"; None: none), in one call; the groups' statistics ``[N, groups]`` in fp32, and what the backward pass reads:
+    the checkpoint of ``x`` as ``[N, ..., C]``, or ``x`` itself with ``checkpoint=False``.  Up to 4096 channels in up to 2048 groups.  What
+    ``layer_norm`` says of means far from 0 holds here, too."""
+    k = _NO_ACT if act is None else _kind_of(act)
+    dtype, device, stream = _begin(x, "group_norm", weight, bias)
+    if stream is None:
+        with torch.cuda.device(device):
+            return group_norm(x, groups, weight, bias, eps, act, checkpoint)
+    samples, positions, channels, stride = _images(x, "group_norm")
+    if groups <= 0 or channels % groups:
+        raise ValueError(f"group_norm: {channels} channels in {groups} groups")
+    w, wk = _param(weight, channels, device, "group_norm: weight")
+    b, bk = _param(bias, channels, device, "group_norm: bias")
+    if wk is not None and bk is not None and wk != bk:
+        raise TypeError("group_norm: weight and bias have one type")
+    y = _like_images(x, stride)
+    mean = torch.empty((samples, groups), dtype=torch.float32, device=device)
+    rstd = torch.empty_like(mean)
+    if checkpoint:
+        held = _empty_checkpoint(x, samples * positions, channels, device)
+        shape = x.shape
+        held.shape = torch.Size((shape[0], *shape[2:], channels))
+        codes, scales = held._at, held._scales_at
+    else:
+        held, codes, scales = x, 0, 0
+    room = lib().cswap_group_norm_workspace_bytes(samples, positions, channels, groups, 0)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    check(lib().cswap_group_norm_forward(k, x.data_ptr(), dtype, samples, positions, channels, groups, stride, w, b, wk or bk or 0, eps,
+                                         y.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), codes, scales, ws.data_ptr() if room else 0, room,
+                                         stream), "cswap_group_norm_forward")
+    return y, mean, rstd, held
+
+
+def group_norm_backward(dy: torch.Tensor, held, mean: torch.Tensor, rstd: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+                        bias: torch.Tensor | None = None, act: str | None = None, param_dtype: torch.dtype | None = None):
+    """``(dx, dweight, dbias)``; ``held`` is what ``group_norm`` returned last, ``weight``, ``bias`` and ``act`` are what it was given.
+    The parameters' gradients come in ``param_dtype`` (the weight's type, else the bias's, else dy's)."""
+    k = _NO_ACT if act is None else _kind_of(act)
+    dtype, device, stream = _begin(dy, "group_norm_backward", held, mean, rstd, weight, bias)
+    if stream is None:
+        with torch.cuda.device(device):
+            return group_norm_backward(dy, held, mean, rstd, groups, weight, bias, act, param_dtype)
+    samples, positions, channels, stride = _images(dy, "group_norm_backward")
+    if groups <= 0 or channels % groups:
+        raise ValueError(f"group_norm_backward: {channels} channels in {groups} groups")
+    shape = dy.shape
+    if isinstance(held, Checkpoint8):
+        fits = held.shape == (shape[0], *shape[2:], channels)
+        x, x_stride, codes, scales = 0, 0, held._at, held._scales_at
+        if fits and held.rows != samples * positions and channels % GROUP:
+            raise ValueError(f"group_norm_backward: a flat checkpoint of rows of {channels} values has no rows of its own")
+    else:
+        fits = held.shape == shape
+        x, codes, scales = held.data_ptr(), 0, 0
+        x_stride = _images(held, "group_norm_backward: x")[3] if fits else 0
+    if not fits or held.dtype != dy.dtype or held.device != device:
+        raise ValueError(f"group_norm_backward: dy is {tuple(shape)} {dy.dtype} on {device}, the input was held as {tuple(held.shape)} "
+                         f"{held.dtype} on {held.device}")
+    for s in (mean, rstd):
+        if s.dtype is not torch.float32 or s.numel() != samples * groups or not s.is_contiguous() or s.device != device:
+            raise ValueError(f"group_norm_backward: mean and rstd are {samples} x {groups} contiguous fp32 values on {device}")
+    w, wk = _param(weight, channels, device, "group_norm_backward: weight")
+    b, bk = _param(bias, channels, device, "group_norm_backward: bias")
+    if wk is not None and bk is not None and wk != bk:
+        raise TypeError("group_norm_backward: weight and bias have one type")
+    given = weight if weight is not None else bias
+    if given is not None and param_dtype not in (None, given.dtype):
+        raise TypeError(f"group_norm_backward: param_dtype {param_dtype}, the parameters have {given.dtype}")
+    param_dtype = param_dtype or (dy.dtype if given is None else given.dtype)
+    pk = _DTYPE.get(param_dtype)
+    if pk is None:
+        raise TypeError(f"group_norm_backward: param_dtype {param_dtype}")
+    dx = _like_images(dy, stride)
+    dw = torch.empty(channels, dtype=param_dtype, device=device)
+    db = torch.empty_like(dw)
+    room = lib().cswap_group_norm_workspace_bytes(samples, positions, channels, groups, 1)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    check(lib().cswap_group_norm_backward(k, dy.data_ptr(), dtype, samples, positions, channels, groups, stride, x, x_stride, codes, scales,
+                                          mean.data_ptr(), rstd.data_ptr(), w, b, pk, dx.data_ptr(), 0, dw.data_ptr(), db.data_ptr(),
+                                          ws.data_ptr() if room else 0, room, stream), "cswap_group_norm_backward")
     return dx, dw, db
 
 

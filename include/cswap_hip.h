@@ -291,7 +291,8 @@ int cswap_q8_unpack_held(const int8_t* d_codes, const uint8_t* d_scales, size_t 
 /* y = f(x) and, where d_codes and d_scales are given, the checkpoint of x in one pass;
  * dx = dy f'(x^) from the checkpoint x^.  f in fp32 whatever the type: x Phi(x), its tanh
  * form, x / (1 + exp(-x)).  Where x is minus infinity y is 0 (at most 1e-35 off it). */
-typedef enum { CSWAP_ACT_GELU = 0, CSWAP_ACT_GELU_TANH = 1, CSWAP_ACT_SILU = 2 } cswap_act;
+typedef enum { CSWAP_ACT_GELU = 0, CSWAP_ACT_GELU_TANH = 1, CSWAP_ACT_SILU = 2,
+               CSWAP_ACT_NONE = 3 /* of a group norm alone */ } cswap_act;
 int cswap_q8_act_forward(int kind, const void* d_x, int dtype, size_t rows, size_t cols, ptrdiff_t x_stride,
                          void* d_y, ptrdiff_t y_stride, int8_t* d_codes, uint8_t* d_scales, cswap_stream_t stream);
 int cswap_q8_act_backward(int kind, const void* d_dy, int dtype, size_t rows, size_t cols, ptrdiff_t dy_stride,
@@ -316,6 +317,25 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
                               const float* d_mean, const float* d_rstd, const void* d_gamma, int param_dtype,
                               void* d_dx, ptrdiff_t dx_stride, void* d_dgamma, void* d_dbeta,
                               void* d_ws, size_t ws_bytes, cswap_stream_t stream);
+
+/* Group norm with an activation function, channels last: `samples` x `positions` rows of `channels` values (up to 4096, in up to
+ * 2048 groups, rows up to 2^31 - 1: CSWAP_E_UNSUPPORTED beyond), strides between rows as above; group k of a sample is its channels k * channels / groups and on,
+ * over all positions.  Forward: y = f((x - mean) * rstd * gamma + beta), rstd = 1 / sqrt(var + eps), mean and rstd in fp32 as
+ * [samples][groups]; gamma and beta (param_dtype, a value for each channel) may be NULL; the checkpoint of x, rows of `channels` values,
+ * is made where d_codes and d_scales are given.  Backward takes x as it is (d_codes = d_scales = NULL) or as its checkpoint (d_x =
+ * NULL), and f and beta as forward; d_dgamma and d_dbeta may be NULL.  All sums are fp32, in a fixed order: the same call gives the
+ * same bits.  d_ws: cswap_group_norm_workspace_bytes (NULL where that is 0), 8-byte aligned, no preparation; calls that overlap must
+ * not share one.  samples may be 0 (gradients of parameters are 0 then). */
+size_t cswap_group_norm_workspace_bytes(size_t samples, size_t positions, size_t channels, size_t groups, int backward);
+int cswap_group_norm_forward(int act, const void* d_x, int dtype, size_t samples, size_t positions, size_t channels,
+                             size_t groups, ptrdiff_t x_stride, const void* d_gamma, const void* d_beta, int param_dtype,
+                             float eps, void* d_y, ptrdiff_t y_stride, float* d_mean, float* d_rstd, int8_t* d_codes,
+                             uint8_t* d_scales, void* d_ws, size_t ws_bytes, cswap_stream_t stream);
+int cswap_group_norm_backward(int act, const void* d_dy, int dtype, size_t samples, size_t positions, size_t channels,
+                              size_t groups, ptrdiff_t dy_stride, const void* d_x, ptrdiff_t x_stride,
+                              const int8_t* d_codes, const uint8_t* d_scales, const float* d_mean, const float* d_rstd,
+                              const void* d_gamma, const void* d_beta, int param_dtype, void* d_dx, ptrdiff_t dx_stride,
+                              void* d_dgamma, void* d_dbeta, void* d_ws, size_t ws_bytes, cswap_stream_t stream);
 
 /* Gradients of a linear layer y = x W^T + b (W: n x k) from the checkpoint x^ of its input
  * (rows x k): dw[n][k] = sum over rows of dy[.][n] x^[.][k], db[n] = sum over rows of dy[.][n]
