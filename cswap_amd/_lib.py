@@ -140,6 +140,9 @@ _SIGNATURES = {
     "cswap_group_norm_backward": (i32, [i32, vp, i32, sz, sz, sz, sz, pd, vp, pd, vp, vp, vp, vp, vp, vp, i32, vp, pd, vp, vp, vp, sz, vp]),
     "cswap_q8_weight_grad_workspace_bytes": (sz, [i32, sz, sz, sz]),
     "cswap_q8_weight_grad": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, vp, vp, i32, vp, sz, vp]),
+    "cswap_f8_pack_weight": (i32, [vp, i32, sz, sz, pd, vp, vp, vp, vp]),
+    "cswap_f8_linear_workspace_bytes": (sz, [sz, sz]),
+    "cswap_f8_linear": (i32, [vp, i32, sz, sz, pd, vp, vp, sz, i32, vp, i32, vp, i32, pd, vp, sz, vp]),
     "cswap_adamw_moment_bytes": (sz, [sz]),
     "cswap_adamw_factors_bytes": (sz, []),
     "cswap_adamw_step": (i32, [vp, sz, i32, C.POINTER(AdamwOptions), C.c_longlong, vp]),

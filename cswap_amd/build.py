@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcswap_hip.so")
 
 SOURCES = ["common.cpp", "zfp_kernels.hip", "zvc_kernels.hip", "q8_kernels.hip", "norm_kernels.hip", "wgrad_kernels.hip",
-           "adamw_kernels.hip", "group_norm_kernels.hip", "link_kernels.hip", "select.cpp", "planner.cpp", "swap_engine.cpp", "compat.cpp"]
+           "adamw_kernels.hip", "group_norm_kernels.hip",
+           "f8_kernels.hip", "link_kernels.hip", "select.cpp", "planner.cpp", "swap_engine.cpp", "compat.cpp"]
 
 HIPCC_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",

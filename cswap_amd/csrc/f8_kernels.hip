@@ -1,0 +1,526 @@
+// f8_kernels.hip -- products of linear layers in 8-bit floating point (e4m3: sign, four bits of exponent, three of mantissa) with a power of two
+// for each 128 values of a row of activations and for each 128 x 128 weights:
+//
+//   y[m][n] = sum over blocks c of 128 of  2^(sx[m][c] + sw[n / 128][c])  sum over k in c of x8[m][k] w8[n][k]  + bias[n]
+//
+// and the gradient of the input, dx = dy W, which is the same product with the codes of W turned round.  The scaled matrix instructions of
+// this chip take a power of two for each lane's 32 values along k, so a block's two scales go into the instruction and nothing is
+// multiplied behind it: that is why the scales are powers of two (it costs up to one bit of range against max / 448, none of precision).
+//
+// Scale of a block: the least 2^s, s >= -126, with max|x| <= 448 * 2^s, held as the byte s + 127.  A block that holds a NaN or an infinity has
+// codes of NaN (0x7f): every result that it goes into is NaN.
+#include <hip/hip_runtime.h>
+#include "../../include/cswap_hip.h"
+#include "common.h"
+#include "q8_block.h"
+#include "q8_params.h"
+
+namespace cswap {
+namespace q8 {
+
+constexpr int kBlock = 128;
+constexpr size_t kMaxFeatures = (size_t)1 << 20;
+
+typedef int i8v __attribute__((ext_vector_type(8)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+inline size_t blocks_of(size_t n) { return (n + kBlock - 1) / kBlock; }
+inline size_t rows16(size_t rows) { return (rows + 15) / 16 * 16; }
+
+// The scale byte of a block whose largest magnitude has these bits; 0 where it is not finite.
+__device__ inline uint32_t f8_scale(uint32_t max_bits)
+{
+  const int s = (int)(max_bits >> 23) - 8 + ((max_bits & 0x7fffffu) > 0x600000u);
+  return max_bits >= 0x7f800000u ? 0u : (uint32_t)max(s, 1);
+}
+
+// Eight codes; a scale of 0: NaN.  The products are exact and at most 448.
+__device__ inline uint2 f8_codes(const float v[8], uint32_t scale)
+{
+  const float inverse = __uint_as_float((254u - scale) << 23);
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inverse, v[5] * inverse, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inverse, v[7] * inverse, hi, true);
+  return scale ? make_uint2((uint32_t)lo, (uint32_t)hi) : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+}
+__device__ inline uint8_t stored_scale(uint32_t scale) { return (uint8_t)(scale ? scale : 127u); }
+
+// The largest magnitude of eight values, NaN if one is; then of the lanes of a row of 16.
+__device__ inline float largest(const float v[8])
+{
+  float m = larger(__builtin_fabsf(v[0]), __builtin_fabsf(v[1]));
+#pragma unroll
+  for (int i = 2; i < 8; i += 2) m = larger(larger(m, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+  return m;
+}
+template <int CTRL> __device__ inline float larger_dpp(float m)
+{
+  return larger(m, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, m), CTRL, 0xf, 0xf, true)));
+}
+__device__ inline float largest_of_16(float m)
+{
+  m = larger_dpp<0xb1>(m);          // lane ^ 1
+  m = larger_dpp<0x4e>(m);          // lane ^ 2
+  m = larger_dpp<0x141>(m);         // 7 - lane
+  return larger_dpp<0x140>(m);      // 15 - lane
+}
+
+// ---------------------------------------------------------------- activations to codes
+// 16 lanes to a block of 128 values of a row, 16 rows a workgroup: their scales, of one block, are neighbours in scales[block][row].
+// Memory bounds it.
+template <typename T>
+__global__ __launch_bounds__(256) void f8_rows_kernel(const typename T::value* __restrict__ x, size_t stride, uint32_t rows, uint32_t cols, uint32_t blocks,
+                                                      uint2* __restrict__ codes, uint8_t* __restrict__ scales, uint32_t scale_pitch)
+{
+  const uint32_t block = blockIdx.x % blocks, row = blockIdx.x / blocks * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  const uint32_t at = min(row, rows - 1), col = block * kBlock + lane * kChunk;
+  float v[8];
+  load_chunk<T>(x + (size_t)at * stride + col, valid_at(col, cols), v);
+  const uint32_t scale = f8_scale(__float_as_uint(largest_of_16(largest(v))) & 0x7fffffffu);
+  const uint2 q = f8_codes(v, scale);
+  if (row < rows) {
+    codes[((size_t)row * blocks + block) * (kBlock / kChunk) + lane] = q;
+    if (lane == 0) scales[(size_t)block * scale_pitch + row] = stored_scale(scale);
+  }
+}
+
+// ---------------------------------------------------------------- weights to codes
+// A workgroup has 128 x 128 weights in registers from load to store; the codes turned round go through LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void f8_weight_kernel(const typename T::value* __restrict__ w, size_t stride, uint32_t n, uint32_t k, uint2* __restrict__ codes,
+                                                        uint4* __restrict__ turned, uint8_t* __restrict__ scales)
+{
+  __shared__ uint32_t tile[kBlock][kBlock / 4 + 1];
+  __shared__ float most[4];
+  const uint32_t kb = (k + kBlock - 1) / kBlock, nb = (n + kBlock - 1) / kBlock;
+  const uint32_t bn = blockIdx.x / kb, bk = blockIdx.x % kb, lane = threadIdx.x & 15, first = threadIdx.x >> 4;
+  const uint32_t col = bk * kBlock + lane * kChunk;
+  const int valid = valid_at(col, k);
+  u4_any raw[8][T::bytes / 2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t row = bn * kBlock + first + 16 * i;
+    load_raw<T>(w + (size_t)min(row, n - 1) * stride + col, row < n ? valid : 0, raw[i]);
+  }
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v[8];
+    widen<T>(raw[i], v);
+    m = larger(m, largest(v));
+  }
+  m = largest_of_16(m);
+  m = larger(m, __shfl_xor(m, 16));
+  m = larger(m, __shfl_xor(m, 32));
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = larger(larger(most[0], most[1]), larger(most[2], most[3]));
+  const uint32_t scale = f8_scale(__float_as_uint(m) & 0x7fffffffu);
+  if (threadIdx.x == 0) scales[(size_t)bn * kb + bk] = stored_scale(scale);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v[8];
+    widen<T>(raw[i], v);
+    const uint2 q = f8_codes(v, scale);
+    const uint32_t r = first + 16 * i;
+    codes[((size_t)(bn * kBlock + r) * kb + bk) * (kBlock / kChunk) + lane] = q;
+    if (turned) tile[r][2 * lane] = q.x, tile[r][2 * lane + 1] = q.y;
+  }
+  if (!turned) return;
+  __syncthreads();
+  // 16 codes of a column, from 16 rows
+  for (uint32_t j = threadIdx.x; j < kBlock * (kBlock / 16); j += 256) {
+    const uint32_t c = j % kBlock, r = j / kBlock * 16;
+    uint32_t out[4];
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word |= ((tile[r + 4 * o + i][c >> 2] >> (8 * (c & 3))) & 0xffu) << (8 * i);
+      out[o] = word;
+    }
+    turned[((size_t)(bk * kBlock + c) * nb + bn) * (kBlock / 16) + r / 16] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+// ---------------------------------------------------------------- products
+struct F8Shape {
+  uint32_t rows, n, blocks;        // of the result; blocks of 128 of what is summed over
+  uint32_t scale_pitch;            // of the activations' scales[block][row]
+  uint32_t step_n, step_k;         // of the weights' scales: from a block of the result's columns, of what is summed over, to the next
+  uint32_t tiles_m, tiles_n;
+  size_t y_stride;
+};
+
+// Four neighbouring results of a row with their bias.
+struct F8Out {
+  void* y;
+  const void* bias;  // NULL: none
+  int dtype, bias_dtype;
+};
+__device__ inline float bias_at(const F8Out& o, uint32_t col)
+{
+  if (!o.bias) return 0.0f;
+  if (o.bias_dtype == CSWAP_DT_F32) return static_cast<const float*>(o.bias)[col];
+  const uint16_t v = static_cast<const uint16_t*>(o.bias)[col];
+  return o.bias_dtype == CSWAP_DT_BF16 ? to_float<BF16>(v) : to_float<F16>(v);
+}
+__device__ inline void store_one(const F8Out& o, size_t at, float v)
+{
+  if (o.dtype == CSWAP_DT_F32) static_cast<float*>(o.y)[at] = v;
+  else static_cast<uint16_t*>(o.y)[at] = o.dtype == CSWAP_DT_BF16 ? from_float<BF16>(v) : from_float<F16>(v);
+}
+
+// Results in 16 bits come from the 8-bit matrix instructions.  These line a call's products up before they add them, and what lies more than 13 bits below
+// the largest product is cut off (measured; the sum with what was there before is fp32): a result is off by about 3e-5 of the products' norm,
+// a tenth of what rounding it to fp16 costs and a fiftieth of bf16's.  Results in fp32 (EXACT) come from the codes as bf16, which hold them
+// and their scales exactly, at half the rate: products are exact and sums fp32.
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+
+// Eight codes as bf16.
+__device__ inline uint4 f8_as_bf16(uint2 q, float unit)
+{
+  uint4 w;
+  w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.x, unit, false));
+  w.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.x, unit, true));
+  w.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.y, unit, false));
+  w.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.y, unit, true));
+  return w;
+}
+
+// Few rows: bound by the weights' bytes, which every workgroup reads once and no other reads.  A workgroup makes 16 columns; its eight wavefronts take
+// blocks of k in turn and add up through LDS.  A lane has 32 codes of one of 16 rows: that is one 16 x 16 x 128 matrix instruction a block, or
+// four of 16 x 16 x 32 in bf16 (which of a lane's codes meet in which does not matter as long as both operands have them alike).
+// The activations are turned into codes in registers, by every workgroup for itself: four lanes have a row's block.
+constexpr int kFewWaves = 8;
+template <typename T, int MF, bool EXACT>
+__global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typename T::value* __restrict__ x, size_t x_stride, uint32_t k, F8Shape s,
+                                                                     const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales, F8Out out)
+{
+  __shared__ __attribute__((aligned(16))) float part[kFewWaves][MF * 256];
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, quarter = lane >> 4;
+  const uint32_t col0 = blockIdx.x * 16, pitch = s.blocks * kBlock;
+  f4v acc[MF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f) acc[f] = (f4v){0, 0, 0, 0};
+  const uint8_t* from = w + (size_t)(col0 + r) * pitch + quarter * 32;  // weights are filled up to whole blocks: the row is there
+  for (uint32_t b = wave; b < s.blocks; b += kFewWaves) {
+    const uint4* at = reinterpret_cast<const uint4*>(from + (size_t)b * kBlock);
+    const uint4 w0 = at[0], w1 = at[1];
+    const int w_scale = w_scales[(size_t)(col0 / kBlock) * s.step_n + (size_t)b * s.step_k];
+    const uint32_t col = b * kBlock + quarter * 32;
+    float v[MF][4][8];
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+      const uint32_t row = f * 16 + r;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        load_chunk<T>(x + (size_t)min(row, s.rows - 1) * x_stride + col + 8 * c, row < s.rows ? valid_at(col + 8 * c, k) : 0, v[f][c]);
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+      float m = larger(larger(largest(v[f][0]), largest(v[f][1])), larger(largest(v[f][2]), largest(v[f][3])));
+      m = larger(m, __shfl_xor(m, 16));
+      m = larger(m, __shfl_xor(m, 32));
+      const uint32_t scale = f8_scale(__float_as_uint(m) & 0x7fffffffu);
+      uint2 q[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) q[c] = f8_codes(v[f][c], scale);
+      const uint2 p[4] = {{w0.x, w0.y}, {w0.z, w0.w}, {w1.x, w1.y}, {w1.z, w1.w}};
+      if constexpr (EXACT) {
+        const float unit = unit_of(stored_scale(scale)), w_unit = unit_of(w_scale);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, f8_as_bf16(p[c], w_unit)), __builtin_bit_cast(bf8, f8_as_bf16(q[c], unit)),
+                                                           acc[f], 0, 0, 0);
+      } else {
+        const i8v wf = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
+        const i8v xf = {(int)q[0].x, (int)q[0].y, (int)q[1].x, (int)q[1].y, (int)q[2].x, (int)q[2].y, (int)q[3].x, (int)q[3].y};
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[f], 0, 0, 0, w_scale, 0, (int)stored_scale(scale));
+      }
+    }
+  }
+  // a lane has columns 4 * quarter and on of row r
+#pragma unroll
+  for (int f = 0; f < MF; ++f) *reinterpret_cast<float4*>(&part[wave][(f * 16 + r) * 16 + 4 * quarter]) = make_float4(acc[f][0], acc[f][1], acc[f][2], acc[f][3]);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < MF * 256; i += 64 * kFewWaves) {
+    const uint32_t row = i / 16, col = col0 + i % 16;
+    float sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kFewWaves; ++p) sum += part[p][i];
+    if (row < s.rows && col < s.n) store_one(out, (size_t)row * s.y_stride + col, sum + bias_at(out, col));
+  }
+}
+
+// Many rows.  Four wavefronts, WM x WN of them, make a tile of TM rows x TN columns, a stage of 128 along k (EXACT: 64) at a time.  Stages lie in
+// LDS row by row, 128 bytes each, as chunks of 16 whose order within a row depends on it, so that eight lanes that read eight rows meet in
+// no bank; two stages, the next one on its way through registers while this one multiplies.  The results go out through LDS, too, in whole rows.
+template <int TM, int TN, int WM, int WN, bool EXACT>
+__global__ __launch_bounds__(256, TM * TN >= 256 * 256 ? 1 : 2) void f8_product_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ x_scales,
+                                                                                       const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales,
+                                                                                       F8Shape s, F8Out out)
+{
+  constexpr int FM = TM / WM / 32, FN = TN / WN / 32, kRows = TM + TN, kLoads = kRows / 32, kStage = kRows * kBlock;
+  constexpr int kDeep = EXACT ? 64 : 128, kSteps = EXACT ? 4 : 2, kOut = EXACT ? 4 : 2;  // k of a stage, matrix instructions along it; bytes of a result
+  static_assert(WM * WN == 4 && TN / WN <= kBlock, "four wavefronts, each within one block of columns");
+  static_assert(TM * TN * kOut <= 2 * kStage, "a tile's results fit the stages");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][kStage];
+  // XCDs take workgroups in turn; each gets neighbouring tiles, up to 16 along n before the next rows
+  const uint32_t count = s.tiles_m * s.tiles_n, xcd = blockIdx.x % 8, each = count / 8, more = count % 8;
+  uint32_t at = xcd * each + min(xcd, more) + blockIdx.x / 8;
+  const uint32_t column = at / (16 * s.tiles_m), width = min(16u, s.tiles_n - 16 * column);
+  at -= column * 16 * s.tiles_m;
+  const uint32_t m0 = at / width * TM, n0 = (16 * column + at % width) * TN;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t pitch = s.blocks * kBlock, n_rows = (s.n + kBlock - 1) / kBlock * kBlock;
+
+  // staging: chunk tid % 8 of rows tid / 8 + 32 i; behind the last row the last one again, which goes into results that nobody stores
+  const int chunk = tid & 7, row = tid >> 3;
+  constexpr int kCodes = kDeep / 8;  // codes of a chunk
+  const uint8_t* const x_from = x + (size_t)m0 * pitch;
+  const uint8_t* const w_from = w + (size_t)n0 * pitch;
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t r = row + 32 * i;
+    const uint32_t there = r < TM ? min(r, s.rows - 1 - m0) : min(r - TM, n_rows - 1 - n0);
+    off[i] = there * pitch + kCodes * chunk;
+  }
+  u4v raw[EXACT ? 1 : kLoads];
+  uint2 raw8[EXACT ? kLoads : 1];
+  uint32_t unit8[EXACT ? kLoads : 1];
+  const uint32_t stages = s.blocks * (kBlock / kDeep), last = stages - 1;
+  auto load = [&](uint32_t stage, int i) __attribute__((always_inline)) {
+    const uint8_t* base = (32 * i < TM ? x_from : w_from) + (size_t)stage * kDeep;
+    if constexpr (EXACT) {
+      raw8[i] = *reinterpret_cast<const uint2*>(base + off[i]);
+      const uint32_t b = stage / 2, r = row + 32 * i;
+      unit8[i] = 32 * i < TM ? x_scales[(size_t)b * s.scale_pitch + min(m0 + r, s.rows - 1)]
+                             : w_scales[(size_t)(min(n0 + 32 * i - TM, s.n - 1) / kBlock) * s.step_n + (size_t)b * s.step_k];
+    } else {
+      raw[i] = *reinterpret_cast<const u4v*>(base + off[i]);
+    }
+  };
+  const int place = row * kBlock + 16 * (chunk ^ (row & 7));
+  auto store = [&](uint8_t* buf, int i) __attribute__((always_inline)) {
+    if constexpr (EXACT) *reinterpret_cast<uint4*>(buf + place + 32 * i * kBlock) = f8_as_bf16(raw8[i], unit_of(unit8[i]));
+    else *reinterpret_cast<u4v*>(buf + place + 32 * i * kBlock) = raw[i];
+  };
+
+  // reading: lane l has 32 codes, or eight bf16, of row l % 32 from that many times l / 32 on
+  const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5;
+  const uint32_t my_n = n0 + wn * (TN / WN), my_m = m0 + wm * (TM / WM);
+  const uint8_t* const ws_from = w_scales + (size_t)(min(my_n, s.n - 1) / kBlock) * s.step_n;
+  uint32_t xs_at[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) xs_at[i] = min(my_m + 32 * i + r, s.rows - 1);
+  int xs[2][FM], ws[2];
+  auto load_scales = [&](uint32_t stage, int which) __attribute__((always_inline)) {
+    if constexpr (!EXACT) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) xs[which][i] = x_scales[(size_t)stage * s.scale_pitch + xs_at[i]];
+      ws[which] = ws_from[(size_t)stage * s.step_k];
+    }
+  };
+  constexpr int kWords = EXACT ? 1 : 2;  // of 16 bytes
+  struct Frag {
+    u4v w[kWords];
+  };
+  auto frag = [&](const uint8_t* buf, int first_row, int step) __attribute__((always_inline)) {
+    Frag f;
+#pragma unroll
+    for (int h = 0; h < kWords; ++h)
+      f.w[h] = *reinterpret_cast<const u4v*>(buf + (first_row + r) * kBlock + 16 * ((2 * kWords * step + kWords * half + h) ^ (r & 7)));
+    return f;
+  };
+  f16v acc[FN][FM] = {};
+  Frag xf[2][FM], wf[2][FN];
+  auto read = [&](const uint8_t* buf, int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) wf[step & 1][i] = frag(buf, TM + wn * (TN / WN) + 32 * i, step);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) xf[step & 1][i] = frag(buf, wm * (TM / WM) + 32 * i, step);
+  };
+  auto multiply = [&](int step, int which) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        const Frag &a = wf[step & 1][i], &b = xf[step & 1][j];
+        if constexpr (EXACT) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a.w[0]), __builtin_bit_cast(bf8, b.w[0]), acc[i][j], 0, 0, 0);
+        } else {
+          const i8v p = {(int)a.w[0].x, (int)a.w[0].y, (int)a.w[0].z, (int)a.w[0].w, (int)a.w[1].x, (int)a.w[1].y, (int)a.w[1].z, (int)a.w[1].w};
+          const i8v q = {(int)b.w[0].x, (int)b.w[0].y, (int)b.w[0].z, (int)b.w[0].w, (int)b.w[1].x, (int)b.w[1].y, (int)b.w[1].z, (int)b.w[1].w};
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(p, q, acc[i][j], 0, 0, 0, ws[which], 0, xs[which][j]);
+        }
+      }
+  };
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load(0, i);
+  load_scales(0, 0);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) store(lds[0], i);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load(min(1u, last), i);
+  __syncthreads();
+  read(lds[0], 0);
+  // A stage: the fragments of a step are read while the step before multiplies, those of the next stage's first step, behind the barrier, beside
+  // the last products of this one.
+  auto one_stage = [&](uint32_t st, int which) __attribute__((always_inline)) {
+    uint8_t *buf = lds[which], *next = lds[which ^ 1];
+    load_scales(min(st + 1, last), which ^ 1);
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step) {
+      if (step + 1 < kSteps) {
+        read(buf, step + 1);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (i * (kSteps - 1) / kLoads == step) {
+            store(next, i);
+            load(min(st + 2, last), i);
+          }
+      } else {
+        __syncthreads();
+        read(next, 0);
+      }
+      multiply(step, which);
+    }
+  };
+  uint32_t st = 0;
+  for (; st + 2 <= stages; st += 2) {
+    one_stage(st, 0);
+    one_stage(st + 1, 1);
+  }
+  if (st < stages) one_stage(st, 0);
+
+  // Results: lane l has row l % 32, columns 8 q + 4 (l / 32) + 0 to 3 for q = 0 to 3.  To LDS as rows of chunks of 16 bytes, in another order in
+  // each row, and from there to memory.
+  __syncthreads();  // the last stage asked for fragments of a stage that is not there
+  constexpr int kChunks = TN * kOut / 16, kEach = 16 / kOut;  // chunks of a row, results of a chunk
+  uint8_t* const tile = lds[0];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = wn * (TN / WN) + 32 * i + 8 * q + 4 * half;
+      float bias[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[e] = bias_at(out, min(n0 + c + e, s.n - 1));
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        const int m = wm * (TM / WM) + 32 * j + r;
+        uint8_t* to = tile + m * (TN * kOut) + 16 * ((c / kEach) ^ (m & (kChunks - 1))) + (c % kEach) * kOut;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] + bias[e];
+        if constexpr (EXACT) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        else if (out.dtype == CSWAP_DT_BF16) *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<BF16>(v[0], v[1]), to_pair<BF16>(v[2], v[3]));
+        else *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<F16>(v[0], v[1]), to_pair<F16>(v[2], v[3]));
+      }
+    }
+  __syncthreads();
+  const uint32_t rows_here = min((uint32_t)TM, s.rows - m0);
+  for (uint32_t i = tid; i < (uint32_t)TM * kChunks; i += 256) {
+    const uint32_t m = i / kChunks, c = i % kChunks, n = n0 + c * kEach;
+    if (m >= rows_here || n >= s.n) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + m * (TN * kOut) + 16 * (c ^ (m & (kChunks - 1))));
+    uint8_t* to = static_cast<uint8_t*>(out.y) + ((size_t)(m0 + m) * s.y_stride + n) * kOut;
+    if (n + kEach <= s.n) {
+      *reinterpret_cast<u4_any*>(to) = (u4_any){v.x, v.y, v.z, v.w};
+    } else {
+      const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < kEach - 1; ++e)
+        if (n + e < s.n) {
+          if constexpr (EXACT) reinterpret_cast<uint32_t*>(to)[e] = word[e];
+          else reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(word[e / 2] >> (16 * (e & 1)));
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches
+constexpr size_t kFewRows = 32;
+
+static bool f8_shape(size_t rows, size_t n, size_t k) { return n <= kMaxFeatures && k <= kMaxFeatures && rows < ((size_t)1 << 31); }
+
+}  // namespace q8
+}  // namespace cswap
+
+using namespace cswap;
+using namespace cswap::q8;
+
+extern "C" size_t cswap_f8_linear_workspace_bytes(size_t rows, size_t k)
+{
+  if (rows <= kFewRows || k == 0 || !f8_shape(rows, 1, k)) return 0;
+  return blocks_of(k) * (rows * kBlock + rows16(rows));
+}
+
+extern "C" int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t k, ptrdiff_t stride, uint8_t* d_codes, uint8_t* d_turned,
+                                    uint8_t* d_scales, cswap_stream_t stream)
+{
+  if (n == 0 || k == 0) return CSWAP_E_ARG;
+  if (!f8_shape(1, n, k)) return CSWAP_E_UNSUPPORTED;
+  if (int e = check_rows(n, k, &stride)) return e;
+  if (!dtype_known(dtype) || !value_ptr(d_w, dtype) || !d_codes || !d_scales || reinterpret_cast<uintptr_t>(d_codes) % 16 ||
+      reinterpret_cast<uintptr_t>(d_turned) % 16)
+    return CSWAP_E_ARG;
+  return with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    hipLaunchKernelGGL(f8_weight_kernel<T>, dim3((unsigned)(blocks_of(n) * blocks_of(k))), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const typename T::value*>(d_w), (size_t)stride, (uint32_t)n, (uint32_t)k, reinterpret_cast<uint2*>(d_codes),
+                       reinterpret_cast<uint4*>(d_turned), d_scales);
+    return check_launch();
+  });
+}
+
+extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k, ptrdiff_t x_stride, const uint8_t* d_codes, const uint8_t* d_scales,
+                               size_t n, int turned, const void* d_bias, int bias_dtype, void* d_y, int out_dtype, ptrdiff_t y_stride, void* d_ws,
+                               size_t ws_bytes, cswap_stream_t stream)
+{
+  if (n == 0 || k == 0) return CSWAP_E_ARG;
+  if (!f8_shape(rows, n, k)) return CSWAP_E_UNSUPPORTED;
+  if (int e = check_rows(rows, k, &x_stride)) return e;
+  if (int e = check_rows(rows, n, &y_stride)) return e;
+  if (!dtype_known(dtype) || !dtype_known(out_dtype) || !dtype_known(bias_dtype) || (turned != 0 && turned != 1)) return CSWAP_E_ARG;
+  if (rows == 0) return CSWAP_OK;
+  if (!value_ptr(d_x, dtype) || !value_ptr(d_y, out_dtype) || (d_bias && !value_ptr(d_bias, bias_dtype)) || !d_codes || !d_scales ||
+      reinterpret_cast<uintptr_t>(d_codes) % 16)
+    return CSWAP_E_ARG;
+  const size_t need = cswap_f8_linear_workspace_bytes(rows, k);
+  if (need && (!d_ws || reinterpret_cast<uintptr_t>(d_ws) % 16)) return CSWAP_E_ARG;
+  if (ws_bytes < need) return CSWAP_E_NOMEM;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint32_t kb = (uint32_t)blocks_of(k), nb = (uint32_t)blocks_of(n);
+  F8Shape s = {(uint32_t)rows, (uint32_t)n, kb, (uint32_t)rows16(rows), turned ? 1u : kb, turned ? nb : 1u, 0, 0, (size_t)y_stride};
+  const F8Out out = {d_y, d_bias, out_dtype, bias_dtype};
+  return with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    const typename T::value* x = static_cast<const typename T::value*>(d_x);
+    if (rows <= kFewRows) {
+      auto f = out_dtype == CSWAP_DT_F32 ? (rows <= 16 ? f8_few_rows_kernel<T, 1, true> : f8_few_rows_kernel<T, 2, true>)
+                                         : (rows <= 16 ? f8_few_rows_kernel<T, 1, false> : f8_few_rows_kernel<T, 2, false>);
+      hipLaunchKernelGGL(f, dim3((unsigned)((n + 15) / 16)), dim3(64 * kFewWaves), 0, st, x, (size_t)x_stride, (uint32_t)k, s, d_codes, d_scales, out);
+      return check_launch();
+    }
+    uint8_t *codes = static_cast<uint8_t*>(d_ws), *scales = codes + rows * kb * kBlock;
+    hipLaunchKernelGGL(f8_rows_kernel<T>, dim3((unsigned)(rows16(rows) / 16 * kb)), dim3(256), 0, st, x, (size_t)x_stride, (uint32_t)rows, (uint32_t)k, kb,
+                       reinterpret_cast<uint2*>(codes), scales, s.scale_pitch);
+    if (int e = check_launch()) return e;
+    auto launch = [&](auto f, uint32_t tm, uint32_t tn) {
+      s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
+      hipLaunchKernelGGL(f, dim3(s.tiles_m * s.tiles_n), dim3(256), 0, st, codes, scales, d_codes, d_scales, s, out);
+      return check_launch();
+    };
+    if (out_dtype == CSWAP_DT_F32) return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128);
+    const size_t large = ((rows + 255) / 256) * ((n + 255) / 256);
+    return large >= 512 ? launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256) : launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128);
+  });
+}

@@ -7,6 +7,7 @@ stays on the device in one byte a value, and the layer's backward pass reads it 
     import cswap_amd.layers8 as layers8
     layers8.checkpoint_layers(model)        # nn.Linear, nn.LayerNorm, nn.GELU, nn.SiLU of a model, in place
     layers8.checkpoint_layers(model, group_norm=True)                   # and nn.GroupNorm, for images that lie channels last
+    layers8.checkpoint_layers(model, f8=True)                           # linear layers whose products are in 8-bit floating point, too
     y = layers8.group_norm(x, 32, weight, bias, act="silu")            # with an activation function in the same call
     y = layers8.linear(x, weight, bias)     # or function by function
 
@@ -27,10 +28,12 @@ import torch.nn.functional as F
 from torch import nn
 from torch.autograd.function import once_differentiable
 
+from . import f8 as _f8
 from . import q8
+from .f8 import F8Weight
 from .q8 import Checkpoint8
 
-__all__ = ["hold", "linear", "layer_norm", "group_norm", "activation", "Linear8", "LayerNorm8", "GroupNorm8", "GELU8", "SiLU8", "checkpoint_layers"]
+__all__ = ["hold", "linear", "linear_f8", "layer_norm", "group_norm", "activation", "Linear8", "LinearF8", "LayerNorm8", "GroupNorm8", "GELU8", "SiLU8", "checkpoint_layers"]
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -113,6 +116,64 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         with torch.autocast("cuda", enabled=False):
             return _Linear.apply(x, weight, bias, held)
     return _Linear.apply(x, weight, bias, held)
+
+
+class _LinearF8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, held, weight8):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if weight8 is None:
+            weight8 = _f8.f8_weight(_rows(weight.detach()), backward=need_x)
+        elif tuple(weight8.shape) != tuple(weight.shape) or weight8.device != weight.device or need_x and weight8.turned is None:
+            raise ValueError(f"linear_f8: weight8 is {weight8} on {weight8.device}, the weight {tuple(weight.shape)} on {weight.device}")
+        if need_w:
+            if held is None:
+                held = hold(x)
+            elif tuple(held.shape) != tuple(x.shape) or held.dtype != x.dtype or held.device != x.device:
+                raise ValueError(f"linear_f8: held is the checkpoint of a {tuple(held.shape)} {held.dtype} tensor on {held.device}, x is "
+                                 f"{tuple(x.shape)} {x.dtype} on {x.device}")
+        # codes go through autograd as bytes, which hooks that take activations leave alone
+        codes = (weight8.turned.view(torch.uint8), weight8.scales) if need_x else (None, None)
+        _keep(ctx, held if need_w else None, *codes)
+        ctx.weight = weight.shape, weight.dtype
+        return _f8.f8_linear(_rows(x), weight8, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        dy = _rows(dy)
+        (n, k), dtype = ctx.weight
+        codes, scales, *held = _kept(ctx, 2) if need_w else ctx.saved_tensors
+        if need_w:
+            dw, db = q8.q8_weight_grad(dy, held[0], bias=need_b, out_dtype=dtype)
+        elif need_b:
+            db = dy.reshape(-1, n).sum(dim=0)
+        if need_x:
+            dx = _f8._product("linear_f8: dy", dy, _Scales(scales, dy.device), codes, n, k, 1, None, None)
+        return dx, dw, db, None, None
+
+
+class _Scales:
+    """What a product reads of an ``F8Weight`` besides its codes."""
+    __slots__ = ("scales", "device")
+
+    def __init__(self, scales, device):
+        self.scales, self.device = scales, device
+
+
+def linear_f8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, held: Checkpoint8 | None = None,
+              weight8: F8Weight | None = None):
+    """``x @ weight.T + bias`` in 8-bit floating point (``cswap_amd.f8``), and so the gradient of x; that of the weight comes from x's 8-bit checkpoint.
+    ``held``: that checkpoint, ``weight8``: the weight as ``f8.f8_weight`` lays it out, where they are there already (a weight that several
+    micro-batches meet is laid out once).  Under autocast in its type."""
+    if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight, bias = (t if t is None else t.to(dtype) for t in (x, weight, bias))
+    if not torch.is_grad_enabled():
+        return _f8.f8_linear(_rows(x), weight8 or _f8.f8_weight(_rows(weight), backward=False), bias)
+    return _LinearF8.apply(x, weight, bias, held, weight8)
 
 
 # ------------------------------------------------------------------- layer norm
@@ -220,6 +281,14 @@ class Linear8(nn.Linear):
         return linear(x, self.weight, self.bias)
 
 
+class LinearF8(nn.Linear):
+    """``nn.Linear`` whose products are in 8-bit floating point and whose input is kept in 8 bits.  The weight is laid out in each call; a
+    program that serves with weights that stay lays them out once and calls ``f8.f8_linear``."""
+
+    def forward(self, x):
+        return linear_f8(x, self.weight, self.bias)
+
+
 class LayerNorm8(nn.LayerNorm):
     """``nn.LayerNorm`` whose input is kept in 8 bits."""
 
@@ -271,15 +340,16 @@ class SiLU8(nn.SiLU):
 _KINDS = {nn.Linear: Linear8, nn.LayerNorm: LayerNorm8, nn.GELU: GELU8, nn.SiLU: SiLU8}
 
 
-def checkpoint_layers(model: nn.Module, group_norm: bool = False) -> nn.Module:
+def checkpoint_layers(model: nn.Module, group_norm: bool = False, f8: bool = False) -> nn.Module:
     """Every ``nn.Linear``, ``nn.LayerNorm``, ``nn.GELU`` and ``nn.SiLU`` of ``model`` (itself among them) becomes its form here, in place:
     parameters, hooks and state stay as they are.  Classes derived from them are left alone, and so are a SiLU that works
     in place, a layer norm over more than 16384 values, a linear layer with more than 2^20 features on one side, and either over
-    none.  ``group_norm=True``: every ``nn.GroupNorm`` of up to 4096 channels in up to 2048 groups, too, for models whose images lie channels last."""
+    none.  ``group_norm=True``: every ``nn.GroupNorm`` of up to 4096 channels in up to 2048 groups, too, for models whose images lie channels last.
+    ``f8=True``: linear layers become ``LinearF8``."""
     for m in model.modules():
         to = _KINDS.get(type(m)) or (GroupNorm8 if group_norm and type(m) is nn.GroupNorm else None)
         if to is not None and _fits(m):
-            m.__class__ = to
+            m.__class__ = LinearF8 if f8 and to is Linear8 else to
     return model
 
 

@@ -351,6 +351,24 @@ int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptr
                          void* d_dw, void* d_db, int out_dtype, void* d_ws, size_t ws_bytes,
                          cswap_stream_t stream);
 
+/* ---------------------------------- products in 8-bit floating point (f8) -----
+ * y = x W^T + bias of a linear layer (W: n x k) with both operands in e4m3 (sign, four bits of exponent, three of mantissa, 448 the
+ * largest) and a power of two for each 128 consecutive values of a row of x and for each 128 x 128 weights, sums in fp32.  The power of a
+ * block is the least 2^s, s >= -126, with max <= 448 * 2^s, held as the byte s + 127; a value is held as x / 2^s rounded to e4m3, to nearest even: off by at
+ * most 2^-4 of itself, or 2^-10 * 2^s.  A block that holds a NaN or an infinity has codes of NaN (0x7f, byte 127): its results are NaN.
+ * Weights are laid out once: codes [n'][k'], n' and k' rounded up to multiples of 128, 0 behind the last ones; `turned` (NULL: not wanted)
+ * the same as [k'][n'], which the product with W itself, dx = dy W, reads; scales [n'/128][k'/128].  Codes are 16-byte aligned.
+ * Up to 2^20 features on either side, 2^31 - 1 rows (CSWAP_E_UNSUPPORTED beyond); strides between rows as for checkpoints. */
+int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t k, ptrdiff_t stride, uint8_t* d_codes, uint8_t* d_turned,
+                         uint8_t* d_scales, cswap_stream_t stream);
+/* d_y (rows x n, out_dtype) from d_x (rows x k, dtype) and the codes of n x k weights; turned = 1: d_codes is `turned` of a k x n
+ * matrix, d_scales its scales.  d_bias may be NULL.  d_ws: cswap_f8_linear_workspace_bytes (NULL where that is 0), 16-byte
+ * aligned, no preparation; calls that overlap must not share one.  Sums are made in a fixed order. */
+size_t cswap_f8_linear_workspace_bytes(size_t rows, size_t k);
+int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k, ptrdiff_t x_stride, const uint8_t* d_codes,
+                    const uint8_t* d_scales, size_t n, int turned, const void* d_bias, int bias_dtype, void* d_y,
+                    int out_dtype, ptrdiff_t y_stride, void* d_ws, size_t ws_bytes, cswap_stream_t stream);
+
 /* ------------------------------------------------ AdamW over many tensors -----
  * No counterpart in the reference, which leaves the optimiser to its framework.  One step, t = 1, 2, ...:
  *   m' = b1 m + (1 - b1) g;  v' = b2 v + (1 - b2) (g g)

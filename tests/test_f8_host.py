@@ -1,0 +1,89 @@
+"""Products in 8-bit floating point without a GPU: the reference is torch's own e4m3, sizes, refusals."""
+import os
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import f8_reference as fref  # noqa: E402
+
+from cswap_amd import _lib, f8, layers8  # noqa: E402
+
+A = 1 << 20
+
+
+def test_the_reference_rounds_as_e4m3_does():
+    x = torch.randn(40, 300, dtype=torch.float64) * torch.exp(3 * torch.randn(40, 300, dtype=torch.float64))
+    x = x.float()
+    for rows in (1, 128):
+        value, scales = fref.held(x, rows)
+        unit = torch.exp2(scales.double() - 127).repeat_interleave(rows, 0)[:40].repeat_interleave(128, 1)[:, :300]
+        codes = (x.double() / unit).float().to(torch.float8_e4m3fn)
+        assert torch.equal(codes.double() * unit, value)
+        assert float((x.double() / unit).abs().max()) <= 448 and bool(((value - x.double()).abs() <= torch.maximum(x.double().abs() / 16, unit * 2.0 ** -10)).all())
+
+
+def test_scales_at_the_border():
+    x = torch.zeros(4, 128)
+    x[0, 0], x[1, 0], x[2, 0], x[3, 5] = 448.0, 448.0 * (1 + 2.0 ** -23), 1.75, 2.0 ** -140
+    assert fref.held(x, 1)[1].flatten().tolist() == [127, 128, 119, 1]
+
+
+def pack(w=A, dtype=0, n=4, k=4, stride=0, codes=A, turned=A, scales=A):
+    return _lib.lib().cswap_f8_pack_weight(w, dtype, n, k, stride, codes, turned, scales, None)
+
+
+def linear(x=A, dtype=0, rows=40, k=4, stride=0, codes=A, scales=A, n=4, turned=0, bias=A, kind=0, y=A, out=0, y_stride=0, ws=A, room=1 << 30):
+    return _lib.lib().cswap_f8_linear(x, dtype, rows, k, stride, codes, scales, n, turned, bias, kind, y, out, y_stride, ws, room, None)
+
+
+def test_argument_errors_do_not_launch():
+    for kw in (dict(w=0), dict(w=A + 2), dict(dtype=3), dict(n=0), dict(k=0), dict(stride=3), dict(codes=0), dict(codes=A + 8), dict(turned=A + 8), dict(scales=0)):
+        assert pack(**kw) == -1, kw
+    for kw in (dict(n=(1 << 20) + 1), dict(k=(1 << 20) + 1)):
+        assert pack(**kw) == -2 and linear(**kw) == -2, kw
+    assert linear(rows=1 << 31) == -2
+    for kw in (dict(x=0), dict(x=A + 2), dict(dtype=3), dict(out=-1), dict(kind=5), dict(k=0), dict(n=0), dict(stride=2), dict(y_stride=3), dict(codes=0), dict(codes=A + 4),
+               dict(scales=0), dict(turned=2), dict(bias=A + 2), dict(y=0), dict(y=A + 1), dict(ws=0), dict(ws=A + 8)):
+        assert linear(**kw) == -1, kw
+    assert linear(room=10) == -4
+    assert linear(rows=0, x=0, y=0, codes=0, scales=0, bias=0, ws=0) == 0
+
+
+def test_workspaces():
+    f = _lib.lib().cswap_f8_linear_workspace_bytes
+    assert f(0, 100) == 0 and f(1, 100) == 0 and f(100, 0) == 0
+    assert f(1000, 129) == 2 * (1000 * 128 + 1008)
+    assert f(1 << 31, 128) == 0 and f(100, (1 << 20) + 1) == 0
+
+
+def test_weights_have_the_arrays_of_their_shape():
+    codes, scales = torch.zeros(256, 128, dtype=torch.float8_e4m3fn), torch.zeros(2, 1, dtype=torch.uint8)
+    held = f8.F8Weight(codes, scales, (200, 100), torch.bfloat16)
+    assert held.turned is None and tuple(held.shape) == (200, 100)
+    assert tuple(f8.f8_weight_values(held).shape) == (200, 100)
+    turned = torch.zeros(128, 256, dtype=torch.float8_e4m3fn)
+    f8.F8Weight(codes, scales, (200, 100), torch.bfloat16, turned)
+    for bad in ((codes[:128], scales), (codes, scales.t()), (codes.view(torch.uint8), scales), (codes, scales.int()), (codes, scales, codes)):
+        with pytest.raises(ValueError):
+            f8.F8Weight(bad[0], bad[1], (200, 100), torch.bfloat16, *bad[2:])
+    with pytest.raises(TypeError):
+        f8.F8Weight(codes, scales, (200, 100), torch.float64)
+    with pytest.raises(ValueError, match="backward=False"):
+        f8.f8_linear_backward(torch.zeros(3, 200), held)
+    with pytest.raises(ValueError, match="device memory"):
+        f8.f8_linear(torch.zeros(3, 100), held)
+    with pytest.raises(ValueError, match="device memory"):
+        f8.f8_weight(torch.zeros(3, 100))
+    with pytest.raises(TypeError):
+        f8.f8_linear(torch.zeros(3, 100, dtype=torch.float64), held)
+
+
+def test_which_layers_are_converted():
+    from torch import nn
+
+    model = nn.Sequential(nn.Linear(3, 4), nn.GELU())
+    assert [type(m) for m in layers8.checkpoint_layers(model, f8=True)] == [layers8.LinearF8, layers8.GELU8]
+    model = nn.Sequential(nn.Linear(3, 4))
+    assert type(layers8.checkpoint_layers(model)[0]) is layers8.Linear8
