@@ -23,11 +23,13 @@ constexpr size_t kMaxFeatures = (size_t)1 << 20;
 
 typedef int i8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 
 inline size_t blocks_of(size_t n) { return (n + kBlock - 1) / kBlock; }
-inline size_t rows16(size_t rows) { return (rows + 15) / 16 * 16; }
+constexpr size_t kRowPad = 256;  // activations' codes have room for whole tiles, so that products need not ask which rows are there
+inline size_t padded(size_t rows) { return (rows + kRowPad - 1) / kRowPad * kRowPad; }
 
 // The scale byte of a block whose largest magnitude has these bits; 0 where it is not finite.
 __device__ inline uint32_t f8_scale(uint32_t max_bits)
@@ -90,25 +92,27 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const typename T::value* _
 
 // ---------------------------------------------------------------- weights to codes
 // A workgroup has 128 x 128 weights in registers from load to store; the codes turned round go through LDS.
+constexpr int kWeightThreads = 1024;
 template <typename T>
-__global__ __launch_bounds__(256) void f8_weight_kernel(const typename T::value* __restrict__ w, size_t stride, uint32_t n, uint32_t k, uint2* __restrict__ codes,
+__global__ __launch_bounds__(kWeightThreads) void f8_weight_kernel(const typename T::value* __restrict__ w, size_t stride, uint32_t n, uint32_t k, uint2* __restrict__ codes,
                                                         uint4* __restrict__ turned, uint8_t* __restrict__ scales)
 {
   __shared__ uint32_t tile[kBlock][kBlock / 4 + 1];
-  __shared__ float most[4];
+  constexpr int kTurns = kBlock * 16 / kWeightThreads, kRows = kBlock / kTurns;  // of 16 lanes a row
+  __shared__ float most[kWeightThreads / 64];
   const uint32_t kb = (k + kBlock - 1) / kBlock, nb = (n + kBlock - 1) / kBlock;
   const uint32_t bn = blockIdx.x / kb, bk = blockIdx.x % kb, lane = threadIdx.x & 15, first = threadIdx.x >> 4;
   const uint32_t col = bk * kBlock + lane * kChunk;
   const int valid = valid_at(col, k);
-  u4_any raw[8][T::bytes / 2];
+  u4_any raw[kTurns][T::bytes / 2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t row = bn * kBlock + first + 16 * i;
+  for (int i = 0; i < kTurns; ++i) {
+    const uint32_t row = bn * kBlock + first + kRows * i;
     load_raw<T>(w + (size_t)min(row, n - 1) * stride + col, row < n ? valid : 0, raw[i]);
   }
   float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kTurns; ++i) {
     float v[8];
     widen<T>(raw[i], v);
     m = larger(m, largest(v));
@@ -118,22 +122,23 @@ __global__ __launch_bounds__(256) void f8_weight_kernel(const typename T::value*
   m = larger(m, __shfl_xor(m, 32));
   if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
   __syncthreads();
-  m = larger(larger(most[0], most[1]), larger(most[2], most[3]));
+#pragma unroll
+  for (int i = 0; i < kWeightThreads / 64; ++i) m = larger(m, most[i]);
   const uint32_t scale = f8_scale(__float_as_uint(m) & 0x7fffffffu);
   if (threadIdx.x == 0) scales[(size_t)bn * kb + bk] = stored_scale(scale);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kTurns; ++i) {
     float v[8];
     widen<T>(raw[i], v);
     const uint2 q = f8_codes(v, scale);
-    const uint32_t r = first + 16 * i;
+    const uint32_t r = first + kRows * i;
     codes[((size_t)(bn * kBlock + r) * kb + bk) * (kBlock / kChunk) + lane] = q;
     if (turned) tile[r][2 * lane] = q.x, tile[r][2 * lane + 1] = q.y;
   }
   if (!turned) return;
   __syncthreads();
   // 16 codes of a column, from 16 rows
-  for (uint32_t j = threadIdx.x; j < kBlock * (kBlock / 16); j += 256) {
+  for (uint32_t j = threadIdx.x; j < kBlock * (kBlock / 16); j += kWeightThreads) {
     const uint32_t c = j % kBlock, r = j / kBlock * 16;
     uint32_t out[4];
 #pragma unroll
@@ -155,6 +160,17 @@ struct F8Shape {
   uint32_t tiles_m, tiles_n;
   size_t y_stride;
 };
+
+// Memory from an address on that is the same in all lanes: loads take it from scalar registers, with a lane's offset and one that the lanes share,
+// both 32 bits.  What is asked for behind its `bytes` reads as 0.
+struct Window {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ inline Window(const uint8_t* p, uint32_t bytes) : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, (int)bytes, 0x00020000)) {}
+  __device__ inline u4v load16(uint32_t lane, uint32_t all) const { return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)lane, (int)all, 0); }
+  __device__ inline u2v load8(uint32_t lane, uint32_t all) const { return __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)lane, (int)all, 0); }
+  __device__ inline uint32_t load1(uint32_t lane, uint32_t all) const { return __builtin_amdgcn_raw_buffer_load_b8(rsrc, (int)lane, (int)all, 0); }
+};
+__device__ inline uint32_t scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Four neighbouring results of a row with their bias.
 struct F8Out {
@@ -258,139 +274,163 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typen
   }
 }
 
+typedef int i4v __attribute__((ext_vector_type(4)));
+template <bool EXACT> struct FragOf {
+  typedef i8v type;
+};
+template <> struct FragOf<true> {
+  typedef bf8 type;
+};
+
 // Many rows.  Four wavefronts, WM x WN of them, make a tile of TM rows x TN columns, a stage of 128 along k (EXACT: 64) at a time.  Stages lie in
 // LDS row by row, 128 bytes each, as chunks of 16 whose order within a row depends on it, so that eight lanes that read eight rows meet in
 // no bank; two stages, the next one on its way through registers while this one multiplies.  The results go out through LDS, too, in whole rows.
 template <int TM, int TN, int WM, int WN, bool EXACT>
-__global__ __launch_bounds__(256, TM * TN >= 256 * 256 ? 1 : 2) void f8_product_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ x_scales,
+__global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void f8_product_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ x_scales,
                                                                                        const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales,
                                                                                        F8Shape s, F8Out out)
 {
-  constexpr int FM = TM / WM / 32, FN = TN / WN / 32, kRows = TM + TN, kLoads = kRows / 32, kStage = kRows * kBlock;
+  constexpr int NT = 64 * WM * WN, FM = TM / WM / 32, FN = TN / WN / 32, kRows = TM + TN, kEach32 = NT / 8, kLoads = kRows / kEach32, kStage = kRows * kBlock;
   constexpr int kDeep = EXACT ? 64 : 128, kSteps = EXACT ? 4 : 2, kOut = EXACT ? 4 : 2;  // k of a stage, matrix instructions along it; bytes of a result
-  static_assert(WM * WN == 4 && TN / WN <= kBlock, "four wavefronts, each within one block of columns");
-  static_assert(TM * TN * kOut <= 2 * kStage, "a tile's results fit the stages");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][kStage];
+  static_assert(TM % kEach32 == 0 && TN % kEach32 == 0 && TN / WN <= kBlock, "loads within one operand, a wavefront within one block of columns");
+  static_assert(TM * TN * kOut <= 2 * kStage && NT % (TN * kOut / 16) == 0, "a tile's results fit the stages, a pass is whole rows");
+  // both stages of activations, then both of weights: a read's place in them is an instruction's 16-bit offset
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStage];
+  __shared__ __attribute__((aligned(16))) float bias[TN];
   // XCDs take workgroups in turn; each gets neighbouring tiles, up to 16 along n before the next rows
   const uint32_t count = s.tiles_m * s.tiles_n, xcd = blockIdx.x % 8, each = count / 8, more = count % 8;
   uint32_t at = xcd * each + min(xcd, more) + blockIdx.x / 8;
   const uint32_t column = at / (16 * s.tiles_m), width = min(16u, s.tiles_n - 16 * column);
   at -= column * 16 * s.tiles_m;
-  const uint32_t m0 = at / width * TM, n0 = (16 * column + at % width) * TN;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t pitch = s.blocks * kBlock, n_rows = (s.n + kBlock - 1) / kBlock * kBlock;
+  const uint32_t m0 = scalar(at / width * TM), n0 = scalar((16 * column + at % width) * TN);
+  const int tid = threadIdx.x, wave = (int)scalar(tid >> 6), lane = tid & 63;
+  for (int i = tid; i < TN; i += NT) bias[i] = bias_at(out, min(n0 + i, s.n - 1));
+  const uint32_t pitch = s.blocks * kBlock;  // up to 2^20
+  const uint32_t n_rows = (s.n + kBlock - 1) / kBlock * kBlock;
 
-  // staging: chunk tid % 8 of rows tid / 8 + 32 i; behind the last row the last one again, which goes into results that nobody stores
+  // Staging: chunk tid % 8 of rows tid / 8 + 32 i.  Behind the last row of activations there is room, behind the last block of weights 0; either
+  // goes into results that nobody stores.
   const int chunk = tid & 7, row = tid >> 3;
   constexpr int kCodes = kDeep / 8;  // codes of a chunk
-  const uint8_t* const x_from = x + (size_t)m0 * pitch;
-  const uint8_t* const w_from = w + (size_t)n0 * pitch;
-  uint32_t off[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const uint32_t r = row + 32 * i;
-    const uint32_t there = r < TM ? min(r, s.rows - 1 - m0) : min(r - TM, n_rows - 1 - n0);
-    off[i] = there * pitch + kCodes * chunk;
-  }
+  const uint32_t stages = s.blocks * (kBlock / kDeep), last = stages - 1, off = row * pitch + kCodes * chunk;
+  const Window x_from(x + (size_t)m0 * pitch, TM * pitch), w_from(w + (size_t)n0 * pitch, min((uint32_t)TN, n_rows - n0) * pitch);
   u4v raw[EXACT ? 1 : kLoads];
-  uint2 raw8[EXACT ? kLoads : 1];
+  u2v raw8[EXACT ? kLoads : 1];
   uint32_t unit8[EXACT ? kLoads : 1];
-  const uint32_t stages = s.blocks * (kBlock / kDeep), last = stages - 1;
   auto load = [&](uint32_t stage, int i) __attribute__((always_inline)) {
-    const uint8_t* base = (32 * i < TM ? x_from : w_from) + (size_t)stage * kDeep;
+    const bool of_x = kEach32 * i < TM;
+    const uint32_t from = (of_x ? kEach32 * i : kEach32 * i - TM) * pitch + stage * kDeep;
     if constexpr (EXACT) {
-      raw8[i] = *reinterpret_cast<const uint2*>(base + off[i]);
-      const uint32_t b = stage / 2, r = row + 32 * i;
-      unit8[i] = 32 * i < TM ? x_scales[(size_t)b * s.scale_pitch + min(m0 + r, s.rows - 1)]
-                             : w_scales[(size_t)(min(n0 + 32 * i - TM, s.n - 1) / kBlock) * s.step_n + (size_t)b * s.step_k];
+      raw8[i] = of_x ? x_from.load8(off, from) : w_from.load8(off, from);
+      const uint32_t b = stage / 2;
+      if (of_x) unit8[i] = x_scales[(size_t)b * s.scale_pitch + m0 + kEach32 * i + row];
+      else unit8[i] = w_scales[(size_t)(min(n0 + kEach32 * i - TM, s.n - 1) / kBlock) * s.step_n + (size_t)b * s.step_k];
     } else {
-      raw[i] = *reinterpret_cast<const u4v*>(base + off[i]);
+      raw[i] = of_x ? x_from.load16(off, from) : w_from.load16(off, from);
     }
   };
-  const int place = row * kBlock + 16 * (chunk ^ (row & 7));
-  auto store = [&](uint8_t* buf, int i) __attribute__((always_inline)) {
-    if constexpr (EXACT) *reinterpret_cast<uint4*>(buf + place + 32 * i * kBlock) = f8_as_bf16(raw8[i], unit_of(unit8[i]));
-    else *reinterpret_cast<u4v*>(buf + place + 32 * i * kBlock) = raw[i];
+  // addresses in LDS: a lane's, which the compiler takes as they are, and what an instruction adds to them
+  typedef __attribute__((address_space(3))) uint8_t* Local;
+  Local const stages_at = (Local)lds;
+  auto as_it_is = [](Local p) __attribute__((always_inline)) {
+    asm("" : "+v"(p));
+    return p;
+  };
+  Local const to_x = as_it_is(stages_at + row * kBlock + 16 * (chunk ^ ((row >> 1) & 7))), to_w = as_it_is(to_x + 2 * TM * kBlock);
+  auto store = [&](int which, int i) __attribute__((always_inline)) {
+    Local const to = kEach32 * i < TM ? to_x + (which * TM + kEach32 * i) * kBlock : to_w + (which * TN + kEach32 * i - TM) * kBlock;
+    if constexpr (EXACT) {
+      const uint4 v = f8_as_bf16(make_uint2(raw8[i].x, raw8[i].y), unit_of(unit8[i]));
+      *(__attribute__((address_space(3))) u4v*)to = (u4v){v.x, v.y, v.z, v.w};
+    } else {
+      *(__attribute__((address_space(3))) u4v*)to = raw[i];
+    }
   };
 
   // reading: lane l has 32 codes, or eight bf16, of row l % 32 from that many times l / 32 on
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5;
   const uint32_t my_n = n0 + wn * (TN / WN), my_m = m0 + wm * (TM / WM);
   const uint8_t* const ws_from = w_scales + (size_t)(min(my_n, s.n - 1) / kBlock) * s.step_n;
-  uint32_t xs_at[FM];
-#pragma unroll
-  for (int i = 0; i < FM; ++i) xs_at[i] = min(my_m + 32 * i + r, s.rows - 1);
   int xs[2][FM], ws[2];
   auto load_scales = [&](uint32_t stage, int which) __attribute__((always_inline)) {
     if constexpr (!EXACT) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) xs[which][i] = x_scales[(size_t)stage * s.scale_pitch + xs_at[i]];
+      for (int i = 0; i < FM; ++i) xs[which][i] = (int)Window(x_scales + (size_t)stage * s.scale_pitch + m0, TM).load1(my_m - m0 + 32 * i + r, 0);
       ws[which] = ws_from[(size_t)stage * s.step_k];
     }
   };
   constexpr int kWords = EXACT ? 1 : 2;  // of 16 bytes
-  struct Frag {
-    u4v w[kWords];
-  };
-  auto frag = [&](const uint8_t* buf, int first_row, int step) __attribute__((always_inline)) {
-    Frag f;
+  typedef typename FragOf<EXACT>::type Frag;
+  Local x_at[kSteps * kWords], w_at[kSteps * kWords];
 #pragma unroll
-    for (int h = 0; h < kWords; ++h)
-      f.w[h] = *reinterpret_cast<const u4v*>(buf + (first_row + r) * kBlock + 16 * ((2 * kWords * step + kWords * half + h) ^ (r & 7)));
-    return f;
+  for (int k = 0; k < kSteps * kWords; ++k) {
+    const int c = 2 * kWords * (k / kWords) + kWords * half + k % kWords;
+    x_at[k] = as_it_is(stages_at + (wm * (TM / WM) + r) * kBlock + 16 * (c ^ ((r >> 1) & 7)));
+    w_at[k] = as_it_is(stages_at + (2 * TM + wn * (TN / WN) + r) * kBlock + 16 * (c ^ ((r >> 1) & 7)));
+  }
+  auto frag = [&](const Local* at, int first_row, int step) __attribute__((always_inline)) {
+    if constexpr (EXACT) {
+      return *(__attribute__((address_space(3))) Frag*)(at[step] + first_row * kBlock);
+    } else {
+      typedef __attribute__((address_space(3))) i4v* Half;
+      return __builtin_shufflevector(*(Half)(at[2 * step] + first_row * kBlock), *(Half)(at[2 * step + 1] + first_row * kBlock), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
   };
   f16v acc[FN][FM] = {};
-  Frag xf[2][FM], wf[2][FN];
-  auto read = [&](const uint8_t* buf, int step) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i) wf[step & 1][i] = frag(buf, TM + wn * (TN / WN) + 32 * i, step);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) xf[step & 1][i] = frag(buf, wm * (TM / WM) + 32 * i, step);
+  Frag xf[FM], wf[2][FN];
+  auto read_x = [&](int which, int step, int j) __attribute__((always_inline)) { xf[j] = frag(x_at, which * TM + 32 * j, step); };
+  auto read_w = [&](int which, int step, int i) __attribute__((always_inline)) {
+    wf[step & 1][i] = frag(w_at, which * TN + 32 * i, step);
   };
-  auto multiply = [&](int step, int which) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < FM; ++j)
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const Frag &a = wf[step & 1][i], &b = xf[step & 1][j];
-        if constexpr (EXACT) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a.w[0]), __builtin_bit_cast(bf8, b.w[0]), acc[i][j], 0, 0, 0);
-        } else {
-          const i8v p = {(int)a.w[0].x, (int)a.w[0].y, (int)a.w[0].z, (int)a.w[0].w, (int)a.w[1].x, (int)a.w[1].y, (int)a.w[1].z, (int)a.w[1].w};
-          const i8v q = {(int)b.w[0].x, (int)b.w[0].y, (int)b.w[0].z, (int)b.w[0].w, (int)b.w[1].x, (int)b.w[1].y, (int)b.w[1].z, (int)b.w[1].w};
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(p, q, acc[i][j], 0, 0, 0, ws[which], 0, xs[which][j]);
-        }
-      }
+  auto multiply = [&](int step, int which, int i, int j) __attribute__((always_inline)) {
+    if constexpr (EXACT) {
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0);
+    } else {
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0, ws[which], 0, xs[which][j]);
+    }
   };
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load(0, i);
   load_scales(0, 0);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) store(lds[0], i);
+  for (int i = 0; i < kLoads; ++i) store(0, i);
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load(min(1u, last), i);
   __syncthreads();
-  read(lds[0], 0);
-  // A stage: the fragments of a step are read while the step before multiplies, those of the next stage's first step, behind the barrier, beside
-  // the last products of this one.
+#pragma unroll
+  for (int i = 0; i < FN; ++i) read_w(0, 0, i);
+#pragma unroll
+  for (int j = 0; j < FM; ++j) read_x(0, 0, j);
+  // A stage is kSteps times FM x FN products.  Beside a step's go the next step's fragments, those of the activations each into the registers of
+  // the one that has just been multiplied for the last time; the last step's are the next stage's, behind a barrier before it.  Beside the
+  // other steps the next stage goes from registers to LDS and the one after it is asked for.  The order is given, or the compiler
+  // brings loads forward until registers run out.
+  constexpr int kSlots = FM * FN, kMoveSlots = (kSteps - 1) * kSlots;
   auto one_stage = [&](uint32_t st, int which) __attribute__((always_inline)) {
-    uint8_t *buf = lds[which], *next = lds[which ^ 1];
     load_scales(min(st + 1, last), which ^ 1);
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      if (step + 1 < kSteps) {
-        read(buf, step + 1);
+      const bool turn = step + 1 == kSteps;
+      const int from = turn ? which ^ 1 : which, next = turn ? 0 : step + 1;
+      if (turn) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          if (i * (kSteps - 1) / kLoads == step) {
-            store(next, i);
-            load(min(st + 2, last), i);
-          }
-      } else {
-        __syncthreads();
-        read(next, 0);
+      for (int t = 0; t < kSlots; ++t) {
+        const int j = t / FN, i = t % FN;
+        multiply(step, which, i, j);
+#pragma unroll
+        for (int f = 0; f < FN; ++f)
+          if (f * kSlots / FN == t) read_w(from, next, f);
+        if (i == FN - 1) read_x(from, next, j);
+        if (!turn) {
+#pragma unroll
+          for (int l = 0; l < kLoads; ++l)
+            if (l * kMoveSlots / kLoads == step * kSlots + t) {
+              store(which ^ 1, l);
+              load(min(st + 2, last), l);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      multiply(step, which);
     }
   };
   uint32_t st = 0;
@@ -404,22 +444,18 @@ __global__ __launch_bounds__(256, TM * TN >= 256 * 256 ? 1 : 2) void f8_product_
   // each row, and from there to memory.
   __syncthreads();  // the last stage asked for fragments of a stage that is not there
   constexpr int kChunks = TN * kOut / 16, kEach = 16 / kOut;  // chunks of a row, results of a chunk
-  uint8_t* const tile = lds[0];
+  uint8_t* const tile = lds;
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int c = wn * (TN / WN) + 32 * i + 8 * q + 4 * half;
-      float bias[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bias[e] = bias_at(out, min(n0 + c + e, s.n - 1));
+      const float4 b = *reinterpret_cast<const float4*>(bias + c);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int m = wm * (TM / WM) + 32 * j + r;
         uint8_t* to = tile + m * (TN * kOut) + 16 * ((c / kEach) ^ (m & (kChunks - 1))) + (c % kEach) * kOut;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] + bias[e];
+        const float v[4] = {acc[i][j][4 * q] + b.x, acc[i][j][4 * q + 1] + b.y, acc[i][j][4 * q + 2] + b.z, acc[i][j][4 * q + 3] + b.w};
         if constexpr (EXACT) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
         else if (out.dtype == CSWAP_DT_BF16) *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<BF16>(v[0], v[1]), to_pair<BF16>(v[2], v[3]));
         else *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<F16>(v[0], v[1]), to_pair<F16>(v[2], v[3]));
@@ -427,8 +463,9 @@ __global__ __launch_bounds__(256, TM * TN >= 256 * 256 ? 1 : 2) void f8_product_
     }
   __syncthreads();
   const uint32_t rows_here = min((uint32_t)TM, s.rows - m0);
-  for (uint32_t i = tid; i < (uint32_t)TM * kChunks; i += 256) {
-    const uint32_t m = i / kChunks, c = i % kChunks, n = n0 + c * kEach;
+#pragma unroll 8
+  for (int pass = 0; pass < TM * kChunks / NT; ++pass) {
+    const uint32_t m = (pass * NT + tid) / kChunks, c = tid % kChunks, n = n0 + c * kEach;
     if (m >= rows_here || n >= s.n) continue;
     const uint4 v = *reinterpret_cast<const uint4*>(tile + m * (TN * kOut) + 16 * (c ^ (m & (kChunks - 1))));
     uint8_t* to = static_cast<uint8_t*>(out.y) + ((size_t)(m0 + m) * s.y_stride + n) * kOut;
@@ -460,7 +497,7 @@ using namespace cswap::q8;
 extern "C" size_t cswap_f8_linear_workspace_bytes(size_t rows, size_t k)
 {
   if (rows <= kFewRows || k == 0 || !f8_shape(rows, 1, k)) return 0;
-  return blocks_of(k) * (rows * kBlock + rows16(rows));
+  return blocks_of(k) * padded(rows) * (kBlock + 1);
 }
 
 extern "C" int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t k, ptrdiff_t stride, uint8_t* d_codes, uint8_t* d_turned,
@@ -474,7 +511,7 @@ extern "C" int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t
     return CSWAP_E_ARG;
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    hipLaunchKernelGGL(f8_weight_kernel<T>, dim3((unsigned)(blocks_of(n) * blocks_of(k))), dim3(256), 0, static_cast<hipStream_t>(stream),
+    hipLaunchKernelGGL(f8_weight_kernel<T>, dim3((unsigned)(blocks_of(n) * blocks_of(k))), dim3(kWeightThreads), 0, static_cast<hipStream_t>(stream),
                        static_cast<const typename T::value*>(d_w), (size_t)stride, (uint32_t)n, (uint32_t)k, reinterpret_cast<uint2*>(d_codes),
                        reinterpret_cast<uint4*>(d_turned), d_scales);
     return check_launch();
@@ -499,7 +536,7 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
   if (ws_bytes < need) return CSWAP_E_NOMEM;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint32_t kb = (uint32_t)blocks_of(k), nb = (uint32_t)blocks_of(n);
-  F8Shape s = {(uint32_t)rows, (uint32_t)n, kb, (uint32_t)rows16(rows), turned ? 1u : kb, turned ? nb : 1u, 0, 0, (size_t)y_stride};
+  F8Shape s = {(uint32_t)rows, (uint32_t)n, kb, (uint32_t)padded(rows), turned ? 1u : kb, turned ? nb : 1u, 0, 0, (size_t)y_stride};
   const F8Out out = {d_y, d_bias, out_dtype, bias_dtype};
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
@@ -510,17 +547,21 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
       hipLaunchKernelGGL(f, dim3((unsigned)((n + 15) / 16)), dim3(64 * kFewWaves), 0, st, x, (size_t)x_stride, (uint32_t)k, s, d_codes, d_scales, out);
       return check_launch();
     }
-    uint8_t *codes = static_cast<uint8_t*>(d_ws), *scales = codes + rows * kb * kBlock;
-    hipLaunchKernelGGL(f8_rows_kernel<T>, dim3((unsigned)(rows16(rows) / 16 * kb)), dim3(256), 0, st, x, (size_t)x_stride, (uint32_t)rows, (uint32_t)k, kb,
+    uint8_t *codes = static_cast<uint8_t*>(d_ws), *scales = codes + padded(rows) * kb * kBlock;
+    hipLaunchKernelGGL(f8_rows_kernel<T>, dim3((unsigned)((rows + 15) / 16 * kb)), dim3(256), 0, st, x, (size_t)x_stride, (uint32_t)rows, (uint32_t)k, kb,
                        reinterpret_cast<uint2*>(codes), scales, s.scale_pitch);
     if (int e = check_launch()) return e;
-    auto launch = [&](auto f, uint32_t tm, uint32_t tn) {
+    auto launch = [&](auto f, uint32_t tm, uint32_t tn, uint32_t threads) {
       s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
-      hipLaunchKernelGGL(f, dim3(s.tiles_m * s.tiles_n), dim3(256), 0, st, codes, scales, d_codes, d_scales, s, out);
+      hipLaunchKernelGGL(f, dim3(s.tiles_m * s.tiles_n), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
       return check_launch();
     };
-    if (out_dtype == CSWAP_DT_F32) return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128);
-    const size_t large = ((rows + 255) / 256) * ((n + 255) / 256);
-    return large >= 512 ? launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256) : launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128);
+    if (out_dtype == CSWAP_DT_F32) return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128, 256);
+    // By what rounds of all compute units take, us, with the stages' number: tiles of 256 x 256, one to a compute unit, 11.5 and 1.43 a stage, of 128 x
+    // 128, two to one, 2.3 and 1.02.  The former : the latter 16384 x 1024 x 4096 58 : 69, 8192^3 400 : 505, 4096^3 58 : 70, 16384 x 4096 x
+    // 1024 93 : 84, 16384 x 768 x 768 20.4 : 17.0, 2048^3 27 : 14.
+    auto rounds = [&](size_t tile, size_t at_once) { return (((rows + tile - 1) / tile) * ((n + tile - 1) / tile) + at_once - 1) / at_once; };
+    if (rounds(256, 256) * (11.5 + 1.43 * kb) < rounds(128, 512) * (2.3 + 1.02 * kb)) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
+    return launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128, 256);
   });
 }

@@ -54,7 +54,7 @@ def test_argument_errors_do_not_launch():
 def test_workspaces():
     f = _lib.lib().cswap_f8_linear_workspace_bytes
     assert f(0, 100) == 0 and f(1, 100) == 0 and f(100, 0) == 0
-    assert f(1000, 129) == 2 * (1000 * 128 + 1008)
+    assert f(1000, 129) == 2 * 1024 * 129                                         # whole tiles of 256 rows
     assert f(1 << 31, 128) == 0 and f(100, (1 << 20) + 1) == 0
 
 
