@@ -7,6 +7,10 @@
 // this chip take a power of two for each lane's 32 values along k, so a block's two scales go into the instruction and nothing is
 // multiplied behind it: that is why the scales are powers of two (it costs up to one bit of range against max / 448, none of precision).
 //
+// Traced: 16384 x 1024 x 4096 58 us (2.37 PFLOP/s; torch's fp8 product with one scale for all 61), 16384 x 4096 x 1024 82 (1.67; torch 70), 8192^3
+// 400 at the clock of a first run (2.75), 500 at that of many; fp32 results 16384 x 768 x 768 30 (torch's bf16 product 26); a token through 4096 x 1024
+// 4.1, through 8192 x 8192 19.5 (3.4 TB/s); 32 tokens 4.2 and 25.6 besides 2.6 and 4.0 to turn them into codes.
+//
 // Scale of a block: the least 2^s, s >= -126, with max|x| <= 448 * 2^s, held as the byte s + 127.  A block that holds a NaN or an infinity has
 // codes of NaN (0x7f): every result that it goes into is NaN.
 #include <hip/hip_runtime.h>
@@ -210,12 +214,14 @@ __device__ inline uint4 f8_as_bf16(uint2 q, float unit)
 }
 
 // Few rows: bound by the weights' bytes, which every workgroup reads once and no other reads.  A workgroup makes 16 columns; its eight wavefronts take
-// blocks of k in turn and add up through LDS.  A lane has 32 codes of one of 16 rows: that is one 16 x 16 x 128 matrix instruction a block, or
-// four of 16 x 16 x 32 in bf16 (which of a lane's codes meet in which does not matter as long as both operands have them alike).
-// The activations are turned into codes in registers, by every workgroup for itself: four lanes have a row's block.
+// blocks of k in turn, two of them under way, and add up through LDS.  A lane has 32 codes of one of 16 rows: that is one 16 x 16 x 128 matrix
+// instruction a block, or four of 16 x 16 x 32 in bf16 (which of a lane's codes meet in which does not matter as long as both operands have
+// them alike).  Up to 16 rows are turned into codes in registers, by every workgroup for itself: four lanes have a row's block.  More rows (PACKED,
+// MF times 16) are codes already.
 constexpr int kFewWaves = 8;
-template <typename T, int MF, bool EXACT>
-__global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typename T::value* __restrict__ x, size_t x_stride, uint32_t k, F8Shape s,
+template <typename T, int MF, bool EXACT, bool PACKED>
+__global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typename T::value* __restrict__ x, size_t x_stride, uint32_t k,
+                                                                     const uint8_t* __restrict__ x_codes, const uint8_t* __restrict__ x_scales, F8Shape s,
                                                                      const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales, F8Out out)
 {
   __shared__ __attribute__((aligned(16))) float part[kFewWaves][MF * 256];
@@ -225,41 +231,69 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typen
 #pragma unroll
   for (int f = 0; f < MF; ++f) acc[f] = (f4v){0, 0, 0, 0};
   const uint8_t* from = w + (size_t)(col0 + r) * pitch + quarter * 32;  // weights are filled up to whole blocks: the row is there
-  for (uint32_t b = wave; b < s.blocks; b += kFewWaves) {
-    const uint4* at = reinterpret_cast<const uint4*>(from + (size_t)b * kBlock);
-    const uint4 w0 = at[0], w1 = at[1];
-    const int w_scale = w_scales[(size_t)(col0 / kBlock) * s.step_n + (size_t)b * s.step_k];
-    const uint32_t col = b * kBlock + quarter * 32;
-    float v[MF][4][8];
+  struct Block {
+    u4v w[2], x[PACKED ? MF : 1][2];
+    u4_any raw[PACKED ? 1 : 4][T::bytes / 2];
+    int w_scale, x_scale[MF];
+  };
+  auto load = [&](uint32_t b, Block& to) __attribute__((always_inline)) {
+    const u4v* at = reinterpret_cast<const u4v*>(from + (size_t)b * kBlock);
+    to.w[0] = at[0], to.w[1] = at[1];
+    to.w_scale = w_scales[(size_t)(col0 / kBlock) * s.step_n + (size_t)b * s.step_k];
+    if constexpr (PACKED) {
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
-      const uint32_t row = f * 16 + r;
+      for (int f = 0; f < MF; ++f) {  // there is room for whole tiles of rows
+        const u4v* row = reinterpret_cast<const u4v*>(x_codes + (size_t)(16 * f + r) * pitch + b * kBlock + quarter * 32);
+        to.x[f][0] = row[0], to.x[f][1] = row[1];
+        to.x_scale[f] = x_scales[(size_t)b * s.scale_pitch + 16 * f + r];
+      }
+    } else {
+      const uint32_t col = b * kBlock + quarter * 32;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        load_chunk<T>(x + (size_t)min(row, s.rows - 1) * x_stride + col + 8 * c, row < s.rows ? valid_at(col + 8 * c, k) : 0, v[f][c]);
+        load_raw<T>(x + (size_t)min(r, s.rows - 1) * x_stride + col + 8 * c, r < s.rows ? valid_at(col + 8 * c, k) : 0, to.raw[c]);
     }
+  };
+  auto multiply = [&](Block& of) __attribute__((always_inline)) {
+    if constexpr (!PACKED) {
+      float v[4][8];
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
-      float m = larger(larger(largest(v[f][0]), largest(v[f][1])), larger(largest(v[f][2]), largest(v[f][3])));
+      for (int c = 0; c < 4; ++c) widen<T>(of.raw[c], v[c]);
+      float m = larger(larger(largest(v[0]), largest(v[1])), larger(largest(v[2]), largest(v[3])));
       m = larger(m, __shfl_xor(m, 16));
       m = larger(m, __shfl_xor(m, 32));
       const uint32_t scale = f8_scale(__float_as_uint(m) & 0x7fffffffu);
-      uint2 q[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) q[c] = f8_codes(v[f][c], scale);
-      const uint2 p[4] = {{w0.x, w0.y}, {w0.z, w0.w}, {w1.x, w1.y}, {w1.z, w1.w}};
+      for (int c = 0; c < 4; ++c) {
+        const uint2 q = f8_codes(v[c], scale);
+        of.x[0][c / 2][2 * (c & 1)] = q.x, of.x[0][c / 2][2 * (c & 1) + 1] = q.y;
+      }
+      of.x_scale[0] = stored_scale(scale);
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
       if constexpr (EXACT) {
-        const float unit = unit_of(stored_scale(scale)), w_unit = unit_of(w_scale);
+        const float unit = unit_of(of.x_scale[f]), w_unit = unit_of(of.w_scale);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, f8_as_bf16(p[c], w_unit)), __builtin_bit_cast(bf8, f8_as_bf16(q[c], unit)),
-                                                           acc[f], 0, 0, 0);
+        for (int c = 0; c < 4; ++c) {
+          const u4v a = of.w[c / 2], b = of.x[f][c / 2];
+          const uint2 p = c & 1 ? make_uint2(a.z, a.w) : make_uint2(a.x, a.y), q = c & 1 ? make_uint2(b.z, b.w) : make_uint2(b.x, b.y);
+          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, f8_as_bf16(p, w_unit)), __builtin_bit_cast(bf8, f8_as_bf16(q, unit)), acc[f], 0, 0, 0);
+        }
       } else {
-        const i8v wf = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
-        const i8v xf = {(int)q[0].x, (int)q[0].y, (int)q[1].x, (int)q[1].y, (int)q[2].x, (int)q[2].y, (int)q[3].x, (int)q[3].y};
-        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[f], 0, 0, 0, w_scale, 0, (int)stored_scale(scale));
+        const i8v wf = __builtin_bit_cast(i8v, __builtin_shufflevector(of.w[0], of.w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        const i8v xf = __builtin_bit_cast(i8v, __builtin_shufflevector(of.x[f][0], of.x[f][1], 0, 1, 2, 3, 4, 5, 6, 7));
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[f], 0, 0, 0, of.w_scale, 0, of.x_scale[f]);
       }
     }
+  };
+  for (uint32_t b = wave; b < s.blocks; b += 2 * kFewWaves) {
+    Block one, two;
+    load(b, one);
+    const bool more = b + kFewWaves < s.blocks;
+    if (more) load(b + kFewWaves, two);
+    multiply(one);
+    if (more) multiply(two);
   }
   // a lane has columns 4 * quarter and on of row r
 #pragma unroll
@@ -484,7 +518,13 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 }
 
 // ---------------------------------------------------------------- launches
-constexpr size_t kFewRows = 32;
+constexpr size_t kFewRows = 16;  // up to which the product's kernel turns activations into codes itself
+constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)1 << 24;
+
+// Few rows read the weights once, a workgroup to 16 columns; tiles of 128 x 128 have fewer workgroups but each value of the activations once for 128
+// columns.  us with codes ready, the former : the latter, 32 rows through 4096 x 1024 4.2 : 7.6, 1024 x 4096 8.3 : 16.8, 8192 x 8192 25.6 :
+// 30.0; 64 rows 6.0 : 7.8, 12.8 : 17.0, 42 : 31.
+static bool few_rows(size_t rows, size_t weights) { return rows <= kFewPacked || (rows <= kFewPackedSmall && weights <= kSmallWeights); }
 
 static bool f8_shape(size_t rows, size_t n, size_t k) { return n <= kMaxFeatures && k <= kMaxFeatures && rows < ((size_t)1 << 31); }
 
@@ -541,16 +581,24 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     const typename T::value* x = static_cast<const typename T::value*>(d_x);
+    const dim3 columns((unsigned)((n + 15) / 16)), threads(64 * kFewWaves);
     if (rows <= kFewRows) {
-      auto f = out_dtype == CSWAP_DT_F32 ? (rows <= 16 ? f8_few_rows_kernel<T, 1, true> : f8_few_rows_kernel<T, 2, true>)
-                                         : (rows <= 16 ? f8_few_rows_kernel<T, 1, false> : f8_few_rows_kernel<T, 2, false>);
-      hipLaunchKernelGGL(f, dim3((unsigned)((n + 15) / 16)), dim3(64 * kFewWaves), 0, st, x, (size_t)x_stride, (uint32_t)k, s, d_codes, d_scales, out);
+      auto f = out_dtype == CSWAP_DT_F32 ? f8_few_rows_kernel<T, 1, true, false> : f8_few_rows_kernel<T, 1, false, false>;
+      hipLaunchKernelGGL(f, columns, threads, 0, st, x, (size_t)x_stride, (uint32_t)k, nullptr, nullptr, s, d_codes, d_scales, out);
       return check_launch();
     }
     uint8_t *codes = static_cast<uint8_t*>(d_ws), *scales = codes + padded(rows) * kb * kBlock;
     hipLaunchKernelGGL(f8_rows_kernel<T>, dim3((unsigned)((rows + 15) / 16 * kb)), dim3(256), 0, st, x, (size_t)x_stride, (uint32_t)rows, (uint32_t)k, kb,
                        reinterpret_cast<uint2*>(codes), scales, s.scale_pitch);
     if (int e = check_launch()) return e;
+    if (few_rows(rows, n * k)) {
+      auto few = [&](auto f) {
+        hipLaunchKernelGGL(f, columns, threads, 0, st, nullptr, 0, (uint32_t)k, codes, scales, s, d_codes, d_scales, out);
+        return check_launch();
+      };
+      if (out_dtype == CSWAP_DT_F32) return rows <= 32 ? few(f8_few_rows_kernel<F32, 2, true, true>) : few(f8_few_rows_kernel<F32, 4, true, true>);
+      return rows <= 32 ? few(f8_few_rows_kernel<F32, 2, false, true>) : few(f8_few_rows_kernel<F32, 4, false, true>);
+    }
     auto launch = [&](auto f, uint32_t tm, uint32_t tn, uint32_t threads) {
       s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
       hipLaunchKernelGGL(f, dim3(s.tiles_m * s.tiles_n), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);

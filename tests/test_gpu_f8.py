@@ -92,7 +92,7 @@ def test_values_that_are_not_finite():
 
 
 # ---------------------------------------------------------------- products
-SIZES = [(1, 16, 16), (1, 1, 1), (1, 4096, 1024), (2, 17, 129), (15, 100, 300), (16, 128, 128), (17, 1000, 193), (32, 33, 4100), (33, 130, 40), (64, 256, 256), (100, 300, 520),
+SIZES = [(1, 16, 16), (1, 1, 1), (1, 4096, 1024), (2, 17, 129), (15, 100, 300), (16, 128, 128), (17, 1000, 193), (32, 33, 4100), (33, 130, 40), (50, 4100, 4200), (64, 256, 256), (100, 300, 520),
          (129, 127, 640), (257, 1000, 193), (1000, 5, 1030), (700, 520, 130), (1576, 1000, 193), (2050, 129, 384), (300, 4100, 256),
          (4100, 8300, 200), (16400, 4000, 136)]                       # the last two: the largest tiles, everything cut off somewhere
 
