@@ -39,53 +39,52 @@ def _dense_order(t: torch.Tensor) -> bool:
 
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
-    __slots__ = ("params", "states", "ptrs", "kept", "contiguous", "table", "device", "strides", "moments", "how")
+    __slots__ = ("params", "states", "rows", "table", "device", "how")
 
     def __init__(self, optimizer, group, params):
-        bits = group["bits"]
-        self.how = bits, group["capturable"]
+        self.how = bits, _ = group["bits"], group["capturable"]
         self.params, self.states = params, [optimizer.state[p] for p in params]
-        self.ptrs = [p.data_ptr() for p in params]
-        self.kept = [(s["exp_avg"], s["exp_avg_sq"], s.get("master")) for s in self.states]
-        self.contiguous = [p.is_contiguous() for p in params]
-        self.strides = [p.stride() for p in params]
         self.device = params[0].device
         # rows of cswap_adamw_tensor: seven words, the type in the last
-        self.table, self.moments = array("Q"), []
-        for p, s, kept in zip(params, self.states, self.kept):
+        self.rows, self.table = [], array("Q")
+        for p, s in zip(params, self.states):
             if p.dtype not in q8._DTYPE:
                 raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
-            _check_state(p, s, kept, bits)
-            m, v, master = kept
-            self.table.extend((p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), p.numel(),
-                               q8._DTYPE[p.dtype]))
-            self.moments.append((m.data_ptr(), v.data_ptr(), p.numel()))
+            m, v, master = s["exp_avg"], s["exp_avg_sq"], s.get("master")
+            _check_state(p, s, (m, v, master), bits)
+            at, n = p.data_ptr(), p.numel()
+            self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m.data_ptr(), v.data_ptr()))
+            self.table.extend((at, 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), n, q8._DTYPE[p.dtype]))
 
     def holds(self, params, group) -> bool:
         """Whether the plan is still that of these parameters and of their state."""
-        if len(params) != len(self.params) or self.how != (group["bits"], group["capturable"]):
+        if len(params) != len(self.rows) or self.how != (group["bits"], group["capturable"]):
             return False
-        for p, mine, ptr, strides, (_, _, n), s, (m, v, master) in zip(params, self.params, self.ptrs, self.strides, self.moments, self.states, self.kept):
-            if p is not mine or p.data_ptr() != ptr or p.stride() != strides or p.numel() != n or p.dtype not in q8._DTYPE:
+        for p, (mine, at, n, strides, _, s, m, v, master, _, _) in zip(params, self.rows):
+            if p is not mine or p.data_ptr() != at or p.numel() != n:
                 return False
-            if s.get("exp_avg") is not m or s.get("exp_avg_sq") is not v or s.get("master") is not master:
+            if (not p.is_contiguous()) if strides is None else p.stride() != strides:
+                return False
+            get = s.get
+            if get("exp_avg") is not m or get("exp_avg_sq") is not v or get("master") is not master:
                 return False
         return True
 
     def set_gradients(self):
         """Fills in the gradients' addresses; gives back what has to live until the launch."""
-        copies, addresses, device = [], array("Q"), self.device
-        for p, contiguous, strides, (_, _, n) in zip(self.params, self.contiguous, self.strides, self.moments):
+        copies, addresses = [], []
+        strided = torch.strided
+        for p, _, n, strides, dtype, *_ in self.rows:
             g = p.grad
-            if g.layout is not torch.strided:
+            if g.layout is not strided:
                 raise RuntimeError("AdamW8: no sparse gradients")
-            if g.dtype is not p.dtype or g.numel() != n or g.device != device:
-                raise TypeError(f"AdamW8: a gradient {tuple(g.shape)} {g.dtype} on {g.device} of a parameter {tuple(p.shape)} {p.dtype} on {device}")
-            if not (contiguous and g.is_contiguous()) and g.stride() != strides or g.is_neg():
+            if g.dtype is not dtype or g.numel() != n:
+                raise TypeError(f"AdamW8: a gradient {tuple(g.shape)} {g.dtype} of a parameter {tuple(p.shape)} {dtype}")
+            if ((not g.is_contiguous()) if strides is None else g.stride() != strides) or g.is_neg():
                 g = torch.empty_like(p).copy_(g)
                 copies.append(g)
             addresses.append(g.data_ptr())
-        self.table[1::7] = addresses
+        self.table[1::7] = array("Q", addresses)
         return copies
 
 
@@ -261,7 +260,7 @@ class AdamW8(torch.optim.Optimizer):
 
 
 def _launch(plan, group, options, lr):
-    table, count, first, stream = plan.table.buffer_info()[0], len(plan.params), plan.states[0], q8._stream_of(plan.device)
+    table, count, first, stream = plan.table.buffer_info()[0], len(plan.rows), plan.states[0], q8._stream_of(plan.device)
     if group["capturable"]:
         if lr is not None and lr.device != plan.device:
             raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
@@ -311,46 +310,54 @@ def _row(m, v, m8, v8):
 
 
 def _convert(rows, name, device):
-    """``rows``: cswap_adamw_moments as five words each."""
-    with torch.cuda.device(device):
-        check(getattr(lib(), name)(rows.buffer_info()[0], len(rows) // 5, q8._stream_of(device)), name)
+    """``rows``: cswap_adamw_moments as five words each; ``device``: or its number."""
+    device = torch.device("cuda", device) if isinstance(device, int) else device
+    stream = q8._stream_of(device)
+    if stream is None:
+        with torch.cuda.device(device):
+            return _convert(rows, name, device)
+    check(getattr(lib(), name)(rows.buffer_info()[0], len(rows) // 5, stream), name)
 
 
-def _unpack_rows(optimizer):
-    """Of the parameters that have made a step, in order: the parameter, its group, its state and, where it is held in 8 bits, the two moments'
-    addresses, checked."""
+def _held(optimizer):
+    """Of the parameters that have made a step, in order: the parameter, its group, its state, its number of values and, where they are held in 8 bits, the two
+    moments' addresses, checked."""
     for number, group in enumerate(optimizer.param_groups):
         params = [p for p in group["params"] if "exp_avg" in optimizer.state.get(p, ())]
         plans = optimizer._plans.get(number, ())
         if len(plans) == 1 and plans[0].holds(params, group):
-            yield from zip(params, [group] * len(params), plans[0].states, plans[0].moments)
+            for p, _, n, _, _, s, _, _, _, m8, v8 in plans[0].rows:
+                yield p, group, s, n, m8, v8
             continue
         for p in params:
             s = optimizer.state[p]
             _check_state(p, s, (s["exp_avg"], s["exp_avg_sq"], None), group["bits"])
-            yield p, group, s, (s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr(), p.numel())
+            yield p, group, s, p.numel(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr()
 
 
 @torch.no_grad()
 def unpack_moments(optimizer: AdamW8, out=None):
     """``[(exp_avg, exp_avg_sq)]`` in fp32 of the parameters that have made a step, in their order and layout; ``out``: such a list to
     write to."""
-    params = list(_unpack_rows(optimizer))
+    held = list(_held(optimizer))
     if out is None:
-        out = [tuple(torch.empty_like(p, dtype=torch.float32) for _ in range(2)) for p, *_ in params]
-    elif len(out) != len(params):
-        raise ValueError(f"unpack_moments: {len(out)} pairs for {len(params)} parameters")
-    rows = {}
-    for (p, group, s, (m8, v8, n)), (m, v) in zip(params, out):
+        out = [tuple(torch.empty_like(p, dtype=torch.float32) for _ in range(2)) for p, *_ in held]
+    elif len(out) != len(held):
+        raise ValueError(f"unpack_moments: {len(out)} pairs for {len(held)} parameters")
+    rows, f32 = {}, torch.float32
+    for (p, group, s, n, m8, v8), (m, v) in zip(held, out):
+        place, contiguous = p.get_device(), p.is_contiguous()
         for t in (m, v):
-            if t.dtype is not torch.float32 or t.device != p.device or t.numel() != n or not (
-                    t.is_contiguous() and p.is_contiguous() or t.stride() == p.stride()):
+            if t.dtype is not f32 or t.numel() != n or t.get_device() != place or not (contiguous and t.is_contiguous() or t.stride() == p.stride()):
                 raise ValueError(f"unpack_moments: {tuple(t.shape)} {t.dtype} on {t.device} for a parameter {tuple(p.shape)} on {p.device}")
         if group["bits"] == 8:
-            rows.setdefault(p.device, array("Q")).extend((m.data_ptr(), v.data_ptr(), m8, v8, n))
+            some = rows.get(place)
+            if some is None:
+                some = rows[place] = []
+            some += (m.data_ptr(), v.data_ptr(), m8, v8, n)
         else:
             m.copy_(s["exp_avg"].view_as(m))
             v.copy_(s["exp_avg_sq"].view_as(v))
-    for device, some in rows.items():
-        _convert(some, "cswap_adamw_unpack", device)
+    for place, some in rows.items():
+        _convert(array("Q", some), "cswap_adamw_unpack", place)
     return out
