@@ -9,8 +9,9 @@ import torch
 
 from cswap_amd import api, swap
 from cswap_amd._lib import Costs
+from cswap_amd.adamw8 import AdamW8
 from cswap_amd.hooks import hold_saved_tensors, swap_saved_tensors
-from cswap_amd.layers8 import checkpoint_layers
+from cswap_amd.layers8 import Linear8, LinearF8, checkpoint_layers
 from cswap_amd.planner import PolicyMaker, run_planned_iteration
 from cswap_amd.workloads import dummy_layer_compute, vgg16_modules
 
@@ -362,4 +363,32 @@ def bench_transformer_step(dev, layers: int = 4, batch: int = 32, seq: int = 512
     checkpoint_layers(net)
     held("layers_8bit", lambda: None)
     held("layers_and_held_8bit", lambda: hold_saved_tensors(min_bytes))
+    # the same layers with their products in 8-bit floating point
+    for m in net.modules():
+        if type(m) is Linear8:
+            m.__class__ = LinearF8
+    held("layers_f8", lambda: None)
+    res["optimizer"] = _optimizer_steps(params)
+    return res
+
+
+def _optimizer_steps(params, reps: int = 20) -> dict:
+    """Time of an AdamW step over a model's tensors, and what its moments hold."""
+    for p in params:
+        p.grad = torch.randn_like(p)
+    res = {"values": sum(p.numel() for p in params), "tensors": len(params)}
+    for label, make in (("torch_fused", lambda: torch.optim.AdamW(params, fused=True)), ("fp32_moments", lambda: AdamW8(params, bits=32)),
+                        ("8bit_moments", lambda: AdamW8(params))):
+        before = torch.cuda.memory_allocated()
+        optimizer = make()
+        for _ in range(3):
+            optimizer.step()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(reps):
+            optimizer.step()
+        torch.cuda.synchronize()
+        res[label] = {"step_ms": round((time.perf_counter() - t0) * 1e3 / reps, 3),
+                      "state_MB": round((torch.cuda.memory_allocated() - before) / 1e6, 1)}
+        del optimizer
     return res

@@ -20,8 +20,11 @@
 // A code hangs on its value's last bits, so m' and v' are rounded after each product and each sum, to the same bits whoever computes them
 // (the build contracts nothing); what only the parameter sees goes through v_sqrt_f32 and v_rcp_f32, one unit off in the last place each.
 //
-// Memory bounds it: bf16 with moments in 8 bits 10.1 bytes a value, fp32 with fp32 moments 28.  The tensors of a launch are in its
-// arguments (so that it needs no table in device memory, which a capture or a second call could find changed), a workgroup finds its tensor by halving.
+// Memory bounds it: bf16 with moments in 8 bits 10.1 bytes a value, fp32 with fp32 moments 28.  Traced: 101.8 M bf16 values in 130 tensors, moments in
+// 8 bits, two launches of 102 us and one of 7 (4.9 TB/s; a copy reaches 5.1), 51.4 M fp32 values with fp32 moments 260 and 10 (5.3 TB/s), the moments as fp32 values 112
+// a launch (4.5 TB/s).  The tensors of a launch are in its
+// arguments (so that it needs no table in device memory, which a
+// capture or a second call could find changed), a workgroup finds its tensor by halving.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include "../../include/cswap_hip.h"
