@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -36,23 +37,25 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
+def _compile(source: str, verbose: bool) -> str:
+    o = os.path.join(HERE, "build", source + ".o")
+    cmd = [hipcc(), *HIPCC_FLAGS, "-x", "hip", "-c", os.path.join(CSRC, source), "-o", o]
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    err = "\n".join(l for l in r.stderr.splitlines() if "packed-fp32-ops" not in l)
+    if r.returncode != 0:
+        raise RuntimeError(f"hipcc failed on {source}:\n{err}")
+    if err.strip() and verbose:
+        print(err)
+    return o
+
+
 def build(verbose: bool = False) -> str:
-    objs = []
-    objdir = os.path.join(HERE, "build")
-    os.makedirs(objdir, exist_ok=True)
+    os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    for s in srcs:
-        o = os.path.join(objdir, s + ".o")
-        cmd = [hipcc(), *HIPCC_FLAGS, "-x", "hip", "-c", os.path.join(CSRC, s), "-o", o]
-        if verbose:
-            print(" ".join(cmd))
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        err = "\n".join(l for l in r.stderr.splitlines() if "packed-fp32-ops" not in l)
-        if r.returncode != 0:
-            raise RuntimeError(f"hipcc failed on {s}:\n{err}")
-        if err.strip() and verbose:
-            print(err)
-        objs.append(o)
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:      # a compiler each, a few hundred MB
+        objs = list(pool.map(lambda s: _compile(s, verbose), srcs))
     cmd = [hipcc(), "-shared", "-fPIC", "--offload-arch=gfx950", "-o", LIB, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
