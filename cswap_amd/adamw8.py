@@ -37,12 +37,16 @@ def _dense_order(t: torch.Tensor) -> bool:
     return True
 
 
+def _how(group):
+    return group["bits"], group["capturable"], group["master"]
+
+
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
     __slots__ = ("params", "states", "rows", "table", "device", "how")
 
     def __init__(self, optimizer, group, params):
-        self.how = bits, _ = group["bits"], group["capturable"]
+        self.how = bits, *_ = _how(group)
         self.params, self.states = params, [optimizer.state[p] for p in params]
         self.device = params[0].device
         # rows of cswap_adamw_tensor: seven words, the type in the last
@@ -52,13 +56,20 @@ class _Plan:
                 raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
             m, v, master = s["exp_avg"], s["exp_avg_sq"], s.get("master")
             _check_state(p, s, (m, v, master), bits)
+            if not _dense_order(p):
+                raise ValueError(f"AdamW8: a parameter {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
             at, n = p.data_ptr(), p.numel()
             self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m.data_ptr(), v.data_ptr()))
             self.table.extend((at, 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), n, q8._DTYPE[p.dtype]))
 
+        # all tensors of a launch are worked on at once
+        ends = sorted((at, at + n * p.element_size()) for p, at, n, *_ in self.rows if n)
+        if any(end > start for (_, end), (start, _) in zip(ends, ends[1:])):
+            raise ValueError("AdamW8: parameters that share memory")
+
     def holds(self, params, group) -> bool:
         """Whether the plan is still that of these parameters and of their state."""
-        if len(params) != len(self.rows) or self.how != (group["bits"], group["capturable"]):
+        if len(params) != len(self.rows) or self.how != _how(group):
             return False
         for p, (mine, at, n, strides, _, s, m, v, master, _, _) in zip(params, self.rows):
             if p is not mine or p.data_ptr() != at or p.numel() != n:
@@ -112,7 +123,8 @@ class AdamW8(torch.optim.Optimizer):
 
     Parameters are float32, bfloat16 or float16 in device memory; the step is computed in fp32 and rounded to the parameter's
     type once, to nearest: 16-bit parameters of steps below their last place keep still, unless ``master=True`` keeps fp32
-    copies of them (their ``state[p]["master"]``).  In 8 bits a moment has three bits of mantissa over 2^14 (the second: 2^30) below the
+    copies of them (their ``state[p]["master"]``, from which a step makes the parameter: what is written to the parameter alone is
+    lost with the next one).  In 8 bits a moment has three bits of mantissa over 2^14 (the second: 2^30) below the
     largest of 32 neighbours, rounded up and down in turn so that it drifts as it should; a NaN or an infinity in a gradient makes its 32
     neighbours' moments NaN.  ``state[p]`` has "step", "exp_avg" and "exp_avg_sq", as ``torch.optim.AdamW``'s, which
     ``load_state_dict`` also takes.
@@ -132,7 +144,11 @@ class AdamW8(torch.optim.Optimizer):
         if group["bits"] not in (8, 32):
             raise ValueError(f"AdamW8: moments in 8 or 32 bits, not {group['bits']}")
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
+        given = self.param_groups[-1]["params"]
+        if len({id(p) for p in given}) != len(given):
+            self.param_groups.pop()
+            raise ValueError("AdamW8: a parameter twice")
+        for p in given:
             if p.dtype not in q8._DTYPE:
                 self.param_groups.pop()
                 raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
@@ -174,6 +190,8 @@ class AdamW8(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # whatever one of the groups refuses is refused before a step of any is made
+        ready = []
         for number, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -188,14 +206,16 @@ class AdamW8(torch.optim.Optimizer):
             if capturable:
                 _all_together(group, params, self.state)
             lr = group["lr"] if isinstance(group["lr"], torch.Tensor) else None
-            copies = [plan.set_gradients() for plan in plans]      # whatever they refuse, they refuse before a step is made
             for plan in plans:
-                if q8._stream_of(plan.device) is not None:
+                if lr is not None and lr.device != plan.device:
+                    raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
+                ready.append((plan, group, options, lr, plan.set_gradients()))
+        for plan, group, options, lr, _ in ready:
+            if q8._stream_of(plan.device) is not None:
+                _launch(plan, group, options, lr)
+            else:
+                with torch.cuda.device(plan.device):
                     _launch(plan, group, options, lr)
-                else:
-                    with torch.cuda.device(plan.device):
-                        _launch(plan, group, options, lr)
-            del copies
         return loss
 
     def _make_plans(self, group, params):
@@ -206,8 +226,15 @@ class AdamW8(torch.optim.Optimizer):
                 self._new_state(p, group, steps)
             step = self.state[p]["step"]
             if isinstance(step, torch.Tensor) != bool(group["capturable"]):      # the option changed
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW8: make a step with capturable=True before capturing one")
                 self._finish_state(p, self.state[p], group, int(step), steps)
                 step = self.state[p]["step"]
+            if bool(group["master"]) != ("master" in self.state[p]) and p.dtype is not torch.float32:
+                if group["master"]:
+                    self.state[p]["master"] = p.detach().to(torch.float32)
+                else:
+                    del self.state[p]["master"]
             split.setdefault((p.device, id(step) if group["capturable"] else step), []).append(p)
         return [_Plan(self, group, some) for some in split.values()]
 
@@ -217,12 +244,15 @@ class AdamW8(torch.optim.Optimizer):
         for saved in state_dict["param_groups"]:
             if saved.get("amsgrad") or saved.get("maximize"):
                 raise ValueError("AdamW8: no amsgrad and no maximize")
+        for kept in state_dict["state"].values():
+            if kept and ("step" not in kept or not all(isinstance(kept.get(k), torch.Tensor) for k in ("exp_avg", "exp_avg_sq"))):
+                raise ValueError(f"AdamW8: expected step, exp_avg and exp_avg_sq in a parameter's state, not {sorted(kept)}")
         own = [{k: group[k] for k in _OWN} for group in self.param_groups]
         super().load_state_dict(state_dict)     # casts moments to the parameters' types: they are read from state_dict again
         self._plans = {}
-        steps = {}
         for group, mine, saved in zip(self.param_groups, own, state_dict["param_groups"]):
             group.update(mine)
+            steps = {}                # each group counts its own
             for p, number in zip(group["params"], saved["params"]):
                 kept = state_dict["state"].get(number)
                 if kept:
@@ -262,8 +292,6 @@ class AdamW8(torch.optim.Optimizer):
 def _launch(plan, group, options, lr):
     table, count, first, stream = plan.table.buffer_info()[0], len(plan.rows), plan.states[0], q8._stream_of(plan.device)
     if group["capturable"]:
-        if lr is not None and lr.device != plan.device:
-            raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
         factors = torch.empty(lib().cswap_adamw_factors_bytes(), dtype=torch.uint8, device=plan.device)
         check(lib().cswap_adamw_step_counted(table, count, group["bits"], C.byref(options), first["step"].data_ptr(),
                                              0 if lr is None else lr.data_ptr(), factors.data_ptr(), stream), "cswap_adamw_step_counted")

@@ -249,6 +249,8 @@ static bool options_fit(const cswap_adamw_options* o)
 
 constexpr size_t kMostValues = kMaxChunks * kChunk - kGroup;  // of a tensor: chunk numbers are 31 bits
 
+constexpr uint64_t kMostGroups = (1u << 24) - 1;          // of a launch: 2^32 threads
+
 // Launches of up to kTensors tensors; `take` puts number i of the caller's into a place of the table and says how many values it has.
 template <typename Table, typename Take, typename Launch> static int for_tables(size_t count, Take&& take, Launch&& launch)
 {
@@ -260,7 +262,7 @@ template <typename Table, typename Take, typename Launch> static int for_tables(
       const size_t n = take(i, table, table.count);
       if (n) {
         const uint64_t more = ((n + kGroup - 1) / kGroup * kChunksPerGroup + kStepThreads - 1) / kStepThreads;
-        if (groups + more < (1u << 31)) {
+        if (table.count == 0 || groups + more <= kMostGroups) {
           table.first[table.count++] = (uint32_t)groups;
           groups += more;
           if (table.count < kTensors) continue;

@@ -169,3 +169,65 @@ def test_which_layouts_fill_their_memory():
     assert _dense_order(t) and _dense_order(t.to(memory_format=torch.channels_last)) and _dense_order(t.permute(2, 0, 3, 1))
     assert _dense_order(torch.zeros(1, 5, 1)) and _dense_order(torch.zeros(())) and _dense_order(torch.zeros(3, 4).t())
     assert not _dense_order(t[:, :5]) and not _dense_order(t[..., ::2]) and not _dense_order(torch.zeros(4).expand(3, 4))
+
+
+def test_a_parameter_twice_is_refused():
+    a, b = (torch.nn.Parameter(torch.zeros(4)) for _ in range(2))
+    for given in ([a, b, a], iter([a, b, a])):
+        with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning, match="duplicate"):
+            AdamW8(given)
+    optimizer = AdamW8([a])
+    with pytest.raises(ValueError):
+        optimizer.add_param_group({"params": [a]})
+    assert len(optimizer.param_groups) == 1
+
+
+@pytest.mark.parametrize("kept", [{"step": 3}, {"exp_avg": torch.zeros(4), "exp_avg_sq": torch.zeros(4)},
+                                  {"step": 3, "exp_avg": torch.zeros(4)}, {"step": 3, "exp_avg": [0.0] * 4, "exp_avg_sq": [0.0] * 4}])
+def test_states_without_moments_are_refused(kept):
+    a = torch.nn.Parameter(torch.zeros(4))
+    optimizer = AdamW8([a], lr=0.5)
+    saved = AdamW8([a]).state_dict()
+    saved["state"] = {0: kept}
+    with pytest.raises(ValueError, match="expected step"):
+        optimizer.load_state_dict(saved)
+    assert not optimizer.state and optimizer.param_groups[0]["lr"] == 0.5
+
+
+def test_parameters_on_another_device_make_that_device_current(monkeypatch):
+    import contextlib
+
+    from cswap_amd import adamw8, api, q8
+
+    current, launched = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        was, current[0] = current[0], d.index
+        yield
+        current[0] = was
+
+    class OnDevice1(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        device = property(lambda self: torch.device("cuda", 1))
+
+    class Lib:
+        cswap_adamw_moment_bytes = staticmethod(_lib.lib().cswap_adamw_moment_bytes)
+
+        @staticmethod
+        def cswap_adamw_step(*a):
+            launched.append((current[0], a[1], a[4], a[-1]))
+            return 0
+
+    monkeypatch.setattr(q8, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(adamw8, "lib", lambda: Lib)
+    made = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **kw: made(*a, **kw).as_subclass(OnDevice1))
+    p = torch.nn.Parameter(made(64).as_subclass(OnDevice1))
+    p.grad = made(64).as_subclass(OnDevice1)
+    optimizer = AdamW8([p])
+    optimizer.step(), optimizer.step()
+    assert launched == [(1, 1, 1, 1001), (1, 1, 2, 1001)] and current == [0]

@@ -417,3 +417,127 @@ def test_options_that_change_under_way():
     square.data = square.data[:32]                             # at the same place, fewer values
     with pytest.raises((TypeError, ValueError)):
         optimizer.step()
+
+
+# ---------------------------------------------------------------- what no other test calls
+def test_groups_that_were_loaded_at_one_step_count_apart():
+    """Each group's launch counts its own steps on: a counter of two groups would count twice."""
+    params = [torch.nn.Parameter(gradient((n,), F32, n, 0.5).cuda()) for n in (100, 200)]
+    first = mod().AdamW8([{"params": [p]} for p in params], capturable=True)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    first.step()
+    again = mod().AdamW8([{"params": [p]} for p in params], capturable=True)
+    again.load_state_dict(copy.deepcopy(first.state_dict()))
+    again.step()
+    assert [int(again.state[p]["step"]) for p in params] == [2, 2]
+    again.step()
+    assert [int(again.state[p]["step"]) for p in params] == [3, 3]
+
+
+def test_what_one_group_refuses_is_refused_before_a_step_of_another():
+    a = torch.nn.Parameter(torch.ones(40).cuda())
+    gap = torch.nn.Parameter(torch.ones(4, 8).cuda()[:, :6])
+    e = torch.nn.Embedding(10, 4, sparse=True).cuda()
+    e(torch.tensor([1]).cuda()).sum().backward()
+    gap.grad = torch.ones_like(gap)
+    for bad, error in ((gap, ValueError), (e.weight, RuntimeError)):
+        a.grad = torch.ones_like(a)
+        optimizer = mod().AdamW8([{"params": [a]}, {"params": [bad]}])
+        with pytest.raises(error):
+            optimizer.step()
+        assert bool((a.detach() == 1).all()) and optimizer.state[a].get("step", 0) == 0 and not optimizer.state[a]["exp_avg"].any()
+
+
+def test_parameters_that_share_memory_are_refused():
+    room = torch.zeros(100).cuda()
+    a, b, c = torch.nn.Parameter(room[:64]), torch.nn.Parameter(room[63:80]), torch.nn.Parameter(room[80:])
+    for p in (a, b, c):
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="share memory"):
+        mod().AdamW8([a, c, b]).step()
+    assert not room.any()
+    mod().AdamW8([b, c]).step()                                  # next to each other
+    assert bool(room[63:].ne(0).all())
+
+
+def test_a_parameter_that_no_longer_fills_its_memory_is_refused():
+    room = torch.ones(8, 8).cuda()
+    p = torch.nn.Parameter(room.clone())
+    p.grad = torch.ones_like(p)
+    optimizer = mod().AdamW8([p], bits=32)
+    optimizer.step()
+    s, wide = optimizer.state[p], torch.ones(8, 9).cuda()
+    p.data = wide[:, :8]
+    p.grad = torch.ones_like(p)
+    for k in ("exp_avg", "exp_avg_sq"):
+        s[k] = torch.zeros(8, 9).cuda()[:, :8]
+    with pytest.raises(ValueError, match="fill"):
+        optimizer.step()
+    assert bool((wide == 1).all())
+
+
+def test_capturable_set_within_a_capture_is_refused():
+    p = torch.nn.Parameter(torch.ones(40).cuda())
+    p.grad = torch.ones_like(p)
+    optimizer = mod().AdamW8([p])
+    optimizer.step()
+    optimizer.param_groups[0]["capturable"] = True
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizer.step()
+    torch.cuda.synchronize()
+    optimizer.step()
+    assert int(optimizer.state[p]["step"]) == 2
+
+
+def test_master_copies_that_are_asked_for_and_given_up_under_way():
+    p = torch.nn.Parameter(torch.ones(300).cuda().to(BF16))
+    optimizer = mod().AdamW8([p], lr=2.0 ** -12, weight_decay=0.0)
+    group = optimizer.param_groups[0]
+
+    def steps(count):
+        for _ in range(count):
+            p.grad = torch.ones_like(p)
+            optimizer.step()
+
+    steps(4)
+    assert bool((p.detach() == 1).all()) and "master" not in optimizer.state[p]      # below bf16's last place
+    group["master"] = True
+    steps(20)                                                                        # 20 of 2^-12: 1.25 of 2^-8
+    assert optimizer.state[p]["master"].dtype is F32 and bool((p.detach() < 1).all())
+    at = p.detach().clone()
+    group["master"] = False
+    steps(1)
+    assert "master" not in optimizer.state[p] and torch.equal(p.detach(), at)
+
+
+def test_two_captured_steps_of_two_optimisers():
+    """Two graphs, replayed in turn and on two streams: each has its counter and its factors."""
+    makes = [torch.nn.Parameter(gradient((n,), d, n, 0.5).cuda()) for n, d in ((5000, F32), (700, BF16))]
+    eager = [torch.nn.Parameter(p.detach().clone()) for p in makes]
+    optimizers = [mod().AdamW8([p], lr=0.01 * (i + 1), capturable=True) for i, p in enumerate(makes)]
+    others = [mod().AdamW8([p], lr=0.01 * (i + 1), capturable=True) for i, p in enumerate(eager)]
+    for i, (p, q) in enumerate(zip(makes, eager)):
+        p.grad = gradient(p.shape, p.dtype, i).cuda()
+        q.grad = p.grad.clone()
+    graphs, streams = [], []
+    for optimizer in optimizers:
+        optimizer.step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            optimizer.step()
+        graphs.append(graph), streams.append(torch.cuda.Stream())
+    torch.cuda.synchronize()
+    for t in range(4):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        torch.randn(1000, device="cuda").sum().item()
+    for other in others:
+        for _ in range(5):
+            other.step()
+    for p, q, a, b in zip(makes, eager, optimizers, others):
+        assert int(a.state[p]["step"]) == int(b.state[q]["step"]) == 5
+        assert torch.equal(p.detach(), q.detach()) and torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"])
