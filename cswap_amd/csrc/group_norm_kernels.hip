@@ -31,6 +31,7 @@ namespace q8 {
 
 constexpr uint32_t kMaxChannels = 4096;
 constexpr uint32_t kMaxGroups = 2048;
+constexpr size_t kMaxSamples = (size_t)1 << 22;  // a launch has fewer than 2^32 threads
 constexpr int NT = 512;  // threads of a workgroup: a chunk of every channel
 // A workgroup's NT threads are `lanes` rows of `width` chunks; a tile is `tile_rows` positions of a sample.
 struct GroupShape {
@@ -372,8 +373,8 @@ __global__ __launch_bounds__(NT) void group_norm_forward_kernel(const typename T
   __syncthreads();
   if (p.tile == 0)
     for (uint32_t g = threadIdx.x; g < s.groups; g += NT) {
-      mean[p.sample * s.groups + g] = group_mean[g];
-      rstd[p.sample * s.groups + g] = group_rstd[g];
+      mean[(size_t)p.sample * s.groups + g] = group_mean[g];
+      rstd[(size_t)p.sample * s.groups + g] = group_rstd[g];
     }
   float mu[8], r[8];
   spread(s, place, group_mean, mu);
@@ -527,7 +528,7 @@ constexpr uint32_t kLeastRows = 8;  // of a thread in a tile, unless a sample ha
 static int group_shape(size_t samples, size_t positions, size_t channels, size_t groups, bool quads, GroupShape* s)
 {
   if (channels == 0 || positions == 0 || groups == 0 || channels % groups) return CSWAP_E_ARG;
-  if (channels > kMaxChannels || groups > kMaxGroups || samples >= ((size_t)1 << 31) || positions >= ((size_t)1 << 31) ||
+  if (channels > kMaxChannels || groups > kMaxGroups || samples > kMaxSamples || positions >= ((size_t)1 << 31) ||
       (samples && positions > (((size_t)1 << 31) - 1) / samples))
     return CSWAP_E_UNSUPPORTED;
   const uint32_t nt = NT;

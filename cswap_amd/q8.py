@@ -421,10 +421,12 @@ def _images(x: torch.Tensor, what: str):
     positions = math.prod(shape[2:])
     if channels == 0 or positions == 0:
         raise ValueError(f"{what}: images without values, {tuple(shape)}")
+    if samples == 0:        # wherever its values would lie
+        return samples, positions, channels, 0
     if channels > 1 and stride[1] != 1:
         raise ValueError(f"{what}: channels have to lie next to each other (torch.channels_last)")
     outer = [(shape[d], stride[d]) for d in (0, *range(2, n)) if shape[d] != 1]
-    if not outer or samples == 0:
+    if not outer:
         return samples, positions, channels, 0
     for (_, a), (size, b) in zip(outer, outer[1:]):
         if a != size * b:

@@ -311,3 +311,70 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         eager = step(sx.clone(), sdy.clone())
         assert all(torch.equal(a, e) for a, e in zip(out, eager))
+
+
+# ---------------------------------------------------------------- what no other test calls
+def test_statistics_beyond_32_bits():
+    """More than 2^32 groups in all, of one value each: its mean is the value itself, and y is beta."""
+    n, c = (1 << 21) + 3, 2048
+    x = torch.zeros(n, c, dtype=BF16, device="cuda")
+    ends = torch.randn(6, c, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(BF16)
+    x[:3], x[-3:] = ends[:3], ends[3:]
+    y, mean, rstd, _ = q8().group_norm(x, c, eps=0.25, checkpoint=False)
+    assert torch.equal(mean[:3], ends[:3].float()) and torch.equal(mean[-3:], ends[3:].float())
+    assert not y.any() and bool((rstd == 2.0).all()) and not mean[3:-3].any()
+
+
+def test_layers_of_no_samples_of_no_positions_and_of_expanded_gradients():
+    from cswap_amd import layers8
+
+    w, b = (t.cuda().requires_grad_() for t in params(40, 1))
+    for shape in ((0, 40, 3, 5), (0, 40)):
+        x = torch.empty(shape, device="cuda", requires_grad=True)
+        y = layers8.group_norm(x, 5, w, b, act="silu")
+        dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+        assert y.shape == shape and dx.shape == shape and not dw.any() and not db.any()
+    with pytest.raises(ValueError, match="without values"):
+        layers8.group_norm(torch.empty(2, 40, 0, 3, device="cuda"), 5, w, b)
+    # [N, C]: groups of a row; images of one channel, one position, channels first
+    for shape, groups in (((6, 40), 5), ((6, 40, 7), 8), ((3, 40, 1, 1), 4), ((1, 40, 2, 3, 2), 10)):
+        x = torch.randn(shape, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_()
+        y = layers8.group_norm(x, groups, w, b)
+        want = torch.nn.functional.group_norm(x, groups, w, b)
+        # fp32 both: a mean and a variance of up to 120 values, two products, each some roundings of values below 8
+        assert float((y - want).detach().abs().max()) <= 64 * 2.0 ** -24 * 8
+        got = torch.autograd.grad(y.sum(), (x, w, b), retain_graph=True)                    # one value, expanded
+        full = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+        assert all(torch.equal(a, e) for a, e in zip(got, full)) and got[0].shape == shape
+    one = torch.randn(4, 1, 9, 9, device="cuda")
+    y = layers8.group_norm(one, 1)
+    assert float((y - torch.nn.functional.group_norm(one, 1)).abs().max()) <= 64 * 2.0 ** -24 * 8
+
+
+def test_two_graphs_that_share_their_memory_and_calls_on_two_streams():
+    (_, x), (_, dy) = images(2, 64, (50, 40), BF16, 1), images(2, 64, (50, 40), BF16, 2)
+    w, b = (t.cuda() for t in params(64, 3))
+    names = ("gelu", "silu")
+    for kind in names:
+        run(x, dy, 8, w, b, kind, True)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in names], []
+    for graph, kind in zip(graphs, names):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if outs else None):
+            outs.append(run(x, dy, 8, w, b, kind, True)[0])
+    for k in range(4):
+        x.mul_(1.5), dy.neg_()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for kind, out in zip(names, outs):
+            assert all(torch.equal(a, e) for a, e in zip(out, run(x, dy, 8, w, b, kind, True)[0]))
+    want = [run(x, dy, 8, w, b, kind, True)[0] for kind in names]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in names]
+    for _ in range(5):
+        got = []
+        for kind, stream in zip(names, streams):
+            with torch.cuda.stream(stream):
+                got.append(run(x, dy, 8, w, b, kind, True)[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for p, q in zip(got, want) for a, e in zip(p, q))

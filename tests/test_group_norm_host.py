@@ -102,3 +102,29 @@ def test_which_layers_are_converted():
     layers8.checkpoint_layers(model, group_norm=True)
     assert [type(m) for m in model] == [layers8.GroupNorm8, nn.GroupNorm, nn.GroupNorm, layers8.Linear8]
     assert model[0].act is None
+
+
+def test_more_samples_than_a_launch_has_room_for():
+    assert forward(n=(1 << 22) + 1) == -2 and backward(n=(1 << 22) + 1) == -2
+    assert _lib.lib().cswap_group_norm_workspace_bytes((1 << 22) + 1, 1, 8, 1, 1) == 0
+
+
+def watched():
+    held = q8.Checkpoint8(torch.zeros(12, 64, dtype=torch.int8), torch.zeros(12, 2, dtype=torch.uint8), (4, 3, 40), torch.float32)
+    plain, s = torch.zeros(4, 3, 40).movedim(-1, 1), torch.zeros(4, 5)
+    return {"forward": lambda x: q8.group_norm(x, 5), "weight": lambda x: q8.group_norm(plain, 5, x[0, :, 0]),
+            "backward": lambda x: q8.group_norm_backward(x, held, s, s, 5), "backward_of_x": lambda x: q8.group_norm_backward(plain, x, s, s, 5),
+            "layer": lambda x: layers8.group_norm(x, 5)}
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", sorted(watched()))
+def test_traces_and_forward_mode_are_refused(name):
+    from torch.autograd import forward_ad
+
+    x = torch.randn(4, 3, 40).movedim(-1, 1)
+    with torch.no_grad():
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            watched()[name](forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(watched()[name], x, check_trace=False)
