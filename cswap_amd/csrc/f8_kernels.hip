@@ -526,7 +526,13 @@ constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)
 // 30.0; 64 rows 6.0 : 7.8, 12.8 : 17.0, 42 : 31.
 static bool few_rows(size_t rows, size_t weights) { return rows <= kFewPacked || (rows <= kFewPackedSmall && weights <= kSmallWeights); }
 
-static bool f8_shape(size_t rows, size_t n, size_t k) { return n <= kMaxFeatures && k <= kMaxFeatures && rows < ((size_t)1 << 31); }
+// Launches have fewer than 2^32 threads: 256 to 16 rows of a block, or to a tile of 128 x 128, 1024 to a block of weights.
+static bool f8_shape(size_t rows, size_t n, size_t k)
+{
+  if (n > kMaxFeatures || k > kMaxFeatures || rows >= ((size_t)1 << 31)) return false;
+  const size_t kb = blocks_of(k), nb = blocks_of(n), launch = (size_t)1 << 24;
+  return (rows + 15) / 16 * kb < launch && blocks_of(rows) * nb < launch && nb * kb < launch / 4;
+}
 
 }  // namespace q8
 }  // namespace cswap

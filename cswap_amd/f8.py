@@ -62,6 +62,8 @@ def f8_weight(w: torch.Tensor, backward: bool = True) -> F8Weight:
             return f8_weight(w, backward)
     if w.dim() != 2 or 0 in w.shape:
         raise ValueError(f"f8_weight: expected out x in features, not {tuple(w.shape)}")
+    if w.is_neg():
+        raise ValueError("f8_weight: a view with its sign turned (resolve_neg)")
     stride = q8._row_stride(w, "f8_weight")
     n, k = w.shape
     nb, kb = -(-n // BLOCK), -(-k // BLOCK)
@@ -92,6 +94,8 @@ def _product(what: str, x: torch.Tensor, held: F8Weight, codes: torch.Tensor, k:
     shape = x.shape
     if len(shape) == 0 or shape[-1] != k:
         raise ValueError(f"{what}: rows of {k} values, not {tuple(shape)}")
+    if x.is_neg():
+        raise ValueError(f"{what}: a view with its sign turned (resolve_neg)")
     stride = 0 if x.is_contiguous() else q8._row_stride(x, what)
     rows, _ = q8._rows_cols(shape)
     b, bk = q8._param(bias, n, device, f"{what}: bias")

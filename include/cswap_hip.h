@@ -319,7 +319,7 @@ int cswap_layer_norm_backward(const void* d_dy, int dtype, size_t rows, size_t c
                               void* d_ws, size_t ws_bytes, cswap_stream_t stream);
 
 /* Group norm with an activation function, channels last: `samples` x `positions` rows of `channels` values (up to 4096, in up to
- * 2048 groups, rows up to 2^31 - 1: CSWAP_E_UNSUPPORTED beyond), strides between rows as above; group k of a sample is its channels k * channels / groups and on,
+ * 2048 groups, up to 2^22 samples and 2^31 - 1 rows: CSWAP_E_UNSUPPORTED beyond), strides between rows as above; group k of a sample is its channels k * channels / groups and on,
  * over all positions.  Forward: y = f((x - mean) * rstd * gamma + beta), rstd = 1 / sqrt(var + eps), mean and rstd in fp32 as
  * [samples][groups]; gamma and beta (param_dtype, a value for each channel) may be NULL; the checkpoint of x, rows of `channels` values,
  * is made where d_codes and d_scales are given.  Backward takes x as it is (d_codes = d_scales = NULL) or as its checkpoint (d_x =
@@ -358,7 +358,9 @@ int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptr
  * most 2^-4 of itself, or 2^-10 * 2^s.  A block that holds a NaN or an infinity has codes of NaN (0x7f, byte 127): its results are NaN.
  * Weights are laid out once: codes [n'][k'], n' and k' rounded up to multiples of 128, 0 behind the last ones; `turned` (NULL: not wanted)
  * the same as [k'][n'], which the product with W itself, dx = dy W, reads; scales [n'/128][k'/128].  Codes are 16-byte aligned.
- * Up to 2^20 features on either side, 2^31 - 1 rows (CSWAP_E_UNSUPPORTED beyond); strides between rows as for checkpoints. */
+ * What is below fp32's normal range (2^-126) may count as 0, what a code makes of values near fp32's largest as infinity.
+ * Up to 2^20 features on either side, 2^31 - 1 rows and, features counted in whole blocks, fewer than 2^36 weights, 2^35 values of x
+ * (rows in whole sixteens) and 2^38 of y (CSWAP_E_UNSUPPORTED beyond); strides between rows as for checkpoints. */
 int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t k, ptrdiff_t stride, uint8_t* d_codes, uint8_t* d_turned,
                          uint8_t* d_scales, cswap_stream_t stream);
 /* d_y (rows x n, out_dtype) from d_x (rows x k, dtype) and the codes of n x k weights; turned = 1: d_codes is `turned` of a k x n

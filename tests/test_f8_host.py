@@ -87,3 +87,81 @@ def test_which_layers_are_converted():
     assert [type(m) for m in layers8.checkpoint_layers(model, f8=True)] == [layers8.LinearF8, layers8.GELU8]
     model = nn.Sequential(nn.Linear(3, 4))
     assert type(layers8.checkpoint_layers(model)[0]) is layers8.Linear8
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    M = 1 << 20
+    for kw in (dict(n=1 << 18, k=1 << 18), dict(n=M, k=1 << 16)):
+        assert pack(**kw, stride=M) == -2, kw
+        assert linear(rows=1, **kw) == -2, kw
+    for kw in (dict(rows=1 << 28, k=1), dict(rows=(1 << 27) + 1, k=129), dict(rows=(1 << 24) - 15, k=2048), dict(rows=1 << 29, n=1 << 9)):
+        assert linear(**kw) == -2, kw
+    f = _lib.lib().cswap_f8_linear_workspace_bytes
+    assert f(1 << 28, 1) == 0 and f((1 << 28) - 16, 1) == (1 << 28) * 129
+
+
+def test_tensors_on_another_device_make_that_device_current(monkeypatch):
+    import contextlib
+
+    from cswap_amd import api, q8
+
+    current, launched = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        was, current[0] = current[0], d.index
+        yield
+        current[0] = was
+
+    class OnDevice1(torch.Tensor):
+        is_cuda = property(lambda self: True)
+        device = property(lambda self: torch.device("cuda", 1))
+
+    class Lib:
+        cswap_f8_linear_workspace_bytes = staticmethod(_lib.lib().cswap_f8_linear_workspace_bytes)
+
+        @staticmethod
+        def cswap_f8_pack_weight(*a):
+            launched.append(("weight", current[0], a[-1]))
+            return 0
+
+        @staticmethod
+        def cswap_f8_linear(*a):
+            launched.append(("product", current[0], a[-1]))
+            return 0
+
+    made = torch.empty
+    monkeypatch.setattr(q8, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
+    monkeypatch.setattr(f8, "lib", lambda: Lib)
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **kw: made(*a, **kw).as_subclass(OnDevice1))
+    held = f8.f8_weight(torch.zeros(30, 40).as_subclass(OnDevice1))
+    f8.f8_linear(torch.zeros(20, 40).as_subclass(OnDevice1), held)
+    f8.f8_linear_backward(torch.zeros(20, 30).as_subclass(OnDevice1), held)
+    assert launched == [("weight", 1, 1001), ("product", 1, 1001), ("product", 1, 1001)] and current == [0]
+    monkeypatch.undo()
+    with pytest.raises(ValueError):
+        f8.f8_linear(torch.zeros(20, 40), held)                     # a tensor elsewhere than the weights
+
+
+def watched():
+    codes, scales = torch.zeros(128, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8)
+    held = f8.F8Weight(codes, scales, (40, 40), torch.float32, codes.clone())
+    plain = torch.zeros(4, 40)
+    return {"weight": f8.f8_weight, "product": lambda x: f8.f8_linear(x, held), "bias": lambda x: f8.f8_linear(plain, held, x[0]),
+            "backward": lambda x: f8.f8_linear_backward(x, held), "layer": lambda x: layers8.linear_f8(x, torch.zeros(40, 40), weight8=held),
+            "layer_weight": lambda x: layers8.linear_f8(plain, x)}
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", sorted(watched()))
+def test_traces_and_forward_mode_are_refused(name):
+    from torch.autograd import forward_ad
+
+    x = torch.randn(4, 40)
+    with torch.no_grad():
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            watched()[name](forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(watched()[name], x, check_trace=False)

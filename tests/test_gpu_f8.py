@@ -309,3 +309,92 @@ def test_a_training_step_of_all_three():
         assert int(oa.state[p]["step"]) == int(ob.state[q]["step"]) == 6
         # the convolutions' gradients are torch's, whose order of sums may differ from run to run: six steps of 1e-3, at most all the other way
         assert float((p.detach().float() - q.detach().float()).abs().max()) <= 2 * 6 * 1e-3 * 4 + 2.0 ** -8 * float(p.detach().float().abs().max())
+
+
+# ---------------------------------------------------------------- what no other test calls
+def test_two_graphs_that_share_their_memory():
+    x = values(300, 260, BF16, 1).cuda()
+    held = f8().f8_weight(values(400, 260, BF16, 2).cuda())
+    dy = values(300, 400, BF16, 3).cuda()
+    f8().f8_linear(x, held), f8().f8_linear_backward(dy, held)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    with torch.cuda.graph(graphs[0]):
+        outs.append(f8().f8_linear(x, held))
+    with torch.cuda.graph(graphs[1], pool=graphs[0].pool()):
+        outs.append(f8().f8_linear_backward(dy, held))
+    for k in range(4):
+        x.mul_(1.25), dy.neg_()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], f8().f8_linear(x, held)) and torch.equal(outs[1], f8().f8_linear_backward(dy, held))
+
+
+def test_calls_on_two_streams_at_once():
+    x = [values(700, 520, BF16, i).cuda() for i in range(4)]
+    held = f8().f8_weight(values(600, 520, BF16, 9).cuda())
+    want = [f8().f8_linear(t, held) for t in x]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in x]
+    for _ in range(5):
+        got = []
+        for t, stream in zip(x, streams):
+            with torch.cuda.stream(stream):
+                got.append(f8().f8_linear(t, held))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+def test_layers_of_no_rows_and_of_expanded_gradients():
+    from cswap_amd import layers8
+
+    w, b = values(24, 40, F32, 1).cuda().requires_grad_(), values(1, 24, F32, 2)[0].cuda().requires_grad_()
+    for shape in ((0, 40), (0, 3, 40), (2, 0, 40)):
+        x = torch.empty(shape, device="cuda", requires_grad=True)
+        y = layers8.linear_f8(x, w, b)
+        dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+        assert y.shape == (*shape[:-1], 24) and dx.shape == shape and not dw.any() and not db.any()
+    x = values(50, 40, F32, 3).cuda().requires_grad_()
+    wide = torch.zeros(24, 60, device="cuda")
+    wide[:, 5:45] = w.detach()
+    for weight in (w, wide[:, 5:45].requires_grad_(), w.detach().t().contiguous().t().requires_grad_()):
+        y = layers8.linear_f8(x, weight, b)
+        got = torch.autograd.grad(y.sum(), (x, weight, b), retain_graph=True)                # one value, expanded
+        want = torch.autograd.grad(y, (x, weight, b), torch.ones_like(y))
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+    with torch.no_grad():
+        assert torch.equal(layers8.linear_f8(x, wide[:, 5:45], b), f8().f8_linear(x, f8().f8_weight(w), b))
+
+
+def test_signs_that_are_turned_in_a_view_are_refused():
+    z = torch.complex(values(1, 1, F32, 1), values(1, 1, F32, 2)).cuda().conj().imag
+    held = f8().f8_weight(values(1, 1, F32, 3).cuda())
+    assert z.is_neg() and z.is_contiguous()
+    for call in (lambda: f8().f8_weight(z), lambda: f8().f8_linear(z, held), lambda: f8().f8_linear_backward(z, held)):
+        with pytest.raises(ValueError, match="sign"):
+            call()
+
+
+def test_hooks_on_saved_tensors_leave_the_layers_as_they_are():
+    """What the layers keep is in 8 bits already: the hooks that hold or swap activations give the same gradients."""
+    from cswap_amd import hooks, layers8, swap
+    from torch import nn
+
+    engine = swap.SwapEngine(pinned_bytes=64 << 20, device_bytes=64 << 20)
+
+    torch.manual_seed(0)
+    net = nn.Sequential(nn.Conv2d(3, 32, 3, padding=1), nn.GroupNorm(4, 32), nn.Flatten(), nn.Linear(32 * 36, 96), nn.Linear(96, 8))
+    net = layers8.checkpoint_layers(net, group_norm=True, f8=True).cuda().to(memory_format=torch.channels_last)
+    assert [type(m).__name__ for m in net] == ["Conv2d", "GroupNorm8", "Flatten", "LinearF8", "LinearF8"]
+    x = torch.randn(5, 32, 6, 6, device="cuda").to(memory_format=torch.channels_last)
+    tail = net[1:]                                                                            # torch's convolution keeps its own input
+
+    dy = torch.randn(5, 8, device="cuda")
+    want = torch.autograd.grad(tail(x), list(tail.parameters()), dy)
+    for ctx in (hooks.hold_saved_tensors(min_bytes=0), hooks.swap_saved_tensors(engine, policy=swap.NONE, min_bytes=4)):
+        with ctx:
+            y = tail(x)
+        got = torch.autograd.grad(y, list(tail.parameters()), dy)
+        assert ctx.stats.get("held", 0) == 0 and all(torch.equal(a, e) for a, e in zip(got, want))
+        ctx.close()
+    engine.close()
