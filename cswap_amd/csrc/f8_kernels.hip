@@ -7,8 +7,8 @@
 // this chip take a power of two for each lane's 32 values along k, so a block's two scales go into the instruction and nothing is
 // multiplied behind it: that is why the scales are powers of two (it costs up to one bit of range against max / 448, none of precision).
 //
-// Traced: 16384 x 1024 x 4096 58 us (2.37 PFLOP/s; torch's fp8 product with one scale for all 61), 16384 x 4096 x 1024 82 (1.67; torch 70), 8192^3
-// 400 at the clock of a first run (2.75), 500 at that of many; fp32 results 16384 x 768 x 768 30 (torch's bf16 product 26); a token through 4096 x 1024
+// Traced: 16384 x 1024 x 4096 57 us (2.41 PFLOP/s; torch's fp8 product with one scale for all 61), 16384 x 4096 x 1024 70 (1.96; torch 70), 8192^3
+// 387 at the clock of a first run (2.84), 480 at that of many; fp32 results 16384 x 768 x 768 30 (torch's bf16 product 26); a token through 4096 x 1024
 // 4.1, through 8192 x 8192 19.5 (3.4 TB/s); 32 tokens 4.2 and 25.6 besides 2.6 and 4.0 to turn them into codes.
 //
 // Scale of a block: the least 2^s, s >= -126, with max|x| <= 448 * 2^s, held as the byte s + 127.  A block that holds a NaN or an infinity has
@@ -182,13 +182,18 @@ struct F8Out {
   const void* bias;  // NULL: none
   int dtype, bias_dtype;
 };
-__device__ inline float bias_at(const F8Out& o, uint32_t col)
+// As it lies in memory, and its value: between the two a load is under way.
+__device__ inline uint32_t bias_bits(const F8Out& o, uint32_t col)
 {
-  if (!o.bias) return 0.0f;
-  if (o.bias_dtype == CSWAP_DT_F32) return static_cast<const float*>(o.bias)[col];
-  const uint16_t v = static_cast<const uint16_t*>(o.bias)[col];
-  return o.bias_dtype == CSWAP_DT_BF16 ? to_float<BF16>(v) : to_float<F16>(v);
+  if (!o.bias) return 0;
+  return o.bias_dtype == CSWAP_DT_F32 ? static_cast<const uint32_t*>(o.bias)[col] : static_cast<const uint16_t*>(o.bias)[col];
 }
+__device__ inline float bias_value(const F8Out& o, uint32_t bits)
+{
+  if (o.bias_dtype == CSWAP_DT_F32) return __uint_as_float(bits);
+  return o.bias_dtype == CSWAP_DT_BF16 ? to_float<BF16>((uint16_t)bits) : to_float<F16>((uint16_t)bits);
+}
+__device__ inline float bias_at(const F8Out& o, uint32_t col) { return bias_value(o, bias_bits(o, col)); }
 __device__ inline void store_one(const F8Out& o, size_t at, float v)
 {
   if (o.dtype == CSWAP_DT_F32) static_cast<float*>(o.y)[at] = v;
@@ -308,6 +313,27 @@ __global__ __launch_bounds__(64 * kFewWaves) void f8_few_rows_kernel(const typen
   }
 }
 
+// 16 bytes of results from place `at` on, of which `left` are wanted.
+template <bool EXACT> __device__ inline void store_results(const F8Out& out, size_t at, uint32_t left, uint4 v)
+{
+  constexpr int kOut = EXACT ? 4 : 2, kEach = 16 / kOut;
+  uint8_t* to = static_cast<uint8_t*>(out.y) + at * kOut;
+  if (left >= kEach) {
+    *reinterpret_cast<u4_any*>(to) = (u4_any){v.x, v.y, v.z, v.w};
+  } else {
+#pragma unroll 1
+    for (uint32_t e = 0; e < left; ++e) {  // the first of them, then the others one place nearer
+      if constexpr (EXACT) {
+        reinterpret_cast<uint32_t*>(to)[e] = v.x;
+        v = make_uint4(v.y, v.z, v.w, 0);
+      } else {
+        reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)v.x;
+        v = make_uint4(v.x >> 16 | v.y << 16, v.y >> 16 | v.z << 16, v.z >> 16 | v.w << 16, v.w >> 16);
+      }
+    }
+  }
+}
+
 typedef int i4v __attribute__((ext_vector_type(4)));
 template <bool EXACT> struct FragOf {
   typedef i8v type;
@@ -319,6 +345,8 @@ template <> struct FragOf<true> {
 // Many rows.  Four wavefronts, WM x WN of them, make a tile of TM rows x TN columns, a stage of 128 along k (EXACT: 64) at a time.  Stages lie in
 // LDS row by row, 128 bytes each, as chunks of 16 whose order within a row depends on it, so that eight lanes that read eight rows meet in
 // no bank; two stages, the next one on its way through registers while this one multiplies.  The results go out through LDS, too, in whole rows.
+// Tiles of 256 x 256 leave a compute unit no room for a second workgroup that would multiply while this one begins or stores.  Their workgroups go on to further
+// tiles instead, whose first two stages are on their way before the results go out (16384 x 4096 x 1024 70 us; 93 with a workgroup to a tile).
 template <int TM, int TN, int WM, int WN, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void f8_product_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ x_scales,
                                                                                        const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales,
@@ -328,17 +356,27 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
   constexpr int kDeep = EXACT ? 64 : 128, kSteps = EXACT ? 4 : 2, kOut = EXACT ? 4 : 2;  // k of a stage, matrix instructions along it; bytes of a result
   static_assert(TM % kEach32 == 0 && TN % kEach32 == 0 && TN / WN <= kBlock, "loads within one operand, a wavefront within one block of columns");
   static_assert(TM * TN * kOut <= 2 * kStage && NT % (TN * kOut / 16) == 0, "a tile's results fit the stages, a pass is whole rows");
+  constexpr bool kOn = TM + TN > 256;  // workgroups go on to further tiles
+  static_assert(!kOn || (!EXACT && TN / WN == 128 && TM / WM == 128), "a wavefront's results leave in parts of 32 x 64");
   // both stages of activations, then both of weights: a read's place in them is an instruction's 16-bit offset
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStage];
-  __shared__ __attribute__((aligned(16))) float bias[TN];
+  __shared__ __attribute__((aligned(16))) uint8_t parts[kOn ? WM * WN * 4096 : 16];
+  __shared__ __attribute__((aligned(16))) float bias[kOn ? WM * WN * 128 : TN];  // (a wavefront's columns for each)
   // XCDs take workgroups in turn; each gets neighbouring tiles, up to 16 along n before the next rows
   const uint32_t count = s.tiles_m * s.tiles_n, xcd = blockIdx.x % 8, each = count / 8, more = count % 8;
-  uint32_t at = xcd * each + min(xcd, more) + blockIdx.x / 8;
-  const uint32_t column = at / (16 * s.tiles_m), width = min(16u, s.tiles_n - 16 * column);
-  at -= column * 16 * s.tiles_m;
-  const uint32_t m0 = scalar(at / width * TM), n0 = scalar((16 * column + at % width) * TN);
+  struct Place {
+    uint32_t m0, n0, stage;
+  };
+  auto begin_of = [&](uint32_t tile) __attribute__((always_inline)) {
+    uint32_t at = xcd * each + min(xcd, more) + tile / 8;
+    const uint32_t column = at / (16 * s.tiles_m), width = min(16u, s.tiles_n - 16 * column);
+    at -= column * 16 * s.tiles_m;
+    return Place{scalar(at / width * TM), scalar((16 * column + at % width) * TN), 0};
+  };
   const int tid = threadIdx.x, wave = (int)scalar(tid >> 6), lane = tid & 63;
-  for (int i = tid; i < TN; i += NT) bias[i] = bias_at(out, min(n0 + i, s.n - 1));
+  Place now = begin_of(blockIdx.x);
+  if constexpr (!kOn)
+    for (int i = tid; i < TN; i += NT) bias[i] = bias_at(out, min(now.n0 + i, s.n - 1));
   const uint32_t pitch = s.blocks * kBlock;  // up to 2^20
   const uint32_t n_rows = (s.n + kBlock - 1) / kBlock * kBlock;
 
@@ -347,20 +385,25 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
   const int chunk = tid & 7, row = tid >> 3;
   constexpr int kCodes = kDeep / 8;  // codes of a chunk
   const uint32_t stages = s.blocks * (kBlock / kDeep), last = stages - 1, off = row * pitch + kCodes * chunk;
-  const Window x_from(x + (size_t)m0 * pitch, TM * pitch), w_from(w + (size_t)n0 * pitch, min((uint32_t)TN, n_rows - n0) * pitch);
   u4v raw[EXACT ? 1 : kLoads];
   u2v raw8[EXACT ? kLoads : 1];
   uint32_t unit8[EXACT ? kLoads : 1];
-  auto load = [&](uint32_t stage, int i) __attribute__((always_inline)) {
+  struct From {
+    Window x, w;
+  };
+  auto from_of = [&](const Place& p) __attribute__((always_inline)) {
+    return From{Window(x + (size_t)p.m0 * pitch, TM * pitch), Window(w + (size_t)p.n0 * pitch, min((uint32_t)TN, n_rows - p.n0) * pitch)};
+  };
+  auto load = [&](const Place& p, const From& window, int i) __attribute__((always_inline)) {
     const bool of_x = kEach32 * i < TM;
-    const uint32_t from = (of_x ? kEach32 * i : kEach32 * i - TM) * pitch + stage * kDeep;
+    const uint32_t from = (of_x ? kEach32 * i : kEach32 * i - TM) * pitch + p.stage * kDeep;
     if constexpr (EXACT) {
-      raw8[i] = of_x ? x_from.load8(off, from) : w_from.load8(off, from);
-      const uint32_t b = stage / 2;
-      if (of_x) unit8[i] = x_scales[(size_t)b * s.scale_pitch + m0 + kEach32 * i + row];
-      else unit8[i] = w_scales[(size_t)(min(n0 + kEach32 * i - TM, s.n - 1) / kBlock) * s.step_n + (size_t)b * s.step_k];
+      raw8[i] = of_x ? window.x.load8(off, from) : window.w.load8(off, from);
+      const uint32_t b = p.stage / 2;
+      if (of_x) unit8[i] = x_scales[(size_t)b * s.scale_pitch + p.m0 + kEach32 * i + row];
+      else unit8[i] = w_scales[(size_t)(min(p.n0 + kEach32 * i - TM, s.n - 1) / kBlock) * s.step_n + (size_t)b * s.step_k];
     } else {
-      raw[i] = of_x ? x_from.load16(off, from) : w_from.load16(off, from);
+      raw[i] = of_x ? window.x.load16(off, from) : window.w.load16(off, from);
     }
   };
   // addresses in LDS: a lane's, which the compiler takes as they are, and what an instruction adds to them
@@ -370,7 +413,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
     asm("" : "+v"(p));
     return p;
   };
-  Local const to_x = as_it_is(stages_at + row * kBlock + 16 * (chunk ^ ((row >> 1) & 7))), to_w = as_it_is(to_x + 2 * TM * kBlock);
+  Local to_x = as_it_is(stages_at + row * kBlock + 16 * (chunk ^ ((row >> 1) & 7))), to_w = as_it_is(to_x + 2 * TM * kBlock);
   auto store = [&](int which, int i) __attribute__((always_inline)) {
     Local const to = kEach32 * i < TM ? to_x + (which * TM + kEach32 * i) * kBlock : to_w + (which * TN + kEach32 * i - TM) * kBlock;
     if constexpr (EXACT) {
@@ -383,14 +426,13 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 
   // reading: lane l has 32 codes, or eight bf16, of row l % 32 from that many times l / 32 on
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5;
-  const uint32_t my_n = n0 + wn * (TN / WN), my_m = m0 + wm * (TM / WM);
-  const uint8_t* const ws_from = w_scales + (size_t)(min(my_n, s.n - 1) / kBlock) * s.step_n;
   int xs[2][FM], ws[2];
-  auto load_scales = [&](uint32_t stage, int which) __attribute__((always_inline)) {
+  auto load_scales = [&](const Place& p, int which) __attribute__((always_inline)) {
     if constexpr (!EXACT) {
+      const Window of_x(x_scales + (size_t)p.stage * s.scale_pitch + p.m0, TM);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) xs[which][i] = (int)Window(x_scales + (size_t)stage * s.scale_pitch + m0, TM).load1(my_m - m0 + 32 * i + r, 0);
-      ws[which] = ws_from[(size_t)stage * s.step_k];
+      for (int i = 0; i < FM; ++i) xs[which][i] = (int)of_x.load1(wm * (TM / WM) + 32 * i + r, 0);
+      ws[which] = w_scales[(size_t)(min(p.n0 + wn * (TN / WN), s.n - 1) / kBlock) * s.step_n + (size_t)p.stage * s.step_k];
     }
   };
   constexpr int kWords = EXACT ? 1 : 2;  // of 16 bytes
@@ -423,96 +465,184 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
       acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0, ws[which], 0, xs[which][j]);
     }
   };
+  {
+    const From window = from_of(now);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) load(0, i);
-  load_scales(0, 0);
+    for (int i = 0; i < kLoads; ++i) load(now, window, i);
+  }
+  load_scales(now, 0);
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) store(0, i);
+  {
+    const Place second = {now.m0, now.n0, min(1u, last)};
+    const From window = from_of(second);
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) load(min(1u, last), i);
+    for (int i = 0; i < kLoads; ++i) load(second, window, i);
+  }
   __syncthreads();
+  auto read_first = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < FN; ++i) read_w(0, 0, i);
+    for (int i = 0; i < FN; ++i) read_w(0, 0, i);
 #pragma unroll
-  for (int j = 0; j < FM; ++j) read_x(0, 0, j);
+    for (int j = 0; j < FM; ++j) read_x(0, 0, j);
+  };
+  read_first();
   // A stage is kSteps times FM x FN products.  Beside a step's go the next step's fragments, those of the activations each into the registers of
   // the one that has just been multiplied for the last time; the last step's are the next stage's, behind a barrier before it.  Beside the
   // other steps the next stage goes from registers to LDS and the one after it is asked for.  The order is given, or the compiler
   // brings loads forward until registers run out.
   constexpr int kSlots = FM * FN, kMoveSlots = (kSteps - 1) * kSlots;
-  auto one_stage = [&](uint32_t st, int which) __attribute__((always_inline)) {
-    load_scales(min(st + 1, last), which ^ 1);
+  auto one_stage = [&](int which, const Place& next, const Place& ahead) __attribute__((always_inline)) {
+    load_scales(next, which ^ 1);
+    const From window = from_of(ahead);
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const bool turn = step + 1 == kSteps;
-      const int from = turn ? which ^ 1 : which, next = turn ? 0 : step + 1;
-      if (turn) __syncthreads();
+      const bool done = step + 1 == kSteps;
+      const int from = done ? which ^ 1 : which, then = done ? 0 : step + 1;
+      if (done) __syncthreads();
 #pragma unroll
       for (int t = 0; t < kSlots; ++t) {
         const int j = t / FN, i = t % FN;
         multiply(step, which, i, j);
 #pragma unroll
         for (int f = 0; f < FN; ++f)
-          if (f * kSlots / FN == t) read_w(from, next, f);
-        if (i == FN - 1) read_x(from, next, j);
-        if (!turn) {
+          if (f * kSlots / FN == t) read_w(from, then, f);
+        if (i == FN - 1) read_x(from, then, j);
+        if (!done) {
 #pragma unroll
           for (int l = 0; l < kLoads; ++l)
             if (l * kMoveSlots / kLoads == step * kSlots + t) {
               store(which ^ 1, l);
-              load(min(st + 2, last), l);
+              load(ahead, window, l);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
-  uint32_t st = 0;
-  for (; st + 2 <= stages; st += 2) {
-    one_stage(st, 0);
-    one_stage(st + 1, 1);
-  }
-  if (st < stages) one_stage(st, 0);
-
-  // Results: lane l has row l % 32, columns 8 q + 4 (l / 32) + 0 to 3 for q = 0 to 3.  To LDS as rows of chunks of 16 bytes, in another order in
-  // each row, and from there to memory.
-  __syncthreads();  // the last stage asked for fragments of a stage that is not there
-  constexpr int kChunks = TN * kOut / 16, kEach = 16 / kOut;  // chunks of a row, results of a chunk
-  uint8_t* const tile = lds;
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int c = wn * (TN / WN) + 32 * i + 8 * q + 4 * half;
-      const float4 b = *reinterpret_cast<const float4*>(bias + c);
-#pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        const int m = wm * (TM / WM) + 32 * j + r;
-        uint8_t* to = tile + m * (TN * kOut) + 16 * ((c / kEach) ^ (m & (kChunks - 1))) + (c % kEach) * kOut;
-        const float v[4] = {acc[i][j][4 * q] + b.x, acc[i][j][4 * q + 1] + b.y, acc[i][j][4 * q + 2] + b.z, acc[i][j][4 * q + 3] + b.w};
-        if constexpr (EXACT) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
-        else if (out.dtype == CSWAP_DT_BF16) *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<BF16>(v[0], v[1]), to_pair<BF16>(v[2], v[3]));
-        else *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<F16>(v[0], v[1]), to_pair<F16>(v[2], v[3]));
-      }
+  // A tile's stages, and the first two of the one that comes then.
+  auto one_tile = [&](const Place& then) __attribute__((always_inline)) {
+    for (uint32_t st = 0; st + 2 <= stages; st += 2) {
+      const bool end = st + 2 >= stages;
+      const Place second = {now.m0, now.n0, st + 1}, ahead = {end ? then.m0 : now.m0, end ? then.n0 : now.n0, end ? 0 : st + 2};
+      one_stage(0, second, ahead);
+      one_stage(1, ahead, Place{ahead.m0, ahead.n0, (uint32_t)min(ahead.stage + 1, last)});
     }
-  __syncthreads();
-  const uint32_t rows_here = min((uint32_t)TM, s.rows - m0);
-#pragma unroll 8
-  for (int pass = 0; pass < TM * kChunks / NT; ++pass) {
-    const uint32_t m = (pass * NT + tid) / kChunks, c = tid % kChunks, n = n0 + c * kEach;
-    if (m >= rows_here || n >= s.n) continue;
-    const uint4 v = *reinterpret_cast<const uint4*>(tile + m * (TN * kOut) + 16 * (c ^ (m & (kChunks - 1))));
-    uint8_t* to = static_cast<uint8_t*>(out.y) + ((size_t)(m0 + m) * s.y_stride + n) * kOut;
-    if (n + kEach <= s.n) {
-      *reinterpret_cast<u4_any*>(to) = (u4_any){v.x, v.y, v.z, v.w};
-    } else {
-      const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+    if (stages & 1) {
+      const Place again = {now.m0, now.n0, last};
+      one_stage(0, again, again);
+    }
+  };
+  if constexpr (kOn) {
+    uint32_t mine[2];
+    auto load_bias = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < kEach - 1; ++e)
-        if (n + e < s.n) {
-          if constexpr (EXACT) reinterpret_cast<uint32_t*>(to)[e] = word[e];
-          else reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(word[e / 2] >> (16 * (e & 1)));
+      for (int e = 0; e < 2; ++e) mine[e] = bias_bits(out, min(now.n0 + wn * 128 + 64 * e + lane, s.n - 1));
+    };
+    load_bias();
+    for (uint32_t tile = blockIdx.x;;) {
+      const uint32_t then = tile + gridDim.x;
+      const Place at = now, follows = then < count ? begin_of(then) : now;
+      one_tile(follows);
+      // Results while the next tile's first stages are in LDS and on their way: each wavefront turns 32 rows x 64 columns at a time in LDS of its own,
+      // whose accesses it makes in order.
+      float* const of_wave = bias + wave * 128;
+      of_wave[lane] = bias_value(out, mine[0]), of_wave[64 + lane] = bias_value(out, mine[1]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      auto results = [&](auto type) __attribute__((always_inline)) {
+        typedef decltype(type) O;
+        int l = lane;
+        asm volatile("" : "+v"(l));  // places are made here, not kept in registers through the stages
+        const int r = l & 31, half = l >> 5, below = l >> 3, c8 = l & 7;
+        uint8_t* const part = parts + wave * 4096;
+        const uint32_t my_m = at.m0 + wm * 128, my_n = at.n0 + wn * 128;
+        const bool whole = my_m + 128 <= s.rows && my_n + 128 <= s.n;
+        uint8_t* const first = static_cast<uint8_t*>(out.y) + ((size_t)(my_m + below) * s.y_stride + my_n + 8 * c8) * 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float4 b[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const float4*>(&of_wave[64 * h + 32 * i + 8 * q + 4 * half]);
+#pragma unroll
+          for (int j = 0; j < FM; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const f16v& of = acc[2 * h + i][j];
+                uint8_t* to = part + r * 128 + 16 * ((4 * i + q) ^ (r & 7)) + 8 * half;
+                *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<O>(of[4 * q] + b[i][q].x, of[4 * q + 1] + b[i][q].y),
+                                                           to_pair<O>(of[4 * q + 2] + b[i][q].z, of[4 * q + 3] + b[i][q].w));
+              }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            uint4 v[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const uint4*>(part + (8 * p + below) * 128 + 16 * (c8 ^ below));
+            if (whole) {
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                *reinterpret_cast<u4_any*>(first + (size_t)(4 * j + p) * s.y_stride * 16 + 128 * h) = (u4_any){v[p].x, v[p].y, v[p].z, v[p].w};
+            } else {
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                const uint32_t m = my_m + 32 * j + 8 * p + below, n = my_n + 64 * h + 8 * c8;
+                if (m < s.rows && n < s.n) store_results<EXACT>(out, (size_t)m * s.y_stride + n, s.n - n, v[p]);
+              }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+          }
         }
+      };
+      if (out.dtype == CSWAP_DT_BF16) results(BF16());
+      else results(F16());
+      if (then >= count) return;
+      tile = then, now = follows;
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = (f16v){};
+      load_bias();
+      read_first();  // again: there is no room for them beside the results
+    }
+  }
+  if constexpr (!kOn) {
+    const uint32_t m0 = now.m0, n0 = now.n0;
+    one_tile(now);  // what it asks for of a next one goes nowhere
+    // Results: lane l has row l % 32, columns 8 q + 4 (l / 32) + 0 to 3 for q = 0 to 3.  To LDS as rows of chunks of 16 bytes, in another order in
+    // each row, and from there to memory.
+    __syncthreads();  // the last stage asked for fragments of a stage that is not there
+    constexpr int kChunks = TN * kOut / 16, kEach = 16 / kOut;  // chunks of a row, results of a chunk
+    uint8_t* const tile = lds;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = wn * (TN / WN) + 32 * i + 8 * q + 4 * half;
+        const float4 b = *reinterpret_cast<const float4*>(bias + c);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          const int m = wm * (TM / WM) + 32 * j + r;
+          uint8_t* to = tile + m * (TN * kOut) + 16 * ((c / kEach) ^ (m & (kChunks - 1))) + (c % kEach) * kOut;
+          const float v[4] = {acc[i][j][4 * q] + b.x, acc[i][j][4 * q + 1] + b.y, acc[i][j][4 * q + 2] + b.z, acc[i][j][4 * q + 3] + b.w};
+          if constexpr (EXACT) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+          else if (out.dtype == CSWAP_DT_BF16) *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<BF16>(v[0], v[1]), to_pair<BF16>(v[2], v[3]));
+          else *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<F16>(v[0], v[1]), to_pair<F16>(v[2], v[3]));
+        }
+      }
+    __syncthreads();
+    const uint32_t rows_here = min((uint32_t)TM, s.rows - m0);
+#pragma unroll 8
+    for (int pass = 0; pass < TM * kChunks / NT; ++pass) {
+      const uint32_t m = (pass * NT + tid) / kChunks, c = tid % kChunks, n = n0 + c * kEach;
+      if (m >= rows_here || n >= s.n) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + m * (TN * kOut) + 16 * (c ^ (m & (kChunks - 1))));
+      store_results<EXACT>(out, (size_t)(m0 + m) * s.y_stride + n, s.n - n, v);
     }
   }
 }
@@ -520,6 +650,10 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 // ---------------------------------------------------------------- launches
 constexpr size_t kFewRows = 16;  // up to which the product's kernel turns activations into codes itself
 constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)1 << 24;
+
+// Tiles of 256 x 256 are made by as many workgroups as there are compute units, each of which goes on to its next tile.  Stages lie in LDS in pairs,
+// so that an odd number of them leaves the next tile's first one where a second would be: then a workgroup makes one tile.
+constexpr uint32_t kOnWorkgroups = 256;
 
 // Few rows read the weights once, a workgroup to 16 columns; tiles of 128 x 128 have fewer workgroups but each value of the activations once for 128
 // columns.  us with codes ready, the former : the latter, 32 rows through 4096 x 1024 4.2 : 7.6, 1024 x 4096 8.3 : 16.8, 8192 x 8192 25.6 :
@@ -607,15 +741,17 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
     }
     auto launch = [&](auto f, uint32_t tm, uint32_t tn, uint32_t threads) {
       s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
-      hipLaunchKernelGGL(f, dim3(s.tiles_m * s.tiles_n), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
+      const uint32_t count = s.tiles_m * s.tiles_n;
+      hipLaunchKernelGGL(f, dim3(tm + tn > 256 && kb % 2 == 0 && count > kOnWorkgroups ? kOnWorkgroups : count), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
       return check_launch();
     };
     if (out_dtype == CSWAP_DT_F32) return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128, 256);
-    // By what rounds of all compute units take, us, with the stages' number: tiles of 256 x 256, one to a compute unit, 11.5 and 1.43 a stage, of 128 x
-    // 128, two to one, 2.3 and 1.02.  The former : the latter 16384 x 1024 x 4096 58 : 69, 8192^3 400 : 505, 4096^3 58 : 70, 16384 x 4096 x
-    // 1024 93 : 84, 16384 x 768 x 768 20.4 : 17.0, 2048^3 27 : 14.
+    // By what rounds of all compute units take, us, with the stages' number: tiles of 256 x 256, one to a compute unit, 1.43 a stage and 11.5, of which further
+    // rounds have 4 where workgroups go on, of 128 x 128, two to one, 1.02 and 2.3.  The former : the latter 16384 x 1024 x 4096 57 : 69, 8192^3 387 : 505, 4096^3
+    // 57 : 69, 16384 x 4096 x 1024 70 : 82, x 256 36 : 43, 32768 x 1024 x 1024 38 : 44, 16384 x 1152 x 1152 37 : 30, 16384 x 768 x 768 19 : 18, 2048^3 25 : 15.
     auto rounds = [&](size_t tile, size_t at_once) { return (((rows + tile - 1) / tile) * ((n + tile - 1) / tile) + at_once - 1) / at_once; };
-    if (rounds(256, 256) * (11.5 + 1.43 * kb) < rounds(128, 512) * (2.3 + 1.02 * kb)) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
+    const double large = rounds(256, 256) * (1.43 * kb + (kb % 2 ? 11.5 : 4.0)) + (kb % 2 ? 0.0 : 7.5);
+    if (large < rounds(128, 512) * (2.3 + 1.02 * kb)) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
     return launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128, 256);
   });
 }

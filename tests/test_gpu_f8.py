@@ -398,3 +398,33 @@ def test_hooks_on_saved_tensors_leave_the_layers_as_they_are():
         assert ctx.stats.get("held", 0) == 0 and all(torch.equal(a, e) for a, e in zip(got, want))
         ctx.close()
     engine.close()
+
+
+@pytest.mark.parametrize("dtype,rows,n,k,kind", [(F16, 8200, 8003, 400, F32), (BF16, 8192, 8192, 512, BF16), (BF16, 9000, 7999, 300, None), (F16, 4100, 4200, 4200, F16),
+                                                 (BF16, 8200, 8100, 4200, BF16), (F16, 17000, 4352, 100, F32)], ids=str)
+def test_whole_numbers_in_many_large_tiles(dtype, rows, n, k, kind):
+    """Sums of products of 0 and +-1 are exact in fp32, so that results are the exact ones rounded once; rows further apart than they are long keep
+    what lies between them.  More tiles than compute units, ends inside a tile on either side, even and odd numbers of stages."""
+    from cswap_amd._lib import lib
+
+    g = torch.Generator(device="cuda").manual_seed(rows + k)
+    x = torch.randint(-1, 2, (rows, k), generator=g, device="cuda").float()
+    w = torch.randint(-1, 2, (n, k), generator=g, device="cuda").float()
+    x[:, 0] = w[0, :] = 1                                           # every block has a value, and one scale
+    bias = None if kind is None else torch.randint(-9, 10, (n,), generator=g, device="cuda").to(kind)
+    want = x @ w.t() if bias is None else x @ w.t() + bias.float()
+    held = f8().f8_weight(w.to(dtype))
+    assert torch.equal(f8().f8_linear(x.to(dtype), held, bias), want.to(dtype))
+    del x
+    dy = torch.randint(-1, 2, (rows, n), generator=g, device="cuda").float()
+    assert torch.equal(f8().f8_linear_backward(dy.to(dtype), held), (dy @ w).to(dtype))
+    # gaps between rows of the result
+    xs, pitch = (want[:, :k] * 0 + 1).to(dtype), n + 5
+    y = torch.full((rows, pitch), -7.0, dtype=dtype, device="cuda")
+    room = lib().cswap_f8_linear_workspace_bytes(rows, k)
+    ws = torch.empty(room, dtype=torch.uint8, device="cuda")
+    code = {F32: 0, BF16: 1, F16: 2}[dtype]
+    assert lib().cswap_f8_linear(xs.data_ptr(), code, rows, k, 0, held.codes.data_ptr(), held.scales.data_ptr(), n, 0, 0, 0, y.data_ptr(), code, pitch, ws.data_ptr(),
+                                 room, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, :n], w.sum(1).to(dtype).expand(rows, n)) and bool((y[:, n:] == -7).all())
