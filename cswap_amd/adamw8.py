@@ -157,7 +157,8 @@ class AdamW8(torch.optim.Optimizer):
         super().__setstate__(state)
         self._plans = {}
 
-    def _new_state(self, p, group, steps):
+    def _new_state(self, p, group, steps, fresh):
+        """``fresh``: gets the moments that are to be 0, all of which are filled at once."""
         if not p.is_cuda:
             raise ValueError("AdamW8: expected parameters in device memory")
         if torch.cuda.is_current_stream_capturing():
@@ -167,10 +168,12 @@ class AdamW8(torch.optim.Optimizer):
         s = self.state[p]
         if group["bits"] == 8:
             size = lib().cswap_adamw_moment_bytes(p.numel())
-            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(size, dtype=torch.uint8, device=p.device) for _ in range(2))
+            pair = [torch.empty(size, dtype=torch.uint8, device=p.device) for _ in range(2)]
             s["strides"] = p.stride()
         else:
-            s["exp_avg"], s["exp_avg_sq"] = (torch.zeros_like(p, dtype=torch.float32) for _ in range(2))
+            pair = [torch.empty_like(p, dtype=torch.float32) for _ in range(2)]
+        s["exp_avg"], s["exp_avg_sq"] = pair
+        fresh += pair
         self._finish_state(p, s, group, 0, steps)
 
     def _finish_state(self, p, s, group, step, steps):
@@ -220,10 +223,15 @@ class AdamW8(torch.optim.Optimizer):
 
     def _make_plans(self, group, params):
         """A plan for the parameters of each device that have made as many steps."""
-        steps, split = {}, {}
+        steps, split, fresh = {}, {}, []
+        try:
+            for p in params:
+                if "exp_avg" not in self.state[p]:
+                    self._new_state(p, group, steps, fresh)
+        finally:
+            if fresh:
+                torch._foreach_zero_(fresh)
         for p in params:
-            if "exp_avg" not in self.state[p]:
-                self._new_state(p, group, steps)
             step = self.state[p]["step"]
             if isinstance(step, torch.Tensor) != bool(group["capturable"]):      # the option changed
                 if torch.cuda.is_current_stream_capturing():
@@ -231,6 +239,8 @@ class AdamW8(torch.optim.Optimizer):
                 self._finish_state(p, self.state[p], group, int(step), steps)
                 step = self.state[p]["step"]
             if bool(group["master"]) != ("master" in self.state[p]) and p.dtype is not torch.float32:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW8: make a step with this master before capturing one")
                 if group["master"]:
                     self.state[p]["master"] = p.detach().to(torch.float32)
                 else:

@@ -225,7 +225,7 @@ def test_parameters_on_another_device_make_that_device_current(monkeypatch):
     monkeypatch.setattr(api, "_raw_stream", lambda index: 1000 + index)
     monkeypatch.setattr(adamw8, "lib", lambda: Lib)
     made = torch.zeros
-    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **kw: made(*a, **kw).as_subclass(OnDevice1))
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **kw: made(*a, **kw).as_subclass(OnDevice1))
     p = torch.nn.Parameter(made(64).as_subclass(OnDevice1))
     p.grad = made(64).as_subclass(OnDevice1)
     optimizer = AdamW8([p])

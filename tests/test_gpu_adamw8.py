@@ -491,6 +491,20 @@ def test_capturable_set_within_a_capture_is_refused():
     assert int(optimizer.state[p]["step"]) == 2
 
 
+def test_master_set_within_a_capture_is_refused():
+    p = torch.nn.Parameter(torch.ones(40).cuda().to(BF16))
+    p.grad = torch.ones_like(p)
+    optimizer = mod().AdamW8([p], capturable=True)
+    optimizer.step()
+    optimizer.param_groups[0]["master"] = True
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizer.step()
+    torch.cuda.synchronize()
+    optimizer.step()
+    assert int(optimizer.state[p]["step"]) == 2 and "master" in optimizer.state[p]
+
+
 def test_master_copies_that_are_asked_for_and_given_up_under_way():
     p = torch.nn.Parameter(torch.ones(300).cuda().to(BF16))
     optimizer = mod().AdamW8([p], lr=2.0 ** -12, weight_decay=0.0)
