@@ -8,7 +8,7 @@
 // multiplied behind it: that is why the scales are powers of two (it costs up to one bit of range against max / 448, none of precision).
 //
 // Traced: 16384 x 1024 x 4096 57 us (2.41 PFLOP/s; torch's fp8 product with one scale for all 61), 16384 x 4096 x 1024 70 (1.96; torch 70), 8192^3
-// 387 at the clock of a first run (2.84), 480 at that of many; fp32 results 16384 x 768 x 768 30 (torch's bf16 product 26); a token through 4096 x 1024
+// 387 at the clock of a first run (2.84), 480 at that of many; fp32 results 16384 x 768 x 768 28 (torch's bf16 product 26), 4096^3 119; a token through 4096 x 1024
 // 4.1, through 8192 x 8192 19.5 (3.4 TB/s); 32 tokens 4.2 and 25.6 besides 2.6 and 4.0 to turn them into codes.
 //
 // Scale of a block: the least 2^s, s >= -126, with max|x| <= 448 * 2^s, held as the byte s + 127.  A block that holds a NaN or an infinity has
@@ -345,8 +345,9 @@ template <> struct FragOf<true> {
 // Many rows.  Four wavefronts, WM x WN of them, make a tile of TM rows x TN columns, a stage of 128 along k (EXACT: 64) at a time.  Stages lie in
 // LDS row by row, 128 bytes each, as chunks of 16 whose order within a row depends on it, so that eight lanes that read eight rows meet in
 // no bank; two stages, the next one on its way through registers while this one multiplies.  The results go out through LDS, too, in whole rows.
-// Tiles of 256 x 256 leave a compute unit no room for a second workgroup that would multiply while this one begins or stores.  Their workgroups go on to further
-// tiles instead, whose first two stages are on their way before the results go out (16384 x 4096 x 1024 70 us; 93 with a workgroup to a tile).
+// Tiles of 256 x 256 and 256 x 192 leave a compute unit no room for a second workgroup that would multiply while this one begins or stores.  Their workgroups go on
+// to further tiles instead, whose first two stages are on their way before the results go out (16384 x 4096 x 1024 71 us; 93 with a workgroup to a tile).  What that
+// leaves is memory's: without storing results 59 to 65.
 template <int TM, int TN, int WM, int WN, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void f8_product_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ x_scales,
                                                                                        const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_scales,
@@ -354,10 +355,10 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 {
   constexpr int NT = 64 * WM * WN, FM = TM / WM / 32, FN = TN / WN / 32, kRows = TM + TN, kEach32 = NT / 8, kLoads = kRows / kEach32, kStage = kRows * kBlock;
   constexpr int kDeep = EXACT ? 64 : 128, kSteps = EXACT ? 4 : 2, kOut = EXACT ? 4 : 2;  // k of a stage, matrix instructions along it; bytes of a result
-  static_assert(TM % kEach32 == 0 && TN % kEach32 == 0 && TN / WN <= kBlock, "loads within one operand, a wavefront within one block of columns");
-  static_assert(TM * TN * kOut <= 2 * kStage && NT % (TN * kOut / 16) == 0, "a tile's results fit the stages, a pass is whole rows");
+  static_assert(TM % kEach32 == 0 && TN % kEach32 == 0 && TN / WN <= kBlock, "loads within one operand, a wavefront's biases have room");
   constexpr bool kOn = TM + TN > 256;  // workgroups go on to further tiles
-  static_assert(!kOn || (!EXACT && TN / WN == 128 && TM / WM == 128), "a wavefront's results leave in parts of 32 x 64");
+  static_assert(kOn || (TM * TN * kOut <= 2 * kStage && NT % (TN * kOut / 16) == 0), "a tile's results fit the stages, a pass is whole rows");
+  constexpr bool kOneBlock = kBlock % (TN / WN) == 0;  // a wavefront's columns are of one block; else each 32 of them are
   // both stages of activations, then both of weights: a read's place in them is an instruction's 16-bit offset
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStage];
   __shared__ __attribute__((aligned(16))) uint8_t parts[kOn ? WM * WN * 4096 : 16];
@@ -426,13 +427,16 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 
   // reading: lane l has 32 codes, or eight bf16, of row l % 32 from that many times l / 32 on
   const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5;
-  int xs[2][FM], ws[2];
+  constexpr int kScales = kOneBlock ? 1 : FN;
+  int xs[2][FM], ws[2][kScales];
   auto load_scales = [&](const Place& p, int which) __attribute__((always_inline)) {
     if constexpr (!EXACT) {
       const Window of_x(x_scales + (size_t)p.stage * s.scale_pitch + p.m0, TM);
 #pragma unroll
       for (int i = 0; i < FM; ++i) xs[which][i] = (int)of_x.load1(wm * (TM / WM) + 32 * i + r, 0);
-      ws[which] = w_scales[(size_t)(min(p.n0 + wn * (TN / WN), s.n - 1) / kBlock) * s.step_n + (size_t)p.stage * s.step_k];
+#pragma unroll
+      for (int i = 0; i < kScales; ++i)
+        ws[which][i] = w_scales[(size_t)(min(p.n0 + wn * (TN / WN) + 32 * i, s.n - 1) / kBlock) * s.step_n + (size_t)p.stage * s.step_k];
     }
   };
   constexpr int kWords = EXACT ? 1 : 2;  // of 16 bytes
@@ -462,7 +466,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
     if constexpr (EXACT) {
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0);
     } else {
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0, ws[which], 0, xs[which][j]);
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[step & 1][i], xf[j], acc[i][j], 0, 0, 0, ws[which][kOneBlock ? 0 : i], 0, xs[which][j]);
     }
   };
   {
@@ -537,15 +541,16 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
     uint32_t mine[2];
     auto load_bias = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) mine[e] = bias_bits(out, min(now.n0 + wn * 128 + 64 * e + lane, s.n - 1));
+      for (int e = 0; e < 2; ++e) mine[e] = bias_bits(out, min(now.n0 + wn * (TN / WN) + 64 * e + lane, s.n - 1));
     };
     load_bias();
     for (uint32_t tile = blockIdx.x;;) {
       const uint32_t then = tile + gridDim.x;
       const Place at = now, follows = then < count ? begin_of(then) : now;
       one_tile(follows);
-      // Results while the next tile's first stages are in LDS and on their way: each wavefront turns 32 rows x 64 columns at a time in LDS of its own,
-      // whose accesses it makes in order.
+      // Results while the next tile's first stages are in LDS and on their way: each wavefront turns 32 rows at a time, kWide of its fragments wide, in LDS of
+      // its own, whose accesses it makes in order.
+      constexpr int kWide = !EXACT && FN % 2 == 0 ? 2 : 1, kChunks = kWide * 2 * kOut, kEach = 16 / kOut, kAtOnce = 64 / kChunks;  // of 16 bytes in a row; results of one; rows
       float* const of_wave = bias + wave * 128;
       of_wave[lane] = bias_value(out, mine[0]), of_wave[64 + lane] = bias_value(out, mine[1]);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -554,43 +559,48 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
         typedef decltype(type) O;
         int l = lane;
         asm volatile("" : "+v"(l));  // places are made here, not kept in registers through the stages
-        const int r = l & 31, half = l >> 5, below = l >> 3, c8 = l & 7;
+        const int r = l & 31, half = l >> 5, below = l / kChunks, c = l % kChunks;
         uint8_t* const part = parts + wave * 4096;
-        const uint32_t my_m = at.m0 + wm * 128, my_n = at.n0 + wn * 128;
-        const bool whole = my_m + 128 <= s.rows && my_n + 128 <= s.n;
-        uint8_t* const first = static_cast<uint8_t*>(out.y) + ((size_t)(my_m + below) * s.y_stride + my_n + 8 * c8) * 2;
+        const uint32_t my_m = at.m0 + wm * (TM / WM), my_n = at.n0 + wn * (TN / WN);
+        const bool whole = my_m + TM / WM <= s.rows && my_n + TN / WN <= s.n;
+        uint8_t* const first = static_cast<uint8_t*>(out.y) + ((size_t)(my_m + below) * s.y_stride + my_n + kEach * c) * kOut;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float4 b[2][4];
+        for (int h = 0; h < FN / kWide; ++h) {
+          float4 b[kWide][4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < kWide; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const float4*>(&of_wave[64 * h + 32 * i + 8 * q + 4 * half]);
+            for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const float4*>(&of_wave[32 * (kWide * h + i) + 8 * q + 4 * half]);
 #pragma unroll
           for (int j = 0; j < FM; ++j) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kWide; ++i)
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const f16v& of = acc[2 * h + i][j];
-                uint8_t* to = part + r * 128 + 16 * ((4 * i + q) ^ (r & 7)) + 8 * half;
-                *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<O>(of[4 * q] + b[i][q].x, of[4 * q + 1] + b[i][q].y),
-                                                           to_pair<O>(of[4 * q + 2] + b[i][q].z, of[4 * q + 3] + b[i][q].w));
+                const f16v& of = acc[kWide * h + i][j];
+                const float v[4] = {of[4 * q] + b[i][q].x, of[4 * q + 1] + b[i][q].y, of[4 * q + 2] + b[i][q].z, of[4 * q + 3] + b[i][q].w};
+                const int byte = (32 * i + 8 * q + 4 * half) * kOut;
+                uint8_t* to = part + (r * kChunks + ((byte / 16) ^ (r & (kChunks - 1)))) * 16 + byte % 16;
+                if constexpr (EXACT) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                else *reinterpret_cast<uint2*>(to) = make_uint2(to_pair<O>(v[0], v[1]), to_pair<O>(v[2], v[3]));
               }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            uint4 v[4];
+            uint4 v[32 / kAtOnce];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const uint4*>(part + (8 * p + below) * 128 + 16 * (c8 ^ below));
+            for (int p = 0; p < 32 / kAtOnce; ++p) {
+              const int row = kAtOnce * p + below;
+              v[p] = *reinterpret_cast<const uint4*>(part + (row * kChunks + (c ^ (row & (kChunks - 1)))) * 16);
+            }
             if (whole) {
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
-                *reinterpret_cast<u4_any*>(first + (size_t)(4 * j + p) * s.y_stride * 16 + 128 * h) = (u4_any){v[p].x, v[p].y, v[p].z, v[p].w};
+              for (int p = 0; p < 32 / kAtOnce; ++p)
+                *reinterpret_cast<u4_any*>(first + ((size_t)(32 * j + kAtOnce * p) * s.y_stride + 32 * kWide * h) * kOut) = (u4_any){v[p].x, v[p].y, v[p].z, v[p].w};
             } else {
 #pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                const uint32_t m = my_m + 32 * j + 8 * p + below, n = my_n + 64 * h + 8 * c8;
+              for (int p = 0; p < 32 / kAtOnce; ++p) {
+                const uint32_t m = my_m + 32 * j + kAtOnce * p + below, n = my_n + 32 * kWide * h + kEach * c;
                 if (m < s.rows && n < s.n) store_results<EXACT>(out, (size_t)m * s.y_stride + n, s.n - n, v[p]);
               }
             }
@@ -599,7 +609,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
           }
         }
       };
-      if (out.dtype == CSWAP_DT_BF16) results(BF16());
+      if (EXACT || out.dtype == CSWAP_DT_BF16) results(BF16());
       else results(F16());
       if (then >= count) return;
       tile = then, now = follows;
@@ -651,7 +661,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM + TN > 256 ? WM * WN / 4 : 2) void
 constexpr size_t kFewRows = 16;  // up to which the product's kernel turns activations into codes itself
 constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)1 << 24;
 
-// Tiles of 256 x 256 are made by as many workgroups as there are compute units, each of which goes on to its next tile.  Stages lie in LDS in pairs,
+// Tiles of 256 rows are made by as many workgroups as there are compute units, each of which goes on to its next tile.  Stages lie in LDS in pairs,
 // so that an odd number of them leaves the next tile's first one where a second would be: then a workgroup makes one tile.
 constexpr uint32_t kOnWorkgroups = 256;
 
@@ -742,16 +752,31 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
     auto launch = [&](auto f, uint32_t tm, uint32_t tn, uint32_t threads) {
       s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
       const uint32_t count = s.tiles_m * s.tiles_n;
-      hipLaunchKernelGGL(f, dim3(tm + tn > 256 && kb % 2 == 0 && count > kOnWorkgroups ? kOnWorkgroups : count), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
+      hipLaunchKernelGGL(f, dim3(tm + tn > 256 && (out_dtype == CSWAP_DT_F32 || kb % 2 == 0) && count > kOnWorkgroups ? kOnWorkgroups : count), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
       return check_launch();
     };
-    if (out_dtype == CSWAP_DT_F32) return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128, 256);
-    // By what rounds of all compute units take, us, with the stages' number: tiles of 256 x 256, one to a compute unit, 1.43 a stage and 11.5, of which further
-    // rounds have 4 where workgroups go on, of 128 x 128, two to one, 1.02 and 2.3.  The former : the latter 16384 x 1024 x 4096 57 : 69, 8192^3 387 : 505, 4096^3
-    // 57 : 69, 16384 x 4096 x 1024 70 : 82, x 256 36 : 43, 32768 x 1024 x 1024 38 : 44, 16384 x 1152 x 1152 37 : 30, 16384 x 768 x 768 19 : 18, 2048^3 25 : 15.
-    auto rounds = [&](size_t tile, size_t at_once) { return (((rows + tile - 1) / tile) * ((n + tile - 1) / tile) + at_once - 1) / at_once; };
-    const double large = rounds(256, 256) * (1.43 * kb + (kb % 2 ? 11.5 : 4.0)) + (kb % 2 ? 0.0 : 7.5);
-    if (large < rounds(128, 512) * (2.3 + 1.02 * kb)) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
+    // By what rounds of tiles on all compute units take, us, in blocks along k: of 256 x 256 and 256 x 192, one to a compute unit (further rounds begin sooner
+    // where workgroups go on), and of 128 x 128, two to one, of which one alone takes 0.62 of the time.  Measured, large : middle : small, bf16 16384 x 1024 x 4096
+    // 57 : 80 : 70, 16384 x 4096 x 1024 70 : 87 : 82, 16384 x 768 x 2304 33 : 31 : 33, 16384 x 768 x 768 18 : 17 : 18, 8192 x 1152 x 1152 22 : 19 : 20, 2048^3 25 : - : 15;
+    // fp32 4096^3 119 : 171 : 142, 16384 x 4096 x 1024 156 : 163 : 167, 25216 x 384 x 1536 51 : 41 : 44, 16384 x 768 x 768 34 : 28 : 29, 2048^3 53 : 45 : 26.
+    const bool exact = out_dtype == CSWAP_DT_F32, on = exact || kb % 2 == 0;
+    auto tiles = [&](size_t tm, size_t tn) { return ((rows + tm - 1) / tm) * ((n + tn - 1) / tn); };
+    auto one_each = [&](size_t count, double first, double further, double block) {
+      const size_t rounds = (count + 255) / 256;
+      return first + (rounds - 1) * (on ? further : first) + rounds * kb * block;
+    };
+    const size_t count = tiles(128, 128), rest = count % 512;
+    const double small = 4.0 + (count / 512 + (rest == 0 ? 0.0 : rest <= 256 ? 0.62 : 1.0)) * (2.3 + (exact ? 2.25 : 1.02) * kb);
+    const double middle = exact ? one_each(tiles(256, 192), 15.0, 9.0, 2.15) : one_each(tiles(256, 192), 10.5, 5.5, 1.12);
+    const double large = exact ? one_each(tiles(256, 256), 13.0, 10.0, 3.34) : one_each(tiles(256, 256), 10.0, 4.3, 1.43);
+    const int pick = large < small && large <= middle ? 2 : middle < small ? 1 : 0;
+    if (exact) {
+      if (pick == 2) return launch(f8_product_kernel<256, 256, 2, 2, true>, 256, 256, 256);
+      if (pick == 1) return launch(f8_product_kernel<256, 192, 2, 2, true>, 256, 192, 256);
+      return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128, 256);
+    }
+    if (pick == 2) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
+    if (pick == 1) return launch(f8_product_kernel<256, 192, 2, 2, false>, 256, 192, 256);
     return launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128, 256);
   });
 }
