@@ -428,3 +428,18 @@ def test_whole_numbers_in_many_large_tiles(dtype, rows, n, k, kind):
                                  room, torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert torch.equal(y[:, :n], w.sum(1).to(dtype).expand(rows, n)) and bool((y[:, n:] == -7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_biases_and_rows_that_start_at_any_element(dtype):
+    room = values(1, 4400, dtype, 5)[0].cuda()
+    for rows, n, k in ((1, 200, 130), (16, 77, 256), (40, 200, 130), (300, 333, 300), (4200, 4300, 256)):
+        wide = values(rows, k + 3, dtype, 1).cuda()
+        held = f8().f8_weight(values(n, k, dtype, 2).cuda())
+        plain = f8().f8_linear(wide[:, 1:k + 1].contiguous(), held, room[1:n + 1].clone())
+        assert torch.equal(f8().f8_linear(wide[:, 1:k + 1], held, room[1:n + 1]), plain)
+        w = values(n, k + 3, dtype, 2).cuda()
+        again = f8().f8_weight(w[:, 1:k + 1])
+        want = f8().f8_weight(w[:, 1:k + 1].contiguous())
+        assert torch.equal(again.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(again.turned.view(torch.uint8), want.turned.view(torch.uint8))
+        assert torch.equal(again.scales, want.scales)

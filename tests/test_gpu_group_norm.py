@@ -378,3 +378,17 @@ def test_two_graphs_that_share_their_memory_and_calls_on_two_streams():
                 got.append(run(x, dy, 8, w, b, kind, True)[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, e) for p, q in zip(got, want) for a, e in zip(p, q))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_parameters_and_images_that_start_at_any_element(dtype):
+    for n, c, spatial, groups in ((2, 64, (6, 7), 8), (3, 30, (5, 4), 5), (1, 64, (100, 90), 4)):
+        (_, x), (_, dy) = images(n, c, spatial, dtype, 1), images(n, c, spatial, dtype, 2)
+        w, b = (t.to(dtype).cuda() for t in params(c + 3, 3))
+        shifted = []
+        for t in (x, dy):
+            room = torch.empty(t.numel() + 3, dtype=dtype, device="cuda")[1:-2].view(n, *spatial, c).movedim(-1, 1)
+            shifted.append(room.copy_(t))
+        want, _ = run(x, dy, groups, w[1:-2].clone(), b[1:-2].clone(), "silu", True)
+        got, _ = run(*shifted, groups, w[1:-2], b[1:-2], "silu", True)
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
