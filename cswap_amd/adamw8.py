@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 from array import array
+from operator import is_
 
 import torch
 
@@ -43,12 +44,13 @@ def _how(group):
 
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
-    __slots__ = ("params", "states", "rows", "table", "device", "how")
+    __slots__ = ("params", "states", "rows", "table", "device", "how", "count")
 
     def __init__(self, optimizer, group, params):
         self.how = bits, *_ = _how(group)
         self.params, self.states = params, [optimizer.state[p] for p in params]
         self.device = params[0].device
+        self.count = self.states[0]["step"]
         # rows of cswap_adamw_tensor: seven words, the type in the last
         self.rows, self.table = [], array("Q")
         for p, s in zip(params, self.states):
@@ -68,16 +70,17 @@ class _Plan:
             raise ValueError("AdamW8: parameters that share memory")
 
     def holds(self, params, group) -> bool:
-        """Whether the plan is still that of these parameters and of their state."""
+        """Whether the plan is still that of these parameters and of what is in their states (which these are: ``AdamW8._same_states``)."""
         if len(params) != len(self.rows) or self.how != _how(group):
             return False
+        count = self.count
         for p, (mine, at, n, strides, _, s, m, v, master, _, _) in zip(params, self.rows):
             if p is not mine or p.data_ptr() != at or p.numel() != n:
                 return False
             if (not p.is_contiguous()) if strides is None else p.stride() != strides:
                 return False
             get = s.get
-            if get("exp_avg") is not m or get("exp_avg_sq") is not v or get("master") is not master:
+            if get("exp_avg") is not m or get("exp_avg_sq") is not v or get("master") is not master or get("step") is not count:
                 return False
         return True
 
@@ -135,7 +138,7 @@ class AdamW8(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, bits: int = 8, master: bool = False,
                  capturable: bool = False):
-        self._plans = {}
+        self._forget()
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, master=master, capturable=capturable))
 
     def add_param_group(self, param_group):
@@ -155,7 +158,16 @@ class AdamW8(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans = {}
+        self._forget()
+
+    def _forget(self):
+        """Plans, and what ``state`` held when they were made: parameters and their dictionaries, one by one."""
+        self._plans, self._seen = {}, ([], [])
+
+    def _same_states(self) -> bool:
+        """Whether ``state`` still has the dictionaries that the plans were made from, whoever cleared or replaced some."""
+        state, (params, states) = self.state, self._seen
+        return len(state) == len(params) and all(map(is_, state, params)) and all(map(is_, state.values(), states))
 
     def _new_state(self, p, group, steps, fresh):
         """``fresh``: gets the moments that are to be 0, all of which are filled at once."""
@@ -194,7 +206,9 @@ class AdamW8(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         # whatever one of the groups refuses is refused before a step of any is made
-        ready = []
+        ready, made = [], False
+        if not self._same_states():
+            self._forget()
         for number, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
@@ -203,7 +217,8 @@ class AdamW8(torch.optim.Optimizer):
             options = _options(group)
             plans = self._plans.get(number)
             if plans is None or not all(plan.holds(some, group) for plan, some in zip(plans, _as_split(plans, params))):
-                plans = self._plans[number] = self._make_plans(group, params)
+                plans, made = self._make_plans(group, params), True
+                self._plans[number] = plans
             if not capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW8: a captured step needs capturable=True")
             if capturable:
@@ -213,6 +228,8 @@ class AdamW8(torch.optim.Optimizer):
                 if lr is not None and lr.device != plan.device:
                     raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
                 ready.append((plan, group, options, lr, plan.set_gradients()))
+        if made:
+            self._seen = list(self.state), list(self.state.values())
         for plan, group, options, lr, _ in ready:
             if q8._stream_of(plan.device) is not None:
                 _launch(plan, group, options, lr)
@@ -233,7 +250,7 @@ class AdamW8(torch.optim.Optimizer):
                 torch._foreach_zero_(fresh)
         for p in params:
             step = self.state[p]["step"]
-            if isinstance(step, torch.Tensor) != bool(group["capturable"]):      # the option changed
+            if not _counts(step, group, p.device):      # the option changed, or it was set
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW8: make a step with capturable=True before capturing one")
                 self._finish_state(p, self.state[p], group, int(step), steps)
@@ -259,7 +276,7 @@ class AdamW8(torch.optim.Optimizer):
                 raise ValueError(f"AdamW8: expected step, exp_avg and exp_avg_sq in a parameter's state, not {sorted(kept)}")
         own = [{k: group[k] for k in _OWN} for group in self.param_groups]
         super().load_state_dict(state_dict)     # casts moments to the parameters' types: they are read from state_dict again
-        self._plans = {}
+        self._forget()
         for group, mine, saved in zip(self.param_groups, own, state_dict["param_groups"]):
             group.update(mine)
             steps = {}                # each group counts its own
@@ -308,8 +325,16 @@ def _launch(plan, group, options, lr):
     else:
         step = first["step"] + 1
         check(lib().cswap_adamw_step(table, count, group["bits"], C.byref(options), step, stream), "cswap_adamw_step")
+        plan.count = step
         for s in plan.states:
             s["step"] = step
+
+
+def _counts(step, group, device) -> bool:
+    """Whether this is how a group counts its steps."""
+    if group["capturable"]:
+        return isinstance(step, torch.Tensor) and step.dtype is torch.int64 and step.numel() == 1 and step.device == device
+    return isinstance(step, int)
 
 
 def _options(group) -> AdamwOptions:
@@ -360,9 +385,10 @@ def _convert(rows, name, device):
 def _held(optimizer):
     """Of the parameters that have made a step, in order: the parameter, its group, its state, its number of values and, where they are held in 8 bits, the two
     moments' addresses, checked."""
+    same = optimizer._same_states()
     for number, group in enumerate(optimizer.param_groups):
         params = [p for p in group["params"] if "exp_avg" in optimizer.state.get(p, ())]
-        plans = optimizer._plans.get(number, ())
+        plans = optimizer._plans.get(number, ()) if same else ()
         if len(plans) == 1 and plans[0].holds(params, group):
             for p, _, n, _, _, s, _, _, _, m8, v8 in plans[0].rows:
                 yield p, group, s, n, m8, v8

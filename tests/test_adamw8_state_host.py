@@ -1,0 +1,156 @@
+"""AdamW8 and the state that its caller replaces, changes or clears, without a GPU: which step and which moments a launch is given."""
+import ctypes as C
+from collections import defaultdict
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from cswap_amd import _lib, adamw8, q8  # noqa: E402
+from cswap_amd.adamw8 import AdamW8, unpack_moments  # noqa: E402
+
+
+class OnDevice(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """What the library's calls are given: of steps (number, [(param, exp_avg, exp_avg_sq, master)]), of conversions ("unpack", [codes of exp_avg])."""
+    made = []
+
+    def words(at, count, each):
+        return [(C.c_uint64 * each).from_address(at + 8 * each * i)[:] for i in range(count)]
+
+    class Lib:
+        cswap_adamw_moment_bytes = staticmethod(_lib.lib().cswap_adamw_moment_bytes)
+        cswap_adamw_factors_bytes = staticmethod(_lib.lib().cswap_adamw_factors_bytes)
+
+        @staticmethod
+        def cswap_adamw_step(table, count, bits, options, step, stream):
+            made.append((step, [(p, m, v, master) for p, g, m, v, master, n, kind in words(table, count, 7)]))
+            return 0
+
+        @staticmethod
+        def cswap_adamw_step_counted(table, count, bits, options, counter, lr, factors, stream):
+            at = C.c_longlong.from_address(counter)
+            at.value += 1
+            return Lib.cswap_adamw_step(table, count, bits, options, at.value, stream)
+
+        @staticmethod
+        def cswap_adamw_unpack(table, count, stream):
+            made.append(("unpack", [m8 for m, v, m8, v8, n in words(table, count, 5)]))
+            return 0
+
+        cswap_adamw_pack = cswap_adamw_unpack
+
+    convert = adamw8._convert
+    monkeypatch.setattr(adamw8, "lib", lambda: Lib)
+    monkeypatch.setattr(adamw8, "_convert", lambda rows, name, device: convert(rows, name, 0))
+    monkeypatch.setattr(q8, "_stream_of", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return made
+
+
+def parameter(n, dtype=torch.float32):
+    p = torch.nn.Parameter(torch.ones(n, dtype=dtype).as_subclass(OnDevice))
+    p.grad = torch.ones(n, dtype=dtype).as_subclass(OnDevice)
+    return p
+
+
+def held(optimizer, *params):
+    """A launch's rows of these parameters, from the optimiser's state."""
+    return [(p.data_ptr(), *(optimizer.state[p][k].data_ptr() for k in ("exp_avg", "exp_avg_sq")),
+             optimizer.state[p]["master"].data_ptr() if "master" in optimizer.state[p] else 0) for p in params]
+
+
+def steps(optimizer, count):
+    for _ in range(count):
+        optimizer.step()
+
+
+CLEARS = {"clear": lambda o: o.state.clear(), "another": lambda o: setattr(o, "state", defaultdict(dict)),
+          "empty": lambda o: o.state.update({p: {} for p in o.state}), "pop": lambda o: [o.state.pop(p) for p in list(o.state)]}
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("how", sorted(CLEARS))
+def test_a_state_that_was_cleared_begins_anew(launches, how, capturable):
+    a, b = parameter(40), parameter(100, torch.bfloat16)
+    optimizer = AdamW8([a, b], master=True, capturable=capturable)
+    steps(optimizer, 6)
+    b.data.fill_(3.0)
+    CLEARS[how](optimizer)
+    optimizer.step()
+    assert launches[-1] == (1, held(optimizer, a, b)) and len(launches) == 7
+    assert not any(optimizer.state[p][k].any() for p in (a, b) for k in ("exp_avg", "exp_avg_sq"))
+    assert torch.equal(optimizer.state[b]["master"], torch.full((100,), 3.0))
+    assert [int(s["step"]) for s in optimizer.state_dict()["state"].values()] == [1, 1]
+    optimizer.step()
+    assert launches[-1] == (2, held(optimizer, a, b))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_that_was_replaced_is_the_one_that_is_used(launches, bits):
+    a, b = parameter(40), parameter(100)
+    optimizer = AdamW8([a, b], bits=bits)
+    steps(optimizer, 3)
+    optimizer.state[a] = {k: v.clone() if isinstance(v, torch.Tensor) else 10 if k == "step" else v for k, v in optimizer.state[a].items()}
+    if bits == 8:
+        unpack_moments(optimizer)
+        assert launches[-1] == ("unpack", [optimizer.state[p]["exp_avg"].data_ptr() for p in (a, b)])
+    del launches[:]
+    optimizer.step()
+    assert launches == [(11, held(optimizer, a)), (4, held(optimizer, b))]
+    assert [optimizer.state[p]["step"] for p in (a, b)] == [11, 4]
+
+
+def test_a_step_that_was_set_is_the_one_that_is_counted_on(launches):
+    a, b = parameter(40), parameter(100)
+    optimizer = AdamW8([a, b])
+    steps(optimizer, 3)
+    for p in (a, b):
+        optimizer.state[p]["step"] = 1000
+    optimizer.step()
+    assert launches[-1] == (1001, held(optimizer, a, b))
+    optimizer.state[b]["step"] = 7
+    del launches[:]
+    optimizer.step()
+    assert launches == [(1002, held(optimizer, a)), (8, held(optimizer, b))]
+    optimizer.state[b]["step"] = torch.tensor(1002.0)               # as torch's optimisers count
+    del launches[:]
+    optimizer.step()
+    assert launches == [(1003, held(optimizer, a, b))] and optimizer.state[b]["step"] == 1003
+
+
+def test_a_counter_that_was_set_is_the_one_that_is_counted_on(launches):
+    a, b = parameter(40), parameter(100)
+    optimizer = AdamW8([a, b], capturable=True)
+    steps(optimizer, 3)
+    assert optimizer.state[a]["step"] is optimizer.state[b]["step"]
+    optimizer.state[b]["step"] = torch.full((1,), 7)
+    del launches[:]
+    optimizer.step()
+    assert launches == [(4, held(optimizer, a)), (8, held(optimizer, b))]
+    for wrong in (torch.tensor(20.0), torch.tensor([20], dtype=torch.int32), 20):     # a float, or four bytes: no counter to count on in place
+        optimizer.state[b]["step"] = wrong
+        del launches[:]
+        optimizer.step()
+        assert launches[1] == (21, held(optimizer, b)), wrong
+        assert optimizer.state[b]["step"].dtype is torch.int64 and int(optimizer.state[b]["step"]) == 21
+
+
+def test_a_group_keeps_its_plan_while_another_changes(launches):
+    a, b = parameter(40), parameter(100)
+    optimizer = AdamW8([{"params": [a]}, {"params": [b], "bits": 32}])
+    steps(optimizer, 2)
+    del optimizer.state[b]
+    del launches[:]
+    optimizer.step()
+    assert launches == [(3, held(optimizer, a)), (1, held(optimizer, b))]
+    b.grad, kept = None, b.grad
+    optimizer.step()
+    b.grad = kept
+    del launches[:]
+    optimizer.step()
+    assert launches == [(5, held(optimizer, a)), (2, held(optimizer, b))]

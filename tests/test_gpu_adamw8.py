@@ -555,3 +555,24 @@ def test_two_captured_steps_of_two_optimisers():
     for p, q, a, b in zip(makes, eager, optimizers, others):
         assert int(a.state[p]["step"]) == int(b.state[q]["step"]) == 5
         assert torch.equal(p.detach(), q.detach()) and torch.equal(a.state[p]["exp_avg"], b.state[q]["exp_avg"])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_optimiser_whose_state_was_cleared_is_a_new_one(bits):
+    shapes, dtypes = [(40,), (300,), (7, 9)], [F32, BF16, F16]
+    model = Model(shapes, dtypes, bits, True)
+    for t in range(3):
+        model.step([gradient(s, d, 10 * t + i) for i, (s, d) in enumerate(zip(shapes, dtypes))])
+    model.optimizer.state.clear()
+    params = [torch.nn.Parameter(p.detach().clone()) for p in model.params]
+    fresh = mod().AdamW8(params, betas=BETAS, eps=EPS, bits=bits, master=True, **model.kw)
+    for t in range(2):
+        for i, (p, q) in enumerate(zip(params, model.params)):
+            p.grad = gradient(p.shape, p.dtype, 50 * t + i).cuda()
+            q.grad = p.grad.clone()
+        fresh.step(), model.optimizer.step()
+    a, b = fresh.state_dict()["state"], model.optimizer.state_dict()["state"]
+    for i, (p, q) in enumerate(zip(params, model.params)):
+        assert torch.equal(p.detach(), q.detach()) and a[i]["step"] == b[i]["step"] == 2
+        for key in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a[i][key], b[i][key])
