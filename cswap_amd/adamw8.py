@@ -16,6 +16,7 @@ from array import array
 from operator import is_
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import q8
 from ._lib import AdamwOptions, check, lib
@@ -44,7 +45,7 @@ def _how(group):
 
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
-    __slots__ = ("params", "states", "rows", "table", "device", "how", "count")
+    __slots__ = ("params", "states", "rows", "written", "table", "device", "how", "count")
 
     def __init__(self, optimizer, group, params):
         self.how = bits, *_ = _how(group)
@@ -52,7 +53,7 @@ class _Plan:
         self.device = params[0].device
         self.count = self.states[0]["step"]
         # rows of cswap_adamw_tensor: seven words, the type in the last
-        self.rows, self.table = [], array("Q")
+        self.rows, self.table, self.written = [], array("Q"), []
         for p, s in zip(params, self.states):
             if p.dtype not in q8._DTYPE:
                 raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
@@ -63,6 +64,9 @@ class _Plan:
             at, n = p.data_ptr(), p.numel()
             self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m.data_ptr(), v.data_ptr()))
             self.table.extend((at, 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), n, q8._DTYPE[p.dtype]))
+            self.written += (p, m, v) if master is None else (p, m, v, master)
+        if group["capturable"]:
+            self.written.append(self.count)
 
         # all tensors of a launch are worked on at once
         ends = sorted((at, at + n * p.element_size()) for p, at, n, *_ in self.rows if n)
@@ -328,6 +332,7 @@ def _launch(plan, group, options, lr):
         plan.count = step
         for s in plan.states:
             s["step"] = step
+    increment_version(plan.written)      # or a backward pass that saved a parameter would not be refused
 
 
 def _counts(step, group, device) -> bool:
@@ -408,7 +413,7 @@ def unpack_moments(optimizer: AdamW8, out=None):
         out = [tuple(torch.empty_like(p, dtype=torch.float32) for _ in range(2)) for p, *_ in held]
     elif len(out) != len(held):
         raise ValueError(f"unpack_moments: {len(out)} pairs for {len(held)} parameters")
-    rows, f32 = {}, torch.float32
+    rows, written, f32 = {}, [], torch.float32
     for (p, group, s, n, m8, v8), (m, v) in zip(held, out):
         place, contiguous = p.get_device(), p.is_contiguous()
         for t in (m, v):
@@ -419,9 +424,11 @@ def unpack_moments(optimizer: AdamW8, out=None):
             if some is None:
                 some = rows[place] = []
             some += (m.data_ptr(), v.data_ptr(), m8, v8, n)
+            written += (m, v)
         else:
             m.copy_(s["exp_avg"].view_as(m))
             v.copy_(s["exp_avg_sq"].view_as(v))
     for place, some in rows.items():
         _convert(array("Q", some), "cswap_adamw_unpack", place)
+    increment_version(written)
     return out

@@ -154,3 +154,54 @@ def test_a_group_keeps_its_plan_while_another_changes(launches):
     del launches[:]
     optimizer.step()
     assert launches == [(5, held(optimizer, a)), (2, held(optimizer, b))]
+
+
+@pytest.mark.parametrize("bits,capturable", [(8, False), (8, True), (32, False)])
+def test_autograd_is_told_what_a_step_writes(launches, bits, capturable):
+    a, b, idle = parameter(40), parameter(100, torch.bfloat16), parameter(8)
+    idle.grad = None
+    optimizer = AdamW8([a, b, idle], bits=bits, master=True, capturable=capturable)
+    optimizer.step()
+
+    def versions():
+        kept = [optimizer.state[p].get(k) for p in (a, b) for k in ("exp_avg", "exp_avg_sq", "master")]
+        return [t._version for t in (a, b, *kept) if t is not None]
+
+    was, others = versions(), [t._version for t in (idle, a.grad, b.grad)]
+    optimizer.step()
+    assert len(was) == 7 and all(now > then for now, then in zip(versions(), was))
+    assert [t._version for t in (idle, a.grad, b.grad)] == others
+
+
+def test_a_backward_pass_after_a_step_is_refused_as_after_torchs(launches):
+    x = torch.ones(2, 4, requires_grad=True)
+    w = torch.nn.Parameter(torch.ones(4, 4).as_subclass(OnDevice))
+    for optimizer in (torch.optim.AdamW([w]), AdamW8([w])):
+        y = (x @ w).sum()
+        w.grad = torch.ones_like(w)
+        optimizer.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_autograd_is_told_where_moments_are_unpacked_to(launches, bits):
+    a, b = parameter(40), parameter(100)
+    optimizer = AdamW8([a, b], bits=bits)
+    optimizer.step()
+    out = [[torch.zeros(p.shape) for _ in range(2)] for p in (a, b)]
+    unpack_moments(optimizer, out)
+    assert all(t._version == 1 for pair in out for t in pair)
+    held8 = [optimizer.state[p][k]._version for p in (a, b) for k in ("exp_avg", "exp_avg_sq")]
+    unpack_moments(optimizer)
+    assert [optimizer.state[p][k]._version for p in (a, b) for k in ("exp_avg", "exp_avg_sq")] == held8
+
+
+def test_steps_in_inference_mode(launches):
+    a = parameter(40)
+    optimizer = AdamW8([a])
+    with torch.inference_mode():
+        optimizer.step()
+    was = a._version
+    optimizer.step()                                # its moments are inference tensors, which have no version
+    assert a._version > was and [s for s, _ in launches] == [1, 2]

@@ -576,3 +576,27 @@ def test_an_optimiser_whose_state_was_cleared_is_a_new_one(bits):
         assert torch.equal(p.detach(), q.detach()) and a[i]["step"] == b[i]["step"] == 2
         for key in ("exp_avg", "exp_avg_sq"):
             assert torch.equal(a[i][key], b[i][key])
+
+
+def test_a_backward_pass_through_weights_that_a_step_has_moved_is_refused():
+    from cswap_amd import hooks, layers8
+
+    x = torch.randn(64, 32, device="cuda", requires_grad=True)
+    net = torch.nn.Sequential(torch.nn.Linear(32, 64), torch.nn.Linear(64, 8)).cuda()
+    for kind in (torch.nn.Linear, layers8.Linear8):
+        for layer in net:
+            layer.__class__ = kind
+        optimizer = mod().AdamW8(net.parameters())
+        loss = net(x).square().sum()
+        loss.backward(retain_graph=True)
+        optimizer.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        net(x).sum().backward()                                      # a forward pass of its own
+    view = net[0].weight.t()
+    key = hooks.swap_saved_tensors._key(view)
+    optimizer.step()
+    assert hooks.swap_saved_tensors._key(view) != key
+    (m, v), *_ = out = [[torch.empty_like(p) for _ in range(2)] for p in net.parameters()]
+    mod().unpack_moments(optimizer, out)
+    assert m._version == v._version == 1
