@@ -45,12 +45,12 @@ def _how(group):
 
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
-    __slots__ = ("params", "states", "rows", "written", "table", "device", "how", "count")
+    __slots__ = ("params", "states", "rows", "written", "table", "device", "place", "how", "count")
 
     def __init__(self, optimizer, group, params):
         self.how = bits, *_ = _how(group)
         self.params, self.states = params, [optimizer.state[p] for p in params]
-        self.device = params[0].device
+        self.device, self.place = params[0].device, params[0].get_device()
         self.count = self.states[0]["step"]
         # rows of cswap_adamw_tensor: seven words, the type in the last
         self.rows, self.table, self.written = [], array("Q"), []
@@ -62,8 +62,9 @@ class _Plan:
             if not _dense_order(p):
                 raise ValueError(f"AdamW8: a parameter {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
             at, n = p.data_ptr(), p.numel()
-            self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m.data_ptr(), v.data_ptr()))
-            self.table.extend((at, 0, m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr(), n, q8._DTYPE[p.dtype]))
+            m_at, v_at, master_at = m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr()
+            self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m_at, v_at, master_at))
+            self.table.extend((at, 0, m_at, v_at, master_at, n, q8._DTYPE[p.dtype]))
             self.written += (p, m, v) if master is None else (p, m, v, master)
         if group["capturable"]:
             self.written.append(self.count)
@@ -78,7 +79,9 @@ class _Plan:
         if len(params) != len(self.rows) or self.how != _how(group):
             return False
         count = self.count
-        for p, (mine, at, n, strides, _, s, m, v, master, _, _) in zip(params, self.rows):
+        if isinstance(count, torch.Tensor) and count.device != self.device:
+            return False
+        for p, (mine, at, n, strides, _, s, m, v, master, m_at, v_at, master_at) in zip(params, self.rows):
             if p is not mine or p.data_ptr() != at or p.numel() != n:
                 return False
             if (not p.is_contiguous()) if strides is None else p.stride() != strides:
@@ -86,18 +89,21 @@ class _Plan:
             get = s.get
             if get("exp_avg") is not m or get("exp_avg_sq") is not v or get("master") is not master or get("step") is not count:
                 return False
+            if m.data_ptr() != m_at or v.data_ptr() != v_at or master is not None and master.data_ptr() != master_at:
+                return False
         return True
 
-    def set_gradients(self):
+    def set_gradients(self, gradients):
         """Fills in the gradients' addresses; gives back what has to live until the launch."""
         copies, addresses = [], []
-        strided = torch.strided
-        for p, _, n, strides, dtype, *_ in self.rows:
-            g = p.grad
+        strided, place = torch.strided, self.place
+        for (p, _, n, strides, dtype, *_), g in zip(self.rows, gradients):
             if g.layout is not strided:
                 raise RuntimeError("AdamW8: no sparse gradients")
             if g.dtype is not dtype or g.numel() != n:
                 raise TypeError(f"AdamW8: a gradient {tuple(g.shape)} {g.dtype} of a parameter {tuple(p.shape)} {dtype}")
+            if g.get_device() != place:
+                raise ValueError(f"AdamW8: a gradient on {g.device} of a parameter on {p.device}")
             if ((not g.is_contiguous()) if strides is None else g.stride() != strides) or g.is_neg():
                 g = torch.empty_like(p).copy_(g)
                 copies.append(g)
@@ -108,6 +114,8 @@ class _Plan:
 
 def _check_state(p, s, kept, bits):
     """A state that did not come from here, or a parameter that changed under it."""
+    if not p.is_cuda:
+        raise ValueError("AdamW8: expected parameters in device memory")
     m, v, master = kept
     n = p.numel()
     for t in (m, v):
@@ -214,7 +222,11 @@ class AdamW8(torch.optim.Optimizer):
         if not self._same_states():
             self._forget()
         for number, group in enumerate(self.param_groups):
-            params = [p for p in group["params"] if p.grad is not None]
+            params, gradients = [], []
+            for p in group["params"]:
+                g = p.grad
+                if g is not None:
+                    params.append(p), gradients.append(g)
             if not params:
                 continue
             capturable = group["capturable"]
@@ -228,10 +240,10 @@ class AdamW8(torch.optim.Optimizer):
             if capturable:
                 _all_together(group, params, self.state)
             lr = group["lr"] if isinstance(group["lr"], torch.Tensor) else None
-            for plan in plans:
+            for plan, some in zip(plans, _as_split(plans, params, gradients)):
                 if lr is not None and lr.device != plan.device:
                     raise ValueError(f"AdamW8: lr on {lr.device}, parameters on {plan.device}")
-                ready.append((plan, group, options, lr, plan.set_gradients()))
+                ready.append((plan, group, options, lr, plan.set_gradients(some)))
         if made:
             self._seen = list(self.state), list(self.state.values())
         for plan, group, options, lr, _ in ready:
@@ -354,14 +366,15 @@ def _options(group) -> AdamwOptions:
     return options
 
 
-def _as_split(plans, params):
-    """params in the plans' order, as far as they are the same ones."""
+def _as_split(plans, params, given=None):
+    """params, or what is given for each of them, in the plans' order, as far as they are the same ones."""
+    given = params if given is None else given
     if len(plans) == 1:
-        return [params]
+        return [given]
     place = {id(p): k for k, plan in enumerate(plans) for p in plan.params}
     split = [[] for _ in plans]
-    for p in params:
-        split[place.get(id(p), 0)].append(p)
+    for p, one in zip(params, given):
+        split[place.get(id(p), 0)].append(one)
     return split
 
 
@@ -388,20 +401,21 @@ def _convert(rows, name, device):
 
 
 def _held(optimizer):
-    """Of the parameters that have made a step, in order: the parameter, its group, its state, its number of values and, where they are held in 8 bits, the two
-    moments' addresses, checked."""
+    """Of the parameters that have made a step, in order: the parameter, its group, its state, its number of values, its device's number, whether it is
+    contiguous and, where they are held in 8 bits, the two moments' addresses, checked."""
     same = optimizer._same_states()
     for number, group in enumerate(optimizer.param_groups):
         params = [p for p in group["params"] if "exp_avg" in optimizer.state.get(p, ())]
         plans = optimizer._plans.get(number, ()) if same else ()
         if len(plans) == 1 and plans[0].holds(params, group):
-            for p, _, n, _, _, s, _, _, _, m8, v8 in plans[0].rows:
-                yield p, group, s, n, m8, v8
+            place = plans[0].place
+            for p, _, n, strides, _, s, _, _, _, m8, v8, _ in plans[0].rows:
+                yield p, group, s, n, place, strides is None, m8, v8
             continue
         for p in params:
             s = optimizer.state[p]
             _check_state(p, s, (s["exp_avg"], s["exp_avg_sq"], None), group["bits"])
-            yield p, group, s, p.numel(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr()
+            yield p, group, s, p.numel(), p.get_device(), p.is_contiguous(), s["exp_avg"].data_ptr(), s["exp_avg_sq"].data_ptr()
 
 
 @torch.no_grad()
@@ -414,8 +428,7 @@ def unpack_moments(optimizer: AdamW8, out=None):
     elif len(out) != len(held):
         raise ValueError(f"unpack_moments: {len(out)} pairs for {len(held)} parameters")
     rows, written, f32 = {}, [], torch.float32
-    for (p, group, s, n, m8, v8), (m, v) in zip(held, out):
-        place, contiguous = p.get_device(), p.is_contiguous()
+    for (p, group, s, n, place, contiguous, m8, v8), (m, v) in zip(held, out):
         for t in (m, v):
             if t.dtype is not f32 or t.numel() != n or t.get_device() != place or not (contiguous and t.is_contiguous() or t.stride() == p.stride()):
                 raise ValueError(f"unpack_moments: {tuple(t.shape)} {t.dtype} on {t.device} for a parameter {tuple(p.shape)} on {p.device}")

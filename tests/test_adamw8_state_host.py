@@ -205,3 +205,55 @@ def test_steps_in_inference_mode(launches):
     was = a._version
     optimizer.step()                                # its moments are inference tensors, which have no version
     assert a._version > was and [s for s, _ in launches] == [1, 2]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_that_moved_are_written_where_they_are(launches, bits):
+    """A program that takes its optimiser's state elsewhere and back through ``.data``: the tensors are the same ones, their memory is not."""
+    a, b = parameter(40), parameter(100, torch.bfloat16)
+    optimizer = AdamW8([a, b], bits=bits, master=True)
+    optimizer.step()
+    old = []
+    for p, key in ((a, "exp_avg"), (a, "exp_avg_sq"), (b, "exp_avg"), (b, "exp_avg_sq"), (b, "master")):
+        kept = optimizer.state[p][key]
+        old.append(kept.data)                       # so that its place is not given out again
+        kept.data = kept.data.clone()
+        if bits == 8:
+            unpack_moments(optimizer)
+            assert launches[-1] == ("unpack", [optimizer.state[p]["exp_avg"].data_ptr() for p in (a, b)])
+        optimizer.step()
+        assert launches[-1][1] == held(optimizer, a, b), key
+    assert launches[-1][0] == 6
+
+
+def test_a_counter_that_moved_is_counted_on_where_it_is(launches):
+    a = parameter(40)
+    optimizer = AdamW8([a], capturable=True)
+    steps(optimizer, 2)
+    old, counter = optimizer.state[a]["step"].data, optimizer.state[a]["step"]
+    counter.data = counter.data.clone()
+    optimizer.step()
+    assert int(counter) == 3 and int(old) == 2
+
+
+class Numbered(OnDevice):
+    def get_device(self):
+        return 0
+
+
+def test_what_lies_in_host_memory_is_refused_before_a_launch(launches):
+    a, b = (torch.nn.Parameter(torch.ones(n).as_subclass(Numbered)) for n in (40, 100))
+    a.grad, b.grad = (torch.ones(n).as_subclass(Numbered) for n in (40, 100))
+    optimizer = AdamW8([a, b])
+    optimizer.step()
+    b.grad = torch.ones(100)                        # a gradient that stayed behind
+    with pytest.raises(ValueError, match="gradient"):
+        optimizer.step()
+    b.grad = torch.ones(100).as_subclass(Numbered)
+    other = torch.nn.Parameter(torch.ones(100))
+    other.grad = torch.ones(100)
+    host = AdamW8([other])
+    host.state[other].update(optimizer.state[b])
+    with pytest.raises(ValueError, match="device memory"):
+        host.step()
+    assert len(launches) == 1 and optimizer.state[a]["step"] == 1
