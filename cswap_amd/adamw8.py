@@ -217,6 +217,9 @@ class AdamW8(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if q8._watched():
+            given = [p for group in self.param_groups for p in group["params"]]
+            q8._refuse_what_torch_would_lose("AdamW8.step", *given, *(p.grad for p in given))
         # whatever one of the groups refuses is refused before a step of any is made
         ready, made = [], False
         if not self._same_states():
@@ -393,6 +396,8 @@ def _row(m, v, m8, v8):
 def _convert(rows, name, device):
     """``rows``: cswap_adamw_moments as five words each; ``device``: or its number."""
     device = torch.device("cuda", device) if isinstance(device, int) else device
+    if q8._watched():
+        q8._refuse_what_torch_would_lose(name)
     stream = q8._stream_of(device)
     if stream is None:
         with torch.cuda.device(device):
@@ -422,6 +427,8 @@ def _held(optimizer):
 def unpack_moments(optimizer: AdamW8, out=None):
     """``[(exp_avg, exp_avg_sq)]`` in fp32 of the parameters that have made a step, in their order and layout; ``out``: such a list to
     write to."""
+    if q8._watched():
+        q8._refuse_what_torch_would_lose("unpack_moments", *(t for pair in out or () for t in pair))
     held = list(_held(optimizer))
     if out is None:
         out = [tuple(torch.empty_like(p, dtype=torch.float32) for _ in range(2)) for p, *_ in held]

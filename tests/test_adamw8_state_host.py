@@ -257,3 +257,46 @@ def test_what_lies_in_host_memory_is_refused_before_a_launch(launches):
     with pytest.raises(ValueError, match="device memory"):
         host.step()
     assert len(launches) == 1 and optimizer.state[a]["step"] == 1
+
+
+def traced(call, p):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def f(g):
+        p.grad = g
+        call()
+        return g * 2
+
+    return make_fx(f)(p.grad)
+
+
+@pytest.mark.parametrize("name", ["step", "first_step", "unpack", "load"])
+def test_traces_are_refused(launches, name):
+    p = parameter(40)
+    optimizer = AdamW8([p])
+    if name != "first_step":
+        optimizer.step()
+    saved = optimizer.state_dict()
+    call = {"step": optimizer.step, "first_step": optimizer.step, "unpack": lambda: unpack_moments(optimizer),
+            "load": lambda: AdamW8([p], bits=32).load_state_dict(saved)}[name]
+    count = len(launches)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        traced(call, p)
+    p.grad = torch.ones(40).as_subclass(OnDevice)
+    with pytest.raises(RuntimeError, match="cannot be traced" if name != "load" else "constant"):       # torch refuses what loading does before it converts
+        torch.jit.trace(lambda g: (call(), g * 2)[1], torch.ones(40), check_trace=False)
+    assert len(launches) == count and optimizer.state[p].get("step", 0) == (0 if name == "first_step" else 1)
+
+
+def test_forward_mode_is_refused(launches):
+    from torch.autograd import forward_ad
+
+    p = parameter(40)
+    optimizer = AdamW8([p])
+    optimizer.step()
+    with forward_ad.dual_level():
+        optimizer.step()                                             # nothing here has a tangent
+        p.grad = forward_ad.make_dual(torch.ones(40).as_subclass(OnDevice), torch.ones(40).as_subclass(OnDevice))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            optimizer.step()
+    assert [s for s, _ in launches] == [1, 2]
