@@ -287,22 +287,34 @@ class AdamW8(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Of an ``AdamW8`` or of a ``torch.optim.AdamW``; this optimiser's own ``bits``, ``master`` and ``capturable`` stay, and moments are
         converted to them (to 8 bits: to nearest)."""
-        for saved in state_dict["param_groups"]:
-            if saved.get("amsgrad") or saved.get("maximize"):
-                raise ValueError("AdamW8: no amsgrad and no maximize")
-        for kept in state_dict["state"].values():
-            if kept and ("step" not in kept or not all(isinstance(kept.get(k), torch.Tensor) for k in ("exp_avg", "exp_avg_sq"))):
-                raise ValueError(f"AdamW8: expected step, exp_avg and exp_avg_sq in a parameter's state, not {sorted(kept)}")
         own = [{k: group[k] for k in _OWN} for group in self.param_groups]
-        super().load_state_dict(state_dict)     # casts moments to the parameters' types: they are read from state_dict again
-        self._forget()
-        for group, mine, saved in zip(self.param_groups, own, state_dict["param_groups"]):
-            group.update(mine)
-            steps = {}                # each group counts its own
-            for p, number in zip(group["params"], saved["params"]):
-                kept = state_dict["state"].get(number)
-                if kept:
-                    self._load(p, group, kept, steps)
+        given = {}
+
+        def look(_, last):             # what the caller's hooks leave
+            for saved in last["param_groups"]:
+                if saved.get("amsgrad") or saved.get("maximize"):
+                    raise ValueError("AdamW8: no amsgrad and no maximize")
+            for kept in last["state"].values():
+                if kept and ("step" not in kept or not all(isinstance(kept.get(k), torch.Tensor) for k in ("exp_avg", "exp_avg_sq"))):
+                    raise ValueError(f"AdamW8: expected step, exp_avg and exp_avg_sq in a parameter's state, not {sorted(kept)}")
+            given.update(last)
+
+        def convert(_):                 # before they see what was loaded; torch has cast moments to the parameters' types
+            for group, mine, saved in zip(self.param_groups, own, given["param_groups"]):
+                group.update(mine)
+                steps = {}              # each group counts its own
+                for p, number in zip(group["params"], saved["params"]):
+                    kept = given["state"].get(number)
+                    if kept:
+                        self._load(p, group, kept, steps)
+
+        hooks = self.register_load_state_dict_pre_hook(look), self.register_load_state_dict_post_hook(convert, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+            self._forget()
 
     @torch.no_grad()
     def _load(self, p, group, kept, steps):

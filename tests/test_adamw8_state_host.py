@@ -300,3 +300,50 @@ def test_forward_mode_is_refused(launches):
         with pytest.raises(RuntimeError, match="forward-mode"):
             optimizer.step()
     assert [s for s, _ in launches] == [1, 2]
+
+
+def test_hooks_on_loading_are_heard(launches):
+    """What a hook before loading gives back is what is loaded, and a hook after it sees the state as it then is."""
+    a, b = parameter(40), parameter(100, torch.bfloat16)
+    saved = {"state": {i: {"step": torch.tensor(5.0), "exp_avg": torch.full((n,), 1.0), "exp_avg_sq": torch.full((n,), 2.0)} for i, n in enumerate((40, 100))},
+             "param_groups": torch.optim.AdamW([torch.nn.Parameter(torch.zeros(1)) for _ in range(2)], lr=0.25).state_dict()["param_groups"]}
+    wrapped = {"optimizer": saved}
+    optimizer = AdamW8([a, b], bits=32, master=True)
+    seen = []
+    hooks = [optimizer.register_load_state_dict_pre_hook(lambda o, given: given["optimizer"]),
+             optimizer.register_load_state_dict_pre_hook(lambda o, given: {**given, "state": {i: {**s, "exp_avg": s["exp_avg"] * 3} for i, s in given["state"].items()}}),
+             optimizer.register_load_state_dict_post_hook(lambda o: seen.append([(type(s["step"]), s["exp_avg"].dtype, float(s["exp_avg"][0])) for s in o.state.values()]))]
+    optimizer.load_state_dict(wrapped)
+    assert seen == [[(int, torch.float32, 3.0)] * 2]
+    for p in (a, b):
+        s = optimizer.state[p]
+        assert s["step"] == 5 and bool((s["exp_avg"] == 3).all()) and bool((s["exp_avg_sq"] == 2).all()) and s["exp_avg"].dtype is torch.float32
+    assert optimizer.param_groups[0]["lr"] == 0.25 and optimizer.param_groups[0]["bits"] == 32
+    assert torch.equal(optimizer.state[b]["master"], torch.ones(100)) and float(saved["state"][0]["exp_avg"][0]) == 1.0
+    # a hook may change what it is given in place; what it gives is checked as what a caller gives
+    for hook in hooks:
+        hook.remove()
+    first = optimizer.register_load_state_dict_pre_hook(lambda o, given: given["param_groups"][0].update(amsgrad=True))
+    with pytest.raises(ValueError, match="amsgrad"):
+        optimizer.load_state_dict(saved)
+    first.remove()
+    saved["param_groups"][0]["amsgrad"] = False
+    optimizer.load_state_dict(saved)
+    optimizer.load_state_dict(optimizer.state_dict())
+    assert len(seen) == 1 and optimizer.state[a]["step"] == 5
+
+
+def test_hooks_on_loading_are_the_callers_alone_after_it(launches):
+    a = parameter(40)
+    optimizer = AdamW8([a])
+    optimizer.step()
+    saved = optimizer.state_dict()
+    for given in (saved, {**saved, "param_groups": []}):
+        try:
+            optimizer.load_state_dict(given)
+        except ValueError:
+            assert given is not saved
+    other = torch.optim.Optimizer.load_state_dict
+    del optimizer.state[a]
+    other(optimizer, saved)                                          # torch's own, with nothing of ours left behind
+    assert optimizer.state[a]["exp_avg"].dtype is torch.float32
