@@ -298,8 +298,11 @@ class AdamW8(torch.optim.Optimizer):
                 if kept and ("step" not in kept or not all(isinstance(kept.get(k), torch.Tensor) for k in ("exp_avg", "exp_avg_sq"))):
                     raise ValueError(f"AdamW8: expected step, exp_avg and exp_avg_sq in a parameter's state, not {sorted(kept)}")
             given.update(last)
+            # torch would cast moments to the parameters' types, all of them before the first is converted
+            numbers = {number for saved in last["param_groups"] for number in saved["params"]}
+            return {**last, "state": {number: kept for number, kept in last["state"].items() if number not in numbers}}
 
-        def convert(_):                 # before they see what was loaded; torch has cast moments to the parameters' types
+        def convert(_):                 # before they see what was loaded
             for group, mine, saved in zip(self.param_groups, own, given["param_groups"]):
                 group.update(mine)
                 steps = {}              # each group counts its own

@@ -347,3 +347,33 @@ def test_hooks_on_loading_are_the_callers_alone_after_it(launches):
     del optimizer.state[a]
     other(optimizer, saved)                                          # torch's own, with nothing of ours left behind
     assert optimizer.state[a]["exp_avg"].dtype is torch.float32
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_loading_moments_of_8_bits_makes_them_in_no_other_type(launches, dtype):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Made(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if isinstance(out, torch.Tensor):
+                made.append((out.dtype, out.numel()))
+            return out
+
+    a, b, made = parameter(4000, dtype), parameter(7000, dtype), []
+    optimizer = AdamW8([a, b])
+    optimizer.step()
+    for i, p in enumerate((a, b)):
+        optimizer.state[p]["exp_avg"].fill_(i + 1), optimizer.state[p]["exp_avg_sq"].fill_(i + 10)
+    saved = optimizer.state_dict()
+    other = AdamW8([a, b])
+    with Made():
+        other.load_state_dict(saved)
+    assert made and all(kind is torch.uint8 for kind, n in made if n >= 4000), made
+    for p in (a, b):
+        for key in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(other.state[p][key], optimizer.state[p][key]) and other.state[p][key] is not optimizer.state[p][key]
+    # what belongs to no parameter is handed on as torch hands it on
+    saved["state"]["extra"] = {}
+    other.load_state_dict(saved)
+    assert other.state["extra"] == {} and other.state[a]["step"] == 1

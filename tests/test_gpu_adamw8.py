@@ -600,3 +600,20 @@ def test_a_backward_pass_through_weights_that_a_step_has_moved_is_refused():
     (m, v), *_ = out = [[torch.empty_like(p) for _ in range(2)] for p in net.parameters()]
     mod().unpack_moments(optimizer, out)
     assert m._version == v._version == 1
+
+
+def test_loading_takes_no_room_beyond_what_is_kept():
+    n = 1 << 24
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    p.grad = torch.ones_like(p)
+    first = mod().AdamW8([p])
+    first.step()
+    saved = {k: v for k, v in first.state_dict().items()}
+    saved["state"] = {0: {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in saved["state"][0].items()}}
+    again = mod().AdamW8([p])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    again.load_state_dict(saved)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (n * 33 // 32) + (2 << 20)      # two moments, and the allocator's rounding
+    assert all(torch.equal(again.state[p][k], first.state[p][k]) for k in ("exp_avg", "exp_avg_sq"))
