@@ -45,15 +45,15 @@ def _how(group):
 
 class _Plan:
     """The call for some parameters: its table, filled in but for the gradients' addresses, and what it was made from."""
-    __slots__ = ("params", "states", "rows", "written", "table", "device", "place", "how", "count")
+    __slots__ = ("params", "states", "rows", "kinds", "written", "table", "device", "place", "how", "count")
 
     def __init__(self, optimizer, group, params):
         self.how = bits, *_ = _how(group)
-        self.params, self.states = params, [optimizer.state[p] for p in params]
+        self.params, self.states = list(params), [optimizer.state[p] for p in params]
         self.device, self.place = params[0].device, params[0].get_device()
         self.count = self.states[0]["step"]
         # rows of cswap_adamw_tensor: seven words, the type in the last
-        self.rows, self.table, self.written = [], array("Q"), []
+        self.rows, self.kinds, self.table, self.written = [], [], array("Q"), []
         for p, s in zip(params, self.states):
             if p.dtype not in q8._DTYPE:
                 raise TypeError(f"AdamW8: float32, bfloat16 or float16, not {p.dtype}")
@@ -63,7 +63,9 @@ class _Plan:
                 raise ValueError(f"AdamW8: a parameter {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
             at, n = p.data_ptr(), p.numel()
             m_at, v_at, master_at = m.data_ptr(), v.data_ptr(), 0 if master is None else master.data_ptr()
-            self.rows.append((p, at, n, None if p.is_contiguous() else p.stride(), p.dtype, s, m, v, master, m_at, v_at, master_at))
+            strides = None if p.is_contiguous() else p.stride()
+            self.rows.append((p, at, n, strides, s, m, v, master, m_at, v_at, master_at))
+            self.kinds.append((n, strides, p.dtype))
             self.table.extend((at, 0, m_at, v_at, master_at, n, q8._DTYPE[p.dtype]))
             self.written += (p, m, v) if master is None else (p, m, v, master)
         if group["capturable"]:
@@ -81,7 +83,7 @@ class _Plan:
         count = self.count
         if isinstance(count, torch.Tensor) and count.device != self.device:
             return False
-        for p, (mine, at, n, strides, _, s, m, v, master, m_at, v_at, master_at) in zip(params, self.rows):
+        for p, (mine, at, n, strides, s, m, v, master, m_at, v_at, master_at) in zip(params, self.rows):
             if p is not mine or p.data_ptr() != at or p.numel() != n:
                 return False
             if (not p.is_contiguous()) if strides is None else p.stride() != strides:
@@ -97,7 +99,7 @@ class _Plan:
         """Fills in the gradients' addresses; gives back what has to live until the launch."""
         copies, addresses = [], []
         strided, place = torch.strided, self.place
-        for (p, _, n, strides, dtype, *_), g in zip(self.rows, gradients):
+        for (n, strides, dtype), g, p in zip(self.kinds, gradients, self.params):
             if g.layout is not strided:
                 raise RuntimeError("AdamW8: no sparse gradients")
             if g.dtype is not dtype or g.numel() != n:
@@ -225,12 +227,11 @@ class AdamW8(torch.optim.Optimizer):
         if not self._same_states():
             self._forget()
         for number, group in enumerate(self.param_groups):
-            params, gradients = [], []
-            for p in group["params"]:
-                g = p.grad
-                if g is not None:
-                    params.append(p), gradients.append(g)
-            if not params:
+            params, gradients = group["params"], [p.grad for p in group["params"]]
+            given = [g for g in gradients if g is not None]
+            if len(given) < len(params):
+                params, gradients = [p for p, g in zip(params, gradients) if g is not None], given
+            if not given:
                 continue
             capturable = group["capturable"]
             options = _options(group)
@@ -429,7 +430,7 @@ def _held(optimizer):
         plans = optimizer._plans.get(number, ()) if same else ()
         if len(plans) == 1 and plans[0].holds(params, group):
             place = plans[0].place
-            for p, _, n, strides, _, s, _, _, _, m8, v8, _ in plans[0].rows:
+            for p, _, n, strides, s, _, _, _, m8, v8, _ in plans[0].rows:
                 yield p, group, s, n, place, strides is None, m8, v8
             continue
         for p in params:

@@ -617,3 +617,20 @@ def test_loading_takes_no_room_beyond_what_is_kept():
     again.load_state_dict(saved)
     assert torch.cuda.max_memory_allocated() - before <= 2 * (n * 33 // 32) + (2 << 20)      # two moments, and the allocator's rounding
     assert all(torch.equal(again.state[p][k], first.state[p][k]) for k in ("exp_avg", "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("eps", [1e-30, 1e-20])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_second_moments_below_the_normal_range_with_a_small_eps(bits, eps):
+    """Gradients whose squares fp32 holds as subnormal numbers: the step is the learning rate, not m / eps."""
+    rows = [[2.0 ** -k] * 32 for k in range(50, 68)] + [[-3e-19] * 32, [2.0 ** -50, -2.0 ** -62] * 16, [0.0] * 32]
+    g = torch.tensor(rows).reshape(-1)
+    p = torch.nn.Parameter(torch.full_like(g, 0.5).cuda())
+    p.grad = g.cuda()
+    optimizer = mod().AdamW8([p], lr=1e-2, betas=BETAS, eps=eps, weight_decay=0.0, bits=bits)
+    optimizer.step()
+    m, v = ref.moments(torch.zeros_like(g), torch.zeros_like(g), g, BETAS)
+    assert bool((v[:32] > 2.0 ** -126).all()) and bool(((v[64:18 * 32] > 0) & (v[64:18 * 32] < 2.0 ** -110)).all()) and int((v == 0).sum()) == 32
+    want, size = ref.update(torch.full_like(g, 0.5).double(), m, v, 1, 1e-2, BETAS, eps, 0.0)
+    assert float((want - 0.5).abs().max()) <= 0.25                      # v is a few bits there, but no step is m / eps
+    assert bool(((p.detach().cpu().double() - want).abs() <= bound(want, size, F32)).all())
