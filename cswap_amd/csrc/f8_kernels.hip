@@ -15,6 +15,7 @@
 // codes of NaN (0x7f): every result that it goes into is NaN.
 #include <hip/hip_runtime.h>
 #include "../../include/cswap_hip.h"
+#include "../../include/cswap_test_hooks.h"
 #include "common.h"
 #include "q8_block.h"
 #include "q8_params.h"
@@ -664,11 +665,36 @@ constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)
 // Tiles of 256 rows are made by as many workgroups as there are compute units, each of which goes on to its next tile.  Stages lie in LDS in pairs,
 // so that an odd number of them leaves the next tile's first one where a second would be: then a workgroup makes one tile.
 constexpr uint32_t kOnWorkgroups = 256;
+static bool goes_on(size_t kb, bool exact) { return exact || kb % 2 == 0; }
 
 // Few rows read the weights once, a workgroup to 16 columns; tiles of 128 x 128 have fewer workgroups but each value of the activations once for 128
 // columns.  us with codes ready, the former : the latter, 32 rows through 4096 x 1024 4.2 : 7.6, 1024 x 4096 8.3 : 16.8, 8192 x 8192 25.6 :
 // 30.0; 64 rows 6.0 : 7.8, 12.8 : 17.0, 42 : 31.
 static bool few_rows(size_t rows, size_t weights) { return rows <= kFewPacked || (rows <= kFewPackedSmall && weights <= kSmallWeights); }
+
+// Which kernel makes a product: 0 the one that turns few rows into codes itself, 32 and 64 the one for so many rows of codes, 128, 192 and 256 the one with tiles
+// of so many columns.
+static int product_form(size_t rows, size_t n, size_t k, bool exact)
+{
+  if (rows <= kFewRows) return 0;
+  if (few_rows(rows, n * k)) return rows <= kFewPacked ? 32 : 64;
+  const size_t kb = blocks_of(k);
+  // By what rounds of tiles on all compute units take, us, in blocks along k: of 256 x 256 and 256 x 192, one to a compute unit (further rounds begin sooner
+  // where workgroups go on), and of 128 x 128, two to one, of which one alone takes 0.62 of the time.  Measured, large : middle : small, bf16 16384 x 1024 x 4096
+  // 57 : 80 : 70, 16384 x 4096 x 1024 70 : 87 : 82, 16384 x 768 x 2304 33 : 31 : 33, 16384 x 768 x 768 18 : 17 : 18, 8192 x 1152 x 1152 22 : 19 : 20, 2048^3 25 : - : 15;
+  // fp32 4096^3 119 : 171 : 142, 16384 x 4096 x 1024 156 : 163 : 167, 25216 x 384 x 1536 51 : 41 : 44, 16384 x 768 x 768 34 : 28 : 29, 2048^3 53 : 45 : 26.
+  const bool on = goes_on(kb, exact);
+  auto tiles = [&](size_t tm, size_t tn) { return ((rows + tm - 1) / tm) * ((n + tn - 1) / tn); };
+  auto one_each = [&](size_t count, double first, double further, double block) {
+    const size_t rounds = (count + 255) / 256;
+    return first + (rounds - 1) * (on ? further : first) + rounds * kb * block;
+  };
+  const size_t count = tiles(128, 128), rest = count % 512;
+  const double small = 4.0 + (count / 512 + (rest == 0 ? 0.0 : rest <= 256 ? 0.62 : 1.0)) * (2.3 + (exact ? 2.25 : 1.02) * kb);
+  const double middle = exact ? one_each(tiles(256, 192), 15.0, 9.0, 2.15) : one_each(tiles(256, 192), 10.5, 5.5, 1.12);
+  const double large = exact ? one_each(tiles(256, 256), 13.0, 10.0, 3.34) : one_each(tiles(256, 256), 10.0, 4.3, 1.43);
+  return large < small && large <= middle ? 256 : middle < small ? 192 : 128;
+}
 
 // Launches have fewer than 2^32 threads: 256 to 16 rows of a block, or to a tile of 128 x 128, 1024 to a block of weights.
 static bool f8_shape(size_t rows, size_t n, size_t k)
@@ -683,6 +709,11 @@ static bool f8_shape(size_t rows, size_t n, size_t k)
 
 using namespace cswap;
 using namespace cswap::q8;
+
+extern "C" int cswap_test_f8_linear_form(size_t rows, size_t n, size_t k, int out_dtype)
+{
+  return n == 0 || k == 0 || !f8_shape(rows, n, k) ? -1 : product_form(rows, n, k, out_dtype == CSWAP_DT_F32);
+}
 
 extern "C" size_t cswap_f8_linear_workspace_bytes(size_t rows, size_t k)
 {
@@ -728,12 +759,14 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
   const uint32_t kb = (uint32_t)blocks_of(k), nb = (uint32_t)blocks_of(n);
   F8Shape s = {(uint32_t)rows, (uint32_t)n, kb, (uint32_t)padded(rows), turned ? 1u : kb, turned ? nb : 1u, 0, 0, (size_t)y_stride};
   const F8Out out = {d_y, d_bias, out_dtype, bias_dtype};
+  const bool exact = out_dtype == CSWAP_DT_F32;
+  const int form = product_form(rows, n, k, exact);
   return with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     const typename T::value* x = static_cast<const typename T::value*>(d_x);
     const dim3 columns((unsigned)((n + 15) / 16)), threads(64 * kFewWaves);
-    if (rows <= kFewRows) {
-      auto f = out_dtype == CSWAP_DT_F32 ? f8_few_rows_kernel<T, 1, true, false> : f8_few_rows_kernel<T, 1, false, false>;
+    if (form == 0) {
+      auto f = exact ? f8_few_rows_kernel<T, 1, true, false> : f8_few_rows_kernel<T, 1, false, false>;
       hipLaunchKernelGGL(f, columns, threads, 0, st, x, (size_t)x_stride, (uint32_t)k, nullptr, nullptr, s, d_codes, d_scales, out);
       return check_launch();
     }
@@ -741,42 +774,27 @@ extern "C" int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k
     hipLaunchKernelGGL(f8_rows_kernel<T>, dim3((unsigned)((rows + 15) / 16 * kb)), dim3(256), 0, st, x, (size_t)x_stride, (uint32_t)rows, (uint32_t)k, kb,
                        reinterpret_cast<uint2*>(codes), scales, s.scale_pitch);
     if (int e = check_launch()) return e;
-    if (few_rows(rows, n * k)) {
+    if (form <= 64) {
       auto few = [&](auto f) {
         hipLaunchKernelGGL(f, columns, threads, 0, st, nullptr, 0, (uint32_t)k, codes, scales, s, d_codes, d_scales, out);
         return check_launch();
       };
-      if (out_dtype == CSWAP_DT_F32) return rows <= 32 ? few(f8_few_rows_kernel<F32, 2, true, true>) : few(f8_few_rows_kernel<F32, 4, true, true>);
-      return rows <= 32 ? few(f8_few_rows_kernel<F32, 2, false, true>) : few(f8_few_rows_kernel<F32, 4, false, true>);
+      if (exact) return form == 32 ? few(f8_few_rows_kernel<F32, 2, true, true>) : few(f8_few_rows_kernel<F32, 4, true, true>);
+      return form == 32 ? few(f8_few_rows_kernel<F32, 2, false, true>) : few(f8_few_rows_kernel<F32, 4, false, true>);
     }
     auto launch = [&](auto f, uint32_t tm, uint32_t tn, uint32_t threads) {
       s.tiles_m = (uint32_t)((rows + tm - 1) / tm), s.tiles_n = (uint32_t)((n + tn - 1) / tn);
       const uint32_t count = s.tiles_m * s.tiles_n;
-      hipLaunchKernelGGL(f, dim3(tm + tn > 256 && (out_dtype == CSWAP_DT_F32 || kb % 2 == 0) && count > kOnWorkgroups ? kOnWorkgroups : count), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
+      hipLaunchKernelGGL(f, dim3(tm + tn > 256 && goes_on(kb, exact) && count > kOnWorkgroups ? kOnWorkgroups : count), dim3(threads), 0, st, codes, scales, d_codes, d_scales, s, out);
       return check_launch();
     };
-    // By what rounds of tiles on all compute units take, us, in blocks along k: of 256 x 256 and 256 x 192, one to a compute unit (further rounds begin sooner
-    // where workgroups go on), and of 128 x 128, two to one, of which one alone takes 0.62 of the time.  Measured, large : middle : small, bf16 16384 x 1024 x 4096
-    // 57 : 80 : 70, 16384 x 4096 x 1024 70 : 87 : 82, 16384 x 768 x 2304 33 : 31 : 33, 16384 x 768 x 768 18 : 17 : 18, 8192 x 1152 x 1152 22 : 19 : 20, 2048^3 25 : - : 15;
-    // fp32 4096^3 119 : 171 : 142, 16384 x 4096 x 1024 156 : 163 : 167, 25216 x 384 x 1536 51 : 41 : 44, 16384 x 768 x 768 34 : 28 : 29, 2048^3 53 : 45 : 26.
-    const bool exact = out_dtype == CSWAP_DT_F32, on = exact || kb % 2 == 0;
-    auto tiles = [&](size_t tm, size_t tn) { return ((rows + tm - 1) / tm) * ((n + tn - 1) / tn); };
-    auto one_each = [&](size_t count, double first, double further, double block) {
-      const size_t rounds = (count + 255) / 256;
-      return first + (rounds - 1) * (on ? further : first) + rounds * kb * block;
-    };
-    const size_t count = tiles(128, 128), rest = count % 512;
-    const double small = 4.0 + (count / 512 + (rest == 0 ? 0.0 : rest <= 256 ? 0.62 : 1.0)) * (2.3 + (exact ? 2.25 : 1.02) * kb);
-    const double middle = exact ? one_each(tiles(256, 192), 15.0, 9.0, 2.15) : one_each(tiles(256, 192), 10.5, 5.5, 1.12);
-    const double large = exact ? one_each(tiles(256, 256), 13.0, 10.0, 3.34) : one_each(tiles(256, 256), 10.0, 4.3, 1.43);
-    const int pick = large < small && large <= middle ? 2 : middle < small ? 1 : 0;
     if (exact) {
-      if (pick == 2) return launch(f8_product_kernel<256, 256, 2, 2, true>, 256, 256, 256);
-      if (pick == 1) return launch(f8_product_kernel<256, 192, 2, 2, true>, 256, 192, 256);
+      if (form == 256) return launch(f8_product_kernel<256, 256, 2, 2, true>, 256, 256, 256);
+      if (form == 192) return launch(f8_product_kernel<256, 192, 2, 2, true>, 256, 192, 256);
       return launch(f8_product_kernel<128, 128, 2, 2, true>, 128, 128, 256);
     }
-    if (pick == 2) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
-    if (pick == 1) return launch(f8_product_kernel<256, 192, 2, 2, false>, 256, 192, 256);
+    if (form == 256) return launch(f8_product_kernel<256, 256, 2, 2, false>, 256, 256, 256);
+    if (form == 192) return launch(f8_product_kernel<256, 192, 2, 2, false>, 256, 192, 256);
     return launch(f8_product_kernel<128, 128, 2, 2, false>, 128, 128, 256);
   });
 }

@@ -61,6 +61,10 @@ int cswap_test_zfp_decode_runs(size_t nx, size_t ny, size_t nz, ptrdiff_t sy, pt
  * tiles of 128 x 256 features, 2000 more with 256 x 256, 3000 more with 64 x 256 (else 128 x 128).  Host only. */
 int cswap_test_weight_grad_plan(int dtype, size_t rows, size_t n, size_t k);
 
+/* Which kernel makes a product of cswap_f8_linear: 0 the one that turns few rows into codes itself, 32 and 64 the one for so many
+ * rows of codes, 128 tiles of 128 x 128 results, 192 of 256 x 192, 256 of 256 x 256; -1: refused.  Host only. */
+int cswap_test_f8_linear_form(size_t rows, size_t n, size_t k, int out_dtype);
+
 #ifdef __cplusplus
 }
 #endif

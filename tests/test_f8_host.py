@@ -165,3 +165,23 @@ def test_traces_and_forward_mode_are_refused(name):
             watched()[name](forward_ad.make_dual(x, torch.ones_like(x)))
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(watched()[name], x, check_trace=False)
+
+
+def test_the_products_that_are_tested_run_every_form():
+    """Whatever the rule that chooses a form becomes, each has a product of its own in either type of results, and large tiles have even and odd numbers
+    of blocks and fewer and more tiles than compute units."""
+    import f8_tile_cases as tiles
+
+    form = _lib.lib().cswap_test_f8_linear_form
+    for want, bits, rows, n, k in tiles.CASES:
+        assert [form(rows, n, k, out) for out in ((1, 2) if bits == 16 else (0,))] == [want] * (2 if bits == 16 else 1), (want, bits, rows, n, k)
+        assert n % 32 and (rows % 32 or want < 128) and k % 128
+    assert {(f, b) for f, b, *_ in tiles.CASES} == {(f, b) for f in (0, 32, 64, 128, 192, 256) for b in (16, 32)}
+    for f in (192, 256):
+        for bits in (16, 32):
+            kinds = {(-(-k // 128) % 2, -(-rows // 256) * -(-n // f) > 256) for g, b, rows, n, k in tiles.CASES if (g, b) == (f, bits)}
+            assert kinds == {(0, False), (0, True), (1, False), (1, True)}, (f, bits)
+    assert form(0, 5, 5, 0) == 0 and form(40, 0, 5, 0) == -1 and form(1 << 31, 5, 5, 0) == -1
+    x = tiles.blocks(300, 300, 1, "cpu", 1)
+    assert set(x.abs().unique().tolist()) == {0.0, 1.0, 2.0, 4.0, 8.0} and fref.held(x, 1)[0].equal(x.double())
+    assert set(fref.held(x, 1)[1].flatten().tolist()) == {119, 120, 121, 122}
