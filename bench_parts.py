@@ -11,7 +11,7 @@ from cswap_amd import api, swap
 from cswap_amd._lib import Costs
 from cswap_amd.adamw8 import AdamW8
 from cswap_amd.hooks import hold_saved_tensors, swap_saved_tensors
-from cswap_amd.layers8 import Linear8, LinearF8, checkpoint_layers
+from cswap_amd.layers8 import checkpoint_layers
 from cswap_amd.planner import PolicyMaker, run_planned_iteration
 from cswap_amd.workloads import dummy_layer_compute, vgg16_modules
 
@@ -364,9 +364,7 @@ def bench_transformer_step(dev, layers: int = 4, batch: int = 32, seq: int = 512
     held("layers_8bit", lambda: None)
     held("layers_and_held_8bit", lambda: hold_saved_tensors(min_bytes))
     # the same layers with their products in 8-bit floating point
-    for m in net.modules():
-        if type(m) is Linear8:
-            m.__class__ = LinearF8
+    checkpoint_layers(net, f8=True)
     held("layers_f8", lambda: None)
     res["optimizer"] = _optimizer_steps(params)
     return res

@@ -345,11 +345,16 @@ def checkpoint_layers(model: nn.Module, group_norm: bool = False, f8: bool = Fal
     parameters, hooks and state stay as they are.  Classes derived from them are left alone, and so are a SiLU that works
     in place, a layer norm over more than 16384 values, a linear layer with more than 2^20 features on one side, and either over
     none.  ``group_norm=True``: every ``nn.GroupNorm`` of up to 4096 channels in up to 2048 groups, too, for models whose images lie channels last.
-    ``f8=True``: linear layers become ``LinearF8``."""
+    ``f8=True``: linear layers become ``LinearF8``, those that are ``Linear8`` already among them."""
+    kinds = dict(_KINDS)
+    if group_norm:
+        kinds[nn.GroupNorm] = GroupNorm8
+    if f8:
+        kinds[nn.Linear] = kinds[Linear8] = LinearF8
     for m in model.modules():
-        to = _KINDS.get(type(m)) or (GroupNorm8 if group_norm and type(m) is nn.GroupNorm else None)
+        to = kinds.get(type(m))
         if to is not None and _fits(m):
-            m.__class__ = LinearF8 if f8 and to is Linear8 else to
+            m.__class__ = to
     return model
 
 
@@ -360,4 +365,4 @@ def _fits(m: nn.Module) -> bool:
         return 0 < math.prod(m.normalized_shape) <= q8.MAX_NORM
     if type(m) is nn.GroupNorm:
         return 0 < m.num_channels <= q8.MAX_CHANNELS and m.num_groups <= q8.MAX_GROUPS
-    return type(m) is not nn.Linear or 0 < min(m.weight.shape) and max(m.weight.shape) <= q8.MAX_FEATURES
+    return type(m) not in (nn.Linear, Linear8) or 0 < min(m.weight.shape) and max(m.weight.shape) <= q8.MAX_FEATURES

@@ -185,3 +185,25 @@ def test_the_products_that_are_tested_run_every_form():
     x = tiles.blocks(300, 300, 1, "cpu", 1)
     assert set(x.abs().unique().tolist()) == {0.0, 1.0, 2.0, 4.0, 8.0} and fref.held(x, 1)[0].equal(x.double())
     assert set(fref.held(x, 1)[1].flatten().tolist()) == {119, 120, 121, 122}
+
+
+def test_layers_that_hold_their_input_become_layers_of_8_bit_products_too():
+    """One call after the other on a model, in whatever order, gives what one call with both gives; classes derived from either are left alone."""
+    from torch import nn
+
+    class Mine(layers8.Linear8):
+        pass
+
+    model = nn.Sequential(nn.Linear(3, 4), Mine(4, 4), nn.GELU(), nn.LayerNorm(4))
+    weights = [p.data_ptr() for p in model.parameters()]
+    layers8.checkpoint_layers(model)
+    assert [type(m) for m in model] == [layers8.Linear8, Mine, layers8.GELU8, layers8.LayerNorm8]
+    layers8.checkpoint_layers(model, f8=True)
+    assert [type(m) for m in model] == [layers8.LinearF8, Mine, layers8.GELU8, layers8.LayerNorm8]
+    layers8.checkpoint_layers(model)                                # what is there stays
+    assert [type(m) for m in model] == [layers8.LinearF8, Mine, layers8.GELU8, layers8.LayerNorm8]
+    assert [p.data_ptr() for p in model.parameters()] == weights
+    wide = nn.Linear(3, 4)
+    wide.__class__ = layers8.Linear8
+    wide.weight = nn.Parameter(torch.empty(0, 3))
+    assert type(layers8.checkpoint_layers(wide, f8=True)) is layers8.Linear8
