@@ -118,14 +118,19 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return _Linear.apply(x, weight, bias, held)
 
 
+def _same_weight(weight8: F8Weight, weight: torch.Tensor, turned: bool) -> None:
+    if tuple(weight8.shape) != tuple(weight.shape) or weight8.device != weight.device or turned and weight8.turned is None:
+        raise ValueError(f"linear_f8: weight8 is {weight8} on {weight8.device}, the weight {tuple(weight.shape)} on {weight.device}")
+
+
 class _LinearF8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, held, weight8):
         need_x, need_w = ctx.needs_input_grad[:2]
         if weight8 is None:
             weight8 = _f8.f8_weight(_rows(weight.detach()), backward=need_x)
-        elif tuple(weight8.shape) != tuple(weight.shape) or weight8.device != weight.device or need_x and weight8.turned is None:
-            raise ValueError(f"linear_f8: weight8 is {weight8} on {weight8.device}, the weight {tuple(weight.shape)} on {weight.device}")
+        else:
+            _same_weight(weight8, weight, need_x)
         if need_w:
             if held is None:
                 held = hold(x)
@@ -172,7 +177,11 @@ def linear_f8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None =
         dtype = torch.get_autocast_dtype("cuda")
         x, weight, bias = (t if t is None else t.to(dtype) for t in (x, weight, bias))
     if not torch.is_grad_enabled():
-        return _f8.f8_linear(_rows(x), weight8 or _f8.f8_weight(_rows(weight), backward=False), bias)
+        if weight8 is None:
+            weight8 = _f8.f8_weight(_rows(weight), backward=False)
+        else:
+            _same_weight(weight8, weight, False)
+        return _f8.f8_linear(_rows(x), weight8, bias)
     return _LinearF8.apply(x, weight, bias, held, weight8)
 
 

@@ -207,3 +207,12 @@ def test_layers_that_hold_their_input_become_layers_of_8_bit_products_too():
     wide.__class__ = layers8.Linear8
     wide.weight = nn.Parameter(torch.empty(0, 3))
     assert type(layers8.checkpoint_layers(wide, f8=True)) is layers8.Linear8
+
+
+def test_codes_of_another_weight_are_refused_with_and_without_gradients():
+    codes, scales = torch.zeros(128, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1, dtype=torch.uint8)
+    held = f8.F8Weight(codes, scales, (40, 30), torch.float32, codes.clone())
+    x, w = torch.zeros(4, 30), torch.zeros(50, 30, requires_grad=True)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode(), pytest.raises(ValueError, match="weight8"):
+            layers8.linear_f8(x, w, None, weight8=held)
