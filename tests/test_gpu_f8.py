@@ -443,3 +443,57 @@ def test_biases_and_rows_that_start_at_any_element(dtype):
         want = f8().f8_weight(w[:, 1:k + 1].contiguous())
         assert torch.equal(again.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(again.turned.view(torch.uint8), want.turned.view(torch.uint8))
         assert torch.equal(again.scales, want.scales)
+
+
+def test_a_captured_training_step_is_the_eager_one_to_the_bit():
+    """Group norm, linear layers in 8-bit floating point, activation functions, layer norm and the 8-bit optimiser make their sums in fixed orders: steps on
+    inputs of their own, captured and eager, leave the same parameters and the same moments."""
+    from cswap_amd import adamw8, layers8
+    from torch import nn
+
+    def build():
+        torch.manual_seed(0)
+        net = nn.Sequential(nn.GroupNorm(4, 32), nn.SiLU(), nn.Flatten(), nn.Linear(32 * 36, 200), nn.GELU(), nn.LayerNorm(200), nn.Linear(200, 10))
+        net = layers8.checkpoint_layers(net, group_norm=True, f8=True).cuda().to(BF16)
+        assert [type(m).__name__ for m in net] == ["GroupNorm8", "SiLU8", "Flatten", "LinearF8", "GELU8", "LayerNorm8", "LinearF8"]
+        return net, adamw8.AdamW8(net.parameters(), lr=1e-2, master=True, capturable=True)
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    inputs = [torch.randn(40, 32, 6, 6, generator=g, device="cuda").to(BF16).to(memory_format=torch.channels_last) for _ in range(7)]
+    targets = [torch.randn(40, 10, generator=g, device="cuda") for _ in inputs]
+    x, t = inputs[0].clone(memory_format=torch.channels_last), targets[0].clone()
+
+    def step(net, optimizer):
+        (net(x).float() - t).square().sum().backward()
+        optimizer.step()
+        for p in net.parameters():
+            p.grad.zero_()
+
+    def kept(net, optimizer):
+        return [v.clone() for p in net.parameters() for v in (p.detach(), *(s for s in optimizer.state[p].values() if isinstance(s, torch.Tensor)))]
+
+    eager, captured = build(), build()
+    start = [p.detach().clone() for p in eager[0].parameters()]
+    wanted = []
+    for k in range(7):
+        x.copy_(inputs[k]), t.copy_(targets[k])
+        step(*eager)
+        wanted.append(kept(*eager))
+    side = torch.cuda.Stream()
+    for k in range(3):
+        x.copy_(inputs[k]), t.copy_(targets[k])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*captured)
+        torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(*captured)
+    for k in range(3, 7):
+        x.copy_(inputs[k]), t.copy_(targets[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        torch.randn(1000, device="cuda").sum().item()
+        assert all(torch.equal(a, e) for a, e in zip(kept(*captured), wanted[k], strict=True)), k
+    assert all(bool((p != q).any()) for p, q in zip(captured[0].parameters(), start))
+    assert all(any(bool((a != b).any()) for a, b in zip(wanted[k], wanted[k + 1])) for k in range(6))
