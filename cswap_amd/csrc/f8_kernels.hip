@@ -201,10 +201,11 @@ __device__ inline void store_one(const F8Out& o, size_t at, float v)
   else static_cast<uint16_t*>(o.y)[at] = o.dtype == CSWAP_DT_BF16 ? from_float<BF16>(v) : from_float<F16>(v);
 }
 
-// Results in 16 bits come from the 8-bit matrix instructions.  These line a call's products up before they add them, and what lies more than 13 bits below
-// the largest product is cut off (measured; the sum with what was there before is fp32): a result is off by about 3e-5 of the products' norm,
-// a tenth of what rounding it to fp16 costs and a fiftieth of bf16's.  Results in fp32 (EXACT) come from the codes as bf16, which hold them
-// and their scales exactly, at half the rate: products are exact and sums fp32.
+// Results in 16 bits come from the 8-bit matrix instructions.  These line up each eight neighbouring products before they add them, and cut each of them
+// to a multiple of 2^-13 of the power of two in the largest (measured; the sums of eights are added in fp32): at most 7 * 2^-13 of the largest of
+// eight, as a rule 3e-5 of the products' norm, a tenth of what rounding to fp16 costs and a fiftieth of bf16's, where values themselves are held to 2^-4.
+// That is why it is taken: exact products are at half the rate.  Results in fp32 (EXACT) have them: they come from the codes as bf16, which hold them
+// and their scales exactly, products are exact and sums fp32.
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 

@@ -8,7 +8,9 @@ a scale for each 128 values of a row of activations and for each 128 x 128 weigh
     dx   = f8_linear_backward(dy, held)     # dy @ w
 
 Tensors are float32, bfloat16 or float16 in device memory, ``[..., features]`` with one distance between rows, on the current stream of
-their device; nothing waits.  A value is off by at most 2^-4 of itself (2^-18 of its block's largest below that), sums are fp32; a NaN or an
+their device; nothing waits.  A value is off by at most 2^-4 of itself (2^-18 of its block's largest below that).  Results in float32 are fp32
+sums of exact products; results in 16 bits come from the 8-bit matrix instructions, which cut each of eight neighbouring products to a multiple of 2^-13 of the
+power of two in the largest of them (as a rule 3e-5 of the products' norm in all) and add up the eights in fp32: ``out_dtype=torch.float32`` where that matters.  A NaN or an
 infinity makes the results of its block's rows (of weights: columns) NaN.  The weight's gradient comes from the input's 8-bit checkpoint
 (``q8.q8_weight_grad``); ``layers8.LinearF8`` has all three.
 """

@@ -353,7 +353,7 @@ int cswap_q8_weight_grad(const void* d_dy, int dtype, size_t rows, size_t n, ptr
 
 /* ---------------------------------- products in 8-bit floating point (f8) -----
  * y = x W^T + bias of a linear layer (W: n x k) with both operands in e4m3 (sign, four bits of exponent, three of mantissa, 448 the
- * largest) and a power of two for each 128 consecutive values of a row of x and for each 128 x 128 weights, sums in fp32.  The power of a
+ * largest) and a power of two for each 128 consecutive values of a row of x and for each 128 x 128 weights.  The power of a
  * block is the least 2^s, s >= -126, with max <= 448 * 2^s, held as the byte s + 127; a value is held as x / 2^s rounded to e4m3, to nearest even: off by at
  * most 2^-4 of itself, or 2^-10 * 2^s.  A block that holds a NaN or an infinity has codes of NaN (0x7f, byte 127): its results are NaN.
  * Weights are laid out once: codes [n'][k'], n' and k' rounded up to multiples of 128, 0 behind the last ones; `turned` (NULL: not wanted)
@@ -365,7 +365,9 @@ int cswap_f8_pack_weight(const void* d_w, int dtype, size_t n, size_t k, ptrdiff
                          uint8_t* d_scales, cswap_stream_t stream);
 /* d_y (rows x n, out_dtype) from d_x (rows x k, dtype) and the codes of n x k weights; turned = 1: d_codes is `turned` of a k x n
  * matrix, d_scales its scales.  d_bias may be NULL.  d_ws: cswap_f8_linear_workspace_bytes (NULL where that is 0), 16-byte
- * aligned, no preparation; calls that overlap must not share one.  Sums are made in a fixed order. */
+ * aligned, no preparation; calls that overlap must not share one.  Results in fp32 are fp32 sums of exact products.  For results in 16 bits
+ * each of eight products that are neighbours along k is cut towards 0 to a multiple of 2^-13 of the power of two in the largest of the eight (at most 7 * 2^-13 of that
+ * product, as a rule 3e-5 of the products' norm in all) and the sums of eights are added in fp32.  Sums are made in a fixed order. */
 size_t cswap_f8_linear_workspace_bytes(size_t rows, size_t k);
 int cswap_f8_linear(const void* d_x, int dtype, size_t rows, size_t k, ptrdiff_t x_stride, const uint8_t* d_codes,
                     const uint8_t* d_scales, size_t n, int turned, const void* d_bias, int bias_dtype, void* d_y,
