@@ -306,6 +306,9 @@ class AdamW8(torch.optim.Optimizer):
         def convert(_):                 # before they see what was loaded
             for group, mine, saved in zip(self.param_groups, own, given["param_groups"]):
                 group.update(mine)
+                lr = group["lr"]
+                if isinstance(lr, torch.Tensor):
+                    group["lr"] = lr.to(next(iter(group["params"]), lr).device, torch.float32) if group["capturable"] else float(lr)
                 steps = {}              # each group counts its own
                 for p, number in zip(group["params"], saved["params"]):
                     kept = given["state"].get(number)

@@ -377,3 +377,26 @@ def test_loading_moments_of_8_bits_makes_them_in_no_other_type(launches, dtype):
     saved["state"]["extra"] = {}
     other.load_state_dict(saved)
     assert other.state["extra"] == {} and other.state[a]["step"] == 1
+
+
+@pytest.mark.parametrize("lr", [torch.tensor(0.25), torch.tensor(0.25, dtype=torch.float64), 0.25])
+def test_options_that_torchs_optimiser_holds_as_tensors_are_loaded(launches, lr):
+    """``torch.optim.AdamW`` may count and hold its learning rate on the device; a loaded one goes on as its own ``capturable`` says."""
+    a = parameter(40)
+    plain = torch.optim.AdamW([torch.nn.Parameter(torch.ones(40))], lr=0.5)
+    saved = plain.state_dict()
+    saved["state"][0] = {"step": torch.tensor(3.0), "exp_avg": torch.ones(40), "exp_avg_sq": torch.ones(40)}
+    saved["param_groups"][0].update(lr=lr, capturable=True)
+    optimizer = AdamW8([a], bits=32)
+    optimizer.load_state_dict(saved)
+    group = optimizer.param_groups[0]
+    assert type(group["lr"]) is float and group["lr"] == 0.25 and group["capturable"] is False
+    optimizer.step()
+    assert launches == [(4, held(optimizer, a))]
+    counted = AdamW8([a], bits=32, capturable=True)
+    counted.load_state_dict(saved)
+    given = counted.param_groups[0]["lr"]
+    if isinstance(lr, torch.Tensor):
+        assert given.dtype is torch.float32 and float(given) == 0.25 and given.device == a.device and given is not lr
+    else:
+        assert given == 0.25
