@@ -95,18 +95,29 @@ class _Plan:
                 return False
         return True
 
+    def moments_hold(self, params, group) -> bool:
+        """The same of what a conversion of the moments reads."""
+        if len(params) != len(self.rows) or self.how != _how(group):
+            return False
+        for p, (mine, _, n, strides, s, m, v, _, m_at, v_at, _) in zip(params, self.rows):
+            if p is not mine or p.numel() != n or ((not p.is_contiguous()) if strides is None else p.stride() != strides):
+                return False
+            if s.get("exp_avg") is not m or s.get("exp_avg_sq") is not v or m.data_ptr() != m_at or v.data_ptr() != v_at:
+                return False
+        return True
+
     def set_gradients(self, gradients):
         """Fills in the gradients' addresses; gives back what has to live until the launch."""
         copies, addresses = [], []
-        strided, place = torch.strided, self.place
+        place = self.place
         for (n, strides, dtype), g, p in zip(self.kinds, gradients, self.params):
-            if g.layout is not strided:
-                raise RuntimeError("AdamW8: no sparse gradients")
             if g.dtype is not dtype or g.numel() != n:
                 raise TypeError(f"AdamW8: a gradient {tuple(g.shape)} {g.dtype} of a parameter {tuple(p.shape)} {dtype}")
             if g.get_device() != place:
                 raise ValueError(f"AdamW8: a gradient on {g.device} of a parameter on {p.device}")
             if ((not g.is_contiguous()) if strides is None else g.stride() != strides) or g.is_neg():
+                if g.layout is not torch.strided:       # (none of these is contiguous)
+                    raise RuntimeError("AdamW8: no sparse gradients")
                 g = torch.empty_like(p).copy_(g)
                 copies.append(g)
             addresses.append(g.data_ptr())
@@ -431,7 +442,7 @@ def _held(optimizer):
     for number, group in enumerate(optimizer.param_groups):
         params = [p for p in group["params"] if "exp_avg" in optimizer.state.get(p, ())]
         plans = optimizer._plans.get(number, ()) if same else ()
-        if len(plans) == 1 and plans[0].holds(params, group):
+        if len(plans) == 1 and plans[0].moments_hold(params, group):
             place = plans[0].place
             for p, _, n, strides, s, _, _, _, m8, v8, _ in plans[0].rows:
                 yield p, group, s, n, place, strides is None, m8, v8
