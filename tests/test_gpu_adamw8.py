@@ -634,3 +634,44 @@ def test_second_moments_below_the_normal_range_with_a_small_eps(bits, eps):
     want, size = ref.update(torch.full_like(g, 0.5).double(), m, v, 1, 1e-2, BETAS, eps, 0.0)
     assert float((want - 0.5).abs().max()) <= 0.25                      # v is a few bits there, but no step is m / eps
     assert bool(((p.detach().cpu().double() - want).abs() <= bound(want, size, F32)).all())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_that_goes_to_the_host_and_comes_back(bits, capturable):
+    """As programs do that need the room between steps: with other tensors, or with other memory for the same ones."""
+    params = [torch.nn.Parameter(gradient((n,), d, n, 0.5).cuda()) for n, d in ((300, F32), (3000, BF16))]
+    stay = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = (mod().AdamW8(some, bits=bits, master=True, capturable=capturable) for some in (params, stay))
+
+    def step(t, refused=False):
+        for i, (p, q) in enumerate(zip(params, stay)):
+            p.grad = gradient(p.shape, p.dtype, 10 * t + i).cuda()
+            q.grad = p.grad.clone()
+        if refused:
+            with pytest.raises(ValueError, match="moment"):
+                a.step()
+        else:
+            a.step(), b.step()
+
+    def move(to, data):
+        for s in a.state.values():
+            for k, v in s.items():
+                if isinstance(v, torch.Tensor):
+                    if data:
+                        v.data = v.data.to(to)
+                    else:
+                        s[k] = v.to(to)
+
+    step(0), step(1)
+    for t, data in ((2, False), (3, True)):
+        move("cpu", data)
+        filler = torch.full((1 << 20,), 0x55, dtype=torch.uint8, device="cuda")         # where the moments were
+        step(t, refused=True)
+        move("cuda", data)
+        step(t)
+        assert bool((filler == 0x55).all())
+    for p, q in zip(params, stay):
+        assert torch.equal(p.detach(), q.detach()) and int(a.state[p]["step"]) == int(b.state[q]["step"]) == 4
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(a.state[p][k], b.state[q][k])
