@@ -7,7 +7,9 @@ optimiser's two moments, 8 bytes a parameter in fp32 and 2.06 here:
     loss.backward();  optimizer.step()
     moments = unpack_moments(optimizer)                         # [(exp_avg, exp_avg_sq)] in fp32
 
-A step is one launch for every 64 tensors, of any mixture of types, on the current stream of their device; nothing waits for it.
+A step is one launch for every 64 tensors, of any mixture of types, on the current stream of their device; nothing waits for it.  It goes by
+``optimizer.state`` as it then is, whoever cleared, replaced or moved what is in it, and autograd is told what it writes: a backward pass through
+weights that a step has moved is refused, as with torch's optimisers.  Steps and conversions refuse to be traced.
 """
 from __future__ import annotations
 
@@ -298,7 +300,7 @@ class AdamW8(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Of an ``AdamW8`` or of a ``torch.optim.AdamW``; this optimiser's own ``bits``, ``master`` and ``capturable`` stay, and moments are
-        converted to them (to 8 bits: to nearest)."""
+        converted to them (to 8 bits: to nearest), one parameter at a time."""
         own = [{k: group[k] for k in _OWN} for group in self.param_groups]
         given = {}
 

@@ -21,7 +21,7 @@
 // (the build contracts nothing); what only the parameter sees goes through v_sqrt_f32 and v_rcp_f32, one unit off in the last place each.
 //
 // Memory bounds it: bf16 with moments in 8 bits 10.1 bytes a value, fp32 with fp32 moments 28.  Traced: 101.8 M bf16 values in 130 tensors, moments in
-// 8 bits, two launches of 102 us and one of 7 (4.9 TB/s; a copy reaches 5.1), 51.4 M fp32 values with fp32 moments 260 and 10 (5.3 TB/s), the moments as fp32 values 112
+// 8 bits, two launches of 99 us and one of 7 (5.0 TB/s; a copy reaches 5.1), 51.4 M fp32 values with fp32 moments 260 and 10 (5.3 TB/s), the moments as fp32 values 111
 // a launch (4.5 TB/s).  The tensors of a launch are in its
 // arguments (so that it needs no table in device memory, which a
 // capture or a second call could find changed), a workgroup finds its tensor by halving.
@@ -136,7 +136,7 @@ __device__ inline void store_moments(const float m[8], const float v[8], uint32_
 }
 
 // v_sqrt_f32 takes a subnormal for 0.  Its root, below 2^-63, is nothing beside an eps of 2^25 times as much; with a smaller eps, which m
-// would be divided by alone, such v are brought up by 2^64 first (with five instructions a value more: 3 us of 102 where no v needs it).
+// would be divided by alone, such v are brought up by 2^64 first (five instructions a value: 3 us more a launch of 99).
 __device__ inline bool roots_matter(const StepFactors& f) { return f.eps < 0x1p-38f * f.root; }
 __device__ inline float root_of(float v, bool matter)
 {

@@ -664,7 +664,8 @@ constexpr size_t kFewRows = 16;  // up to which the product's kernel turns activ
 constexpr size_t kFewPacked = 32, kFewPackedSmall = 64, kSmallWeights = (size_t)1 << 24;
 
 // Tiles of 256 rows are made by as many workgroups as there are compute units, each of which goes on to its next tile.  Stages lie in LDS in pairs,
-// so that an odd number of them leaves the next tile's first one where a second would be: then a workgroup makes one tile.
+// so that an odd number of them leaves the next tile's first one where a second would be: then a workgroup makes one tile (16384 x 4096 by 1024, 1152 and
+// 1280 along k, 8, 9 and 10 blocks: 71, 85 and 83 us).
 constexpr uint32_t kOnWorkgroups = 256;
 static bool goes_on(size_t kb, bool exact) { return exact || kb % 2 == 0; }
 

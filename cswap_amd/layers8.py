@@ -11,8 +11,8 @@ stays on the device in one byte a value, and the layer's backward pass reads it 
     y = layers8.group_norm(x, 32, weight, bias, act="silu")            # with an activation function in the same call
     y = layers8.linear(x, weight, bias)     # or function by function
 
-Outputs are those of the layers without checkpoints (linear layers run torch's own product; norms and activation
-functions are computed in fp32 and rounded once, which may differ from torch's in the last place); gradients are
+Outputs are those of the layers without checkpoints (linear layers run torch's own product, those with ``f8=True`` that of ``cswap_amd.f8``, whose
+operands are held to 2^-4; norms and activation functions are computed in fp32 and rounded once, which may differ from torch's in the last place); gradients are
 computed from inputs that are off by at most 2^-7 of the largest magnitude among 32 neighbours (a layer norm whose
 rows have a mean of many times their deviation is better left as it is).  Without gradients to come nothing is
 kept.  Layers that share an input (the projections of an attention layer) can
